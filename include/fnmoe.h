@@ -31,6 +31,8 @@
  *   fnmoe_dequantize         mx.dequantize affine Q4 (metal_runtime.py:751-758)
  *   fnmoe_swiglu             fused up-SwiGLU bfloat16 epilogue (metal_runtime.py:262-285)
  *   fnmoe_paged_decode       paged_attention decode (models/qwen27b/paged_kv.py:417-495)
+ *   fnmoe_page_plan, fnmoe_kv_append_q8, fnmoe_paged_attention_q8
+ *       PagedKVCache bookkeeping, append and attention (paged_kv.py:54-495) on an 8-bit cache
  *   fnmoe_tile_experts       no direct counterpart: the B200 analogue of packing
  *       expert records once for fast reads (models/flashnext/slab_pack.py:96-153),
  *       into a tile-major HBM layout the decode kernels stream with bulk copies
@@ -267,6 +269,125 @@ typedef struct FnPagedArgs {
   uint64_t workspace_bytes;
 } FnPagedArgs;
 
+/* ---- Paged 8-bit KV cache ----
+ * Keys and values as codes of 8 bits in pages [num_pages, page_size, kv_heads,
+ * head_dim], with one float32 scale for each `block` consecutive tokens of a
+ * page and each kv head ([num_pages, page_size / block, kv_heads]); a stored
+ * value is code * scale.  Slot s of the cache is token s % page_size of page
+ * s / page_size.  The reference holds its paged cache in the model's type
+ * (models/qwen27b/paged_kv.py:54-400) or in Q4 (models/bonsai2/
+ * q4_attention_kernel.py:141-258); 8 bits with a scale per block is this
+ * library's own form. */
+#define FNMOE_Q8_INT8 0u /* int8 codes in [-127, 127], scale = |x|max / 127     */
+#define FNMOE_Q8_E4M3 1u /* float8 e4m3 codes (finite), scale = |x|max / 448    */
+
+typedef struct FnQ8Cache {
+  void *k_codes;               /* [num_pages, page_size, kv_heads, head_dim], 16-byte aligned */
+  void *v_codes;
+  float *k_scale;              /* [num_pages, page_size / block, kv_heads] */
+  float *v_scale;
+  uint32_t num_pages;
+  uint32_t page_size;          /* tokens per page, a multiple of block */
+  uint32_t block;              /* tokens that share a scale: 16, 32, 64 or 128 */
+  uint32_t kv_heads;
+  uint32_t head_dim;           /* 64, 128 or 256 */
+  uint32_t code_type;          /* FNMOE_Q8_* */
+} FnQ8Cache;
+
+/* One serving step's block tables, slot map and free pages from the requests'
+ * lengths (fnmoe_page_plan); no host read.  Per sequence b, in order:
+ *   held   = release[b] ? 0 : seq_lens[b];   n = new_lens[b]
+ *   need   = pages(held + n) - pages(held)
+ * A sequence is admitted when held + n fits its table row, its pages are among
+ * the free ones (need == 0, or the inclusive sum of `need` over the sequences
+ * that fit their rows is at most the free count) and its tokens are among
+ * max_tokens (n == 0, or the inclusive sum of n over those is).  One that is
+ * not gets neither pages nor slots and keeps its length; the caller sees
+ * admitted[b] == 0.  Pages come from the head of the free ring in order;
+ * pages of released rows join its end (in order of sequence and column) and
+ * can be given from the next call on.  Unused table cells hold -1. */
+typedef struct FnPagePlanArgs {
+  uint32_t abi_version;
+  uint32_t batch;              /* sequences (table rows), at most 8192 */
+  uint32_t page_size;
+  uint32_t max_pages;          /* block_table row length */
+  uint32_t num_pages;          /* length of the free ring */
+  uint32_t max_tokens;         /* length of slot_map, token_seq and positions */
+  const int32_t *seq_lens;     /* [batch] tokens held; negative counts as 0 */
+  const int32_t *new_lens;     /* [batch] tokens to add; negative counts as 0 */
+  const int32_t *release;      /* [batch] nonzero: the row's request has ended; or NULL */
+  const int32_t *block_table;  /* [batch, max_pages] */
+  int32_t *free_pages;         /* [num_pages] ring of free pages, updated in place */
+  const int32_t *free_state;   /* [2]: head of the ring, free pages */
+  int32_t *block_table_out;    /* [batch, max_pages]; may be block_table */
+  int32_t *seq_lens_out;       /* [batch]; not seq_lens */
+  int32_t *free_state_out;     /* [2]; not free_state */
+  int64_t *slot_map;           /* [max_tokens] slot of each packed new token, -1 past the last */
+  int32_t *token_seq;          /* [max_tokens] its sequence, or -1 */
+  int32_t *positions;          /* [max_tokens] its position, or -1 */
+  int32_t *cu_new;             /* [batch + 1] first packed token of each sequence */
+  int32_t *admitted;           /* [batch] 1 or 0 */
+} FnPagePlanArgs;
+
+/* Quantise K/V rows into their slots (fnmoe_kv_append_q8).  For each block
+ * that gets rows and each kv head, with `first` the least slot of the block
+ * written by this call:
+ *   scale = max(first is the block's first slot ? 0 : its scale,
+ *               max(|x|max of the rows, 2^-100) / top)
+ * the codes before `first` become round(code * (old scale / scale)), the rows'
+ * codes round(x * (1 / scale)), ties to even, clamped to +-top (top = 127 or
+ * 448; the e4m3 rounding is to e4m3).  |x|max leaves out infinities and NaN;
+ * infinities are stored as +-top, NaN as 0.  The rows of one block are
+ * adjacent in the map with ascending consecutive slots, as fnmoe_page_plan
+ * writes them, and no two runs share a block.  Rows whose slot lies outside
+ * the cache are skipped. */
+typedef struct FnQ8AppendArgs {
+  uint32_t abi_version;
+  uint32_t tokens;             /* 0 is a no-op */
+  FnQ8Cache cache;
+  const void *k;               /* [tokens, kv_heads, head_dim] bf16, heads contiguous, 16-byte aligned */
+  const void *v;
+  uint64_t k_stride;           /* elements from one token to the next, a multiple of 8 */
+  uint64_t v_stride;
+  const int64_t *slot_map;     /* [tokens] */
+} FnQ8AppendArgs;
+
+/* The values that slots hold, bf16(code * scale) (fnmoe_kv_read_q8); a slot
+ * outside the cache reads as zeros. */
+typedef struct FnQ8ReadArgs {
+  uint32_t abi_version;
+  uint32_t count;              /* 0 is a no-op */
+  FnQ8Cache cache;
+  const int64_t *slots;        /* [count] */
+  void *k_out;                 /* [count, kv_heads, head_dim] bf16, 16-byte aligned */
+  void *v_out;
+} FnQ8ReadArgs;
+
+/* Causal attention of packed query rows over the cache
+ * (fnmoe_paged_attention_q8).  Sequence b's n = cu_q[b+1] - cu_q[b] rows are
+ * its last n tokens: row i is at position context_lens[b] - n + i and sees the
+ * positions up to its own (cu_q NULL: one row per sequence, seeing the whole
+ * context).  Positions whose page is outside the cache or past the table row
+ * are not seen.  A row that sees nothing is 0.  Softmax statistics and sums
+ * are float32; rows of q outside cu_q are not written. */
+typedef struct FnQ8AttentionArgs {
+  uint32_t abi_version;
+  uint32_t batch;
+  uint32_t q_rows;             /* rows of q and out (batch when cu_q is NULL); 0 is a no-op */
+  uint32_t q_heads;            /* multiple of kv_heads, at most 32 per kv head */
+  uint32_t max_pages;
+  float scale;                 /* finite, > 0 */
+  FnQ8Cache cache;
+  const void *q;               /* [q_rows, q_heads, head_dim] bf16, heads contiguous, 16-byte aligned */
+  uint64_t q_stride;           /* elements from one row to the next, a multiple of 8 */
+  const int32_t *block_table;  /* [batch, max_pages] */
+  const int32_t *context_lens; /* [batch] */
+  const int32_t *cu_q;         /* [batch + 1] ascending from 0, at most q_rows; or NULL */
+  void *out;                   /* [q_rows, q_heads, head_dim] bf16, 16-byte aligned */
+  void *workspace;
+  uint64_t workspace_bytes;
+} FnQ8AttentionArgs;
+
 /* Quantized embedding / n-gram row lookup (fnmoe_rows_dequantize).  The
  * table -- every shard of a sharded table, concatenated in shard order -- is
  * resident on the device: weight [table_rows][dims * bits / 32] uint32 (value
@@ -422,6 +543,17 @@ FNMOE_API int fnmoe_swiglu(const void *gate, const void *up, void *out, uint64_t
 
 FNMOE_API int fnmoe_paged_decode_workspace_size(const FnPagedArgs *args, uint64_t *bytes);
 FNMOE_API int fnmoe_paged_decode(const FnPagedArgs *args, void *stream);
+
+/* The paged 8-bit KV cache (see FnQ8Cache): plan a step's pages and slots,
+ * quantise its K/V rows into them, attend over the cache, read values back.
+ * The plan replaces the host-side page bookkeeping of PagedKVCache
+ * (paged_kv.py:54-400); the attention is paged_attention's computation
+ * (paged_kv.py:417-495) on 8-bit pages, for one or many query rows. */
+FNMOE_API int fnmoe_page_plan(const FnPagePlanArgs *args, void *stream);
+FNMOE_API int fnmoe_kv_append_q8(const FnQ8AppendArgs *args, void *stream);
+FNMOE_API int fnmoe_kv_read_q8(const FnQ8ReadArgs *args, void *stream);
+FNMOE_API int fnmoe_paged_attention_q8_workspace_size(const FnQ8AttentionArgs *args, uint64_t *bytes);
+FNMOE_API int fnmoe_paged_attention_q8(const FnQ8AttentionArgs *args, void *stream);
 
 /* Gather and dequantise table rows (see FnRowsArgs) on `stream`.  Replaces
  * StreamingQuantizedEmbedding.__call__ (ngram.py:62-69, rows read by

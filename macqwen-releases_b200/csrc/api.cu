@@ -17,6 +17,7 @@
 
 #include "../../include/fnmoe.h"
 #include "attention.cuh"
+#include "paged_q8.cuh"
 #include "rows.cuh"
 #include "common.cuh"
 #include "moe_kernels.cuh"
@@ -1061,6 +1062,26 @@ int fnmoe_paged_decode_workspace_size(const FnPagedArgs *args, uint64_t *bytes) 
 
 int fnmoe_paged_decode(const FnPagedArgs *args, void *stream) {
   return paged_decode(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_page_plan(const FnPagePlanArgs *args, void *stream) {
+  return page_plan(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_kv_append_q8(const FnQ8AppendArgs *args, void *stream) {
+  return kv_append_q8(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_kv_read_q8(const FnQ8ReadArgs *args, void *stream) {
+  return kv_read_q8(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_paged_attention_q8_workspace_size(const FnQ8AttentionArgs *args, uint64_t *bytes) {
+  return paged_attention_q8_workspace_size(args, bytes, g_last_error);
+}
+
+int fnmoe_paged_attention_q8(const FnQ8AttentionArgs *args, void *stream) {
+  return paged_attention_q8(args, static_cast<cudaStream_t>(stream), g_last_error);
 }
 
 int fnmoe_rows_dequantize(const FnRowsArgs *args, void *stream) {

@@ -132,6 +132,52 @@ class FnPagedArgs(ctypes.Structure):
     ]
 
 
+Q8_INT8 = 0
+Q8_E4M3 = 1
+
+
+class FnQ8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", _vp), ("v_codes", _vp), ("k_scale", _vp), ("v_scale", _vp),
+        ("num_pages", _u32), ("page_size", _u32), ("block", _u32), ("kv_heads", _u32),
+        ("head_dim", _u32), ("code_type", _u32),
+    ]
+
+
+class FnPagePlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("batch", _u32), ("page_size", _u32), ("max_pages", _u32),
+        ("num_pages", _u32), ("max_tokens", _u32),
+        ("seq_lens", _vp), ("new_lens", _vp), ("release", _vp), ("block_table", _vp),
+        ("free_pages", _vp), ("free_state", _vp),
+        ("block_table_out", _vp), ("seq_lens_out", _vp), ("free_state_out", _vp),
+        ("slot_map", _vp), ("token_seq", _vp), ("positions", _vp), ("cu_new", _vp), ("admitted", _vp),
+    ]
+
+
+class FnQ8AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("tokens", _u32), ("cache", FnQ8Cache),
+        ("k", _vp), ("v", _vp), ("k_stride", _u64), ("v_stride", _u64), ("slot_map", _vp),
+    ]
+
+
+class FnQ8ReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("count", _u32), ("cache", FnQ8Cache),
+        ("slots", _vp), ("k_out", _vp), ("v_out", _vp),
+    ]
+
+
+class FnQ8AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("batch", _u32), ("q_rows", _u32), ("q_heads", _u32), ("max_pages", _u32),
+        ("scale", ctypes.c_float), ("cache", FnQ8Cache),
+        ("q", _vp), ("q_stride", _u64), ("block_table", _vp), ("context_lens", _vp), ("cu_q", _vp),
+        ("out", _vp), ("workspace", _vp), ("workspace_bytes", _u64),
+    ]
+
+
 class FnRowsArgs(ctypes.Structure):
     _fields_ = [
         ("abi_version", _u32), ("dims", _u32), ("bits", _u32), ("group_size", _u32),
@@ -184,6 +230,12 @@ SIGNATURES = {
     "fnmoe_swiglu": ([_vp, _vp, _vp, _u64, _vp], ctypes.c_int),
     "fnmoe_paged_decode_workspace_size": ([ctypes.POINTER(FnPagedArgs), ctypes.POINTER(_u64)], ctypes.c_int),
     "fnmoe_paged_decode": ([ctypes.POINTER(FnPagedArgs), _vp], ctypes.c_int),
+    "fnmoe_page_plan": ([ctypes.POINTER(FnPagePlanArgs), _vp], ctypes.c_int),
+    "fnmoe_kv_append_q8": ([ctypes.POINTER(FnQ8AppendArgs), _vp], ctypes.c_int),
+    "fnmoe_kv_read_q8": ([ctypes.POINTER(FnQ8ReadArgs), _vp], ctypes.c_int),
+    "fnmoe_paged_attention_q8_workspace_size": ([ctypes.POINTER(FnQ8AttentionArgs), ctypes.POINTER(_u64)],
+                                                ctypes.c_int),
+    "fnmoe_paged_attention_q8": ([ctypes.POINTER(FnQ8AttentionArgs), _vp], ctypes.c_int),
     "fnmoe_rows_dequantize": ([ctypes.POINTER(FnRowsArgs), _vp], ctypes.c_int),
     "fnmoe_read_device_errors": ([ctypes.POINTER(_u32), ctypes.c_int], ctypes.c_int),
     "fnmoe_profile_enable": ([ctypes.c_int], ctypes.c_int),

@@ -1,0 +1,236 @@
+"""Paged KV cache in 8 bits: page planning, quantising append, attention.
+
+Keys and values are codes of 8 bits (int8, or float8 e4m3) in HBM pages
+``[pages, page_size, kv_heads, head_dim]`` with one float32 scale for each
+``block`` consecutive tokens of a page and each kv head; a stored value is
+``code * scale``.  Half the bytes of the bfloat16 cache of
+:mod:`~flashnext_b200.paged_attention`, so about twice the contexts in a GPU's
+memory and half the time of a decode step, which reads the cache once.
+
+* :func:`page_plan` builds a serving step's block tables and slot map on the
+  device from the requests' lengths (the bookkeeping of ``PagedKVCache``,
+  ``models/qwen27b/paged_kv.py:54-400``, without a host read);
+* :func:`kv_append_q8` quantises the step's K/V rows into their slots;
+* :func:`paged_attention_q8` is ``paged_attention``'s computation
+  (``paged_kv.py:417-495``) over such a cache, causal, for one query row per
+  sequence or packed rows (multi-token verify, prefill chunks);
+* :func:`kv_read_q8` takes values out as bfloat16;
+* :class:`PagedKVCacheQ8` keeps the buffers and runs the four together.
+
+Every call is ordered on torch's current stream and reads nothing on the
+host, so a step can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Any
+
+from . import _lib
+from .cuda_runtime import _torch
+
+BLOCKS = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128, 256)
+_CODES: dict[Any, int] = {}  # torch dtype -> FNMOE_Q8_*, filled at the first use
+_workspaces: dict[tuple[int, int], Any] = {}  # (device, stream) -> scratch, so that streams do not share one
+
+
+@dataclass
+class PagePlan:
+    """A serving step's pages and slots (:func:`page_plan`)."""
+
+    block_table: Any  # [batch, max_pages] int32, -1 in unused cells
+    seq_lens: Any     # [batch] int32, the admitted tokens included
+    free_pages: Any   # [pages] int32 ring of free pages
+    free_state: Any   # [2] int32: head of the ring, free pages
+    slot_map: Any     # [max_tokens] int64 slot of each packed new token, -1 past the last
+    token_seq: Any    # [max_tokens] int32 its sequence, or -1
+    positions: Any    # [max_tokens] int32 its position, or -1
+    cu_new: Any       # [batch + 1] int32 first packed token of each sequence
+    admitted: Any     # [batch] int32: 0 where pages, tokens or table columns ran out
+
+
+def _want(t, dtype, shape, what):
+    """A contiguous CUDA tensor of this type and shape (None: any extent)."""
+    if t.dtype != dtype or not t.is_cuda:
+        raise TypeError(f"{what} must be a {dtype} CUDA tensor")
+    have = t.shape
+    if len(have) != len(shape) or any(w is not None and w != h for w, h in zip(shape, have)):
+        raise ValueError(f"{what} has shape {tuple(have)}, not {tuple('any' if w is None else w for w in shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _rows(t, heads, dim, what):
+    """Pointer and token stride of bfloat16 rows [n, heads, dim]; a row is contiguous, rows may be apart."""
+    torch = _torch()
+    if t.dtype != torch.bfloat16 or not t.is_cuda:
+        raise TypeError(f"{what} must be a bfloat16 CUDA tensor")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
+        raise ValueError(f"{what} must be [tokens, {heads}, {dim}], not {tuple(t.shape)}")
+    n, (s0, s1, s2) = t.shape[0], t.stride()
+    if n == 0:
+        return t.data_ptr(), heads * dim
+    if (s2 != 1 and dim > 1) or (s1 != dim and heads > 1):
+        raise ValueError(f"{what}'s heads must be contiguous within a token")
+    return t.data_ptr(), s0 if n > 1 else heads * dim
+
+
+def _cache(k_cache, v_cache, k_scale, v_scale):
+    torch = _torch()
+    if not _CODES:
+        _CODES.update({torch.int8: _lib.Q8_INT8, torch.float8_e4m3fn: _lib.Q8_E4M3})
+    dtype = k_cache.dtype
+    code = _CODES.get(dtype)
+    if code is None:
+        raise TypeError("k_cache must be an int8 or float8_e4m3fn tensor")
+    if k_cache.dim() != 4 or k_scale.dim() != 3:
+        raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] and scales [pages, page_size / block, kv_heads]")
+    shape = pages, page, heads, dim = k_cache.shape
+    blocks = k_scale.shape[1]
+    if blocks == 0 or page % blocks:
+        raise ValueError("a page must hold a whole number of scale blocks")
+    ss = (pages, blocks, heads)
+    f32 = torch.float32
+    return _lib.FnQ8Cache(_want(k_cache, dtype, shape, "k_cache"), _want(v_cache, dtype, shape, "v_cache"),
+                          _want(k_scale, f32, ss, "k_scale"), _want(v_scale, f32, ss, "v_scale"),
+                          pages, page, page // blocks, heads, dim, code)
+
+
+def _stream_of(t):
+    """Current stream of torch's current device, which must be ``t``'s."""
+    torch = _torch()
+    s = torch.cuda.current_stream()
+    if t.device != s.device:
+        raise ValueError(f"tensors are on {t.device}, the current device is {s.device}")
+    return s.cuda_stream
+
+
+def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size: int, max_tokens: int,
+              release=None, out: PagePlan | None = None) -> PagePlan:
+    """Pages and slots for ``new_lens[b]`` more tokens of every sequence.
+
+    ``seq_lens`` / ``new_lens`` / ``release`` [batch], ``block_table``
+    [batch, max_pages], ``free_pages`` [pages] (a ring) and ``free_state`` [2]
+    (head, count) are int32.  A row with ``release`` set has ended: its pages
+    join the ring's end (to be given from the next call on) and the row
+    starts over with its ``new_lens``.  Sequences are served in order;
+    one whose pages or tokens do not fit has ``admitted`` 0 and keeps what it
+    had.  ``free_pages`` is updated in place; the rest is written to ``out``
+    (a plan of the same sizes, whose ``block_table`` may be the input) or to
+    new tensors.
+    """
+    torch = _torch()
+    lib = _lib.ensure_device()
+    i32, batch = torch.int32, seq_lens.shape[0]
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [batch, max_pages]")
+    width, max_tokens = block_table.shape[1], int(max_tokens)
+    if batch == 0 or width == 0 or max_tokens <= 0:
+        raise ValueError("page_plan needs sequences, table columns and max_tokens > 0")
+    one, cells = (batch,), (batch, width)
+    ins = (_want(seq_lens, i32, one, "seq_lens"), _want(new_lens, i32, one, "new_lens"),
+           None if release is None else _want(release, i32, one, "release"),
+           _want(block_table, i32, cells, "block_table"), _want(free_pages, i32, (None,), "free_pages"),
+           _want(free_state, i32, (2,), "free_state"))
+    if out is None:
+        dev = seq_lens.device
+        words = torch.empty(batch * (width + 3) + 1 + 2 + 2 * max_tokens, dtype=i32, device=dev)
+        t, lens, state, seq, pos, cu, ok = words.split((batch * width, batch, 2, max_tokens, max_tokens, batch + 1, batch))
+        out = PagePlan(t.view(cells), lens, free_pages, state, torch.empty(max_tokens, dtype=torch.int64, device=dev),
+                       seq, pos, cu, ok)
+    tok = (max_tokens,)
+    a = _lib.FnPagePlanArgs(
+        _lib.ABI_VERSION, batch, int(page_size), width, free_pages.shape[0], max_tokens, *ins,
+        _want(out.block_table, i32, cells, "out.block_table"), _want(out.seq_lens, i32, one, "out.seq_lens"),
+        _want(out.free_state, i32, (2,), "out.free_state"), _want(out.slot_map, torch.int64, tok, "out.slot_map"),
+        _want(out.token_seq, i32, tok, "out.token_seq"), _want(out.positions, i32, tok, "out.positions"),
+        _want(out.cu_new, i32, (batch + 1,), "out.cu_new"), _want(out.admitted, i32, one, "out.admitted"))
+    _lib.check(lib.fnmoe_page_plan(ctypes.byref(a), _stream_of(seq_lens)), "page_plan")
+    out.free_pages = free_pages
+    return out
+
+
+def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
+    """Quantise rows ``k``, ``v`` [tokens, kv_heads, head_dim] (bfloat16; rows
+    may be slices of a wider row) into the slots ``slot_map`` [tokens] int64.
+
+    A block's scale is the largest magnitude it holds over the code type's
+    largest value; a row that raises it has the block's earlier codes rounded
+    again to the new scale.  Rows of one block must be adjacent with
+    ascending slots, as :func:`page_plan` maps them; slots outside the cache
+    (-1) are skipped.  Infinities store the largest code, NaN stores 0.
+    """
+    lib = _lib.ensure_device()
+    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    kp, ks = _rows(k, c.kv_heads, c.head_dim, "k")
+    vp, vs = _rows(v, c.kv_heads, c.head_dim, "v")
+    tokens = k.shape[0]
+    if v.shape[0] != tokens:
+        raise ValueError("k and v must have the same number of rows")
+    a = _lib.FnQ8AppendArgs(_lib.ABI_VERSION, tokens, c, kp, vp, ks, vs,
+                            _want(slot_map, _torch().int64, (tokens,), "slot_map"))
+    _lib.check(lib.fnmoe_kv_append_q8(ctypes.byref(a), _stream_of(k)), "kv_append_q8")
+
+
+def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
+    """The values ``(k, v)`` that ``slots`` [n] int64 hold, bfloat16
+    [n, kv_heads, head_dim]; slots outside the cache (-1) read as zeros."""
+    torch = _torch()
+    lib = _lib.ensure_device()
+    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    n = slots.shape[0]
+    shape = (n, c.kv_heads, c.head_dim)
+    if out is None:
+        out = (torch.empty(shape, dtype=torch.bfloat16, device=slots.device),
+               torch.empty(shape, dtype=torch.bfloat16, device=slots.device))
+    a = _lib.FnQ8ReadArgs(_lib.ABI_VERSION, n, c, _want(slots, torch.int64, (n,), "slots"),
+                          _want(out[0], torch.bfloat16, shape, "out[0]"), _want(out[1], torch.bfloat16, shape, "out[1]"))
+    _lib.check(lib.fnmoe_kv_read_q8(ctypes.byref(a), _stream_of(slots)), "kv_read_q8")
+    return out
+
+
+def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, scale: float, cu_q=None,
+                       out=None, workspace=None):
+    """Causal attention of bfloat16 rows ``q`` [rows, q_heads, head_dim]
+    (rows may be slices of a wider row) over the cache; -> like ``q``.
+
+    With ``cu_q`` [batch + 1] int32, rows ``cu_q[b] .. cu_q[b + 1]`` are the
+    last tokens of sequence b's ``context_lens[b]``, each seeing the positions
+    up to its own; without it, row b sees all of sequence b's context.  A row
+    that sees nothing is 0.  ``workspace``: a uint8 tensor of
+    :func:`attention_workspace_bytes` bytes, or None for one kept per stream.
+    """
+    torch = _torch()
+    lib = _lib.ensure_device()
+    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 3:
+        raise ValueError("q must be [rows, q_heads, head_dim]")
+    rows, heads, dim = q.shape
+    if dim != c.head_dim:
+        raise ValueError("cache head_dim differs from q")
+    qp, qs = _rows(q, heads, dim, "q")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [batch, max_pages]")
+    batch, width = block_table.shape
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device=q.device)
+    i32 = torch.int32
+    a = _lib.FnQ8AttentionArgs(
+        _lib.ABI_VERSION, batch, rows, heads, width, float(scale), c, qp, qs,
+        _want(block_table, i32, (batch, width), "block_table"), _want(context_lens, i32, (batch,), "context_lens"),
+        None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q"),
+        _want(out, torch.bfloat16, (rows, heads, dim), "out"))
+    stream = _stream_of(q)
+    need = ctypes.c_uint64(0)
+    ref = ctypes.byref(a)
+    _lib.check(lib.fnmoe_paged_attention_q8_workspace_size(ref, ctypes.byref(need)), "paged attention q8 workspace")
+    if workspace is None:
+        key = (q.device.index, stream)
+        workspace = _workspaces.get(key)
+        if workspace is None or workspace.numel() < need.value:
+            workspace = _workspaces[key] = torch.empty(max(need.value, 256), dtype=torch.uint8, device=q.device)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _lib.check(lib.fnmoe_paged_attention_q8(ref, stream), "paged_attention_q8")
+    return out
