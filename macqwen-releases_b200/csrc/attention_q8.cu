@@ -4,15 +4,26 @@
 //   k_j = ks[block of j] * kcode_j,  v_j = vs[block of j] * vcode_j,
 //   j over the positions up to row i's own whose page is in the cache.
 //
-// Simplest form: one CTA per (row, query head); each warp takes every fourth
-// token, a lane D / 32 dims of it.
+// Codes go to the tensor cores as bfloat16, in which they are exact (int8 has
+// 7 bits and a sign, e4m3 4 bits), next to the queries as they are; the two
+// block scales enter in float32.  With
+//   t_j = (scale * log2 e * ks) (q . kcode_j) + log2 vs,   u_j = 2^(t_j - m),
+// m a running reference of the t_j,
+//   out = sum_j u_j vcode_j / sum_blocks (1 / vs) sum_(j in block) u_j :
+// the value scale rides in the exponent.  The weights enter the second product
+// as two bfloat16 terms, u = hi + lo with 16 bits: one term alone would cost
+// up to 2^-9 of an output (as much as its final rounding), and float16 loses
+// weights below 2^-24 of the largest, which are all that is left of an output
+// whose heaviest tokens hold zeros.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
+#include "async.cuh"
 #include "common.cuh"
 #include "moe_kernels.cuh"
 #include "paged_q8.cuh"
@@ -21,6 +32,9 @@ namespace fnmoe {
 
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.0f;  // a reference may fall this far (log2) below the largest t
+
 struct Q8View {
   const uint16_t *q;
   const uint8_t *kc, *vc;
@@ -28,84 +42,551 @@ struct Q8View {
   const int32_t *table, *ctx, *cu;
   uint16_t *out;
   uint64_t q_stride;
-  int B, rows, Hq, Hkv, gq, page, block, width, pages;
+  int B, rows, Hq, Hkv, gq, page, block_shift, width, pages;
   float scale;
+  // workspace
+  long long *prefix;  // [B + 1] units of work before each sequence
+  float *part;        // [2 * CTAs][8][D] unfinished sums
+  float2 *part_ml;    // [2 * CTAs][8] their reference and weight sum
 };
 
-template <bool E4M3>
-__device__ __forceinline__ float code_value(uint8_t c) {
-  if (!E4M3) return static_cast<float>(static_cast<int8_t>(c));
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(c)));
-  return __half2float(__ushort_as_half(static_cast<uint16_t>(h)));
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+  return d;
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// a and b as bfloat16 pairs hi + lo.
+__device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t &hi, uint32_t &lo) {
+  hi = pack_bf16x2(a, b);
+  lo = pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
+}
+__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two codes in bytes (0, 1) (HALF 0) or (2, 3) (HALF 1) of w, as bfloat16 pairs.
+// int8: under the high byte 0x43, the low seven bits l of a code read as
+// 128 + l and its sign bit alone as 128 (clear) or 256 (set); the difference
+// is l or l - 128, the code.
+// e4m3: to float16, to float32, to bfloat16, all exact.
+template <bool E4M3, int HALF>
+__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+  uint32_t d;
+  if (E4M3) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(HALF ? w >> 16 : w)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    d = pack_bf16x2(f.x, f.y);
+  } else {
+    const uint32_t x = prmt(w, 0x43434343u, HALF ? 0x4342u : 0x4140u);
+    asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
+  }
+  return d;
+}
+
+__device__ __forceinline__ uint4 ldg_stream(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Rows of sequence b: first packed row and their number.
+__device__ __forceinline__ int2 rows_of(const Q8View &p, int b) {
+  if (p.cu == nullptr) return make_int2(b, 1);
+  const int r0 = max(p.cu[b], 0), r1 = min(p.cu[b + 1], p.rows);
+  return make_int2(r0, max(r1 - r0, 0));
+}
+// Tokens of sequence b that the cache can hold.
+__device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
+  return max(0, min(p.ctx[b], p.width * p.page));
+}
+
+// ---- few rows per sequence --------------------------------------------------
+//
+// Bound by HBM (one byte a value, 2 * D * Hkv bytes a token).  Work is cut
+// into units of 64 tokens of one (sequence, kv head, tile of 8 rows); the
+// units of all sequences, laid end to end, are dealt to the CTAs in equal
+// contiguous ranges, so ragged contexts load every SM alike.  A CTA's range
+// covers whole segments, which it finishes, and at most two cut ones (its
+// first and last), whose sums go to the workspace for k_q8_join.
+//
+// A warp takes 16 tokens at a time straight from global memory into MMA
+// fragments (no shared memory, no barriers: at 23 bytes a clock and SM the
+// conversions and MMAs of eight warps keep up with HBM):
+//   S^T = K Q^T   (m16n8k16, M = 16 tokens, N = 8 rows): the order of the
+//     contraction is free, so lane (g, t) takes 16 consecutive dims of tokens
+//     g and g + 8, one 16-byte load for four k-steps;
+//   O^T += V^T P^T (M = 16 dims, N = 8 rows, K = 16 tokens): lane (g, t)
+//     loads 16 consecutive dims of tokens 2t, 2t+1, 2t+8, 2t+9 and pairs the
+//     tokens' bytes with prmt.
+// 16 tokens lie in one page and one scale block.  The next step's K is
+// requested when this one's K has been consumed, the next V likewise.
+
+constexpr int kUnit = 64;       // tokens of a unit: 4 warps x 16
+constexpr int kFewThreads = 128;
+
+template <int D>
+struct Few {
+  static constexpr int kCtas = D == 256 ? 2 : D == 128 ? 3 : 5;  // per SM
+  static constexpr int kMax = 148 * kCtas;
+};
+
+// Units of one (kv head, row tile) of sequence b, and its row tiles.
+__device__ __forceinline__ int2 units_of(const Q8View &p, int b) {
+  const int rows = rows_of(p, b).y * p.gq;
+  return make_int2((tokens_of(p, b) + kUnit - 1) / kUnit, (rows + 7) / 8);
+}
+
+// The sequence that holds unit `at` of all units, and its first unit; the
+// total.  CTA 0 leaves the sums for the join.  Every thread gets the result.
+struct Found {
+  int b;
+  long long before, total;
+};
+__device__ __forceinline__ long long seq_units(const Q8View &p, int b) {
+  const int2 u = units_of(p, b);
+  return static_cast<long long>(u.x) * u.y * p.Hkv;
+}
+
+template <int THREADS>
+__device__ Found find_unit(const Q8View &p, int cta, int ctas, long long &start, long long &end) {
+  __shared__ long long s_w[THREADS / 32];
+  __shared__ long long s_before;
+  __shared__ int s_b;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  long long total = 0;
+  for (int b = tid; b < p.B; b += THREADS) total += seq_units(p, b);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+  if (lane == 0) s_w[warp] = total;
+  if (tid == 0) {
+    s_b = p.B;
+    s_before = 0;
+  }
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) total += s_w[w];
+  // At most a CTA per unit, so that no range between two others is empty.
+  const int used = static_cast<int>(min(static_cast<long long>(ctas), max(total, 1ll)));
+  start = total * min(cta, used) / used;
+  end = total * min(cta + 1, used) / used;
+  long long carry = 0;
+  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+    const int b = b0 + tid;
+    const long long u = b < p.B ? seq_units(p, b) : 0;
+    long long v = u;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long o = __shfl_up_sync(0xFFFFFFFFu, v, off);
+      if (lane >= off) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) s_w[warp] = v;
+    __syncthreads();
+    long long before = carry;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += s_w[w];
+      carry += s_w[w];
+    }
+    before += v - u;
+    if (b < p.B && before <= start && start < before + u) {
+      s_b = b;
+      s_before = before;
+    }
+    if (cta == 0 && b < p.B) p.prefix[b] = before;
+    if (cta != 0 && carry > start) break;
+  }
+  if (cta == 0 && tid == 0) p.prefix[p.B] = total;
+  __syncthreads();
+  return Found{s_b, s_before, total};
 }
 
 template <int D, bool E4M3>
-__global__ void __launch_bounds__(128) k_q8_attention(Q8View p) {
-  constexpr int N = D / 32;
-  __shared__ float s_o[4][D], s_m[4], s_l[4];
-  const int r = blockIdx.x / p.Hq, head = blockIdx.x - r * p.Hq, h = head / p.gq;
+__global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p) {
+  constexpr int KC = D / 64;               // 16-byte pieces of a K row per lane
+  constexpr int VC = D == 64 ? 1 : D / 128;  // pieces of a V row per lane
+  constexpr int VW = D == 64 ? 2 : 4;      // words of a V piece
+  constexpr int MT = D / 16;               // 16-dim tiles of O^T
+  __shared__ __align__(16) float s_o[4][8][D];
+  __shared__ float s_m[4][8], s_l[4][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int b = r, last;
-  if (p.cu) {
-    int lo = 0, hi = p.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.cu[mid] <= r) lo = mid; else hi = mid;
+  const int g = lane >> 2, tq = lane & 3;
+  pdl_trigger();
+  long long cur, end;
+  const Found f = find_unit<kFewThreads>(p, blockIdx.x, gridDim.x, cur, end);
+  const long long first = cur;
+  int b = f.b;
+  long long off = cur - f.before;  // within the sequence
+
+  while (cur < end) {
+    int2 u = units_of(p, b);
+    while (off >= static_cast<long long>(u.x) * u.y * p.Hkv) {  // next sequence with work
+      off -= static_cast<long long>(u.x) * u.y * p.Hkv;
+      u = units_of(p, ++b);
     }
-    b = lo;
-    if (r < p.cu[b] || r >= p.cu[b + 1]) return;
-    last = p.ctx[b] - p.cu[b + 1] + r;
-  } else {
-    last = p.ctx[b] - 1;
+    const int seg = static_cast<int>(off / u.x);
+    const int u0 = static_cast<int>(off - static_cast<long long>(seg) * u.x);
+    const int n = static_cast<int>(min(static_cast<long long>(u.x - u0), end - cur));
+    const int h = seg / u.y, rt = seg - h * u.y;
+    const int2 qr = rows_of(p, b);
+    const int ctx = tokens_of(p, b);
+    const int rows = qr.y * p.gq;
+    const int lim0 = p.ctx[b] - qr.y;  // last position that row 0 sees
+
+    // ---- this tile's query rows as the B operand, and the last position each sees ----
+    uint32_t qf[MT][2];
+    int lim[2];
+    {
+      const int r = rt * 8 + g;
+      const bool live = r < rows;
+      const int qi = live ? r / p.gq : 0;
+      const int head = h * p.gq + (live ? r - qi * p.gq : 0);
+      const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D + 16 * tq;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        uint4 w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          w[e] = live ? *reinterpret_cast<const uint4 *>(src + 64 * i + 8 * e) : make_uint4(0, 0, 0, 0);
+        qf[4 * i][0] = w[0].x;
+        qf[4 * i][1] = w[0].y;
+        qf[4 * i + 1][0] = w[0].z;
+        qf[4 * i + 1][1] = w[0].w;
+        qf[4 * i + 2][0] = w[1].x;
+        qf[4 * i + 2][1] = w[1].y;
+        qf[4 * i + 3][0] = w[1].z;
+        qf[4 * i + 3][1] = w[1].w;
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int rr = rt * 8 + 2 * tq + hh;
+        lim[hh] = rr < rows ? lim0 + rr / p.gq : -1;
+      }
+    }
+
+    float o[MT][4];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    // ---- this warp's 16-token steps ----
+    const int t_end = min(ctx, (u0 + n) * kUnit);
+    int t = u0 * kUnit + 16 * warp;
+    int col = t / p.page, at = t - col * p.page;  // table column and offset in the page of step t
+    const int32_t *trow = p.table + static_cast<size_t>(b) * p.width;
+    const int bpp = p.page >> p.block_shift;
+    auto advance = [&](int &cc, int &aa) {
+      aa += kUnit;
+      while (aa >= p.page) {
+        aa -= p.page;
+        ++cc;
+      }
+    };
+    uint4 kf[KC][2];
+    uint4 vf[VC][4];
+    float ks, vs;
+    auto load_k = [&](int pg, int a) {
+      const size_t row = (static_cast<size_t>(pg) * p.page + a + g) * p.Hkv + h;
+      const uint8_t *r0 = p.kc + row * D + 16 * tq;
+      const uint8_t *r1 = r0 + static_cast<size_t>(8) * p.Hkv * D;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        kf[i][0] = ldg_stream(r0 + 64 * i);
+        kf[i][1] = ldg_stream(r1 + 64 * i);
+      }
+      ks = __ldg(p.ks + (static_cast<size_t>(pg) * bpp + (a >> p.block_shift)) * p.Hkv + h);
+    };
+    auto load_v = [&](int pg, int a) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const size_t row = (static_cast<size_t>(pg) * p.page + a + 2 * tq + (k & 1) + 8 * (k >> 1)) * p.Hkv + h;
+        const uint8_t *r = p.vc + row * D;
+        if (D == 64) {
+          const uint2 w = ldg_stream8(r + 8 * g);
+          vf[0][k] = make_uint4(w.x, w.y, 0, 0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VC; ++i) vf[i][k] = ldg_stream(r + 128 * i + 16 * g);
+        }
+      }
+      vs = __ldg(p.vs + (static_cast<size_t>(pg) * bpp + (a >> p.block_shift)) * p.Hkv + h);
+    };
+    // A page outside the cache: its tokens are masked and page 0 read instead.
+    auto page_at = [&](int cc) { return cc < p.width ? trow[cc] : -1; };
+    int pg = -1, pg_next = -1;
+    int col2 = col, at2 = at;  // the step after
+    if (t < t_end) {
+      pg = page_at(col);
+      advance(col2, at2);
+      if (t + kUnit < t_end) pg_next = page_at(col2);
+      const int safe = pg >= 0 && pg < p.pages ? pg : 0;
+      load_k(safe, at);
+      load_v(safe, at);
+    }
+    for (; t < t_end; t += kUnit) {
+      const bool ok = pg >= 0 && pg < p.pages;
+      const bool more = t + kUnit < t_end;
+      const int safe = pg_next >= 0 && pg_next < p.pages ? pg_next : 0;
+      const int at_now2 = at2;
+      int col3 = col2, at3 = at2, pg3 = -1;
+      advance(col3, at3);
+      if (t + 2 * kUnit < t_end) pg3 = page_at(col3);
+
+      // S^T = K Q^T, two chains
+      float sa[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const uint32_t w0[4] = {kf[i][0].x, kf[i][0].y, kf[i][0].z, kf[i][0].w};
+        const uint32_t w1[4] = {kf[i][1].x, kf[i][1].y, kf[i][1].z, kf[i][1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x0 = w0[j], x1 = w1[j];
+          const uint32_t a[4] = {widen2<E4M3, 0>(x0), widen2<E4M3, 0>(x1), widen2<E4M3, 1>(x0), widen2<E4M3, 1>(x1)};
+          mma_bf16(j & 1 ? sb : sa, a, qf[4 * i + j][0], qf[4 * i + j][1]);
+        }
+      }
+      const float k_scale = ks;
+      if (more) load_k(safe, at_now2);
+
+      // t_j, the running reference, the weights
+      const float v_scale = fmaxf(vs, 0x1p-110f);
+      const float lv = __log2f(v_scale), rv = __frcp_rn(v_scale);
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = t + g + 8 * (e >> 1), hh = e & 1;
+        const float s = __fadd_rn(sa[e], sb[e]);
+        x[e] = ok && tok <= lim[hh] ? __fmaf_rn(s, p.scale * kLog2e * k_scale, lv) : -INFINITY;
+      }
+      if (__any_sync(0xFFFFFFFFu, fmaxf(x[0], x[2]) > m[0] + kLazy || fmaxf(x[1], x[3]) > m[1] + kLazy)) {
+        float al[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          float cm = fmaxf(x[hh], x[hh + 2]);
+#pragma unroll
+          for (int s = 4; s <= 16; s <<= 1) cm = fmaxf(cm, __shfl_xor_sync(0xFFFFFFFFu, cm, s));
+          cm = fmaxf(cm, m[hh]);
+          al[hh] = cm == -INFINITY ? 1.0f : ex2(m[hh] - cm);
+          m[hh] = cm;
+          l[hh] *= al[hh];
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          o[j][0] *= al[0];
+          o[j][1] *= al[1];
+          o[j][2] *= al[0];
+          o[j][3] *= al[1];
+        }
+      }
+      const float r0 = m[0] == -INFINITY ? 0.0f : m[0], r1 = m[1] == -INFINITY ? 0.0f : m[1];
+      const float p0 = ex2(x[0] - r0), p1 = ex2(x[1] - r1), p2 = ex2(x[2] - r0), p3 = ex2(x[3] - r1);
+      l[0] = __fmaf_rn(p0 + p2, rv, l[0]);
+      l[1] = __fmaf_rn(p1 + p3, rv, l[1]);
+      uint32_t hi0, lo0, hi1, lo1;
+      split_bf16x2(p0, p1, hi0, lo0);
+      split_bf16x2(p2, p3, hi1, lo1);
+      hi0 = movm_t(hi0);
+      hi1 = movm_t(hi1);
+      lo0 = movm_t(lo0);
+      lo1 = movm_t(lo1);
+
+      // Slots past the context (or of a page outside the cache) may hold
+      // anything, NaN codes too: their value bytes are zeroed.
+      const int live = ok ? min(16, ctx - t) : 0;
+      if (live < 16) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (2 * tq + (k & 1) + 8 * (k >> 1) >= live) {
+#pragma unroll
+            for (int i = 0; i < VC; ++i) vf[i][k] = make_uint4(0u, 0u, 0u, 0u);
+          }
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        const uint32_t v0[4] = {vf[i][0].x, vf[i][0].y, vf[i][0].z, vf[i][0].w};
+        const uint32_t v1[4] = {vf[i][1].x, vf[i][1].y, vf[i][1].z, vf[i][1].w};
+        const uint32_t v2[4] = {vf[i][2].x, vf[i][2].y, vf[i][2].z, vf[i][2].w};
+        const uint32_t v3[4] = {vf[i][3].x, vf[i][3].y, vf[i][3].z, vf[i][3].w};
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t la = prmt(v0[w], v1[w], 0x5140u), ha = prmt(v0[w], v1[w], 0x7362u);
+          const uint32_t lb = prmt(v2[w], v3[w], 0x5140u), hb = prmt(v2[w], v3[w], 0x7362u);
+          const uint32_t a0[4] = {widen2<E4M3, 0>(la), widen2<E4M3, 1>(la), widen2<E4M3, 0>(lb), widen2<E4M3, 1>(lb)};
+          const uint32_t a1[4] = {widen2<E4M3, 0>(ha), widen2<E4M3, 1>(ha), widen2<E4M3, 0>(hb), widen2<E4M3, 1>(hb)};
+          mma_bf16(o[2 * VW * i + 2 * w], a0, hi0, hi1);
+          mma_bf16(o[2 * VW * i + 2 * w + 1], a1, hi0, hi1);
+          mma_bf16(o[2 * VW * i + 2 * w], a0, lo0, lo1);
+          mma_bf16(o[2 * VW * i + 2 * w + 1], a1, lo0, lo1);
+        }
+      }
+      if (more) load_v(safe, at_now2);
+      pg = pg_next;
+      pg_next = pg3;
+      col2 = col3;
+      at2 = at3;
+    }
+
+    // ---- join the four warps ----
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+      for (int s = 4; s <= 16; s <<= 1) l[hh] += __shfl_xor_sync(0xFFFFFFFFu, l[hh], s);
+      if (g == 0) {
+        s_m[warp][2 * tq + hh] = m[hh];
+        s_l[warp][2 * tq + hh] = l[hh];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int r = 2 * tq + hh;
+      const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+      const float fac = m[hh] == -INFINITY ? 0.0f : ex2(m[hh] - mm);
+#pragma unroll
+      for (int i = 0; i < VC; ++i)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const float *a = o[2 * VW * i + 2 * w], *bb = o[2 * VW * i + 2 * w + 1];
+          *reinterpret_cast<float4 *>(&s_o[warp][r][128 * i + 4 * VW * g + 4 * w]) =
+              make_float4(a[hh] * fac, a[2 + hh] * fac, bb[hh] * fac, bb[2 + hh] * fac);
+        }
+    }
+    __syncthreads();
+    const bool whole = u0 == 0 && n == u.x;
+    const int slot = 2 * blockIdx.x + (cur == first ? 0 : 1);
+    for (int i = threadIdx.x; i < 8 * D / 4; i += kFewThreads) {
+      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+      const int rr = rt * 8 + r;
+      if (rr >= rows) continue;
+      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, s_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 v = *reinterpret_cast<const float4 *>(&s_o[w][r][d]);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+        if (s_m[w][r] != -INFINITY) ll += s_l[w][r] * ex2(s_m[w][r] - mm);
+      }
+      if (whole) {
+        const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
+        const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
+        const uint32_t lo = static_cast<uint32_t>(f32_to_bf16(s.x * inv)) | (static_cast<uint32_t>(f32_to_bf16(s.y * inv)) << 16);
+        const uint32_t hi = static_cast<uint32_t>(f32_to_bf16(s.z * inv)) | (static_cast<uint32_t>(f32_to_bf16(s.w * inv)) << 16);
+        *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + d) = make_uint2(lo, hi);
+      } else {
+        *reinterpret_cast<float4 *>(p.part + (static_cast<size_t>(slot) * 8 + r) * D + d) = s;
+        if (d == 0) p.part_ml[slot * 8 + r] = make_float2(mm, ll);
+      }
+    }
+    __syncthreads();  // s_m, s_l and s_o are rewritten by the next piece
+    cur += n;
+    off += n;
   }
-  const int seen = min(last + 1, p.width * p.page);
-  float q[N], o[N], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = bf16_to_f32(p.q[static_cast<uint64_t>(r) * p.q_stride + static_cast<uint64_t>(head) * D + i * 32 + lane]) *
-           p.scale;
-    o[i] = 0.0f;
+}
+
+// The CTA whose range holds unit `unit` of `total`.
+__device__ __forceinline__ int owner_of(long long unit, long long total, int ctas) {
+  return static_cast<int>(((unit + 1) * ctas - 1) / total);
+}
+
+// One CTA per (sequence, kv head, tile, row): joins the cut segments' sums in
+// CTA order, and zeroes rows whose sequence has no token.
+template <int D>
+__global__ void __launch_bounds__(256) k_q8_join(Q8View p, int tiles, int ctas) {
+  constexpr int L = D / 4, G = 256 / L;  // lanes of a row, groups of partial sums
+  __shared__ float4 s_o[G][L];
+  __shared__ float s_l[G];
+  pdl_wait();
+  const int r = blockIdx.x & 7;
+  int seg = blockIdx.x >> 3;
+  const int rt = seg % tiles;
+  seg /= tiles;
+  const int h = seg % p.Hkv, b = seg / p.Hkv;
+  const int2 qr = rows_of(p, b);
+  const int rows = qr.y * p.gq, rr = rt * 8 + r;
+  if (rr >= rows) return;
+  const int2 u = units_of(p, b);
+  const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
+  uint16_t *dst = p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D;
+  const int lane = threadIdx.x % L, grp = threadIdx.x / L;
+  if (u.x == 0) {
+    if (grp == 0) *reinterpret_cast<uint2 *>(dst + 4 * lane) = make_uint2(0, 0);
+    return;
   }
-  for (int t = warp; t < seen; t += 4) {
-    const int c = t / p.page;
-    const int pg = p.table[static_cast<size_t>(b) * p.width + c];
-    if (pg < 0 || pg >= p.pages) continue;
-    const size_t slot = static_cast<size_t>(pg) * p.page + (t - c * p.page);
-    const size_t at = (slot * p.Hkv + h) * D + lane, sc = slot / p.block * p.Hkv + h;
-    float s = 0.0f;
+  const long long total = p.prefix[p.B];
+  ctas = static_cast<int>(min(static_cast<long long>(ctas), total));
+  const long long a = p.prefix[b] + static_cast<long long>(h * u.y + rt) * u.x;
+  const int c0 = owner_of(a, total, ctas), c1 = owner_of(a + u.x - 1, total, ctas);
+  if (c0 == c1) return;  // finished by its CTA
+  // CTA c0's piece is its first one only if its range begins with the segment.
+  auto slot_of = [&](int c) { return 2 * c + (c == c0 && total * c / ctas < a ? 1 : 0); };
+  float mm = -INFINITY;
+  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, p.part_ml[slot_of(c) * 8 + r].x);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += q[i] * code_value<E4M3>(p.kc[at + 32 * i]);
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, off);
-    s *= p.ks[sc];
-    const float mn = fmaxf(m, s), al = expf(m - mn), w = expf(s - mn);
-    m = mn;
-    l = l * al + w;
-    const float wv = w * p.vs[sc];
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * al + wv * code_value<E4M3>(p.vc[at + 32 * i]);
+  for (int s = 16; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, s));
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float ll = 0.0f;
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += G) {
+    const int slot = slot_of(c);
+    const float2 ml = p.part_ml[slot * 8 + r];
+    const float4 v = *reinterpret_cast<const float4 *>(p.part + (static_cast<size_t>(slot) * 8 + r) * D + 4 * lane);
+    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
+    ll += ml.y * w;
+    acc.x += v.x * w;
+    acc.y += v.y * w;
+    acc.z += v.z * w;
+    acc.w += v.w * w;
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) s_o[warp][32 * i + lane] = o[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
+  s_o[grp][lane] = acc;
+  if (lane == 0) s_l[grp] = ll;
   __syncthreads();
-  const float mm = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float w[4], L = 0.0f;
+  if (grp != 0) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = s_m[i] == -INFINITY ? 0.0f : expf(s_m[i] - mm);
-    L += w[i] * s_l[i];
+  for (int i = 1; i < G; ++i) {
+    const float4 v = s_o[i][lane];
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+    ll += s_l[i];
   }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v += w[i] * s_o[i][d];
-    p.out[(static_cast<size_t>(r) * p.Hq + head) * D + d] = f32_to_bf16(L > 0.0f ? v / L : 0.0f);
-  }
+  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
+  const uint32_t lo = static_cast<uint32_t>(f32_to_bf16(acc.x * inv)) | (static_cast<uint32_t>(f32_to_bf16(acc.y * inv)) << 16);
+  const uint32_t hi = static_cast<uint32_t>(f32_to_bf16(acc.z * inv)) | (static_cast<uint32_t>(f32_to_bf16(acc.w * inv)) << 16);
+  *reinterpret_cast<uint2 *>(dst + 4 * lane) = make_uint2(lo, hi);
 }
 
 int check(const FnQ8AttentionArgs *a, std::string &err) {
@@ -138,15 +619,35 @@ int check(const FnQ8AttentionArgs *a, std::string &err) {
   return FNMOE_OK;
 }
 
-constexpr uint64_t kWorkspaceBytes = 256;  // nothing kept there yet
+uint64_t align256(uint64_t n) { return (n + 255) & ~static_cast<uint64_t>(255); }
+
+// Workspace: prefix sums, then the cut segments' sums.
+struct Carve {
+  uint64_t ml, part, bytes;
+};
+Carve carve(const FnQ8AttentionArgs *a) {
+  const uint64_t d = a->cache.head_dim;
+  const uint64_t slots = 2ull * (d == 256 ? Few<256>::kMax : d == 128 ? Few<128>::kMax : Few<64>::kMax);
+  Carve c{};
+  c.ml = align256(8 * (static_cast<uint64_t>(a->batch) + 1));
+  c.part = c.ml + align256(slots * 8 * sizeof(float2));
+  c.bytes = c.part + slots * 8 * d * sizeof(float) + 256;  // the start is rounded up to 256 bytes
+  return c;
+}
+
+template <int D, bool E4M3>
+cudaError_t launch_few(const Q8View &p, cudaStream_t s) {
+  constexpr int ctas = Few<D>::kMax;
+  const uint64_t tiles = p.cu ? (static_cast<uint64_t>(p.rows) * p.gq + 7) / 8 : (p.gq + 7) / 8;
+  const uint64_t joins = static_cast<uint64_t>(p.B) * p.Hkv * tiles * 8;
+  if (joins > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+  k_q8_few<D, E4M3><<<ctas, kFewThreads, 0, s>>>(p);
+  return launch_pdl(k_q8_join<D>, dim3(static_cast<unsigned>(joins)), dim3(256), 0, s, p, static_cast<int>(tiles), ctas);
+}
 
 template <int D>
-void launch(const Q8View &p, bool e4m3, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(p.rows) * p.Hq;
-  if (e4m3)
-    k_q8_attention<D, true><<<grid, 128, 0, s>>>(p);
-  else
-    k_q8_attention<D, false><<<grid, 128, 0, s>>>(p);
+cudaError_t launch(const Q8View &p, bool e4m3, cudaStream_t s) {
+  return e4m3 ? launch_few<D, true>(p, s) : launch_few<D, false>(p, s);
 }
 
 }  // namespace
@@ -154,15 +655,16 @@ void launch(const Q8View &p, bool e4m3, cudaStream_t s) {
 int paged_attention_q8_workspace_size(const FnQ8AttentionArgs *a, uint64_t *bytes, std::string &err) {
   if (bytes == nullptr) { err = "bytes is NULL"; return FNMOE_ERR_NULL; }
   if (const int rc = check(a, err)) return rc;
-  *bytes = kWorkspaceBytes;
+  *bytes = carve(a).bytes;
   return FNMOE_OK;
 }
 
 int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &err) {
   if (const int rc = check(a, err)) return rc;
   if (a->q_rows == 0) return FNMOE_OK;
-  if (a->workspace == nullptr || a->workspace_bytes < kWorkspaceBytes) {
-    err = "workspace needs " + std::to_string(kWorkspaceBytes) + " bytes";
+  const Carve w = carve(a);
+  if (a->workspace == nullptr || a->workspace_bytes < w.bytes) {
+    err = "workspace needs " + std::to_string(w.bytes) + " bytes";
     return FNMOE_ERR_WORKSPACE;
   }
   const FnQ8Cache &c = a->cache;
@@ -183,17 +685,22 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
   p.Hkv = static_cast<int>(c.kv_heads);
   p.gq = p.Hq / p.Hkv;
   p.page = static_cast<int>(c.page_size);
-  p.block = static_cast<int>(c.block);
+  p.block_shift = 31 - __builtin_clz(c.block);
   p.width = static_cast<int>(a->max_pages);
   p.pages = static_cast<int>(c.num_pages);
   p.scale = a->scale;
+  uint8_t *ws = reinterpret_cast<uint8_t *>(align256(reinterpret_cast<uintptr_t>(a->workspace)));
+  p.prefix = reinterpret_cast<long long *>(ws);
+  p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
+  p.part = reinterpret_cast<float *>(ws + w.part);
   const bool e4m3 = c.code_type == FNMOE_Q8_E4M3;
+  cudaError_t e;
   switch (c.head_dim) {
-    case 64: launch<64>(p, e4m3, s); break;
-    case 128: launch<128>(p, e4m3, s); break;
-    default: launch<256>(p, e4m3, s); break;
+    case 64: e = launch<64>(p, e4m3, s); break;
+    case 128: e = launch<128>(p, e4m3, s); break;
+    default: e = launch<256>(p, e4m3, s); break;
   }
-  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     err = std::string("paged attention q8: ") + cudaGetErrorString(e);
     return FNMOE_ERR_LAUNCH;
