@@ -320,6 +320,15 @@ def ensure_device() -> ctypes.CDLL:
     return lib
 
 
+def ensure_device_of(index: int) -> ctypes.CDLL:
+    """:func:`ensure_device` for a tensor of CUDA device ``index``, which must be the current one."""
+    import torch
+
+    if torch.cuda.current_device() != index:
+        raise ValueError(f"tensors are on device {index}, the current device is {torch.cuda.current_device()}")
+    return _handle if _available.get(index) else ensure_device()
+
+
 def read_device_errors(clear: bool = True) -> int:
     lib = ensure_device()
     flags = _u32(0)

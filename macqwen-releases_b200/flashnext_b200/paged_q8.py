@@ -26,16 +26,17 @@ import ctypes
 from dataclasses import dataclass
 from typing import Any
 
+import torch
+
 from . import _lib
-from .cuda_runtime import _torch
 
 BLOCKS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
-_CODES: dict[Any, int] = {}  # torch dtype -> FNMOE_Q8_*, filled at the first use
+_CODES = {torch.int8: _lib.Q8_INT8, torch.float8_e4m3fn: _lib.Q8_E4M3}
 _workspaces: dict[tuple[int, int], Any] = {}  # (device, stream) -> scratch, so that streams do not share one
 
 
-@dataclass
+@dataclass(slots=True)
 class PagePlan:
     """A serving step's pages and slots (:func:`page_plan`)."""
 
@@ -50,61 +51,59 @@ class PagePlan:
     admitted: Any     # [batch] int32: 0 where pages, tokens or table columns ran out
 
 
-def _want(t, dtype, shape, what):
-    """A contiguous CUDA tensor of this type and shape (None: any extent)."""
+def _refuse(t, dtype, shape, what):
     if t.dtype != dtype or not t.is_cuda:
         raise TypeError(f"{what} must be a {dtype} CUDA tensor")
-    have = t.shape
-    if len(have) != len(shape) or any(w is not None and w != h for w, h in zip(shape, have)):
-        raise ValueError(f"{what} has shape {tuple(have)}, not {tuple('any' if w is None else w for w in shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    return t.data_ptr()
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    raise ValueError(f"{what} must be contiguous")
+
+
+def _want(t, dtype, shape, what):
+    """Pointer of a contiguous CUDA tensor of this type and shape."""
+    if t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(t, dtype, shape, what)
 
 
 def _rows(t, heads, dim, what):
     """Pointer and token stride of bfloat16 rows [n, heads, dim]; a row is contiguous, rows may be apart."""
-    torch = _torch()
-    if t.dtype != torch.bfloat16 or not t.is_cuda:
+    if t.dtype is not torch.bfloat16 or not t.is_cuda:
         raise TypeError(f"{what} must be a bfloat16 CUDA tensor")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{what} must be [tokens, {heads}, {dim}], not {tuple(t.shape)}")
-    n, (s0, s1, s2) = t.shape[0], t.stride()
-    if n == 0:
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{what} must be [tokens, {heads}, {dim}], not {tuple(shape)}")
+    if shape[0] < 2 and t.is_contiguous():
         return t.data_ptr(), heads * dim
+    s0, s1, s2 = t.stride()
     if (s2 != 1 and dim > 1) or (s1 != dim and heads > 1):
         raise ValueError(f"{what}'s heads must be contiguous within a token")
-    return t.data_ptr(), s0 if n > 1 else heads * dim
+    return t.data_ptr(), s0 if shape[0] > 1 else heads * dim
 
 
 def _cache(k_cache, v_cache, k_scale, v_scale):
-    torch = _torch()
-    if not _CODES:
-        _CODES.update({torch.int8: _lib.Q8_INT8, torch.float8_e4m3fn: _lib.Q8_E4M3})
     dtype = k_cache.dtype
     code = _CODES.get(dtype)
     if code is None:
         raise TypeError("k_cache must be an int8 or float8_e4m3fn tensor")
-    if k_cache.dim() != 4 or k_scale.dim() != 3:
-        raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] and scales [pages, page_size / block, kv_heads]")
-    shape = pages, page, heads, dim = k_cache.shape
-    blocks = k_scale.shape[1]
+    shape, scales = k_cache.shape, k_scale.shape
+    if len(shape) != 4 or len(scales) != 3:
+        raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] and scales "
+                         "[pages, page_size / block, kv_heads]")
+    pages, page, heads, dim = shape
+    blocks = scales[1]
     if blocks == 0 or page % blocks:
         raise ValueError("a page must hold a whole number of scale blocks")
-    ss = (pages, blocks, heads)
-    f32 = torch.float32
+    ss, f32 = (pages, blocks, heads), torch.float32
     return _lib.FnQ8Cache(_want(k_cache, dtype, shape, "k_cache"), _want(v_cache, dtype, shape, "v_cache"),
                           _want(k_scale, f32, ss, "k_scale"), _want(v_scale, f32, ss, "v_scale"),
                           pages, page, page // blocks, heads, dim, code)
 
 
-def _stream_of(t):
-    """Current stream of torch's current device, which must be ``t``'s."""
-    torch = _torch()
-    s = torch.cuda.current_stream()
-    if t.device != s.device:
-        raise ValueError(f"tensors are on {t.device}, the current device is {s.device}")
-    return s.cuda_stream
+def _ready(t):
+    """The library and the current stream of the current device, which must be ``t``'s."""
+    lib = _lib.ensure_device_of(t.get_device())
+    return lib, torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size: int, max_tokens: int,
@@ -121,19 +120,17 @@ def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size
     (a plan of the same sizes, whose ``block_table`` may be the input) or to
     new tensors.
     """
-    torch = _torch()
-    lib = _lib.ensure_device()
     i32, batch = torch.int32, seq_lens.shape[0]
     if block_table.dim() != 2:
         raise ValueError("block_table must be [batch, max_pages]")
     width, max_tokens = block_table.shape[1], int(max_tokens)
     if batch == 0 or width == 0 or max_tokens <= 0:
         raise ValueError("page_plan needs sequences, table columns and max_tokens > 0")
-    one, cells = (batch,), (batch, width)
+    one, cells, two = (batch,), (batch, width), (2,)
     ins = (_want(seq_lens, i32, one, "seq_lens"), _want(new_lens, i32, one, "new_lens"),
            None if release is None else _want(release, i32, one, "release"),
-           _want(block_table, i32, cells, "block_table"), _want(free_pages, i32, (None,), "free_pages"),
-           _want(free_state, i32, (2,), "free_state"))
+           _want(block_table, i32, cells, "block_table"), _want(free_pages, i32, (free_pages.numel(),), "free_pages"),
+           _want(free_state, i32, two, "free_state"))
     if out is None:
         dev = seq_lens.device
         words = torch.empty(batch * (width + 3) + 1 + 2 + 2 * max_tokens, dtype=i32, device=dev)
@@ -144,10 +141,11 @@ def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size
     a = _lib.FnPagePlanArgs(
         _lib.ABI_VERSION, batch, int(page_size), width, free_pages.shape[0], max_tokens, *ins,
         _want(out.block_table, i32, cells, "out.block_table"), _want(out.seq_lens, i32, one, "out.seq_lens"),
-        _want(out.free_state, i32, (2,), "out.free_state"), _want(out.slot_map, torch.int64, tok, "out.slot_map"),
+        _want(out.free_state, i32, two, "out.free_state"), _want(out.slot_map, torch.int64, tok, "out.slot_map"),
         _want(out.token_seq, i32, tok, "out.token_seq"), _want(out.positions, i32, tok, "out.positions"),
         _want(out.cu_new, i32, (batch + 1,), "out.cu_new"), _want(out.admitted, i32, one, "out.admitted"))
-    _lib.check(lib.fnmoe_page_plan(ctypes.byref(a), _stream_of(seq_lens)), "page_plan")
+    lib, stream = _ready(seq_lens)
+    _lib.check(lib.fnmoe_page_plan(ctypes.byref(a), stream), "page_plan")
     out.free_pages = free_pages
     return out
 
@@ -162,7 +160,6 @@ def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
     ascending slots, as :func:`page_plan` maps them; slots outside the cache
     (-1) are skipped.  Infinities store the largest code, NaN stores 0.
     """
-    lib = _lib.ensure_device()
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     kp, ks = _rows(k, c.kv_heads, c.head_dim, "k")
     vp, vs = _rows(v, c.kv_heads, c.head_dim, "v")
@@ -170,15 +167,14 @@ def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
     if v.shape[0] != tokens:
         raise ValueError("k and v must have the same number of rows")
     a = _lib.FnQ8AppendArgs(_lib.ABI_VERSION, tokens, c, kp, vp, ks, vs,
-                            _want(slot_map, _torch().int64, (tokens,), "slot_map"))
-    _lib.check(lib.fnmoe_kv_append_q8(ctypes.byref(a), _stream_of(k)), "kv_append_q8")
+                            _want(slot_map, torch.int64, (tokens,), "slot_map"))
+    lib, stream = _ready(k)
+    _lib.check(lib.fnmoe_kv_append_q8(ctypes.byref(a), stream), "kv_append_q8")
 
 
 def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
     """The values ``(k, v)`` that ``slots`` [n] int64 hold, bfloat16
     [n, kv_heads, head_dim]; slots outside the cache (-1) read as zeros."""
-    torch = _torch()
-    lib = _lib.ensure_device()
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     n = slots.shape[0]
     shape = (n, c.kv_heads, c.head_dim)
@@ -187,7 +183,8 @@ def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
                torch.empty(shape, dtype=torch.bfloat16, device=slots.device))
     a = _lib.FnQ8ReadArgs(_lib.ABI_VERSION, n, c, _want(slots, torch.int64, (n,), "slots"),
                           _want(out[0], torch.bfloat16, shape, "out[0]"), _want(out[1], torch.bfloat16, shape, "out[1]"))
-    _lib.check(lib.fnmoe_kv_read_q8(ctypes.byref(a), _stream_of(slots)), "kv_read_q8")
+    lib, stream = _ready(slots)
+    _lib.check(lib.fnmoe_kv_read_q8(ctypes.byref(a), stream), "kv_read_q8")
     return out
 
 
@@ -199,11 +196,10 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
     With ``cu_q`` [batch + 1] int32, rows ``cu_q[b] .. cu_q[b + 1]`` are the
     last tokens of sequence b's ``context_lens[b]``, each seeing the positions
     up to its own; without it, row b sees all of sequence b's context.  A row
-    that sees nothing is 0.  ``workspace``: a uint8 tensor of
-    :func:`attention_workspace_bytes` bytes, or None for one kept per stream.
+    that sees nothing is 0.  ``workspace``: a uint8 tensor of as many bytes as
+    ``fnmoe_paged_attention_q8_workspace_size`` reports, or None for one that
+    is kept for the current stream.
     """
-    torch = _torch()
-    lib = _lib.ensure_device()
     c = _cache(k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3:
         raise ValueError("q must be [rows, q_heads, head_dim]")
@@ -222,15 +218,17 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
         _want(block_table, i32, (batch, width), "block_table"), _want(context_lens, i32, (batch,), "context_lens"),
         None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q"),
         _want(out, torch.bfloat16, (rows, heads, dim), "out"))
-    stream = _stream_of(q)
-    need = ctypes.c_uint64(0)
+    lib, stream = _ready(q)
     ref = ctypes.byref(a)
-    _lib.check(lib.fnmoe_paged_attention_q8_workspace_size(ref, ctypes.byref(need)), "paged attention q8 workspace")
-    if workspace is None:
-        key = (q.device.index, stream)
-        workspace = _workspaces.get(key)
-        if workspace is None or workspace.numel() < need.value:
-            workspace = _workspaces[key] = torch.empty(max(need.value, 256), dtype=torch.uint8, device=q.device)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    _lib.check(lib.fnmoe_paged_attention_q8(ref, stream), "paged_attention_q8")
+    kept = workspace if workspace is not None else _workspaces.get((q.get_device(), stream))
+    if kept is not None:
+        a.workspace, a.workspace_bytes = kept.data_ptr(), kept.numel()
+    code = lib.fnmoe_paged_attention_q8(ref, stream)
+    if code == _lib.ERR_WORKSPACE and workspace is None:  # none kept for this stream yet, or too small a one
+        need = ctypes.c_uint64(0)
+        _lib.check(lib.fnmoe_paged_attention_q8_workspace_size(ref, ctypes.byref(need)), "paged attention q8 workspace")
+        kept = _workspaces[(q.get_device(), stream)] = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = kept.data_ptr(), kept.numel()
+        code = lib.fnmoe_paged_attention_q8(ref, stream)
+    _lib.check(code, "paged_attention_q8")
     return out
