@@ -1,130 +1,19 @@
-// attention_q8.cu -- causal attention over the paged 8-bit KV cache (sm_100a).
-//
-//   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale * q_i . k_j - m_i),
-//   k_j = ks[block of j] * kcode_j,  v_j = vs[block of j] * vcode_j,
-//   j over the positions up to row i's own whose page is in the cache.
-//
-// Codes go to the tensor cores as bfloat16, in which they are exact (int8 has
-// 7 bits and a sign, e4m3 4 bits), next to the queries as they are; the two
-// block scales enter in float32.  With
-//   t_j = (scale * log2 e * ks) (q . kcode_j) + log2 vs,   u_j = 2^(t_j - m),
-// m a running reference of the t_j,
-//   out = sum_j u_j vcode_j / sum_blocks (1 / vs) sum_(j in block) u_j :
-// the value scale rides in the exponent.  The weights enter the second product
-// as two bfloat16 terms, u = hi + lo with 16 bits: one term alone would cost
-// up to 2^-9 of an output (as much as its final rounding), and float16 loses
-// weights below 2^-24 of the largest, which are all that is left of an output
-// whose heaviest tokens hold zeros.
-#include <cuda_fp16.h>
+// attention_q8.cu -- causal attention over the paged 8-bit KV cache (sm_100a):
+// the entry points and the kernels for sequences with few query rows (decode).
+// The arithmetic: attention_q8.cuh; many rows: attention_q8_many.cu.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <algorithm>
 #include <cmath>
 #include <string>
 
-#include "async.cuh"
-#include "common.cuh"
+#include "attention_q8.cuh"
 #include "moe_kernels.cuh"
 #include "paged_q8.cuh"
 
 namespace fnmoe {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 8.0f;  // a reference may fall this far (log2) below the largest t
-
-struct Q8View {
-  const uint16_t *q;
-  const uint8_t *kc, *vc;
-  const float *ks, *vs;
-  const int32_t *table, *ctx, *cu;
-  uint16_t *out;
-  uint64_t q_stride;
-  int B, rows, Hq, Hkv, gq, page, block_shift, width, pages;
-  float scale;
-  // workspace
-  long long *prefix;  // [B + 1] units of work before each sequence
-  float *part;        // [2 * CTAs][8][D] unfinished sums
-  float2 *part_ml;    // [2 * CTAs][8] their reference and weight sum
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
-  return d;
-}
-__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-// a and b as bfloat16 pairs hi + lo.
-__device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t &hi, uint32_t &lo) {
-  hi = pack_bf16x2(a, b);
-  lo = pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
-}
-__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two codes in bytes (0, 1) (HALF 0) or (2, 3) (HALF 1) of w, as bfloat16 pairs.
-// int8: under the high byte 0x43, the low seven bits l of a code read as
-// 128 + l and its sign bit alone as 128 (clear) or 256 (set); the difference
-// is l or l - 128, the code.
-// e4m3: to float16, to float32, to bfloat16, all exact.
-template <bool E4M3, int HALF>
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
-  uint32_t d;
-  if (E4M3) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(HALF ? w >> 16 : w)));
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-    d = pack_bf16x2(f.x, f.y);
-  } else {
-    const uint32_t x = prmt(w, 0x43434343u, HALF ? 0x4342u : 0x4140u);
-    asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
-  }
-  return d;
-}
-
-__device__ __forceinline__ uint4 ldg_stream(const void *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
-// Rows of sequence b: first packed row and their number.
-__device__ __forceinline__ int2 rows_of(const Q8View &p, int b) {
-  if (p.cu == nullptr) return make_int2(b, 1);
-  const int r0 = max(p.cu[b], 0), r1 = min(p.cu[b + 1], p.rows);
-  return make_int2(r0, max(r1 - r0, 0));
-}
-// Tokens of sequence b that the cache can hold.
-__device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
-  return max(0, min(p.ctx[b], p.width * p.page));
-}
 
 // ---- few rows per sequence --------------------------------------------------
 //
@@ -133,7 +22,7 @@ __device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
 // units of all sequences, laid end to end, are dealt to the CTAs in equal
 // contiguous ranges, so ragged contexts load every SM alike.  A CTA's range
 // covers whole segments, which it finishes, and at most two cut ones (its
-// first and last), whose sums go to the workspace for k_q8_join.
+// first and last), whose sums go to the workspace for k_q8_few_join.
 //
 // A warp takes 16 tokens at a time straight from global memory into MMA
 // fragments (no shared memory, no barriers: at 23 bytes a clock and SM the
@@ -147,8 +36,8 @@ __device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
 // 16 tokens lie in one page and one scale block.  The next step's K is
 // requested when this one's K has been consumed, the next V likewise.
 
-constexpr int kUnit = 64;       // tokens of a unit: 4 warps x 16
-constexpr int kFewThreads = 128;
+constexpr int kFewThreads = 128;  // 4 warps x 16 tokens = a unit
+constexpr int kFewRows = 16;
 
 template <int D>
 struct Few {
@@ -159,7 +48,7 @@ struct Few {
 // Units of one (kv head, row tile) of sequence b, and its row tiles.
 __device__ __forceinline__ int2 units_of(const Q8View &p, int b) {
   const int rows = rows_of(p, b).y * p.gq;
-  return make_int2((tokens_of(p, b) + kUnit - 1) / kUnit, (rows + 7) / 8);
+  return make_int2((tokens_of(p, b) + kUnit - 1) / kUnit, rows <= p.few_rows ? (rows + 7) / 8 : 0);
 }
 
 // The sequence that holds unit `at` of all units, and its first unit; the
@@ -192,10 +81,9 @@ __device__ Found find_unit(const Q8View &p, int cta, int ctas, long long &start,
   total = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) total += s_w[w];
-  // At most a CTA per unit, so that no range between two others is empty.
-  const int used = static_cast<int>(min(static_cast<long long>(ctas), max(total, 1ll)));
-  start = total * min(cta, used) / used;
-  end = total * min(cta + 1, used) / used;
+  const int used = ranges_of(total, ctas);
+  start = range_start(total, used, cta);
+  end = range_start(total, used, cta + 1);
   long long carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += THREADS) {
     const int b = b0 + tid;
@@ -241,6 +129,14 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
   pdl_trigger();
   long long cur, end;
   const Found f = find_unit<kFewThreads>(p, blockIdx.x, gridDim.x, cur, end);
+  // rows of sequences without a token
+  for (int e = blockIdx.x; e < p.B; e += gridDim.x) {
+    const int2 u = units_of(p, e);
+    if (u.x != 0 || u.y == 0) continue;
+    const int2 qr = rows_of(p, e);
+    uint2 *dst = reinterpret_cast<uint2 *>(p.out + static_cast<size_t>(qr.x) * p.Hq * D);
+    for (int i = threadIdx.x; i < qr.y * p.Hq * (D / 4); i += kFewThreads) dst[i] = make_uint2(0, 0);
+  }
   const long long first = cur;
   int b = f.b;
   long long off = cur - f.before;  // within the sequence
@@ -502,9 +398,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
       if (whole) {
         const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
         const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
-        const uint32_t lo = static_cast<uint32_t>(f32_to_bf16(s.x * inv)) | (static_cast<uint32_t>(f32_to_bf16(s.y * inv)) << 16);
-        const uint32_t hi = static_cast<uint32_t>(f32_to_bf16(s.z * inv)) | (static_cast<uint32_t>(f32_to_bf16(s.w * inv)) << 16);
-        *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + d) = make_uint2(lo, hi);
+        *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + d) =
+            make_uint2(pack_bf16x2(s.x * inv, s.y * inv), pack_bf16x2(s.z * inv, s.w * inv));
       } else {
         *reinterpret_cast<float4 *>(p.part + (static_cast<size_t>(slot) * 8 + r) * D + d) = s;
         if (d == 0) p.part_ml[slot * 8 + r] = make_float2(mm, ll);
@@ -516,77 +411,34 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
   }
 }
 
-// The CTA whose range holds unit `unit` of `total`.
-__device__ __forceinline__ int owner_of(long long unit, long long total, int ctas) {
-  return static_cast<int>(((unit + 1) * ctas - 1) / total);
-}
-
-// One CTA per (sequence, kv head, tile, row): joins the cut segments' sums in
-// CTA order, and zeroes rows whose sequence has no token.
+// One CTA per (cut, row): the segment that unit range_start(i) cuts, once for
+// the first cut inside it.
 template <int D>
-__global__ void __launch_bounds__(256) k_q8_join(Q8View p, int tiles, int ctas) {
-  constexpr int L = D / 4, G = 256 / L;  // lanes of a row, groups of partial sums
-  __shared__ float4 s_o[G][L];
-  __shared__ float s_l[G];
+__global__ void __launch_bounds__(256) k_q8_few_join(Q8View p, int ctas) {
   pdl_wait();
-  const int r = blockIdx.x & 7;
-  int seg = blockIdx.x >> 3;
-  const int rt = seg % tiles;
-  seg /= tiles;
-  const int h = seg % p.Hkv, b = seg / p.Hkv;
-  const int2 qr = rows_of(p, b);
-  const int rows = qr.y * p.gq, rr = rt * 8 + r;
-  if (rr >= rows) return;
-  const int2 u = units_of(p, b);
-  const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
-  uint16_t *dst = p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D;
-  const int lane = threadIdx.x % L, grp = threadIdx.x / L;
-  if (u.x == 0) {
-    if (grp == 0) *reinterpret_cast<uint2 *>(dst + 4 * lane) = make_uint2(0, 0);
-    return;
-  }
+  const int r = blockIdx.x & 7, cut = (blockIdx.x >> 3) + 1;
   const long long total = p.prefix[p.B];
-  ctas = static_cast<int>(min(static_cast<long long>(ctas), total));
-  const long long a = p.prefix[b] + static_cast<long long>(h * u.y + rt) * u.x;
-  const int c0 = owner_of(a, total, ctas), c1 = owner_of(a + u.x - 1, total, ctas);
-  if (c0 == c1) return;  // finished by its CTA
-  // CTA c0's piece is its first one only if its range begins with the segment.
-  auto slot_of = [&](int c) { return 2 * c + (c == c0 && total * c / ctas < a ? 1 : 0); };
-  float mm = -INFINITY;
-  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, p.part_ml[slot_of(c) * 8 + r].x);
-#pragma unroll
-  for (int s = 16; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, s));
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float ll = 0.0f;
-#pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += G) {
-    const int slot = slot_of(c);
-    const float2 ml = p.part_ml[slot * 8 + r];
-    const float4 v = *reinterpret_cast<const float4 *>(p.part + (static_cast<size_t>(slot) * 8 + r) * D + 4 * lane);
-    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
-    ll += ml.y * w;
-    acc.x += v.x * w;
-    acc.y += v.y * w;
-    acc.z += v.z * w;
-    acc.w += v.w * w;
+  const int used = ranges_of(total, ctas);
+  if (cut >= used) return;
+  const long long unit = range_start(total, used, cut);
+  int lo = 0, hi = p.B;  // the last sequence that begins at or before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.prefix[mid] <= unit) lo = mid; else hi = mid;
   }
-  s_o[grp][lane] = acc;
-  if (lane == 0) s_l[grp] = ll;
-  __syncthreads();
-  if (grp != 0) return;
-#pragma unroll
-  for (int i = 1; i < G; ++i) {
-    const float4 v = s_o[i][lane];
-    acc.x += v.x;
-    acc.y += v.y;
-    acc.z += v.z;
-    acc.w += v.w;
-    ll += s_l[i];
-  }
-  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
-  const uint32_t lo = static_cast<uint32_t>(f32_to_bf16(acc.x * inv)) | (static_cast<uint32_t>(f32_to_bf16(acc.y * inv)) << 16);
-  const uint32_t hi = static_cast<uint32_t>(f32_to_bf16(acc.z * inv)) | (static_cast<uint32_t>(f32_to_bf16(acc.w * inv)) << 16);
-  *reinterpret_cast<uint2 *>(dst + 4 * lane) = make_uint2(lo, hi);
+  const int2 u = units_of(p, lo);
+  const int seg = static_cast<int>((unit - p.prefix[lo]) / u.x);
+  const int h = seg / u.y, rt = seg - h * u.y;
+  const long long a = p.prefix[lo] + static_cast<long long>(seg) * u.x;
+  if (a == unit) return;  // between two segments
+  const int c0 = owner_of(a, total, used), c1 = owner_of(a + u.x - 1, total, used);
+  if (c0 != cut - 1) return;
+  const int2 qr = rows_of(p, lo);
+  const int rr = rt * 8 + r;
+  if (rr >= qr.y * p.gq) return;
+  const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
+  join_row<D, 8>(p.part, p.part_ml, c0, c1, range_start(total, used, c0) < a, r,
+                 p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D);
 }
 
 int check(const FnQ8AttentionArgs *a, std::string &err) {
@@ -599,6 +451,10 @@ int check(const FnQ8AttentionArgs *a, std::string &err) {
       (a->cu_q == nullptr && a->q_rows != a->batch)) {
     err = "attention needs sequences, a table row below 2^31 tokens, q_heads a multiple of kv_heads and, "
           "without cu_q, one row per sequence";
+    return FNMOE_ERR_SHAPE;
+  }
+  if (static_cast<uint64_t>(a->q_rows) * (a->q_heads / c.kv_heads) > 0x7FFFFF00ull) {
+    err = "too many query rows";
     return FNMOE_ERR_SHAPE;
   }
   if (a->q_heads / c.kv_heads > 32) { err = "at most 32 query heads per kv head"; return FNMOE_ERR_UNSUPPORTED; }
@@ -621,52 +477,46 @@ int check(const FnQ8AttentionArgs *a, std::string &err) {
 
 uint64_t align256(uint64_t n) { return (n + 255) & ~static_cast<uint64_t>(255); }
 
-// Workspace: prefix sums, then the cut segments' sums.
+// Workspace: prefix sums and tiles, then the cut segments' sums.
 struct Carve {
-  uint64_t ml, part, bytes;
+  uint64_t ml, part, seq_tile, tiles, tprefix, tml, tpart, bytes;
 };
-Carve carve(const FnQ8AttentionArgs *a) {
+Carve carve(const FnQ8AttentionArgs *a, const Q8View &p, bool few, bool many) {
   const uint64_t d = a->cache.head_dim;
-  const uint64_t slots = 2ull * (d == 256 ? Few<256>::kMax : d == 128 ? Few<128>::kMax : Few<64>::kMax);
+  const uint64_t slots = few ? 2ull * (d == 256 ? Few<256>::kMax : d == 128 ? Few<128>::kMax : Few<64>::kMax) : 0;
+  const uint64_t tiles = many ? many_tiles(p) : 0, tslots = many ? 2ull * many_ctas(static_cast<int>(d)) : 0;
+  uint64_t at = 0;
+  auto take = [&](uint64_t n) {
+    const uint64_t here = at;
+    at += align256(n);
+    return here;
+  };
   Carve c{};
-  c.ml = align256(8 * (static_cast<uint64_t>(a->batch) + 1));
-  c.part = c.ml + align256(slots * 8 * sizeof(float2));
-  c.bytes = c.part + slots * 8 * d * sizeof(float) + 256;  // the start is rounded up to 256 bytes
+  take(8 * (static_cast<uint64_t>(a->batch) + 1));
+  c.ml = take(slots * 8 * sizeof(float2));
+  c.part = take(slots * 8 * d * sizeof(float));
+  c.seq_tile = take(4 * (static_cast<uint64_t>(a->batch) + 1));
+  c.tiles = take(sizeof(int4) * tiles);
+  c.tprefix = take(8 * (tiles + 1));
+  c.tml = take(tslots * 128 * sizeof(float2));
+  c.tpart = take(tslots * 128 * d * sizeof(float));
+  c.bytes = at + 256;  // the start is rounded up to 256 bytes
   return c;
 }
 
 template <int D, bool E4M3>
 cudaError_t launch_few(const Q8View &p, cudaStream_t s) {
   constexpr int ctas = Few<D>::kMax;
-  const uint64_t tiles = p.cu ? (static_cast<uint64_t>(p.rows) * p.gq + 7) / 8 : (p.gq + 7) / 8;
-  const uint64_t joins = static_cast<uint64_t>(p.B) * p.Hkv * tiles * 8;
-  if (joins > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
   k_q8_few<D, E4M3><<<ctas, kFewThreads, 0, s>>>(p);
-  return launch_pdl(k_q8_join<D>, dim3(static_cast<unsigned>(joins)), dim3(256), 0, s, p, static_cast<int>(tiles), ctas);
+  return launch_pdl(k_q8_few_join<D>, dim3((ctas - 1) * 8), dim3(256), 0, s, p, ctas);
 }
 
 template <int D>
-cudaError_t launch(const Q8View &p, bool e4m3, cudaStream_t s) {
+cudaError_t launch_few_d(const Q8View &p, bool e4m3, cudaStream_t s) {
   return e4m3 ? launch_few<D, true>(p, s) : launch_few<D, false>(p, s);
 }
 
-}  // namespace
-
-int paged_attention_q8_workspace_size(const FnQ8AttentionArgs *a, uint64_t *bytes, std::string &err) {
-  if (bytes == nullptr) { err = "bytes is NULL"; return FNMOE_ERR_NULL; }
-  if (const int rc = check(a, err)) return rc;
-  *bytes = carve(a).bytes;
-  return FNMOE_OK;
-}
-
-int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &err) {
-  if (const int rc = check(a, err)) return rc;
-  if (a->q_rows == 0) return FNMOE_OK;
-  const Carve w = carve(a);
-  if (a->workspace == nullptr || a->workspace_bytes < w.bytes) {
-    err = "workspace needs " + std::to_string(w.bytes) + " bytes";
-    return FNMOE_ERR_WORKSPACE;
-  }
+Q8View view_of(const FnQ8AttentionArgs *a) {
   const FnQ8Cache &c = a->cache;
   Q8View p{};
   p.q = static_cast<const uint16_t *>(a->q);
@@ -688,18 +538,55 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
   p.block_shift = 31 - __builtin_clz(c.block);
   p.width = static_cast<int>(a->max_pages);
   p.pages = static_cast<int>(c.num_pages);
+  p.page_magic = static_cast<uint32_t>(((1ull << 32) + c.page_size - 1) / c.page_size);
   p.scale = a->scale;
+  p.few_rows = kFewRows;
+  return p;
+}
+
+// Which kernels a call can need: a sequence's rows are not known on the host,
+// but without cu_q each has one, and no sequence has more than all of them.
+bool wants_few(const Q8View &p) { return p.cu != nullptr || p.gq <= p.few_rows; }
+bool wants_many(const Q8View &p) {
+  return p.cu != nullptr ? static_cast<uint64_t>(p.rows) * p.gq > static_cast<uint64_t>(p.few_rows) : p.gq > p.few_rows;
+}
+
+}  // namespace
+
+int paged_attention_q8_workspace_size(const FnQ8AttentionArgs *a, uint64_t *bytes, std::string &err) {
+  if (bytes == nullptr) { err = "bytes is NULL"; return FNMOE_ERR_NULL; }
+  if (const int rc = check(a, err)) return rc;
+  const Q8View p = view_of(a);
+  *bytes = carve(a, p, wants_few(p), wants_many(p)).bytes;
+  return FNMOE_OK;
+}
+
+int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &err) {
+  if (const int rc = check(a, err)) return rc;
+  if (a->q_rows == 0) return FNMOE_OK;
+  Q8View p = view_of(a);
+  const bool few = wants_few(p), many = wants_many(p);
+  const Carve w = carve(a, p, few, many);
+  if (a->workspace == nullptr || a->workspace_bytes < w.bytes) {
+    err = "workspace needs " + std::to_string(w.bytes) + " bytes";
+    return FNMOE_ERR_WORKSPACE;
+  }
   uint8_t *ws = reinterpret_cast<uint8_t *>(align256(reinterpret_cast<uintptr_t>(a->workspace)));
   p.prefix = reinterpret_cast<long long *>(ws);
   p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
   p.part = reinterpret_cast<float *>(ws + w.part);
-  const bool e4m3 = c.code_type == FNMOE_Q8_E4M3;
-  cudaError_t e;
-  switch (c.head_dim) {
-    case 64: e = launch<64>(p, e4m3, s); break;
-    case 128: e = launch<128>(p, e4m3, s); break;
-    default: e = launch<256>(p, e4m3, s); break;
-  }
+  p.max_tiles = many ? static_cast<int>(many_tiles(p)) : 0;
+  p.seq_tile = reinterpret_cast<int *>(ws + w.seq_tile);
+  p.tiles = reinterpret_cast<int4 *>(ws + w.tiles);
+  p.tprefix = reinterpret_cast<long long *>(ws + w.tprefix);
+  p.tpart_ml = reinterpret_cast<float2 *>(ws + w.tml);
+  p.tpart = reinterpret_cast<float *>(ws + w.tpart);
+  const int d = static_cast<int>(a->cache.head_dim);
+  const bool e4m3 = a->cache.code_type == FNMOE_Q8_E4M3;
+  cudaError_t e = cudaSuccess;
+  if (many) e = launch_many(p, d, e4m3, s);
+  if (e == cudaSuccess && few)
+    e = d == 64 ? launch_few_d<64>(p, e4m3, s) : d == 128 ? launch_few_d<128>(p, e4m3, s) : launch_few_d<256>(p, e4m3, s);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     err = std::string("paged attention q8: ") + cudaGetErrorString(e);

@@ -1,0 +1,209 @@
+// attention_q8.cuh -- what the kernels of the attention over the paged 8-bit
+// KV cache share: the call's view, code conversion, the row and token counts
+// of a sequence and the division of work.
+//
+//   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale * q_i . k_j - m_i),
+//   k_j = ks[block of j] * kcode_j,  v_j = vs[block of j] * vcode_j,
+//   j over the positions up to row i's own whose page is in the cache.
+//
+// Codes go to the tensor cores as bfloat16, in which they are exact (int8 has
+// 7 bits and a sign, e4m3 4 bits), next to the queries as they are; the two
+// block scales enter in float32.  With
+//   t_j = (scale * log2 e * ks) (q . kcode_j) + log2 vs,   u_j = 2^(t_j - m),
+// m a running reference of the t_j,
+//   out = sum_j u_j vcode_j / sum_blocks (1 / vs) sum_(j in block) u_j :
+// the value scale rides in the exponent.  The weights enter the second product
+// as two bfloat16 terms, u = hi + lo with 16 bits: one term alone would cost
+// up to 2^-9 of an output (as much as its final rounding), and float16 loses
+// weights below 2^-24 of the largest, which are all that is left of an output
+// whose heaviest tokens hold zeros.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "async.cuh"
+#include "common.cuh"
+
+namespace fnmoe {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.0f;  // a reference may fall this far (log2) below the largest t
+
+constexpr int kUnit = 64;  // tokens of a unit of work
+
+struct Q8View {
+  const uint16_t *q;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  const int32_t *table, *ctx, *cu;
+  uint16_t *out;
+  uint64_t q_stride;
+  int B, rows, Hq, Hkv, gq, page, block_shift, width, pages;
+  uint32_t page_magic;  // 2^32 / page, rounded up
+  float scale;
+  int few_rows;         // sequences of more (row, head) pairs per kv head take the many-row kernel
+  // workspace of the few-row kernel (8 rows a tile)
+  long long *prefix;    // [B + 1] units of work before each sequence
+  float *part;          // [2 * CTAs][8][D] unfinished sums
+  float2 *part_ml;      // [2 * CTAs][8] their reference and weight sum
+  // workspace of the many-row kernel (128 rows a tile)
+  int max_tiles;
+  int *seq_tile;        // [B + 1] tiles before each sequence
+  int4 *tiles;          // [tiles] {sequence, tile of it, units of one kv head, 0}
+  long long *tprefix;   // [tiles + 1] units of work before each tile
+  float *tpart;         // [2 * CTAs][128][D]
+  float2 *tpart_ml;     // [2 * CTAs][128]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+  return d;
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// a and b as bfloat16 pairs hi + lo.
+__device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t &hi, uint32_t &lo) {
+  hi = pack_bf16x2(a, b);
+  lo = pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
+}
+__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two codes in bytes (0, 1) (HALF 0) or (2, 3) (HALF 1) of w, as bfloat16 pairs.
+// int8: under the high byte 0x43, the low seven bits l of a code read as
+// 128 + l and its sign bit alone as 128 (clear) or 256 (set); the difference
+// is l or l - 128, the code.
+// e4m3: to float16, to float32, to bfloat16, all exact.
+template <bool E4M3, int HALF>
+__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+  uint32_t d;
+  if (E4M3) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(HALF ? w >> 16 : w)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    d = pack_bf16x2(f.x, f.y);
+  } else {
+    const uint32_t x = prmt(w, 0x43434343u, HALF ? 0x4342u : 0x4140u);
+    asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
+  }
+  return d;
+}
+
+__device__ __forceinline__ uint4 ldg_stream(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Rows of sequence b: first packed row and their number.
+__device__ __forceinline__ int2 rows_of(const Q8View &p, int b) {
+  if (p.cu == nullptr) return make_int2(b, 1);
+  const int r0 = max(p.cu[b], 0), r1 = min(p.cu[b + 1], p.rows);
+  return make_int2(r0, max(r1 - r0, 0));
+}
+// pos / page for pos < 2^31.
+__device__ __forceinline__ int page_col(const Q8View &p, int pos) {
+  int c = static_cast<int>(__umulhi(static_cast<uint32_t>(pos), p.page_magic));
+  if (c * p.page > pos) --c;
+  return c;
+}
+// Tokens of sequence b that the cache can hold.
+__device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
+  return max(0, min(p.ctx[b], p.width * p.page));
+}
+
+// Equal contiguous ranges of `total` units for the CTAs: CTA i takes
+// [range_start(i), range_start(i + 1)).  At most a CTA per unit is used, so
+// that no range between two others is empty.
+__device__ __forceinline__ int ranges_of(long long total, int ctas) {
+  return static_cast<int>(min(static_cast<long long>(ctas), max(total, 1ll)));
+}
+__device__ __forceinline__ long long range_start(long long total, int used, int i) {
+  return total * min(i, used) / used;
+}
+// The CTA whose range holds `unit`.
+__device__ __forceinline__ int owner_of(long long unit, long long total, int used) {
+  return static_cast<int>(((unit + 1) * used - 1) / total);
+}
+
+// Joins the sums of a segment that several CTAs worked on (CTA c0 to c1, in
+// CTA order) for one row: `row` of the R rows of a workspace slot.  256
+// threads: L = D / 4 lanes, G groups that take every G-th CTA.  A CTA's first
+// piece of work is in slot 2c, a later cut one in 2c + 1; `late0`: CTA c0's
+// range begins before the segment.
+template <int D, int R>
+__device__ __forceinline__ void join_row(const float *part, const float2 *part_ml, int c0, int c1, bool late0, int row,
+                                         uint16_t *dst) {
+  constexpr int L = D / 4, G = 256 / L;
+  __shared__ float4 s_o[G][L];
+  __shared__ float s_l[G];
+  const int lane = threadIdx.x % L, grp = threadIdx.x / L;
+  auto at = [&](int c) { return static_cast<size_t>(2 * c + (c == c0 && late0 ? 1 : 0)) * R + row; };
+  float mm = -INFINITY;
+  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, part_ml[at(c)].x);
+#pragma unroll
+  for (int s = 16; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, s));
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float ll = 0.0f;
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += G) {
+    const float2 ml = part_ml[at(c)];
+    const float4 v = *reinterpret_cast<const float4 *>(part + at(c) * D + 4 * lane);
+    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
+    ll += ml.y * w;
+    acc.x += v.x * w;
+    acc.y += v.y * w;
+    acc.z += v.z * w;
+    acc.w += v.w * w;
+  }
+  s_o[grp][lane] = acc;
+  if (lane == 0) s_l[grp] = ll;
+  __syncthreads();
+  if (grp != 0) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    const float4 v = s_o[i][lane];
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+    ll += s_l[i];
+  }
+  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
+  *reinterpret_cast<uint2 *>(dst + 4 * lane) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+// The many-row kernels (attention_q8_many.cu).
+int many_ctas(int head_dim);
+uint64_t many_tiles(const Q8View &p);  // at most so many tiles of 128 rows
+cudaError_t launch_many(const Q8View &p, int head_dim, bool e4m3, cudaStream_t s);
+
+}  // namespace fnmoe

@@ -1,0 +1,744 @@
+// attention_q8_many.cu -- causal attention over the paged 8-bit KV cache for
+// sequences with many query rows (multi-token verify, prefill chunks), on
+// tcgen05.  The arithmetic: attention_q8.cuh.
+//
+// A tile is 128 (row, head) pairs of one sequence and kv head (MMA M); a unit
+// of work is a tile times 64 tokens.  k_q8_tiles lists the tiles with the
+// units that causality leaves them; the units of all tiles, laid end to end,
+// are dealt to persistent CTAs in equal contiguous ranges, so neither ragged
+// lengths nor the causal triangle load one SM more than another.  Tiles that
+// a range cuts are joined by k_q8_many_join.
+//
+// Per unit, S = Q K^T (M128 N64, K = D) and O += P V (M128 N = D, K = 64, for
+// each of the two terms of P) run on the tensor cores with Q and P as TMEM
+// operands, S and O as TMEM accumulators: 6 D * 128 * 64 multiply-adds where
+// the formula has 4, which bounds the kernel (1,536 clocks a unit at D 256).
+// Roles:
+//   warps 0-3   softmax, one row a thread: S from TMEM, running reference and
+//               sum, P back to TMEM; Q in and the result out of TMEM;
+//   warp 4      issues the MMAs;
+//   warps 8-..  read K and V codes (16 bytes a thread) one unit ahead in
+//               registers, widen them to bfloat16 and store them to shared
+//               memory as 128B-swizzled tiles, [D / 64][64 tokens][128 bytes]:
+//               K-major for K, MN-major for V.
+// The warpgroups trade registers (setmaxnreg): a softmax thread holds a row of
+// S, the issuer next to nothing.
+// Widening in the kernel reads a byte a value from L2 where a widened copy
+// would write and re-read two.
+// TMEM columns at D 256: O 0-255, Q 256-383, S 384-447, P 448-511, so the next
+// unit's Q K^T runs while this one's P is made.  At D 64 and 128 P takes S's
+// columns and a CTA needs 256 of the 512: two CTAs share an SM and fill each
+// other's waits.
+// Every wait is bounded: a timeout sets the device error word and marks the
+// CTA dead, whereupon every role runs to the end.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "attention_q8.cuh"
+#include "moe_kernels.cuh"
+#include "umma.cuh"
+
+namespace fnmoe {
+
+namespace {
+
+constexpr int kTile = 128;
+constexpr int kMmaWarp = 4, kConvWarp0 = 8;  // warps 5-7 only fill the MMA issuer's warpgroup
+constexpr int kInfo = 8;  // units whose scales are kept
+constexpr uint32_t kSpin = 1u << 22;
+
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+template <int D>
+struct Many {
+  static constexpr bool kShared = D < 256;  // P takes S's columns
+  static constexpr int kCtas = D < 256 ? 2 : 1;  // per SM
+  static constexpr int kConvWarps = D < 256 ? 4 : 8;
+  static constexpr int kThreads = 32 * (kConvWarp0 + kConvWarps);
+  // Registers a thread: at launch 512 x 128 or 384 x 80; the shares add up to as many.
+  static constexpr int kRegSoftmax = D < 256 ? 136 : 208, kRegIssue = D < 256 ? 40 : 48, kRegConv = D < 256 ? 64 : 128;
+  static constexpr int kSlots = 3;               // tiles of K and of V in shared memory
+  static constexpr int kSlotBytes = 64 * D * 2;
+  static constexpr int kCols = D < 256 ? 256 : 512;
+  static constexpr int kColQ = D;
+  static constexpr int kColS = D < 256 ? 192 : 384;
+  static constexpr int kColP = D < 256 ? 192 : 448;
+  // barriers
+  static constexpr int kKFull = 0, kKEmpty = kKFull + kSlots, kVFull = kKEmpty + kSlots, kVEmpty = kVFull + kSlots,
+                       kSFull = kVEmpty + kSlots, kSEmpty = kSFull + 1, kPFull = kSEmpty + 1, kPEmpty = kPFull + 1,
+                       kQFull = kPEmpty + 1, kInfoFull = kQFull + 1, kBars = kInfoFull + kInfo;
+  static constexpr int kOffV = kSlots * kSlotBytes;
+  static constexpr int kOffInfo = 2 * kSlots * kSlotBytes;  // float4 [kInfo][4]
+  static constexpr int kOffBar = kOffInfo + kInfo * 64;
+  static constexpr int kOffMisc = kOffBar + 8 * kBars;      // TMEM base, dead flag
+  static constexpr int kSmem = kOffMisc + 16 + 1024;        // + slack for the 1024-byte alignment of the tiles
+  static constexpr int kMax = 148 * kCtas;
+};
+static_assert(Many<256>::kSmem <= 227 * 1024, "shared memory");
+static_assert(2 * Many<128>::kSmem <= 227 * 1024, "shared memory of two CTAs");
+
+// kind::f16, bfloat16 A and B, float32 D, M 128.
+constexpr uint32_t idesc(int n, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+// Descriptor of a 128B-swizzled MN-major tile: 64-value groups of the MN
+// dimension 8192 bytes apart (LBO), 8-token groups 1024 bytes apart (SBO).
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (512ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// D[tmem] (+)= A[tmem] B[smem].
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t s, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(s), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+// Bounded wait on `bar` for the phase of parity `parity`; false when it gives
+// up or the CTA is dead.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *dead, uint32_t *err) {
+  uint32_t spins = 0;
+  while (!mbar_try_wait_u32(bar, parity)) {
+    if (*dead) return false;
+    if (++spins >= kSpin) {
+      *dead = 1u;
+      set_error(err, kErrTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+// ---- tiles ------------------------------------------------------------------
+
+__device__ __forceinline__ int tiles_of(const Q8View &p, int b) {
+  const int rows = rows_of(p, b).y * p.gq;
+  return rows > p.few_rows ? (rows + kTile - 1) / kTile : 0;
+}
+
+constexpr int kScanThreads = 1024;
+
+// Inclusive sum over the CTA's threads plus `carry`, which becomes the total.
+__device__ __forceinline__ long long scan1(long long v, long long &carry, long long *red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long o = __shfl_up_sync(0xFFFFFFFFu, v, off);
+    if (lane >= off) v += o;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    long long w = red[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long o = __shfl_up_sync(0xFFFFFFFFu, w, off);
+      if (lane >= off) w += o;
+    }
+    red[lane] = w;
+  }
+  __syncthreads();
+  const long long before = warp > 0 ? red[warp - 1] : 0;
+  const long long out = carry + before + v;
+  carry += red[31];
+  return out;
+}
+
+// One CTA: the tiles of all sequences and the units before each.
+__global__ void __launch_bounds__(kScanThreads) k_q8_tiles(Q8View p) {
+  __shared__ long long red[32];
+  long long carry = 0;
+  pdl_trigger();
+  for (int b0 = 0; b0 < p.B; b0 += kScanThreads) {
+    const int b = b0 + threadIdx.x;
+    const int n = b < p.B ? tiles_of(p, b) : 0;
+    const long long s = scan1(n, carry, red);
+    if (b < p.B) p.seq_tile[b] = static_cast<int>(s - n);
+  }
+  // Ascending cu_q never gives more than max_tiles.
+  const int tiles = static_cast<int>(min(carry, static_cast<long long>(p.max_tiles)));
+  if (threadIdx.x == 0) p.seq_tile[p.B] = tiles;
+  __syncthreads();
+  carry = 0;
+  for (int t0 = 0; t0 < tiles; t0 += kScanThreads) {
+    const int t = t0 + threadIdx.x;
+    long long units = 0;
+    if (t < tiles) {
+      int lo = 0, hi = p.B;  // the last sequence whose tiles begin at or before t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.seq_tile[mid] <= t) lo = mid; else hi = mid;
+      }
+      const int mt = t - p.seq_tile[lo];
+      const int n = rows_of(p, lo).y, rows = n * p.gq;
+      const int last = (min((mt + 1) * kTile, rows) - 1) / p.gq;  // the tile's last query
+      const int seen = max(0, min(p.ctx[lo] - n + last + 1, p.width * p.page));
+      const int steps = (seen + kUnit - 1) / kUnit;
+      p.tiles[t] = make_int4(lo, mt, steps, 0);
+      units = static_cast<long long>(steps) * p.Hkv;
+    }
+    const long long s = scan1(units, carry, red);
+    if (t < tiles) p.tprefix[t] = s - units;
+  }
+  if (threadIdx.x == 0) p.tprefix[tiles] = carry;
+}
+
+// The last of `tiles` tiles that begins at or before `unit`; a whole warp.
+__device__ __forceinline__ int find_tile(const Q8View &p, int tiles, long long unit) {
+  int lo = 0, hi = tiles;
+  const int lane = threadIdx.x & 31;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int t = lo + lane * step;
+    const unsigned m = __ballot_sync(0xFFFFFFFFu, t < hi && p.tprefix[min(t, tiles)] <= unit);
+    const int k = 31 - __clz(m);  // lane 0 always holds
+    lo += k * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// A piece of work: units [u0, u0 + n) of tile `tile` and kv head h.
+struct Piece {
+  int b, mt, h, u0, n, steps;
+};
+struct Walk {
+  long long cur, end, off, first;
+  int tile;
+};
+__device__ __forceinline__ bool next_piece(const Q8View &p, Walk &w, Piece &q) {
+  if (w.cur >= w.end) return false;
+  int4 t = p.tiles[w.tile];
+  while (w.off >= static_cast<long long>(t.z) * p.Hkv) {
+    w.off -= static_cast<long long>(t.z) * p.Hkv;
+    t = p.tiles[++w.tile];
+  }
+  q.b = t.x;
+  q.mt = t.y;
+  q.steps = t.z;
+  q.h = static_cast<int>(w.off / t.z);
+  q.u0 = static_cast<int>(w.off - static_cast<long long>(q.h) * t.z);
+  q.n = static_cast<int>(min(static_cast<long long>(t.z - q.u0), w.end - w.cur));
+  w.cur += q.n;
+  w.off += q.n;
+  return true;
+}
+
+// 16 codes to 16 bfloat16.
+template <bool E4M3>
+__device__ __forceinline__ void widen16(uint4 c, uint4 &lo, uint4 &hi) {
+  lo = make_uint4(widen2<E4M3, 0>(c.x), widen2<E4M3, 1>(c.x), widen2<E4M3, 0>(c.y), widen2<E4M3, 1>(c.y));
+  hi = make_uint4(widen2<E4M3, 0>(c.z), widen2<E4M3, 1>(c.z), widen2<E4M3, 0>(c.w), widen2<E4M3, 1>(c.w));
+}
+
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q8View p, uint32_t *err) {
+  using M = Many<D>;
+  extern __shared__ uint8_t many_raw[];
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t raw0 = smem_u32(many_raw);
+  const uint32_t sbase = (raw0 + 1023u) & ~1023u;
+  uint8_t *sm = many_raw + (sbase - raw0);
+  const uint32_t bars = sbase + M::kOffBar;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + M::kOffMisc);
+  volatile uint32_t *dead = reinterpret_cast<volatile uint32_t *>(sm + M::kOffMisc + 4);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  const int tiles = p.seq_tile[p.B];
+  // Tiles that see no token: their rows are zero.
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int4 ti = p.tiles[t];
+    if (ti.z != 0) continue;
+    const int2 qr = rows_of(p, ti.x);
+    const int r0 = ti.y * kTile, nr = min(kTile, qr.y * p.gq - r0);
+    for (int i = tid; i < nr * p.Hkv * (D / 8); i += M::kThreads) {
+      const int d = i % (D / 8), rh = i / (D / 8);
+      const int r = r0 + rh % nr, h = rh / nr;
+      const int qi = r / p.gq, head = h * p.gq + r - qi * p.gq;
+      *reinterpret_cast<uint4 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 8 * d) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const long long total = p.tprefix[tiles];
+  const int used = ranges_of(total, gridDim.x);
+  Walk w;
+  w.cur = w.first = range_start(total, used, blockIdx.x);
+  w.end = range_start(total, used, blockIdx.x + 1);
+  if (w.cur >= w.end) return;
+  w.tile = find_tile(p, tiles, w.cur);
+  w.off = w.cur - p.tprefix[w.tile];
+
+  if (tid == 0) {
+    for (int i = 0; i < M::kBars; ++i) {
+      uint32_t count = 1;
+      if ((i >= M::kKFull && i < M::kKFull + M::kSlots) || (i >= M::kVFull && i < M::kVFull + M::kSlots)) count = M::kConvWarps;
+      if (i == M::kSEmpty || i == M::kPFull || i == M::kQFull) count = 4;
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bars + 8 * i), "r"(count));
+    }
+    *dead = 0u;
+    mbar_init_fence();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
+                 "r"(static_cast<uint32_t>(M::kCols)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto bar = [&](int i) { return bars + 8 * i; };
+  Piece q;
+
+  if (warp < 4) {
+    // ---------------- softmax, one row a thread ----------------
+    reg_inc<M::kRegSoftmax>();
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+    uint32_t i = 0;  // units so far
+    bool live = true;
+    while (live && next_piece(p, w, q)) {
+      const int2 qr = rows_of(p, q.b);
+      const int rows = qr.y * p.gq;
+      const int r = q.mt * kTile + tid;
+      const bool valid = r < rows;
+      const int qi = valid ? r / p.gq : 0, head = q.h * p.gq + (valid ? r - qi * p.gq : 0);
+      // Last position the row sees; rows past the end are left unmasked (and unwritten).
+      const int lim = valid ? p.ctx[q.b] - qr.y + qi : 0x7FFFFFFF;
+      const int lim_min = __reduce_min_sync(0xFFFFFFFFu, lim);
+      const bool idle = !__any_sync(0xFFFFFFFFu, valid);
+      {  // Q into TMEM; the last piece's products are done (its sums were read)
+        const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t v[32];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 x = valid ? __ldg(reinterpret_cast<const uint4 *>(src + 64 * c + 8 * e)) : make_uint4(0, 0, 0, 0);
+            v[4 * e] = x.x;
+            v[4 * e + 1] = x.y;
+            v[4 * e + 2] = x.z;
+            v[4 * e + 3] = x.w;
+          }
+          __syncwarp();
+          tmem_st32(lanes + M::kColQ + 32 * c, v);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(M::kQFull));
+      }
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < q.n; ++j, ++i) {
+        live = bar_wait(bar(M::kInfoFull + i % kInfo), (i / kInfo) & 1u, dead, err) &&
+               bar_wait(bar(M::kSFull), i & 1u, dead, err);
+        live = __all_sync(0xFFFFFFFFu, live);
+        if (!live) break;
+        tc_fence_after();
+        float s[64];
+        if (!idle) {
+          tmem_ld32_nowait(lanes + M::kColS, reinterpret_cast<uint32_t *>(s));
+          tmem_ld32_nowait(lanes + M::kColS + 32, reinterpret_cast<uint32_t *>(s + 32));
+          tmem_wait_ld();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (!M::kShared && lane == 0) mbar_arrive(bar(M::kSEmpty));
+        if (!idle) {
+          const int t0 = (q.u0 + j) * kUnit;
+          if (t0 + kUnit - 1 > lim_min) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) s[e] = t0 + e <= lim ? s[e] : -INFINITY;
+          }
+          const float4 *info = reinterpret_cast<const float4 *>(sm + M::kOffInfo) + (i % kInfo) * 4;
+          float4 f[4];
+          float tm = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f[g] = info[g];  // scale * log2 e * ks, log2 vs, 1 / vs
+            float a = fmaxf(s[16 * g], s[16 * g + 1]), b = fmaxf(s[16 * g + 2], s[16 * g + 3]);
+#pragma unroll
+            for (int e = 4; e < 16; e += 4) {
+              a = fmaxf(a, fmaxf(s[16 * g + e], s[16 * g + e + 1]));
+              b = fmaxf(b, fmaxf(s[16 * g + e + 2], s[16 * g + e + 3]));
+            }
+            tm = fmaxf(tm, __fmaf_rn(fmaxf(a, b), f[g].x, f[g].y));
+          }
+          if (__any_sync(0xFFFFFFFFu, tm > m + kLazy)) {
+            const float mn = fmaxf(m, tm);
+            const float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
+            m = mn;
+            l *= al;
+            if (j > 0) {
+              live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err));
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld32_nowait(lanes + 32 * c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * al);
+                tmem_st32(lanes + 32 * c, v);
+              }
+              tmem_wait_st();
+            }
+          }
+          const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int g2 = 0; g2 < 2; ++g2) {
+              const int g = 2 * half + g2;
+              const float add = f[g].y - ref;
+              float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const float u0 = ex2(__fmaf_rn(s[16 * g + e], f[g].x, add));
+                const float u1 = ex2(__fmaf_rn(s[16 * g + e + 1], f[g].x, add));
+                sum0 += u0;
+                sum1 += u1;
+                // hi: the upper 16 bits of each; lo: what is left, rounded
+                const uint32_t a0 = __float_as_uint(u0), a1 = __float_as_uint(u1);
+                hi[8 * g2 + e / 2] = prmt(a0, a1, 0x7632u);
+                lo[8 * g2 + e / 2] = pack_bf16x2(u0 - __uint_as_float(a0 & 0xFFFF0000u), u1 - __uint_as_float(a1 & 0xFFFF0000u));
+              }
+              l = __fmaf_rn(sum0 + sum1, f[g].z, l);
+            }
+            if (half == 0) {  // P may be written once the last unit's P V is done
+              live = live && bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err);
+              live = __all_sync(0xFFFFFFFFu, live);
+              if (!live) break;
+              tc_fence_after();
+            }
+            tmem_st16(lanes + M::kColP + 16 * half, hi);
+            tmem_st16(lanes + M::kColP + 32 + 16 * half, lo);
+          }
+          if (!live) break;
+          tmem_wait_st();
+        } else {
+          live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err));
+          if (!live) break;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(M::kPFull));
+      }
+      if (!live) break;
+      // ---- the tile's (or the piece's) sums ----
+      live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPEmpty), (i - 1) & 1u, dead, err));
+      if (!live) break;
+      tc_fence_after();
+      const bool whole = q.u0 == 0 && q.n == q.steps;
+      const float inv = l > 0.0f ? __frcp_rn(l) : 0.0f;
+      uint16_t *dst = p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D;
+      const int slot = 2 * blockIdx.x + (w.cur - q.n == w.first ? 0 : 1);
+      float *part = p.tpart + (static_cast<size_t>(slot) * kTile + tid) * D;
+      if (!idle) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld32_nowait(lanes + 32 * c, v);
+          tmem_wait_ld();
+          if (!valid) continue;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t o[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                o[k] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * k]) * inv, __uint_as_float(v[8 * e + 2 * k + 1]) * inv);
+              *reinterpret_cast<uint4 *>(dst + 32 * c + 8 * e) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4 *>(part + 32 * c + 4 * e) =
+                  make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+        }
+        if (valid && !whole) p.tpart_ml[slot * kTile + tid] = make_float2(m, l);
+      }
+      tc_fence_before();  // the next piece's products overwrite what was read
+    }
+  } else if (warp < kConvWarp0) {
+    // ---------------- MMA issuer ----------------
+    reg_dec<M::kRegIssue>();
+    if (warp == kMmaWarp && lane == 0) {
+      uint32_t nk = 0, nv = 0, pieces = 0;  // units whose Q K^T / P V were issued
+      bool live = true;
+      auto pv = [&](bool accumulate) {
+        const uint32_t slot = nv % M::kSlots;
+        live = bar_wait(bar(M::kVFull + slot), (nv / M::kSlots) & 1u, dead, err) &&
+               bar_wait(bar(M::kPFull), nv & 1u, dead, err);
+        if (!live) return;
+        tc_fence_after();
+        const uint64_t vd = sw128_mn_desc(sbase + M::kOffV + slot * M::kSlotBytes);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ts(tmem, tmem + M::kColP + 32 * half + 8 * kk, vd + 128 * kk, idesc(D, true),
+                    accumulate || half + kk > 0 ? 1u : 0u);
+        umma_commit(bar(M::kVEmpty + slot));
+        umma_commit(bar(M::kPEmpty));
+        ++nv;
+      };
+      while (live && next_piece(p, w, q)) {
+        live = bar_wait(bar(M::kQFull), pieces & 1u, dead, err);
+        ++pieces;
+        for (int j = 0; live && j < q.n; ++j) {
+          const uint32_t slot = nk % M::kSlots;
+          // S free: read by the softmax, or (shared columns) P consumed by P V
+          live = bar_wait(bar(M::kShared ? M::kPEmpty : M::kSEmpty), (nk & 1u) ^ 1u, dead, err) &&
+                 bar_wait(bar(M::kKFull + slot), (nk / M::kSlots) & 1u, dead, err);
+          if (!live) break;
+          tc_fence_after();
+          const uint64_t kd = sw128_desc(sbase + slot * M::kSlotBytes);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_ts(tmem + M::kColS, tmem + M::kColQ + 8 * kk, kd + 512 * (kk / 4) + 2 * (kk % 4), idesc(64, false),
+                    kk > 0 ? 1u : 0u);
+          umma_commit(bar(M::kKEmpty + slot));
+          umma_commit(bar(M::kSFull));
+          ++nk;
+          if (M::kShared)
+            pv(j > 0);
+          else if (j > 0)
+            pv(j > 1);
+        }
+        if (!M::kShared && live) pv(q.n > 1);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- codes to shared memory ----------------
+    if constexpr (M::kRegConv < 128) reg_dec<M::kRegConv>();
+    constexpr int kPer = D / 16;                           // 16-code chunks of a row
+    constexpr int kRowsPass = 32 * M::kConvWarps / kPer;  // rows of a pass: 16 or 32
+    constexpr int kPasses = kUnit / kRowsPass;
+    const int ct = tid - 32 * kConvWarp0;
+    const int row0 = ct / kPer, c16 = ct % kPer;
+    const int bpp = p.page >> p.block_shift;
+    uint32_t i = 0;
+    bool live = true;
+    while (live && next_piece(p, w, q)) {
+      const int ctx = tokens_of(p, q.b);
+      const int32_t *trow = p.table + static_cast<size_t>(q.b) * p.width;
+      const int last = q.u0 + q.n;
+      int pg[kPasses];       // page of each pass's token, one unit ahead of the codes
+      uint4 ck[kPasses], cv[kPasses];
+      float ks = 0.0f, vs = 0.0f;  // lanes 0-3 of the first warp: scales of a granule
+      int info_pg = -1;
+      auto fetch_pages = [&](int u) {
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int t = u * kUnit + k * kRowsPass + row0;
+          pg[k] = u < last && t < ctx ? trow[page_col(p, t)] : -1;
+        }
+        const int t = u * kUnit + 16 * lane;
+        if (ct < 4) info_pg = u < last && t < ctx ? trow[page_col(p, t)] : -1;
+      };
+      auto fetch = [&](int u, const uint8_t *codes, uint4 (&c)[kPasses]) {
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          c[k] = make_uint4(0, 0, 0, 0);  // tokens past the context or without a page: zero codes
+          if (pg[k] >= 0 && pg[k] < p.pages) {
+            const int t = u * kUnit + k * kRowsPass + row0;
+            const size_t row = static_cast<size_t>(pg[k]) * p.page + (t - page_col(p, t) * p.page);
+            c[k] = ldg_stream(codes + (row * p.Hkv + q.h) * D + 16 * c16);
+          }
+        }
+      };
+      auto fetch_scales = [&](int u) {
+        if (ct >= 4) return;
+        ks = 0.0f;
+        vs = -1.0f;
+        if (info_pg >= 0 && info_pg < p.pages) {
+          const int t = u * kUnit + 16 * lane;
+          const size_t at = (static_cast<size_t>(info_pg) * bpp + ((t - page_col(p, t) * p.page) >> p.block_shift)) * p.Hkv + q.h;
+          ks = __ldg(p.ks + at);
+          vs = fmaxf(__ldg(p.vs + at), 0x1p-110f);
+        }
+      };
+      fetch_pages(q.u0);
+      fetch(q.u0, p.kc, ck);
+      fetch(q.u0, p.vc, cv);
+      fetch_scales(q.u0);
+      fetch_pages(q.u0 + 1);
+      for (int u = q.u0; u < last; ++u, ++i) {
+        const uint32_t slot = i % M::kSlots, ph = (i / M::kSlots) & 1u;
+        auto store = [&](uint32_t tile, const uint4 (&c)[kPasses]) {
+#pragma unroll
+          for (int k = 0; k < kPasses; ++k) {
+            const int n = k * kRowsPass + row0;
+            uint4 a, b;
+            widen16<E4M3>(c[k], a, b);
+            const uint32_t row = tile + (c16 >> 2) * 8192 + n * 128;
+            const int j = 2 * (c16 & 3);
+            const uint32_t sa = row + (((j) ^ (n & 7)) << 4), sb = row + (((j + 1) ^ (n & 7)) << 4);
+            // lanes of odd 64-value groups store their second half first: all eight bank groups are hit
+            const bool odd = (c16 >> 2) & 1;
+            sts128(odd ? sb : sa, odd ? b : a);
+            sts128(odd ? sa : sb, odd ? a : b);
+          }
+        };
+        live = bar_wait(bar(M::kKEmpty + slot), ph ^ 1u, dead, err);
+        live = __all_sync(0xFFFFFFFFu, live);
+        if (!live) break;
+        store(sbase + slot * M::kSlotBytes, ck);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(M::kKFull + slot));
+        if (u + 1 < last) fetch(u + 1, p.kc, ck);
+        if (warp == kConvWarp0) {
+          if (lane < 4) {
+            const bool ok = vs > 0.0f;
+            reinterpret_cast<float4 *>(sm + M::kOffInfo)[(i % kInfo) * 4 + lane] =
+                make_float4(fmaxf(p.scale * kLog2e * ks, 1e-37f), ok ? __log2f(vs) : -INFINITY, ok ? __frcp_rn(vs) : 0.0f, 0.0f);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(M::kInfoFull + i % kInfo));
+          if (u + 1 < last) fetch_scales(u + 1);
+        }
+        live = bar_wait(bar(M::kVEmpty + slot), ph ^ 1u, dead, err);
+        live = __all_sync(0xFFFFFFFFu, live);
+        if (!live) break;
+        store(sbase + M::kOffV + slot * M::kSlotBytes, cv);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(M::kVFull + slot));
+        if (u + 1 < last) {
+          fetch(u + 1, p.vc, cv);
+          fetch_pages(u + 2);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
+                 "r"(static_cast<uint32_t>(M::kCols)));
+}
+
+// Joins the tiles that several CTAs worked on.  BY_CUT: one CTA per (cut, 8
+// rows), at the first cut inside a segment -- for calls with more segments
+// than cuts; otherwise one CTA per (tile, kv head, row).
+template <int D, bool BY_CUT>
+__global__ void __launch_bounds__(256) k_q8_many_join(Q8View p, int ctas) {
+  pdl_wait();
+  const int tiles = p.seq_tile[p.B];
+  const long long total = p.tprefix[tiles];
+  const int used = ranges_of(total, ctas);
+  int tile, h, row0;
+  long long a, unit = -1;
+  int cut = 0;
+  if (BY_CUT) {
+    cut = (blockIdx.x >> 4) + 1;
+    row0 = (blockIdx.x & 15) * 8;
+    if (cut >= used) return;
+    unit = range_start(total, used, cut);
+    tile = find_tile(p, tiles, unit);
+    h = static_cast<int>((unit - p.tprefix[tile]) / p.tiles[tile].z);
+  } else {
+    row0 = blockIdx.x & 127;
+    const int seg = blockIdx.x >> 7;
+    tile = seg / p.Hkv;
+    h = seg - tile * p.Hkv;
+    if (tile >= tiles) return;
+  }
+  const int4 ti = p.tiles[tile];
+  if (ti.z == 0) return;
+  a = p.tprefix[tile] + static_cast<long long>(h) * ti.z;
+  if (a == unit) return;
+  const int c0 = owner_of(a, total, used), c1 = owner_of(a + ti.z - 1, total, used);
+  if (c0 == c1 || (BY_CUT && c0 != cut - 1)) return;
+  const int2 qr = rows_of(p, ti.x);
+  const bool late0 = range_start(total, used, c0) < a;
+  for (int r = row0; r < row0 + (BY_CUT ? 8 : 1); ++r) {
+    const int rr = ti.y * kTile + r;
+    if (rr >= qr.y * p.gq) return;
+    const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
+    if (BY_CUT && r > row0) __syncthreads();  // join_row's shared arrays
+    join_row<D, kTile>(p.tpart, p.tpart_ml, c0, c1, late0, r, p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D);
+  }
+}
+
+template <int D, bool E4M3>
+cudaError_t launch(const Q8View &p, cudaStream_t s) {
+  using M = Many<D>;
+  // Set for every call: the attribute belongs to the current device.
+  cudaError_t e = cudaFuncSetAttribute(k_q8_many<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
+  if (e != cudaSuccess) return e;
+  k_q8_tiles<<<1, kScanThreads, 0, s>>>(p);
+  e = launch_pdl(k_q8_many<D, E4M3>, dim3(M::kMax), dim3(M::kThreads), M::kSmem, s, p, device_error_word());
+  if (e != cudaSuccess) return e;
+  const uint64_t segs = many_tiles(p) * p.Hkv;
+  if (segs <= 32)
+    return launch_pdl(k_q8_many_join<D, false>, dim3(static_cast<unsigned>(segs * kTile)), dim3(256), 0, s, p, +M::kMax);
+  return launch_pdl(k_q8_many_join<D, true>, dim3((M::kMax - 1) * 16), dim3(256), 0, s, p, +M::kMax);
+}
+
+}  // namespace
+
+int many_ctas(int head_dim) { return head_dim == 256 ? Many<256>::kMax : Many<128>::kMax; }
+
+uint64_t many_tiles(const Q8View &p) {
+  const uint64_t pairs = static_cast<uint64_t>(p.rows) * p.gq;
+  // a full tile per 128 pairs, a partial one per sequence that can be here
+  return pairs / kTile + std::min<uint64_t>(p.B, pairs / (p.few_rows + 1) + 1);
+}
+
+cudaError_t launch_many(const Q8View &p, int head_dim, bool e4m3, cudaStream_t s) {
+  switch (head_dim) {
+    case 64: return e4m3 ? launch<64, true>(p, s) : launch<64, false>(p, s);
+    case 128: return e4m3 ? launch<128, true>(p, s) : launch<128, false>(p, s);
+    default: return e4m3 ? launch<256, true>(p, s) : launch<256, false>(p, s);
+  }
+}
+
+}  // namespace fnmoe
