@@ -53,7 +53,7 @@ struct Q8View {
   int *seq_tile;        // [B + 1] tiles before each sequence
   int4 *tiles;          // [tiles] {sequence, tile of it, units of one kv head, 0}
   long long *tprefix;   // [tiles + 1] units of work before each tile
-  float *tpart;         // [2 * CTAs][128][D]
+  float *tpart;         // [2 * CTAs][D / 4][128][4]
   float2 *tpart_ml;     // [2 * CTAs][128]
 };
 
@@ -76,6 +76,22 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
+}
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n"
+      : "=l"(d)
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+        "l"(reinterpret_cast<unsigned long long &>(c)));
+  return reinterpret_cast<float2 &>(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;\n"
+      : "=l"(d)
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+  return reinterpret_cast<float2 &>(d);
 }
 // a and b as bfloat16 pairs hi + lo.
 __device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t &hi, uint32_t &lo) {

@@ -14,15 +14,18 @@
 // operands, S and O as TMEM accumulators: 6 D * 128 * 64 multiply-adds where
 // the formula has 4, which bounds the kernel (1,536 clocks a unit at D 256).
 // Roles:
-//   warps 0-3   softmax, one row a thread: S from TMEM, running reference and
-//               sum, P back to TMEM; Q in and the result out of TMEM;
-//   warp 4      issues the MMAs;
-//   warps 8-..  read K and V codes (16 bytes a thread) one unit ahead in
+//   softmax     a row a thread (at D 256 two threads, 32 tokens each, which
+//               exchange their maxima through shared memory): S from TMEM,
+//               running reference and sum, P back to TMEM; Q in and the
+//               result out of TMEM, through a shared-memory stage that turns
+//               row-a-thread into coalesced 64-byte pieces;
+//   one warp    issues the MMAs;
+//   codes       read K and V codes (16 bytes a thread) one unit ahead in
 //               registers, widen them to bfloat16 and store them to shared
 //               memory as 128B-swizzled tiles, [D / 64][64 tokens][128 bytes]:
 //               K-major for K, MN-major for V.
-// The warpgroups trade registers (setmaxnreg): a softmax thread holds a row of
-// S, the issuer next to nothing.
+// The warpgroups trade registers (setmaxnreg): a softmax thread holds its part
+// of a row of S, the issuer next to nothing.
 // Widening in the kernel reads a byte a value from L2 where a widened copy
 // would write and re-read two.
 // TMEM columns at D 256: O 0-255, Q 256-383, S 384-447, P 448-511, so the next
@@ -46,7 +49,6 @@ namespace fnmoe {
 namespace {
 
 constexpr int kTile = 128;
-constexpr int kMmaWarp = 4, kConvWarp0 = 8;  // warps 5-7 only fill the MMA issuer's warpgroup
 constexpr int kInfo = 8;  // units whose scales are kept
 constexpr uint32_t kSpin = 1u << 22;
 
@@ -59,10 +61,16 @@ template <int D>
 struct Many {
   static constexpr bool kShared = D < 256;  // P takes S's columns
   static constexpr int kCtas = D < 256 ? 2 : 1;  // per SM
+  static constexpr int kHalves = D < 256 ? 1 : 2;  // softmax threads a row
+  static constexpr int kSoftWarps = 4 * kHalves;
+  static constexpr int kMmaWarp = kSoftWarps;       // the three warps after it only fill its warpgroup
+  static constexpr int kConvWarp0 = kMmaWarp + 4;
   static constexpr int kConvWarps = D < 256 ? 4 : 8;
   static constexpr int kThreads = 32 * (kConvWarp0 + kConvWarps);
-  // Registers a thread: at launch 512 x 128 or 384 x 80; the shares add up to as many.
-  static constexpr int kRegSoftmax = D < 256 ? 136 : 208, kRegIssue = D < 256 ? 40 : 48, kRegConv = D < 256 ? 64 : 128;
+  // Registers a thread: at launch 640 x 96 or 384 x 80; the shares add up to as many.
+  static constexpr int kRegLaunch = D < 256 ? 80 : 96;
+  static constexpr int kRegSoftmax = D < 256 ? 136 : 120, kRegIssue = D < 256 ? 40 : 48, kRegConv = D < 256 ? 64 : 96;
+  static_assert(kHalves * kRegSoftmax + kRegIssue + kConvWarps / 4 * kRegConv <= kThreads / 128 * kRegLaunch, "registers");
   static constexpr int kSlots = 3;               // tiles of K and of V in shared memory
   static constexpr int kSlotBytes = 64 * D * 2;
   static constexpr int kCols = D < 256 ? 256 : 512;
@@ -72,10 +80,12 @@ struct Many {
   // barriers
   static constexpr int kKFull = 0, kKEmpty = kKFull + kSlots, kVFull = kKEmpty + kSlots, kVEmpty = kVFull + kSlots,
                        kSFull = kVEmpty + kSlots, kSEmpty = kSFull + 1, kPFull = kSEmpty + 1, kPEmpty = kPFull + 1,
-                       kQFull = kPEmpty + 1, kInfoFull = kQFull + 1, kBars = kInfoFull + kInfo;
+                       kQFull = kPEmpty + 1, kPair = kQFull + 1, kInfoFull = kPair + 4, kBars = kInfoFull + kInfo;
   static constexpr int kOffV = kSlots * kSlotBytes;
   static constexpr int kOffInfo = 2 * kSlots * kSlotBytes;  // float4 [kInfo][4]
-  static constexpr int kOffBar = kOffInfo + kInfo * 64;
+  static constexpr int kOffMax = kOffInfo + kInfo * 64;      // float [2][2][128]: the halves' maxima, sums
+  static constexpr int kOffStage = kOffMax + 2048;           // 32 rows x 64 bytes a softmax warp
+  static constexpr int kOffBar = kOffStage + 2048 * kSoftWarps;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;      // TMEM base, dead flag
   static constexpr int kSmem = kOffMisc + 16 + 1024;        // + slack for the 1024-byte alignment of the tiles
   static constexpr int kMax = 148 * kCtas;
@@ -100,6 +110,11 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(desc), "r"(accumulate)
       : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+  return ok != 0;
 }
 __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t *v) {
   asm volatile(
@@ -155,6 +170,12 @@ __device__ __forceinline__ int tiles_of(const Q8View &p, int b) {
   const int rows = rows_of(p, b).y * p.gq;
   return rows > p.few_rows ? (rows + kTile - 1) / kTile : 0;
 }
+
+// Beginning and ending a tile costs about as much as kCost units (queries in,
+// results out, the pipeline's start), which the ranges count: a tile and kv
+// head of n units weighs n + kCost, and its real units are the last n of
+// those.
+constexpr int kCost = 3;
 
 constexpr int kScanThreads = 1024;
 
@@ -216,7 +237,7 @@ __global__ void __launch_bounds__(kScanThreads) k_q8_tiles(Q8View p) {
       const int seen = max(0, min(p.ctx[lo] - n + last + 1, p.width * p.page));
       const int steps = (seen + kUnit - 1) / kUnit;
       p.tiles[t] = make_int4(lo, mt, steps, 0);
-      units = static_cast<long long>(steps) * p.Hkv;
+      units = steps > 0 ? static_cast<long long>(steps + kCost) * p.Hkv : 0;
     }
     const long long s = scan1(units, carry, red);
     if (t < tiles) p.tprefix[t] = s - units;
@@ -239,30 +260,38 @@ __device__ __forceinline__ int find_tile(const Q8View &p, int tiles, long long u
   return lo;
 }
 
-// A piece of work: units [u0, u0 + n) of tile `tile` and kv head h.
+// A piece of work: units [u0, u0 + n) of a tile and kv head h.
 struct Piece {
   int b, mt, h, u0, n, steps;
+  bool first;  // of the CTA's range
 };
 struct Walk {
   long long cur, end, off, first;
   int tile;
 };
 __device__ __forceinline__ bool next_piece(const Q8View &p, Walk &w, Piece &q) {
-  if (w.cur >= w.end) return false;
-  int4 t = p.tiles[w.tile];
-  while (w.off >= static_cast<long long>(t.z) * p.Hkv) {
-    w.off -= static_cast<long long>(t.z) * p.Hkv;
-    t = p.tiles[++w.tile];
+  while (w.cur < w.end) {
+    int4 t = p.tiles[w.tile];
+    long long seg = t.z > 0 ? t.z + kCost : 0;
+    while (w.off >= seg * p.Hkv) {
+      w.off -= seg * p.Hkv;
+      t = p.tiles[++w.tile];
+      seg = t.z > 0 ? t.z + kCost : 0;
+    }
+    q.b = t.x;
+    q.mt = t.y;
+    q.steps = t.z;
+    q.h = static_cast<int>(w.off / seg);
+    const int v0 = static_cast<int>(w.off - q.h * seg);
+    const int n = static_cast<int>(min(seg - v0, w.end - w.cur));
+    q.u0 = max(v0 - kCost, 0);
+    q.n = max(v0 + n - kCost, 0) - q.u0;
+    q.first = w.cur == w.first;
+    w.cur += n;
+    w.off += n;
+    if (q.n > 0) return true;  // else the range ends in the tile's overhead
   }
-  q.b = t.x;
-  q.mt = t.y;
-  q.steps = t.z;
-  q.h = static_cast<int>(w.off / t.z);
-  q.u0 = static_cast<int>(w.off - static_cast<long long>(q.h) * t.z);
-  q.n = static_cast<int>(min(static_cast<long long>(t.z - q.u0), w.end - w.cur));
-  w.cur += q.n;
-  w.off += q.n;
-  return true;
+  return false;
 }
 
 // 16 codes to 16 bfloat16.
@@ -313,13 +342,14 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
     for (int i = 0; i < M::kBars; ++i) {
       uint32_t count = 1;
       if ((i >= M::kKFull && i < M::kKFull + M::kSlots) || (i >= M::kVFull && i < M::kVFull + M::kSlots)) count = M::kConvWarps;
-      if (i == M::kSEmpty || i == M::kPFull || i == M::kQFull) count = 4;
+      if (i == M::kSEmpty || i == M::kPFull || i == M::kQFull) count = M::kSoftWarps;
+      if (i >= M::kPair && i < M::kPair + 4) count = 2;
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bars + 8 * i), "r"(count));
     }
     *dead = 0u;
     mbar_init_fence();
   }
-  if (warp == kMmaWarp) {
+  if (warp == M::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
                  "r"(static_cast<uint32_t>(M::kCols)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -331,37 +361,79 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
   auto bar = [&](int i) { return bars + 8 * i; };
   Piece q;
 
-  if (warp < 4) {
-    // ---------------- softmax, one row a thread ----------------
+  if (warp < M::kSoftWarps) {
+    // ---------------- softmax: a row and kTok tokens of each unit a thread ----------------
     reg_inc<M::kRegSoftmax>();
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * warp) << 16);
-    uint32_t i = 0;  // units so far
+    constexpr int kTok = kUnit / M::kHalves;  // tokens of this thread
+    constexpr int kDims = D / M::kHalves;     // dims of Q and O that it moves
+    const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    const uint32_t stage = sbase + M::kOffStage + 2048 * warp;
+    // This thread's 16-byte chunk c of its own row in the stage, and the chunk
+    // of row 8 e + lane / 4 that it moves to or from global memory.
+    auto own = [&](int c) { return stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4); };
+    auto other = [&](int e) {
+      const int r = 8 * e + (lane >> 2);
+      return stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4);
+    };
+    // The other half's value for this row; buffers alternate, so that one is
+    // rewritten only after both halves have read it.
+    uint32_t exchanges = 0;
     bool live = true;
+    auto swap = [&](float mine) {
+      volatile float *sx = reinterpret_cast<volatile float *>(sm + M::kOffMax) + (exchanges & 1u) * 256;
+      sx[half * 128 + row] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(M::kPair + quarter));
+      live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPair + quarter), exchanges & 1u, dead, err));
+      ++exchanges;
+      return sx[(half ^ 1) * 128 + row];
+    };
+    uint32_t i = 0;  // units so far
     while (live && next_piece(p, w, q)) {
       const int2 qr = rows_of(p, q.b);
       const int rows = qr.y * p.gq;
-      const int r = q.mt * kTile + tid;
+      const int r = q.mt * kTile + row;
       const bool valid = r < rows;
       const int qi = valid ? r / p.gq : 0, head = q.h * p.gq + (valid ? r - qi * p.gq : 0);
       // Last position the row sees; rows past the end are left unmasked (and unwritten).
       const int lim = valid ? p.ctx[q.b] - qr.y + qi : 0x7FFFFFFF;
       const int lim_min = __reduce_min_sync(0xFFFFFFFFu, lim);
       const bool idle = !__any_sync(0xFFFFFFFFu, valid);
+      // Rows of the warp that this thread moves: row 8 e + lane / 4.
+      long long q_at[4], o_at[4];
+      {
+        const long long qa = valid ? static_cast<long long>(static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D) : -1;
+        const long long oa = (static_cast<long long>(qr.x + qi) * p.Hq + head) * D;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          q_at[e] = __shfl_sync(0xFFFFFFFFu, qa, 8 * e + (lane >> 2));
+          o_at[e] = __shfl_sync(0xFFFFFFFFu, oa, 8 * e + (lane >> 2));
+          if (q_at[e] < 0) o_at[e] = -1;
+        }
+      }
       {  // Q into TMEM; the last piece's products are done (its sums were read)
-        const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D;
+        const int c0 = half * kDims + 8 * (lane & 3);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t v[32];
+        for (int c = 0; c < kDims / 32; ++c) {
+          uint4 x[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint4 x = valid ? __ldg(reinterpret_cast<const uint4 *>(src + 64 * c + 8 * e)) : make_uint4(0, 0, 0, 0);
-            v[4 * e] = x.x;
-            v[4 * e + 1] = x.y;
-            v[4 * e + 2] = x.z;
-            v[4 * e + 3] = x.w;
-          }
+          for (int e = 0; e < 4; ++e)
+            x[e] = q_at[e] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.q + q_at[e] + c0 + 32 * c)) : make_uint4(0, 0, 0, 0);
           __syncwarp();
-          tmem_st32(lanes + M::kColQ + 32 * c, v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sts128(other(e), x[e]);
+          __syncwarp();
+          uint32_t v[16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint4 y = lds128(own(e));
+            v[4 * e] = y.x;
+            v[4 * e + 1] = y.y;
+            v[4 * e + 2] = y.z;
+            v[4 * e + 3] = y.w;
+          }
+          tmem_st16(lanes + M::kColQ + (half * kDims) / 2 + 16 * c, v);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -375,34 +447,40 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         live = __all_sync(0xFFFFFFFFu, live);
         if (!live) break;
         tc_fence_after();
-        float s[64];
+        float s[kTok];
         if (!idle) {
-          tmem_ld32_nowait(lanes + M::kColS, reinterpret_cast<uint32_t *>(s));
-          tmem_ld32_nowait(lanes + M::kColS + 32, reinterpret_cast<uint32_t *>(s + 32));
+#pragma unroll
+          for (int c = 0; c < kTok / 32; ++c)
+            tmem_ld32_nowait(lanes + M::kColS + half * kTok + 32 * c, reinterpret_cast<uint32_t *>(s + 32 * c));
           tmem_wait_ld();
         }
         tc_fence_before();
         __syncwarp();
         if (!M::kShared && lane == 0) mbar_arrive(bar(M::kSEmpty));
         if (!idle) {
-          const int t0 = (q.u0 + j) * kUnit;
-          if (t0 + kUnit - 1 > lim_min) {
+          const int t0 = (q.u0 + j) * kUnit + half * kTok;
+          if (t0 + kTok - 1 > lim_min) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e) s[e] = t0 + e <= lim ? s[e] : -INFINITY;
+            for (int e = 0; e < kTok; ++e) s[e] = t0 + e <= lim ? s[e] : -INFINITY;
           }
-          const float4 *info = reinterpret_cast<const float4 *>(sm + M::kOffInfo) + (i % kInfo) * 4;
-          float4 f[4];
+          const float4 *info = reinterpret_cast<const float4 *>(sm + M::kOffInfo) + (i % kInfo) * 4 + half * (kTok / 16);
+          float4 f[kTok / 16];
           float tm = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < kTok / 16; ++g) {
             f[g] = info[g];  // scale * log2 e * ks, log2 vs, 1 / vs
-            float a = fmaxf(s[16 * g], s[16 * g + 1]), b = fmaxf(s[16 * g + 2], s[16 * g + 3]);
+            float a = s[16 * g], b = s[16 * g + 1];
 #pragma unroll
-            for (int e = 4; e < 16; e += 4) {
-              a = fmaxf(a, fmaxf(s[16 * g + e], s[16 * g + e + 1]));
-              b = fmaxf(b, fmaxf(s[16 * g + e + 2], s[16 * g + e + 3]));
+            for (int e = 2; e < 16; e += 2) {
+              a = fmaxf(a, s[16 * g + e]);
+              b = fmaxf(b, s[16 * g + e + 1]);
             }
             tm = fmaxf(tm, __fmaf_rn(fmaxf(a, b), f[g].x, f[g].y));
+          }
+          if (M::kHalves == 2) {
+            const float o = swap(tm);
+            if (!live) break;
+            tm = fmaxf(tm, o);
           }
           if (__any_sync(0xFFFFFFFFu, tm > m + kLazy)) {
             const float mn = fmaxf(m, tm);
@@ -413,47 +491,48 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
               live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err));
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
+              for (int c = 0; c < kDims / 32; ++c) {
                 uint32_t v[32];
-                tmem_ld32_nowait(lanes + 32 * c, v);
+                tmem_ld32_nowait(lanes + half * kDims + 32 * c, v);
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * al);
-                tmem_st32(lanes + 32 * c, v);
+                tmem_st32(lanes + half * kDims + 32 * c, v);
               }
               tmem_wait_st();
             }
           }
           const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int h2 = 0; h2 < kTok / 32; ++h2) {
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int g2 = 0; g2 < 2; ++g2) {
-              const int g = 2 * half + g2;
-              const float add = f[g].y - ref;
-              float sum0 = 0.0f, sum1 = 0.0f;
+              const int g = 2 * h2 + g2;
+              const float2 mul = make_float2(f[g].x, f[g].x), add = make_float2(f[g].y - ref, f[g].y - ref);
+              float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                const float u0 = ex2(__fmaf_rn(s[16 * g + e], f[g].x, add));
-                const float u1 = ex2(__fmaf_rn(s[16 * g + e + 1], f[g].x, add));
-                sum0 += u0;
-                sum1 += u1;
+                const float2 x = fma2(make_float2(s[16 * g + e], s[16 * g + e + 1]), mul, add);
+                const float2 u = make_float2(ex2(x.x), ex2(x.y));
+                sum = add2(sum, u);
                 // hi: the upper 16 bits of each; lo: what is left, rounded
-                const uint32_t a0 = __float_as_uint(u0), a1 = __float_as_uint(u1);
+                const uint32_t a0 = __float_as_uint(u.x), a1 = __float_as_uint(u.y);
                 hi[8 * g2 + e / 2] = prmt(a0, a1, 0x7632u);
-                lo[8 * g2 + e / 2] = pack_bf16x2(u0 - __uint_as_float(a0 & 0xFFFF0000u), u1 - __uint_as_float(a1 & 0xFFFF0000u));
+                const float2 left = add2(u, make_float2(__uint_as_float((a0 & 0xFFFF0000u) ^ 0x80000000u),
+                                                        __uint_as_float((a1 & 0xFFFF0000u) ^ 0x80000000u)));
+                lo[8 * g2 + e / 2] = pack_bf16x2(left.x, left.y);
               }
-              l = __fmaf_rn(sum0 + sum1, f[g].z, l);
+              l = __fmaf_rn(sum.x + sum.y, f[g].z, l);
             }
-            if (half == 0) {  // P may be written once the last unit's P V is done
+            if (h2 == 0) {  // P may be written once the last unit's P V is done
               live = live && bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err);
               live = __all_sync(0xFFFFFFFFu, live);
               if (!live) break;
               tc_fence_after();
             }
-            tmem_st16(lanes + M::kColP + 16 * half, hi);
-            tmem_st16(lanes + M::kColP + 32 + 16 * half, lo);
+            tmem_st16(lanes + M::kColP + 16 * (half + h2), hi);
+            tmem_st16(lanes + M::kColP + 32 + 16 * (half + h2), lo);
           }
           if (!live) break;
           tmem_wait_st();
@@ -470,19 +549,23 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
       live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPEmpty), (i - 1) & 1u, dead, err));
       if (!live) break;
       tc_fence_after();
-      const bool whole = q.u0 == 0 && q.n == q.steps;
-      const float inv = l > 0.0f ? __frcp_rn(l) : 0.0f;
-      uint16_t *dst = p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D;
-      const int slot = 2 * blockIdx.x + (w.cur - q.n == w.first ? 0 : 1);
-      float *part = p.tpart + (static_cast<size_t>(slot) * kTile + tid) * D;
       if (!idle) {
+        if (M::kHalves == 2) {
+          const float o = swap(l);
+          if (!live) break;
+          l += o;
+        }
+        const bool whole = q.u0 == 0 && q.n == q.steps;
+        const float inv = l > 0.0f ? __frcp_rn(l) : 0.0f;
+        const int slot = 2 * blockIdx.x + (q.first ? 0 : 1);
+        // cut tiles: float4 d of row r at [d][r], so that a warp's stores are contiguous
+        float4 *part = reinterpret_cast<float4 *>(p.tpart) + (static_cast<size_t>(slot) * (D / 4) + half * (kDims / 4)) * kTile + row;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < kDims / 32; ++c) {
           uint32_t v[32];
           __syncwarp();
-          tmem_ld32_nowait(lanes + 32 * c, v);
+          tmem_ld32_nowait(lanes + half * kDims + 32 * c, v);
           tmem_wait_ld();
-          if (!valid) continue;
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -490,141 +573,169 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 o[k] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * k]) * inv, __uint_as_float(v[8 * e + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4 *>(dst + 32 * c + 8 * e) = make_uint4(o[0], o[1], o[2], o[3]);
+              sts128(own(e), make_uint4(o[0], o[1], o[2], o[3]));
             }
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (o_at[e] >= 0)
+                *reinterpret_cast<uint4 *>(p.out + o_at[e] + half * kDims + 32 * c + 8 * (lane & 3)) = lds128(other(e));
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4 *>(part + 32 * c + 4 * e) =
-                  make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+              part[(8 * c + e) * kTile] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                                      __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
           }
         }
-        if (valid && !whole) p.tpart_ml[slot * kTile + tid] = make_float2(m, l);
+        if (!whole && half == 0) p.tpart_ml[slot * kTile + row] = make_float2(m, l);
       }
       tc_fence_before();  // the next piece's products overwrite what was read
+      __syncwarp();
     }
-  } else if (warp < kConvWarp0) {
+  } else if (warp < M::kConvWarp0) {
     // ---------------- MMA issuer ----------------
     reg_dec<M::kRegIssue>();
-    if (warp == kMmaWarp && lane == 0) {
+    if (warp == M::kMmaWarp) {
+      // The whole warp walks the units (so that descriptors stay in uniform
+      // registers); one elected lane issues.
       uint32_t nk = 0, nv = 0, pieces = 0;  // units whose Q K^T / P V were issued
+      uint32_t kslot = 0, kph = 0, vslot = 0, vph = 0;
       bool live = true;
+      const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+      auto wait = [&](int i, uint32_t parity) { return __all_sync(0xFFFFFFFFu, bar_wait(bar(i), parity, dead, err)) != 0; };
       auto pv = [&](bool accumulate) {
-        const uint32_t slot = nv % M::kSlots;
-        live = bar_wait(bar(M::kVFull + slot), (nv / M::kSlots) & 1u, dead, err) &&
-               bar_wait(bar(M::kPFull), nv & 1u, dead, err);
+        live = wait(M::kVFull + vslot, vph) && wait(M::kPFull, nv & 1u);
         if (!live) return;
         tc_fence_after();
-        const uint64_t vd = sw128_mn_desc(sbase + M::kOffV + slot * M::kSlotBytes);
+        const uint64_t vd = sw128_mn_desc(sbase + M::kOffV + vslot * M::kSlotBytes);
+        if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_ts(tmem, tmem + M::kColP + 32 * half + 8 * kk, vd + 128 * kk, idesc(D, true),
-                    accumulate || half + kk > 0 ? 1u : 0u);
-        umma_commit(bar(M::kVEmpty + slot));
-        umma_commit(bar(M::kPEmpty));
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ts(tm, tm + M::kColP + 32 * half + 8 * kk, vd + 128 * kk, idesc(D, true),
+                      accumulate || half + kk > 0 ? 1u : 0u);
+          umma_commit(bar(M::kVEmpty + vslot));
+          umma_commit(bar(M::kPEmpty));
+        }
+        __syncwarp();
         ++nv;
+        if (++vslot == M::kSlots) {
+          vslot = 0;
+          vph ^= 1u;
+        }
       };
       while (live && next_piece(p, w, q)) {
-        live = bar_wait(bar(M::kQFull), pieces & 1u, dead, err);
+        const int n = __shfl_sync(0xFFFFFFFFu, q.n, 0);
+        live = wait(M::kQFull, pieces & 1u);
         ++pieces;
-        for (int j = 0; live && j < q.n; ++j) {
-          const uint32_t slot = nk % M::kSlots;
+        for (int j = 0; live && j < n; ++j) {
           // S free: read by the softmax, or (shared columns) P consumed by P V
-          live = bar_wait(bar(M::kShared ? M::kPEmpty : M::kSEmpty), (nk & 1u) ^ 1u, dead, err) &&
-                 bar_wait(bar(M::kKFull + slot), (nk / M::kSlots) & 1u, dead, err);
+          live = wait(M::kShared ? M::kPEmpty : M::kSEmpty, (nk & 1u) ^ 1u) && wait(M::kKFull + kslot, kph);
           if (!live) break;
           tc_fence_after();
-          const uint64_t kd = sw128_desc(sbase + slot * M::kSlotBytes);
+          const uint64_t kd = sw128_desc(sbase + kslot * M::kSlotBytes);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_ts(tmem + M::kColS, tmem + M::kColQ + 8 * kk, kd + 512 * (kk / 4) + 2 * (kk % 4), idesc(64, false),
-                    kk > 0 ? 1u : 0u);
-          umma_commit(bar(M::kKEmpty + slot));
-          umma_commit(bar(M::kSFull));
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_ts(tm + M::kColS, tm + M::kColQ + 8 * kk, kd + 512 * (kk / 4) + 2 * (kk % 4), idesc(64, false),
+                      kk > 0 ? 1u : 0u);
+            umma_commit(bar(M::kKEmpty + kslot));
+            umma_commit(bar(M::kSFull));
+          }
+          __syncwarp();
           ++nk;
+          if (++kslot == M::kSlots) {
+            kslot = 0;
+            kph ^= 1u;
+          }
           if (M::kShared)
             pv(j > 0);
           else if (j > 0)
             pv(j > 1);
         }
-        if (!M::kShared && live) pv(q.n > 1);
+        if (!M::kShared && live) pv(n > 1);
       }
     }
     __syncwarp();
   } else {
     // ---------------- codes to shared memory ----------------
-    if constexpr (M::kRegConv < 128) reg_dec<M::kRegConv>();
-    constexpr int kPer = D / 16;                           // 16-code chunks of a row
+    if constexpr (M::kRegConv < M::kRegLaunch) reg_dec<M::kRegConv>();
+    constexpr int kPer = D / 16;                          // 16-code chunks of a row
     constexpr int kRowsPass = 32 * M::kConvWarps / kPer;  // rows of a pass: 16 or 32
     constexpr int kPasses = kUnit / kRowsPass;
-    const int ct = tid - 32 * kConvWarp0;
-    const int row0 = ct / kPer, c16 = ct % kPer;
+    // Four lanes take a 64-value group of one row, the next four the same group
+    // of the next row: their eight 16-byte stores hit all eight bank groups.
+    constexpr int kGroups = D / 64;
+    const int ct = tid - 32 * M::kConvWarp0;
+    const int grp = (ct >> 3) % kGroups, c4 = ct & 3;
+    const int row0 = 2 * (ct / (8 * kGroups)) + ((ct >> 2) & 1);
+    const uint32_t soff = grp * 8192 + row0 * 128 + (((2 * c4) ^ (row0 & 7)) << 4);  // second half: ^ 16
     const int bpp = p.page >> p.block_shift;
+    const uint32_t row_bytes = static_cast<uint32_t>(p.Hkv) * D;
     uint32_t i = 0;
     bool live = true;
     while (live && next_piece(p, w, q)) {
       const int ctx = tokens_of(p, q.b);
       const int32_t *trow = p.table + static_cast<size_t>(q.b) * p.width;
       const int last = q.u0 + q.n;
-      int pg[kPasses];       // page of each pass's token, one unit ahead of the codes
+      const size_t head_off = static_cast<size_t>(q.h) * D + 64 * grp + 16 * c4;
+      const uint8_t *kbase = p.kc + head_off, *vbase = p.vc + head_off;
+      int pg[kPasses];        // page of each pass's token, one unit ahead of the codes
+      uint32_t in[kPasses];   // and the token's place in it
       uint4 ck[kPasses], cv[kPasses];
       float ks = 0.0f, vs = 0.0f;  // lanes 0-3 of the first warp: scales of a granule
-      int info_pg = -1;
+      int info_pg = -1, info_in = 0;
       auto fetch_pages = [&](int u) {
 #pragma unroll
         for (int k = 0; k < kPasses; ++k) {
           const int t = u * kUnit + k * kRowsPass + row0;
-          pg[k] = u < last && t < ctx ? trow[page_col(p, t)] : -1;
+          const int c = page_col(p, t);
+          in[k] = t - c * p.page;
+          pg[k] = t < ctx ? trow[c] : -1;
         }
-        const int t = u * kUnit + 16 * lane;
-        if (ct < 4) info_pg = u < last && t < ctx ? trow[page_col(p, t)] : -1;
+        if (ct < 4) {
+          const int t = u * kUnit + 16 * lane;
+          const int c = page_col(p, t);
+          info_in = t - c * p.page;
+          info_pg = t < ctx ? trow[c] : -1;
+        }
       };
-      auto fetch = [&](int u, const uint8_t *codes, uint4 (&c)[kPasses]) {
+      auto fetch = [&](const uint8_t *codes, uint4 (&c)[kPasses]) {
 #pragma unroll
         for (int k = 0; k < kPasses; ++k) {
           c[k] = make_uint4(0, 0, 0, 0);  // tokens past the context or without a page: zero codes
-          if (pg[k] >= 0 && pg[k] < p.pages) {
-            const int t = u * kUnit + k * kRowsPass + row0;
-            const size_t row = static_cast<size_t>(pg[k]) * p.page + (t - page_col(p, t) * p.page);
-            c[k] = ldg_stream(codes + (row * p.Hkv + q.h) * D + 16 * c16);
-          }
+          if (static_cast<uint32_t>(pg[k]) < static_cast<uint32_t>(p.pages))
+            c[k] = ldg_stream(codes + static_cast<uint64_t>(static_cast<uint32_t>(pg[k]) * static_cast<uint32_t>(p.page) + in[k]) * row_bytes);
         }
       };
-      auto fetch_scales = [&](int u) {
+      auto fetch_scales = [&]() {
         if (ct >= 4) return;
         ks = 0.0f;
         vs = -1.0f;
-        if (info_pg >= 0 && info_pg < p.pages) {
-          const int t = u * kUnit + 16 * lane;
-          const size_t at = (static_cast<size_t>(info_pg) * bpp + ((t - page_col(p, t) * p.page) >> p.block_shift)) * p.Hkv + q.h;
+        if (static_cast<uint32_t>(info_pg) < static_cast<uint32_t>(p.pages)) {
+          const size_t at = (static_cast<size_t>(info_pg) * bpp + (info_in >> p.block_shift)) * p.Hkv + q.h;
           ks = __ldg(p.ks + at);
           vs = fmaxf(__ldg(p.vs + at), 0x1p-110f);
         }
       };
+      auto store = [&](uint32_t tile, const uint4 (&c)[kPasses]) {
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          uint4 a, b;
+          widen16<E4M3>(c[k], a, b);
+          const uint32_t at = tile + soff + k * (kRowsPass * 128);
+          sts128(at, a);
+          sts128(at ^ 16u, b);
+        }
+      };
       fetch_pages(q.u0);
-      fetch(q.u0, p.kc, ck);
-      fetch(q.u0, p.vc, cv);
-      fetch_scales(q.u0);
+      fetch(kbase, ck);
+      fetch(vbase, cv);
+      fetch_scales();
       fetch_pages(q.u0 + 1);
       for (int u = q.u0; u < last; ++u, ++i) {
         const uint32_t slot = i % M::kSlots, ph = (i / M::kSlots) & 1u;
-        auto store = [&](uint32_t tile, const uint4 (&c)[kPasses]) {
-#pragma unroll
-          for (int k = 0; k < kPasses; ++k) {
-            const int n = k * kRowsPass + row0;
-            uint4 a, b;
-            widen16<E4M3>(c[k], a, b);
-            const uint32_t row = tile + (c16 >> 2) * 8192 + n * 128;
-            const int j = 2 * (c16 & 3);
-            const uint32_t sa = row + (((j) ^ (n & 7)) << 4), sb = row + (((j + 1) ^ (n & 7)) << 4);
-            // lanes of odd 64-value groups store their second half first: all eight bank groups are hit
-            const bool odd = (c16 >> 2) & 1;
-            sts128(odd ? sb : sa, odd ? b : a);
-            sts128(odd ? sa : sb, odd ? a : b);
-          }
-        };
         live = bar_wait(bar(M::kKEmpty + slot), ph ^ 1u, dead, err);
         live = __all_sync(0xFFFFFFFFu, live);
         if (!live) break;
@@ -632,8 +743,8 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(M::kKFull + slot));
-        if (u + 1 < last) fetch(u + 1, p.kc, ck);
-        if (warp == kConvWarp0) {
+        if (u + 1 < last) fetch(kbase, ck);
+        if (warp == M::kConvWarp0) {
           if (lane < 4) {
             const bool ok = vs > 0.0f;
             reinterpret_cast<float4 *>(sm + M::kOffInfo)[(i % kInfo) * 4 + lane] =
@@ -641,7 +752,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(M::kInfoFull + i % kInfo));
-          if (u + 1 < last) fetch_scales(u + 1);
+          if (u + 1 < last) fetch_scales();
         }
         live = bar_wait(bar(M::kVEmpty + slot), ph ^ 1u, dead, err);
         live = __all_sync(0xFFFFFFFFu, live);
@@ -651,7 +762,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(M::kVFull + slot));
         if (u + 1 < last) {
-          fetch(u + 1, p.vc, cv);
+          fetch(vbase, cv);
           fetch_pages(u + 2);
         }
       }
@@ -660,52 +771,87 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp)
+  if (warp == M::kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
                  "r"(static_cast<uint32_t>(M::kCols)));
 }
 
-// Joins the tiles that several CTAs worked on.  BY_CUT: one CTA per (cut, 8
-// rows), at the first cut inside a segment -- for calls with more segments
-// than cuts; otherwise one CTA per (tile, kv head, row).
-template <int D, bool BY_CUT>
-__global__ void __launch_bounds__(256) k_q8_many_join(Q8View p, int ctas) {
+// Joins the tiles that several CTAs worked on, in CTA order: one CTA per four
+// rows, a thread per row and float4, G groups of threads that take every G-th
+// piece.  BY_CUT: at the first cut inside a segment, for calls with more
+// segments than cuts (few pieces each: G 1); otherwise per (tile, kv head).
+template <int D, int G, bool BY_CUT>
+__global__ void __launch_bounds__(D * G) k_q8_many_join(Q8View p, int ctas) {
+  constexpr int kRowsCta = 4;
+  __shared__ float4 s_o[G][D];
+  __shared__ float s_l[G][kRowsCta];
   pdl_wait();
   const int tiles = p.seq_tile[p.B];
   const long long total = p.tprefix[tiles];
   const int used = ranges_of(total, ctas);
-  int tile, h, row0;
-  long long a, unit = -1;
-  int cut = 0;
+  constexpr int kPer = kTile / kRowsCta;
+  const int row0 = (blockIdx.x % kPer) * kRowsCta, at = blockIdx.x / kPer;
+  int tile, h;
+  long long unit = -1;
   if (BY_CUT) {
-    cut = (blockIdx.x >> 4) + 1;
-    row0 = (blockIdx.x & 15) * 8;
-    if (cut >= used) return;
-    unit = range_start(total, used, cut);
+    if (at + 1 >= used) return;
+    unit = range_start(total, used, at + 1);
     tile = find_tile(p, tiles, unit);
-    h = static_cast<int>((unit - p.tprefix[tile]) / p.tiles[tile].z);
+    h = static_cast<int>((unit - p.tprefix[tile]) / (p.tiles[tile].z + kCost));
   } else {
-    row0 = blockIdx.x & 127;
-    const int seg = blockIdx.x >> 7;
-    tile = seg / p.Hkv;
-    h = seg - tile * p.Hkv;
+    tile = at / p.Hkv;
+    h = at - tile * p.Hkv;
     if (tile >= tiles) return;
   }
   const int4 ti = p.tiles[tile];
   if (ti.z == 0) return;
-  a = p.tprefix[tile] + static_cast<long long>(h) * ti.z;
-  if (a == unit) return;
-  const int c0 = owner_of(a, total, used), c1 = owner_of(a + ti.z - 1, total, used);
-  if (c0 == c1 || (BY_CUT && c0 != cut - 1)) return;
+  const long long a = p.tprefix[tile] + static_cast<long long>(h) * (ti.z + kCost);
+  const int c0 = owner_of(a + kCost, total, used), c1 = owner_of(a + kCost + ti.z - 1, total, used);
+  if (c0 == c1 || (BY_CUT && c0 != at)) return;
   const int2 qr = rows_of(p, ti.x);
+  const int rows = qr.y * p.gq;
+  if (ti.y * kTile + row0 >= rows) return;
   const bool late0 = range_start(total, used, c0) < a;
-  for (int r = row0; r < row0 + (BY_CUT ? 8 : 1); ++r) {
-    const int rr = ti.y * kTile + r;
-    if (rr >= qr.y * p.gq) return;
-    const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
-    if (BY_CUT && r > row0) __syncthreads();  // join_row's shared arrays
-    join_row<D, kTile>(p.tpart, p.tpart_ml, c0, c1, late0, r, p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D);
+  const int r = threadIdx.x & 3, d4 = (threadIdx.x >> 2) % (D / 4), grp = threadIdx.x / D;
+  auto slot_of = [&](int c) { return 2 * c + (c == c0 && late0 ? 1 : 0); };
+  float mm = -INFINITY;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, p.tpart_ml[slot_of(c) * kTile + row0 + r].x);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float ll = 0.0f;
+  const float4 *part = reinterpret_cast<const float4 *>(p.tpart) + static_cast<size_t>(d4) * kTile + row0 + r;
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += G) {
+    const float2 ml = p.tpart_ml[slot_of(c) * kTile + row0 + r];
+    const float4 v = part[static_cast<size_t>(slot_of(c)) * (D / 4) * kTile];
+    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
+    ll += ml.y * w;
+    acc.x += v.x * w;
+    acc.y += v.y * w;
+    acc.z += v.z * w;
+    acc.w += v.w * w;
   }
+  if (G > 1) {
+    s_o[grp][threadIdx.x % D] = acc;
+    if (d4 == 0) s_l[grp][r] = ll;
+    __syncthreads();
+    if (grp != 0) return;
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+      const float4 v = s_o[g][threadIdx.x];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+      ll += s_l[g][r];
+    }
+  }
+  const int rr = ti.y * kTile + row0 + r;
+  if (rr >= rows) return;
+  const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
+  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
+  *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 4 * d4) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 template <int D, bool E4M3>
@@ -717,10 +863,12 @@ cudaError_t launch(const Q8View &p, cudaStream_t s) {
   k_q8_tiles<<<1, kScanThreads, 0, s>>>(p);
   e = launch_pdl(k_q8_many<D, E4M3>, dim3(M::kMax), dim3(M::kThreads), M::kSmem, s, p, device_error_word());
   if (e != cudaSuccess) return e;
+  constexpr int kPer = kTile / 4;
   const uint64_t segs = many_tiles(p) * p.Hkv;
   if (segs <= 32)
-    return launch_pdl(k_q8_many_join<D, false>, dim3(static_cast<unsigned>(segs * kTile)), dim3(256), 0, s, p, +M::kMax);
-  return launch_pdl(k_q8_many_join<D, true>, dim3((M::kMax - 1) * 16), dim3(256), 0, s, p, +M::kMax);
+    return launch_pdl(k_q8_many_join<D, 1024 / D, false>, dim3(static_cast<unsigned>(segs * kPer)), dim3(1024), 0, s, p,
+                      +M::kMax);
+  return launch_pdl(k_q8_many_join<D, 1, true>, dim3((M::kMax - 1) * kPer), dim3(D), 0, s, p, +M::kMax);
 }
 
 }  // namespace
