@@ -45,13 +45,14 @@ struct Q8View {
   float scale;
   int few_rows;         // sequences of more (row, head) pairs per kv head take the many-row kernel
   // workspace of the few-row kernel (8 rows a tile)
-  long long *prefix;    // [B + 1] units of work before each sequence
+  int4 *cuts;           // [CTAs] where each range begins (Cut)
   float *part;          // [2 * CTAs][8][D] unfinished sums
   float2 *part_ml;      // [2 * CTAs][8] their reference and weight sum
   // workspace of the many-row kernel (128 rows a tile)
   int max_tiles;
   int *seq_tile;        // [B + 1] tiles before each sequence
   int4 *tiles;          // [tiles] {sequence, tile of it, units of one kv head, 0}
+  int4 *tcuts;          // [CTAs]
   long long *tprefix;   // [tiles + 1] units of work before each tile
   float *tpart;         // [2 * CTAs][D / 4][128][4]
   float2 *tpart_ml;     // [2 * CTAs][128]
@@ -169,57 +170,22 @@ __device__ __forceinline__ int owner_of(long long unit, long long total, int use
   return static_cast<int>(((unit + 1) * used - 1) / total);
 }
 
-// Joins the sums of a segment that several CTAs worked on (CTA c0 to c1, in
-// CTA order) for one row: `row` of the R rows of a workspace slot.  256
-// threads: L = D / 4 lanes, G groups that take every G-th CTA.  A CTA's first
-// piece of work is in slot 2c, a later cut one in 2c + 1; `late0`: CTA c0's
-// range begins before the segment.
-template <int D, int R>
-__device__ __forceinline__ void join_row(const float *part, const float2 *part_ml, int c0, int c1, bool late0, int row,
-                                         uint16_t *dst) {
-  constexpr int L = D / 4, G = 256 / L;
-  __shared__ float4 s_o[G][L];
-  __shared__ float s_l[G];
-  const int lane = threadIdx.x % L, grp = threadIdx.x / L;
-  auto at = [&](int c) { return static_cast<size_t>(2 * c + (c == c0 && late0 ? 1 : 0)) * R + row; };
-  float mm = -INFINITY;
-  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, part_ml[at(c)].x);
-#pragma unroll
-  for (int s = 16; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, s));
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float ll = 0.0f;
-#pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += G) {
-    const float2 ml = part_ml[at(c)];
-    const float4 v = *reinterpret_cast<const float4 *>(part + at(c) * D + 4 * lane);
-    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
-    ll += ml.y * w;
-    acc.x += v.x * w;
-    acc.y += v.y * w;
-    acc.z += v.z * w;
-    acc.w += v.w * w;
-  }
-  s_o[grp][lane] = acc;
-  if (lane == 0) s_l[grp] = ll;
-  __syncthreads();
-  if (grp != 0) return;
-#pragma unroll
-  for (int i = 1; i < G; ++i) {
-    const float4 v = s_o[i][lane];
-    acc.x += v.x;
-    acc.y += v.y;
-    acc.z += v.z;
-    acc.w += v.w;
-    ll += s_l[i];
-  }
-  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
-  *reinterpret_cast<uint2 *>(dst + 4 * lane) =
-      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+// Where a CTA's range begins.  When that is the first cut inside a segment
+// (work of one sequence, kv head and tile that several CTAs share), the join
+// finds here all it needs: {sequence, kv head, tile, last CTA of the segment,
+// with bit 30 set when the CTA before, the segment's first, began earlier than
+// the segment}; otherwise the sequence is -1.
+__device__ __forceinline__ int4 cut_of(int b, int h, int tile, long long seg_begin, long long first_unit, long long last_unit,
+                                       long long total, int used, int cta) {
+  if (owner_of(first_unit, total, used) != cta - 1) return make_int4(-1, 0, 0, 0);
+  const int late = range_start(total, used, cta - 1) < seg_begin ? 1 << 30 : 0;
+  return make_int4(b, h, tile, owner_of(last_unit, total, used) | late);
 }
 
 // The many-row kernels (attention_q8_many.cu).
 int many_ctas(int head_dim);
 uint64_t many_tiles(const Q8View &p);  // at most so many tiles of 128 rows
+int few_ctas(int head_dim);
 cudaError_t launch_many(const Q8View &p, int head_dim, bool e4m3, cudaStream_t s);
 
 }  // namespace fnmoe

@@ -7,7 +7,7 @@
 // units that causality leaves them; the units of all tiles, laid end to end,
 // are dealt to persistent CTAs in equal contiguous ranges, so neither ragged
 // lengths nor the causal triangle load one SM more than another.  Tiles that
-// a range cuts are joined by k_q8_many_join.
+// a range cuts are joined by k_q8_join.
 //
 // Per unit, S = Q K^T (M128 N64, K = D) and O += P V (M128 N = D, K = 64, for
 // each of the two terms of P) run on the tensor cores with Q and P as TMEM
@@ -301,6 +301,23 @@ __device__ __forceinline__ void widen16(uint4 c, uint4 &lo, uint4 &hi) {
   hi = make_uint4(widen2<E4M3, 0>(c.z), widen2<E4M3, 1>(c.z), widen2<E4M3, 0>(c.w), widen2<E4M3, 1>(c.w));
 }
 
+// Tiles that see no token: their rows are zero.
+template <int D>
+__device__ __forceinline__ void zero_tiles(const Q8View &p, int tiles) {
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int4 ti = p.tiles[t];
+    if (ti.z != 0) continue;
+    const int2 qr = rows_of(p, ti.x);
+    const int r0 = ti.y * kTile, nr = min(kTile, qr.y * p.gq - r0);
+    for (int i = threadIdx.x; i < nr * p.Hkv * (D / 8); i += blockDim.x) {
+      const int d = i % (D / 8), rh = i / (D / 8);
+      const int r = r0 + rh % nr, h = rh / nr;
+      const int qi = r / p.gq, head = h * p.gq + r - qi * p.gq;
+      *reinterpret_cast<uint4 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 8 * d) = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q8View p, uint32_t *err) {
   using M = Many<D>;
@@ -316,25 +333,16 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   const int tiles = p.seq_tile[p.B];
-  // Tiles that see no token: their rows are zero.
-  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int4 ti = p.tiles[t];
-    if (ti.z != 0) continue;
-    const int2 qr = rows_of(p, ti.x);
-    const int r0 = ti.y * kTile, nr = min(kTile, qr.y * p.gq - r0);
-    for (int i = tid; i < nr * p.Hkv * (D / 8); i += M::kThreads) {
-      const int d = i % (D / 8), rh = i / (D / 8);
-      const int r = r0 + rh % nr, h = rh / nr;
-      const int qi = r / p.gq, head = h * p.gq + r - qi * p.gq;
-      *reinterpret_cast<uint4 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 8 * d) = make_uint4(0, 0, 0, 0);
-    }
-  }
   const long long total = p.tprefix[tiles];
   const int used = ranges_of(total, gridDim.x);
   Walk w;
   w.cur = w.first = range_start(total, used, blockIdx.x);
   w.end = range_start(total, used, blockIdx.x + 1);
-  if (w.cur >= w.end) return;
+  if (w.cur >= w.end) {
+    if (tid == 0) p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    zero_tiles<D>(p, tiles);
+    return;
+  }
   w.tile = find_tile(p, tiles, w.cur);
   w.off = w.cur - p.tprefix[w.tile];
 
@@ -348,6 +356,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
     }
     *dead = 0u;
     mbar_init_fence();
+    p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // until the first piece shows a cut
   }
   if (warp == M::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
@@ -400,6 +409,10 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
       const int lim = valid ? p.ctx[q.b] - qr.y + qi : 0x7FFFFFFF;
       const int lim_min = __reduce_min_sync(0xFFFFFFFFu, lim);
       const bool idle = !__any_sync(0xFFFFFFFFu, valid);
+      if (tid == 0 && q.first && q.u0 > 0) {
+        const long long a = w.cur - (kCost + q.u0 + q.n);  // the segment's first unit
+        p.tcuts[blockIdx.x] = cut_of(q.b, q.h, q.mt, a, a + kCost, a + kCost + q.steps - 1, total, used, blockIdx.x);
+      }
       // Rows of the warp that this thread moves: row 8 e + lane / 4.
       long long q_at[4], o_at[4];
       {
@@ -771,87 +784,10 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  zero_tiles<D>(p, tiles);
   if (warp == M::kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
                  "r"(static_cast<uint32_t>(M::kCols)));
-}
-
-// Joins the tiles that several CTAs worked on, in CTA order: one CTA per four
-// rows, a thread per row and float4, G groups of threads that take every G-th
-// piece.  BY_CUT: at the first cut inside a segment, for calls with more
-// segments than cuts (few pieces each: G 1); otherwise per (tile, kv head).
-template <int D, int G, bool BY_CUT>
-__global__ void __launch_bounds__(D * G) k_q8_many_join(Q8View p, int ctas) {
-  constexpr int kRowsCta = 4;
-  __shared__ float4 s_o[G][D];
-  __shared__ float s_l[G][kRowsCta];
-  pdl_wait();
-  const int tiles = p.seq_tile[p.B];
-  const long long total = p.tprefix[tiles];
-  const int used = ranges_of(total, ctas);
-  constexpr int kPer = kTile / kRowsCta;
-  const int row0 = (blockIdx.x % kPer) * kRowsCta, at = blockIdx.x / kPer;
-  int tile, h;
-  long long unit = -1;
-  if (BY_CUT) {
-    if (at + 1 >= used) return;
-    unit = range_start(total, used, at + 1);
-    tile = find_tile(p, tiles, unit);
-    h = static_cast<int>((unit - p.tprefix[tile]) / (p.tiles[tile].z + kCost));
-  } else {
-    tile = at / p.Hkv;
-    h = at - tile * p.Hkv;
-    if (tile >= tiles) return;
-  }
-  const int4 ti = p.tiles[tile];
-  if (ti.z == 0) return;
-  const long long a = p.tprefix[tile] + static_cast<long long>(h) * (ti.z + kCost);
-  const int c0 = owner_of(a + kCost, total, used), c1 = owner_of(a + kCost + ti.z - 1, total, used);
-  if (c0 == c1 || (BY_CUT && c0 != at)) return;
-  const int2 qr = rows_of(p, ti.x);
-  const int rows = qr.y * p.gq;
-  if (ti.y * kTile + row0 >= rows) return;
-  const bool late0 = range_start(total, used, c0) < a;
-  const int r = threadIdx.x & 3, d4 = (threadIdx.x >> 2) % (D / 4), grp = threadIdx.x / D;
-  auto slot_of = [&](int c) { return 2 * c + (c == c0 && late0 ? 1 : 0); };
-  float mm = -INFINITY;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, p.tpart_ml[slot_of(c) * kTile + row0 + r].x);
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float ll = 0.0f;
-  const float4 *part = reinterpret_cast<const float4 *>(p.tpart) + static_cast<size_t>(d4) * kTile + row0 + r;
-#pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += G) {
-    const float2 ml = p.tpart_ml[slot_of(c) * kTile + row0 + r];
-    const float4 v = part[static_cast<size_t>(slot_of(c)) * (D / 4) * kTile];
-    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
-    ll += ml.y * w;
-    acc.x += v.x * w;
-    acc.y += v.y * w;
-    acc.z += v.z * w;
-    acc.w += v.w * w;
-  }
-  if (G > 1) {
-    s_o[grp][threadIdx.x % D] = acc;
-    if (d4 == 0) s_l[grp][r] = ll;
-    __syncthreads();
-    if (grp != 0) return;
-#pragma unroll
-    for (int g = 1; g < G; ++g) {
-      const float4 v = s_o[g][threadIdx.x];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
-      ll += s_l[g][r];
-    }
-  }
-  const int rr = ti.y * kTile + row0 + r;
-  if (rr >= rows) return;
-  const int qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
-  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
-  *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 4 * d4) =
-      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 template <int D, bool E4M3>
@@ -861,14 +797,7 @@ cudaError_t launch(const Q8View &p, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(k_q8_many<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
   if (e != cudaSuccess) return e;
   k_q8_tiles<<<1, kScanThreads, 0, s>>>(p);
-  e = launch_pdl(k_q8_many<D, E4M3>, dim3(M::kMax), dim3(M::kThreads), M::kSmem, s, p, device_error_word());
-  if (e != cudaSuccess) return e;
-  constexpr int kPer = kTile / 4;
-  const uint64_t segs = many_tiles(p) * p.Hkv;
-  if (segs <= 32)
-    return launch_pdl(k_q8_many_join<D, 1024 / D, false>, dim3(static_cast<unsigned>(segs * kPer)), dim3(1024), 0, s, p,
-                      +M::kMax);
-  return launch_pdl(k_q8_many_join<D, 1, true>, dim3((M::kMax - 1) * kPer), dim3(D), 0, s, p, +M::kMax);
+  return launch_pdl(k_q8_many<D, E4M3>, dim3(M::kMax), dim3(M::kThreads), M::kSmem, s, p, device_error_word());
 }
 
 }  // namespace
