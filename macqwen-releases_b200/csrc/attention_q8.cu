@@ -1,15 +1,19 @@
 // attention_q8.cu -- causal attention over the paged 8-bit KV cache (sm_100a):
 // the entry points and the kernels for sequences with few query rows (decode).
 // The arithmetic: attention_q8.cuh; many rows: attention_q8_many.cu.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <cmath>
+#include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "attention_q8.cuh"
 #include "moe_kernels.cuh"
 #include "paged_q8.cuh"
+#include "umma.cuh"
 
 namespace fnmoe {
 
@@ -18,43 +22,165 @@ namespace {
 // ---- few rows per sequence --------------------------------------------------
 //
 // Bound by HBM (one byte a value, 2 * D * Hkv bytes a token).  Work is cut
-// into units of 64 tokens of one (sequence, kv head, tile of 8 rows); the
+// into units of 128 tokens of one (sequence, kv head, tile of 8 rows); the
 // units of all sequences, laid end to end, are dealt to the CTAs in equal
 // contiguous ranges, so ragged contexts load every SM alike.  A CTA's range
 // covers whole segments, which it finishes, and at most two cut ones (its
-// first and last), whose sums go to the workspace for k_q8_few_join.
+// first and last), whose sums go to the workspace for k_q8_join.
 //
-// A warp takes 16 tokens at a time.  Each lane copies exactly the codes that it
-// will feed to its MMA fragments (cp.async into a ring of its own, kStages
-// steps deep), so the copies need no swizzle and no barrier, and the ring,
-// not the register file, holds the bytes in flight that HBM's latency asks
-// for:
-//   S^T = K Q^T   (m16n8k16, M = 16 tokens, N = 8 rows): the order of the
-//     contraction is free, so lane (g, t) takes 16 consecutive dims of tokens
-//     g and g + 8, one 16-byte load for four k-steps;
+// A warp takes 32 tokens at a time, as two tiles of 16 whose chains of
+// dependent instructions overlap.  It fetches them for itself: TMA boxes of
+// 16 tokens x 128 bytes (128-byte swizzle; 64 bytes at D 64) into shared memory
+// of its own, the next step's K as soon as this one's scores are done, the next
+// V when its products are; no warp waits for another inside a piece of work.
+// (Loads by the lanes themselves, to registers or by cp.async, stayed at
+// 3.5 TB/s whatever the occupancy.)
+//   S^T = K Q^T   (M = 16 tokens, N = 8 rows): A fragments by ldmatrix
+//     (QueryInt8, QueryE4M3);
 //   O^T += V^T P^T (M = 16 dims, N = 8 rows, K = 16 tokens): lane (g, t)
-//     loads 16 consecutive dims of tokens 2t, 2t+1, 2t+8, 2t+9 and pairs the
+//     takes 16 consecutive dims of tokens 2t, 2t+1, 2t+8, 2t+9 and pairs the
 //     tokens' bytes with prmt.
 // 16 tokens lie in one page and one scale block.
 
-constexpr int kFewThreads = 128;  // 4 warps x 16 tokens = a unit
+constexpr int kFewThreads = 128;
+constexpr int kFewUnit = 128;  // 4 warps x 32 tokens
 constexpr int kFewRows = 16;
+constexpr uint32_t kFewSpin = 1u << 22;  // mbarrier polls before a wait gives up
 
+// Byte offset, in a 16-token tile of codes, of the 16-byte chunk `c` of token
+// `row`: boxes of 16 rows x 128 bytes, chunk c at c ^ (row & 7), or one of 16 x
+// 64 bytes, c at c ^ ((row >> 1) & 3).
 template <int D>
+__device__ __forceinline__ uint32_t tile_offset(int row, int c) {
+  if (D == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+  return (c >> 3) * 2048 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// The query rows as B operands in shared memory (fragment order, shared by the
+// CTA's warps), and the scores of two tiles of 16 tokens at at[0], at[1].
+// ldmatrix gives lane (g, t) the codes of tokens g and g + 8 at dims 32 s + 4 t
+// .. + 3 and 32 s + 16 + 4 t .. + 3; put() stores this lane's share of 32-dim
+// step s of its row (eight dims, as two words a, b of four: the raw bfloat16
+// pairs); scale_of() is the power of two that a row's scores are to be
+// multiplied by, from the bits of its largest magnitude.
+//
+// e4m3 codes and queries as float16: the codes are exact, one conversion for
+// two; a row is scaled so that its largest element lies in [1, 2) (exact for
+// elements within 2^-14 of it).
+template <int D>
+struct QueryE4M3 {
+  static constexpr int kBytes = D / 16 * 256;
+  static __device__ __forceinline__ uint32_t exponent(uint32_t peak) { return min(max(peak >> 7, 1u), 253u); }
+  static __device__ __forceinline__ float scale_of(uint32_t peak) { return __uint_as_float(exponent(peak) << 23); }
+  static __device__ __forceinline__ void put(uint2 *q, int s, uint2 a, uint2 b, uint32_t peak) {
+    const float down = __uint_as_float((254u - exponent(peak)) << 23);
+    auto pair = [&](uint32_t w) { return pack_f16x2(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down); };
+    const int lane = threadIdx.x & 31;
+    q[2 * s * 32 + lane] = make_uint2(pair(a.x), pair(a.y));
+    q[(2 * s + 1) * 32 + lane] = make_uint2(pair(b.x), pair(b.y));
+  }
+  static __device__ __forceinline__ void scores(const uint32_t (&at)[2], uint32_t q, float (&s)[2][4]) {
+    const int lane = threadIdx.x & 31, row = lane & 15, half = lane >> 4;
+    float c[2][2][4] = {};  // two chains a tile
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st) {
+      uint32_t w[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) ldsm_x4(at[u] + tile_offset<D>(row, 2 * st + half), w[u]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint2 b = lds64(q + (2 * st + k) * 256);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t x0 = w[u][2 * k], x1 = w[u][2 * k + 1];
+          const uint32_t a[4] = {e4m3_f16<0>(x0), e4m3_f16<0>(x1), e4m3_f16<1>(x0), e4m3_f16<1>(x1)};
+          mma_16816(c[u][k], a, b.x, b.y);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[u][e] = __fadd_rn(c[u][0][e], c[u][1][e]);
+  }
+};
+
+// int8 codes as they are, on the integer tensor cores: a row as the fixed
+// point X = round(q 2^(21 - E)), E the exponent of its largest element, in
+// three byte planes X = X0 + 2^8 X1 + 2^16 X2 (X2 signed); sums of code times
+// plane stay below 2^24, exact in float32.  X is exact for elements within
+// 2^-14 of the largest.
+template <int D>
+struct QueryInt8 {
+  static constexpr int kBytes = 3 * (D / 32) * 256;
+  static __device__ __forceinline__ uint32_t exponent(uint32_t peak) { return min(max(peak >> 7, 24u), 253u); }
+  static __device__ __forceinline__ float scale_of(uint32_t peak) {  // NaN for a row with an infinity or NaN
+    return (peak >> 7) == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float((exponent(peak) - 21u) << 23);
+  }
+  static __device__ __forceinline__ void put(uint2 *q, int s, uint2 a, uint2 b, uint32_t peak) {
+    const float up = __uint_as_float((275u - exponent(peak)) << 23);  // 2^(21 - E)
+    const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+    uint32_t plane[3][2] = {};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)  // four dims: one word of each plane
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t v = w[2 * k + (t >> 1)];
+        const int x = __float2int_rn(__uint_as_float(t & 1 ? v & 0xFFFF0000u : v << 16) * up);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) plane[p][k] |= ((static_cast<uint32_t>(x) >> (8 * p)) & 0xFFu) << (8 * t);
+      }
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) q[(p * (D / 32) + s) * 32 + lane] = make_uint2(plane[p][0], plane[p][1]);
+  }
+  static __device__ __forceinline__ void scores(const uint32_t (&at)[2], uint32_t q, float (&s)[2][4]) {
+    const int lane = threadIdx.x & 31, row = lane & 15, half = lane >> 4;
+    int c[2][3][4] = {};
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st) {
+      const uint2 b0 = lds64(q + st * 256), b1 = lds64(q + (D / 32 + st) * 256), b2 = lds64(q + (2 * (D / 32) + st) * 256);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a[4];
+        ldsm_x4(at[u] + tile_offset<D>(row, 2 * st + half), a);
+        mma_s8<false>(c[u][0], a[0], a[1], a[2], a[3], b0.x, b0.y);
+        mma_s8<false>(c[u][1], a[0], a[1], a[2], a[3], b1.x, b1.y);
+        mma_s8<true>(c[u][2], a[0], a[1], a[2], a[3], b2.x, b2.y);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s[u][e] = __fmaf_rn(__int2float_rn(c[u][2][e]), 65536.0f,
+                            __fmaf_rn(__int2float_rn(c[u][1][e]), 256.0f, __int2float_rn(c[u][0][e])));
+  }
+};
+
+template <int D, bool E4M3>
 struct Few {
+  using Query = typename std::conditional<E4M3, QueryE4M3<D>, QueryInt8<D>>::type;
   static constexpr int kCtas = D == 256 ? 3 : D == 128 ? 4 : 6;  // per SM
-  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 3 : 4;
-  static constexpr int kHalf = 16 * D;                          // bytes of a step's K (or V) codes
-  static constexpr int kWarpBytes = kStages * 2 * kHalf;        // 12 warps or more: 192 KB an SM
-  static constexpr int kSmem = 4 * kWarpBytes;                  // the warps' sums are joined in the same space
+  static constexpr int kTileBytes = 16 * D;                     // K (or V) codes of 16 tokens
+  static constexpr int kWarpBytes = 4 * kTileBytes;             // two tiles of K, two of V
+  static constexpr int kOffQ = 4 * kWarpBytes;                  // the warps' sums are joined in the first part
+  static constexpr int kOffBar = kOffQ + Query::kBytes;         // per warp: K has arrived, V has arrived
+  static constexpr int kSmem = kOffBar + 64 + 1024;             // + slack for the 1024-byte alignment of the tiles
   static constexpr int kMax = 148 * kCtas;
-  static_assert(kSmem >= 4 * 8 * D * 4, "the four warps' sums");
+  static_assert(kOffQ >= 4 * 8 * D * 4, "the four warps' sums");
 };
 
 // Units of one (kv head, row tile) of sequence b, and its row tiles.
 __device__ __forceinline__ int2 units_of(const Q8View &p, int b) {
   const int rows = rows_of(p, b).y * p.gq;
-  return make_int2((tokens_of(p, b) + kUnit - 1) / kUnit, rows <= p.few_rows ? (rows + 7) / 8 : 0);
+  return make_int2((tokens_of(p, b) + kFewUnit - 1) / kFewUnit, rows <= p.few_rows ? (rows + 7) / 8 : 0);
 }
 
 // The sequence that holds this CTA's first unit, the units before that
@@ -121,19 +247,30 @@ __device__ Found find_unit(const Q8View &p, int cta, int ctas, long long &start,
 }
 
 template <int D, bool E4M3>
-__global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p) {
+__global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8View p, const __grid_constant__ CUtensorMap kmap,
+                                                                                 const __grid_constant__ CUtensorMap vmap, uint32_t *err) {
   constexpr int KC = D / 64;               // 16-byte pieces of a K row per lane
   constexpr int VC = D == 64 ? 1 : D / 128;  // pieces of a V row per lane
   constexpr int VW = D == 64 ? 2 : 4;      // words of a V piece
   constexpr int MT = D / 16;               // 16-dim tiles of O^T
-  using F = Few<D>;
-  extern __shared__ __align__(16) uint8_t few_ring[];
+  using F = Few<D, E4M3>;
+  extern __shared__ uint8_t few_raw[];
+  const uint32_t sbase = (smem_u32(few_raw) + 1023u) & ~1023u;
+  uint8_t *few_ring = few_raw + (sbase - smem_u32(few_raw));
   float (*s_o)[8][D] = reinterpret_cast<float (*)[8][D]>(few_ring);
   __shared__ float s_m[4][8], s_l[4][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tq = lane & 3;
   pdl_wait();  // launched after the many-row kernel, whose workspace the join reads
   pdl_trigger();
+  const uint32_t kbar = sbase + F::kOffBar + 16 * warp, vbar = kbar + 8;
+  if (lane == 0) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(kbar));
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(vbar));
+    mbar_init_fence();
+  }
+  uint32_t phase = 0;  // of both: they complete once a step
+  bool dead = false;
   long long cur, end;
   const Found f = find_unit<kFewThreads>(p, blockIdx.x, gridDim.x, cur, end);
   const long long first = cur;
@@ -155,32 +292,34 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
     const int rows = qr.y * p.gq;
     const int lim0 = p.ctx[b] - qr.y;  // last position that row 0 sees
 
-    // ---- this tile's query rows as the B operand, and the last position each sees ----
-    uint32_t qf[MT][2];
+    // ---- this tile's query rows, their scale and the last position each sees ----
+    float c[2];
     int lim[2];
     {
       const int r = rt * 8 + g;
       const bool live = r < rows;
       const int qi = live ? r / p.gq : 0;
       const int head = h * p.gq + (live ? r - qi * p.gq : 0);
-      const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D + 16 * tq;
+      const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D + 4 * tq;
+      uint2 raw[D / 32][2];
+      uint32_t peak = 0;
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        uint4 w[2];
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          w[e] = live ? *reinterpret_cast<const uint4 *>(src + 64 * i + 8 * e) : make_uint4(0, 0, 0, 0);
-        qf[4 * i][0] = w[0].x;
-        qf[4 * i][1] = w[0].y;
-        qf[4 * i + 1][0] = w[0].z;
-        qf[4 * i + 1][1] = w[0].w;
-        qf[4 * i + 2][0] = w[1].x;
-        qf[4 * i + 2][1] = w[1].y;
-        qf[4 * i + 3][0] = w[1].z;
-        qf[4 * i + 3][1] = w[1].w;
-      }
+        for (int e = 0; e < 2; ++e) {
+          raw[i][e] = live ? *reinterpret_cast<const uint2 *>(src + 32 * i + 16 * e) : make_uint2(0, 0);
+          peak = max(peak, max(max(raw[i][e].x & 0x7FFFu, (raw[i][e].x >> 16) & 0x7FFFu),
+                               max(raw[i][e].y & 0x7FFFu, (raw[i][e].y >> 16) & 0x7FFFu)));
+        }
+      peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 1));
+      peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 2));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        if ((i & 3) == warp) F::Query::put(reinterpret_cast<uint2 *>(few_ring + F::kOffQ), i, raw[i][0], raw[i][1], peak);
+      const float up = F::Query::scale_of(peak);
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
+        c[hh] = p.scale * kLog2e * __shfl_sync(0xFFFFFFFFu, up, (2 * tq + hh) * 4);
         const int rr = rt * 8 + 2 * tq + hh;
         lim[hh] = rr < rows ? lim0 + rr / p.gq : -1;
       }
@@ -191,114 +330,99 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
     for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-    // ---- this warp's 16-token steps ----
-    const int t_end = min(ctx, (u0 + n) * kUnit);
-    int t = u0 * kUnit + 16 * warp;
+    // ---- this warp's steps of 32 tokens ----
+    const int t_end = min(ctx, (u0 + n) * kFewUnit);
+    int t = u0 * kFewUnit + 32 * warp;
     const int32_t *trow = p.table + static_cast<size_t>(b) * p.width;
-    const int bpp = p.page >> p.block_shift;
-    // Where step t's tokens are: the table column, then (a step later) the page.
-    int col = page_col(p, t), at = t - col * p.page;
-    int ft = t;          // the next step to request, its column and place in the page
-    int fpg = ft < t_end ? trow[col] : -1;  // its page
-    const uint32_t row_bytes = static_cast<uint32_t>(p.Hkv) * D;
-    const uint32_t ring = smem_u32(few_ring) + warp * F::kWarpBytes;
-    const uint8_t *kbase = p.kc + static_cast<size_t>(h) * D + static_cast<size_t>(g) * row_bytes + 16 * tq;
-    const uint8_t *vbase = p.vc + static_cast<size_t>(h) * D + static_cast<size_t>(2 * tq) * row_bytes + (D == 64 ? 8 : 16) * g;
-    float ks[F::kStages], vs[F::kStages];  // scales of the requested steps, oldest first
-    bool ok[F::kStages];                   // and whether their page is in the cache
-    auto row_of = [&]() {  // a page outside the cache: page 0 is read and its tokens masked
-      const bool in = static_cast<uint32_t>(fpg) < static_cast<uint32_t>(p.pages);
-      return static_cast<uint64_t>((in ? static_cast<uint32_t>(fpg) : 0u) * static_cast<uint32_t>(p.page) + static_cast<uint32_t>(at)) * row_bytes;
-    };
-    auto request_k = [&](uint32_t slot, int e) {
-      if (ft < t_end) {
-        const uint8_t *src = kbase + row_of();
-        const uint32_t dst = ring + slot * (2 * F::kHalf) + 16 * lane;
+    const uint32_t ring = sbase + warp * F::kWarpBytes;
+    const uint32_t qat = sbase + F::kOffQ + 8 * lane;
+    const uint32_t kat[2] = {ring, ring + F::kTileBytes}, vat[2] = {ring + 2 * F::kTileBytes, ring + 3 * F::kTileBytes};
+    // The two tiles of the step to request next: their pages (looked up a step
+    // ahead; -1 where there is none) and the scales that come with their codes.
+    int pg[2];
+    float ks[2], vs[2];
+    auto look_up = [&](int tt) {
 #pragma unroll
-        for (int i = 0; i < KC; ++i) {
-          cp_async16_u32(dst + (2 * i) * 512, src + 64 * i);
-          cp_async16_u32(dst + (2 * i + 1) * 512, src + 64 * i + 8ull * row_bytes);
-        }
-        ok[e] = static_cast<uint32_t>(fpg) < static_cast<uint32_t>(p.pages);
-        const size_t sc = (static_cast<size_t>(ok[e] ? fpg : 0) * bpp + (at >> p.block_shift)) * p.Hkv + h;
+      for (int e = 0; e < 2; ++e) {
+        const int pos = tt + 16 * e;
+        pg[e] = pos < t_end ? trow[page_col(p, pos)] : -1;
+      }
+    };
+    auto slot_of = [&](int e, int tt) {  // first slot of a tile, or -1 without a page in the cache
+      const int pos = tt + 16 * e;
+      return static_cast<uint32_t>(pg[e]) < static_cast<uint32_t>(p.pages) ? pg[e] * p.page + (pos - page_col(p, pos) * p.page) : -1;
+    };
+    auto request = [&](const CUtensorMap &map, const uint32_t (&dst)[2], uint32_t bar, int slot0, int slot1) {
+      mbar_expect_tx_u32(bar, ((slot0 >= 0) + (slot1 >= 0)) * F::kTileBytes);
+#pragma unroll
+      for (int c = 0; c < (D + 127) / 128; ++c) {
+        if (slot0 >= 0) tma_box2d(dst[0] + 2048 * c, &map, h * D + 128 * c, slot0, bar);
+        if (slot1 >= 0) tma_box2d(dst[1] + 2048 * c, &map, h * D + 128 * c, slot1, bar);
+      }
+    };
+    auto request_k = [&](int tt, bool (&in)[2]) {
+      if (tt >= t_end) return;
+      const int s0 = slot_of(0, tt), s1 = slot_of(1, tt);
+      in[0] = s0 >= 0;
+      in[1] = s1 >= 0;
+      if (lane == 0 && !dead) request(kmap, kat, kbar, s0, s1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const size_t sc = static_cast<size_t>(max(e ? s1 : s0, 0) >> p.block_shift) * p.Hkv + h;
         ks[e] = __ldg(p.ks + sc);
         vs[e] = __ldg(p.vs + sc);
       }
-      cp_async_commit();
     };
-    auto request_v = [&](uint32_t slot) {  // and on to the next step
-      if (ft < t_end) {
-        const uint8_t *src = vbase + row_of();
-        const uint32_t dst = ring + slot * (2 * F::kHalf) + F::kHalf + (D == 64 ? 8 : 16) * lane;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t *r = src + static_cast<uint64_t>((k & 1) + 8 * (k >> 1)) * row_bytes;
-          if (D == 64) {
-            cp_async8_u32(dst + k * 256, r);
-          } else {
-#pragma unroll
-            for (int i = 0; i < VC; ++i) cp_async16_u32(dst + (k * VC + i) * 512, r + 128 * i);
-          }
-        }
-        ft += kUnit;
-        at += kUnit;
-        while (at >= p.page) {
-          at -= p.page;
-          ++col;
-        }
-        fpg = ft < t_end ? trow[col] : -1;
-      }
-      cp_async_commit();
+    auto request_v = [&](int tt) {
+      if (tt < t_end && lane == 0 && !dead) request(vmap, vat, vbar, slot_of(0, tt), slot_of(1, tt));
     };
-#pragma unroll
-    for (int e = 0; e < F::kStages; ++e) {
-      request_k(e, e);
-      request_v(e);
-    }
-    uint32_t slot = 0;
-    for (; t < t_end; t += kUnit) {
-      const uint32_t kst = ring + slot * (2 * F::kHalf), vst = kst + F::kHalf;
-      // Groups in flight behind this step's K: its V and the steps after it.
-      cp_async_wait<2 * F::kStages - 1>();
-      // S^T = K Q^T, two chains
-      float sa[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const uint4 k0 = lds128(kst + 16 * lane + (2 * i) * 512), k1 = lds128(kst + 16 * lane + (2 * i + 1) * 512);
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w};
-        const uint32_t w1[4] = {k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x0 = w0[j], x1 = w1[j];
-          const uint32_t a[4] = {widen2<E4M3, 0>(x0), widen2<E4M3, 0>(x1), widen2<E4M3, 1>(x0), widen2<E4M3, 1>(x1)};
-          mma_bf16(j & 1 ? sb : sa, a, qf[4 * i + j][0], qf[4 * i + j][1]);
+    auto arrived = [&](uint32_t bar) {  // bounded: a copy that never lands sets the error word
+      uint32_t spins = 0;
+      while (!dead && !mbar_try_wait_u32(bar, phase))
+        if (++spins >= kFewSpin) {
+          set_error(err, kErrTimeout);
+          dead = true;
         }
-      }
-      const float k_scale = ks[0], v_raw = vs[0];
-      const bool in = ok[0];
+      dead = __any_sync(0xFFFFFFFFu, dead);
+    };
+    bool in_next[2] = {false, false};
+    look_up(t);
+    request_k(t, in_next);
+    request_v(t);
+    look_up(t + kFewUnit);
+    __syncthreads();  // the query rows are in place
+    for (; t < t_end; t += kFewUnit) {
+      const bool in[2] = {in_next[0], in_next[1]};
+      float sc[2][4];  // (token g, row 2 tq), (g, 2 tq + 1), (g + 8, 2 tq), (g + 8, 2 tq + 1)
+      arrived(kbar);
+      F::Query::scores(kat, qat, sc);
+      const float k_scale[2] = {ks[0], ks[1]};
+      float lv[2], rv[2];
 #pragma unroll
-      for (int e = 0; e + 1 < F::kStages; ++e) {
-        ks[e] = ks[e + 1];
-        vs[e] = vs[e + 1];
-        ok[e] = ok[e + 1];
+      for (int e = 0; e < 2; ++e) {
+        const float v_scale = fmaxf(vs[e], 0x1p-110f);
+        lv[e] = lg2(v_scale);
+        rv[e] = rcp(v_scale);
       }
-      request_k(slot, F::kStages - 1);
+      __syncwarp();  // every lane has read its K
+      request_k(t + kFewUnit, in_next);
 
       // t_j, the running reference, the weights
-      const float v_scale = fmaxf(v_raw, 0x1p-110f);
-      const float lv = __log2f(v_scale), rv = __frcp_rn(v_scale);
-      float x[4];
+      float x[2][4];
+      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int tok = t + g + 8 * (e >> 1), hh = e & 1;
-        const float s = __fadd_rn(sa[e], sb[e]);
-        x[e] = in && tok <= lim[hh] ? __fmaf_rn(s, p.scale * kLog2e * k_scale, lv) : -INFINITY;
-      }
-      if (__any_sync(0xFFFFFFFFu, fmaxf(x[0], x[2]) > m[0] + kLazy || fmaxf(x[1], x[3]) > m[1] + kLazy)) {
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int tok = t + 16 * e + g + 8 * (k >> 1), hh = k & 1;
+          x[e][k] = in[e] && tok <= lim[hh] ? __fmaf_rn(sc[e][k], c[hh] * k_scale[e], lv[e]) : -INFINITY;
+          top[hh] = fmaxf(top[hh], x[e][k]);
+        }
+      if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
         float al[2];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          float cm = fmaxf(x[hh], x[hh + 2]);
+          float cm = top[hh];
 #pragma unroll
           for (int s = 4; s <= 16; s <<= 1) cm = fmaxf(cm, __shfl_xor_sync(0xFFFFFFFFu, cm, s));
           cm = fmaxf(cm, m[hh]);
@@ -314,65 +438,70 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
           o[j][3] *= al[1];
         }
       }
-      const float r0 = m[0] == -INFINITY ? 0.0f : m[0], r1 = m[1] == -INFINITY ? 0.0f : m[1];
-      const float p0 = ex2(x[0] - r0), p1 = ex2(x[1] - r1), p2 = ex2(x[2] - r0), p3 = ex2(x[3] - r1);
-      l[0] = __fmaf_rn(p0 + p2, rv, l[0]);
-      l[1] = __fmaf_rn(p1 + p3, rv, l[1]);
-      uint32_t hi0, lo0, hi1, lo1;
-      split_bf16x2(p0, p1, hi0, lo0);
-      split_bf16x2(p2, p3, hi1, lo1);
-      hi0 = movm_t(hi0);
-      hi1 = movm_t(hi1);
-      lo0 = movm_t(lo0);
-      lo1 = movm_t(lo1);
-
-      // Slots past the context (or of a page outside the cache) may hold
-      // anything, NaN codes too: their value bytes are zeroed.
-      const int live = in ? min(16, ctx - t) : 0;
-      uint32_t keep[4];
+      const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+      uint32_t hi[2][2], lo[2][2];  // [tile][tokens g | g + 8 transposed]
 #pragma unroll
-      for (int k = 0; k < 4; ++k) keep[k] = 2 * tq + (k & 1) + 8 * (k >> 1) < live ? 0xFFFFFFFFu : 0u;
-      // O^T += V^T P^T
-      cp_async_wait<2 * F::kStages - 1>();
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = ex2(x[e][0] - ref[0]), p1 = ex2(x[e][1] - ref[1]);
+        const float p2 = ex2(x[e][2] - ref[0]), p3 = ex2(x[e][3] - ref[1]);
+        l[0] = __fmaf_rn(p0 + p2, rv[e], l[0]);
+        l[1] = __fmaf_rn(p1 + p3, rv[e], l[1]);
+        split_bf16x2(p0, p1, hi[e][0], lo[e][0]);
+        split_bf16x2(p2, p3, hi[e][1], lo[e][1]);
 #pragma unroll
-      for (int i = 0; i < VC; ++i) {
-        uint32_t v[4][4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (D == 64) {
-            const uint2 y = lds64(vst + 8 * lane + k * 256);
-            v[k][0] = y.x;
-            v[k][1] = y.y;
-          } else {
-            const uint4 y = lds128(vst + 16 * lane + (k * VC + i) * 512);
-            v[k][0] = y.x;
-            v[k][1] = y.y;
-            v[k][2] = y.z;
-            v[k][3] = y.w;
-          }
-        }
-        if (live < 16) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) v[k][w] &= keep[k];
-        }
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          const uint32_t la = prmt(v[0][w], v[1][w], 0x5140u), ha = prmt(v[0][w], v[1][w], 0x7362u);
-          const uint32_t lb = prmt(v[2][w], v[3][w], 0x5140u), hb = prmt(v[2][w], v[3][w], 0x7362u);
-          const uint32_t a0[4] = {widen2<E4M3, 0>(la), widen2<E4M3, 1>(la), widen2<E4M3, 0>(lb), widen2<E4M3, 1>(lb)};
-          const uint32_t a1[4] = {widen2<E4M3, 0>(ha), widen2<E4M3, 1>(ha), widen2<E4M3, 0>(hb), widen2<E4M3, 1>(hb)};
-          mma_bf16(o[2 * VW * i + 2 * w], a0, hi0, hi1);
-          mma_bf16(o[2 * VW * i + 2 * w + 1], a1, hi0, hi1);
-          mma_bf16(o[2 * VW * i + 2 * w], a0, lo0, lo1);
-          mma_bf16(o[2 * VW * i + 2 * w + 1], a1, lo0, lo1);
+        for (int k = 0; k < 2; ++k) {
+          hi[e][k] = movm_t(hi[e][k]);
+          lo[e][k] = movm_t(lo[e][k]);
         }
       }
-      request_v(slot);
-      slot = slot + 1 == F::kStages ? 0 : slot + 1;
+
+      // O^T += V^T P^T.  Slots past the context (or of a page outside the
+      // cache) may hold anything, NaN codes too: their value bytes are zeroed.
+      arrived(vbar);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int live = in[e] ? min(16, ctx - t - 16 * e) : 0;
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+          uint32_t v[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (D == 64) {
+              const uint2 y = lds64(vat[e] + tile_offset<D>(2 * tq + (k & 1) + 8 * (k >> 1), g >> 1) + 8 * (g & 1));
+              v[k][0] = y.x;
+              v[k][1] = y.y;
+            } else {
+              const uint4 y = lds128(vat[e] + tile_offset<D>(2 * tq + (k & 1) + 8 * (k >> 1), 8 * i + g));
+              v[k][0] = y.x;
+              v[k][1] = y.y;
+              v[k][2] = y.z;
+              v[k][3] = y.w;
+            }
+          }
+          if (live < 16) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) v[k][w] = 2 * tq + (k & 1) + 8 * (k >> 1) < live ? v[k][w] : 0u;
+          }
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            const uint32_t la = prmt(v[0][w], v[1][w], 0x5140u), ha = prmt(v[0][w], v[1][w], 0x7362u);
+            const uint32_t lb = prmt(v[2][w], v[3][w], 0x5140u), hb = prmt(v[2][w], v[3][w], 0x7362u);
+            const uint32_t a0[4] = {widen2<E4M3, 0>(la), widen2<E4M3, 1>(la), widen2<E4M3, 0>(lb), widen2<E4M3, 1>(lb)};
+            const uint32_t a1[4] = {widen2<E4M3, 0>(ha), widen2<E4M3, 1>(ha), widen2<E4M3, 0>(hb), widen2<E4M3, 1>(hb)};
+            mma_bf16(o[2 * VW * i + 2 * w], a0, hi[e][0], hi[e][1]);
+            mma_bf16(o[2 * VW * i + 2 * w + 1], a1, hi[e][0], hi[e][1]);
+            mma_bf16(o[2 * VW * i + 2 * w], a0, lo[e][0], lo[e][1]);
+            mma_bf16(o[2 * VW * i + 2 * w + 1], a1, lo[e][0], lo[e][1]);
+          }
+        }
+      }
+      phase ^= 1u;
+      __syncwarp();  // every lane has read its V
+      request_v(t + kFewUnit);
+      look_up(t + 2 * kFewUnit);
     }
-    cp_async_wait<0>();
 
     // ---- join the four warps ----
 #pragma unroll
@@ -433,10 +562,14 @@ __global__ void __launch_bounds__(kFewThreads, Few<D>::kCtas) k_q8_few(Q8View p)
         if (d == 0) p.part_ml[part_slot * 8 + r] = make_float2(mm, ll);
       }
     }
-    __syncthreads();  // s_m, s_l and s_o are rewritten by the next piece
+    fence_proxy_async();  // the next piece's copies land where the sums were
+    __syncthreads();      // and s_m, s_l and s_o are rewritten
     cur += n;
     off += n;
   }
+  if (dead)  // give what is still in flight as long again before the CTA may end
+    for (uint32_t spins = 0; spins < kFewSpin && !(mbar_try_wait_u32(kbar, phase) && mbar_try_wait_u32(vbar, phase)); ++spins) {
+    }
   if (first >= end && threadIdx.x == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
   // rows of sequences without a token
   for (int e = blockIdx.x; e < p.B; e += gridDim.x) {
@@ -585,14 +718,49 @@ Carve carve(const FnQ8AttentionArgs *a, const Q8View &p, bool few, bool many) {
   return c;
 }
 
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no -lcuda).
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn q8_encode_fn() {
+  static std::once_flag once;
+  static EncodeTiledFn fn = nullptr;
+  std::call_once(once, [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// Codes as a byte matrix [slots][Hkv * D]: boxes of 16 slots x 128 (or 64) bytes.
+bool make_codes_map(CUtensorMap *map, const void *base, uint64_t slots, uint64_t cols, int D) {
+  EncodeTiledFn fn = q8_encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {cols, slots};
+  const cuuint64_t strides[1] = {cols};
+  const cuuint32_t box[2] = {D == 64 ? 64u : 128u, 16};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool E4M3>
 cudaError_t launch_few(const Q8View &p, bool pdl, cudaStream_t s) {
-  using F = Few<D>;
+  using F = Few<D, E4M3>;
+  CUtensorMap km, vm;
+  const uint64_t slots = static_cast<uint64_t>(p.pages) * p.page, cols = static_cast<uint64_t>(p.Hkv) * D;
+  if (!make_codes_map(&km, p.kc, slots, cols, D) || !make_codes_map(&vm, p.vc, slots, cols, D)) return cudaErrorInvalidValue;
   // Set for every call: the attribute belongs to the current device.
   const cudaError_t e = cudaFuncSetAttribute(k_q8_few<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
-  if (pdl) return launch_pdl(k_q8_few<D, E4M3>, dim3(F::kMax), dim3(kFewThreads), F::kSmem, s, p);
-  k_q8_few<D, E4M3><<<F::kMax, kFewThreads, F::kSmem, s>>>(p);
+  uint32_t *err = device_error_word();
+  if (pdl) return launch_pdl(k_q8_few<D, E4M3>, dim3(F::kMax), dim3(kFewThreads), F::kSmem, s, p, km, vm, err);
+  k_q8_few<D, E4M3><<<F::kMax, kFewThreads, F::kSmem, s>>>(p, km, vm, err);
   return cudaSuccess;
 }
 
@@ -644,7 +812,7 @@ bool wants_many(const Q8View &p) {
 }  // namespace
 
 int few_ctas(int head_dim) {
-  return head_dim == 256 ? Few<256>::kMax : head_dim == 128 ? Few<128>::kMax : Few<64>::kMax;
+  return head_dim == 256 ? Few<256, false>::kMax : head_dim == 128 ? Few<128, false>::kMax : Few<64, false>::kMax;
 }
 
 int paged_attention_q8_workspace_size(const FnQ8AttentionArgs *a, uint64_t *bytes, std::string &err) {

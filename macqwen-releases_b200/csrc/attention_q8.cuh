@@ -6,9 +6,9 @@
 //   k_j = ks[block of j] * kcode_j,  v_j = vs[block of j] * vcode_j,
 //   j over the positions up to row i's own whose page is in the cache.
 //
-// Codes go to the tensor cores as bfloat16, in which they are exact (int8 has
-// 7 bits and a sign, e4m3 4 bits), next to the queries as they are; the two
-// block scales enter in float32.  With
+// Codes go to the tensor cores as numbers in which they are exact (bfloat16
+// holds int8's 7 bits and sign and e4m3's 4 bits); the two block scales enter
+// in float32.  With
 //   t_j = (scale * log2 e * ks) (q . kcode_j) + log2 vs,   u_j = 2^(t_j - m),
 // m a running reference of the t_j,
 //   out = sum_j u_j vcode_j / sum_blocks (1 / vs) sum_(j in block) u_j :
@@ -63,6 +63,17 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+// Of normal numbers; within 2^-22 and 2^-23.
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t d;
   asm("prmt.b32 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
@@ -106,6 +117,31 @@ __device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// m16n8k32 with signed A bytes and unsigned (or signed) B bytes.
+template <bool SIGNED_B>
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (SIGNED_B)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two e4m3 codes in bytes (0, 1) or (2, 3) of w as float16.
+template <int HALF>
+__device__ __forceinline__ uint32_t e4m3_f16(uint32_t w) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(HALF ? w >> 16 : w)));
+  return h;
+}
+
 // Two codes in bytes (0, 1) (HALF 0) or (2, 3) (HALF 1) of w, as bfloat16 pairs.
 // int8: under the high byte 0x43, the low seven bits l of a code read as
 // 128 + l and its sign bit alone as 128 (clear) or 256 (set); the difference
@@ -115,8 +151,7 @@ template <bool E4M3, int HALF>
 __device__ __forceinline__ uint32_t widen2(uint32_t w) {
   uint32_t d;
   if (E4M3) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(HALF ? w >> 16 : w)));
+    const uint32_t h = e4m3_f16<HALF>(w);
     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
     d = pack_bf16x2(f.x, f.y);
   } else {

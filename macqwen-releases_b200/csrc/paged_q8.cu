@@ -510,8 +510,8 @@ int check_q8_cache(const FnQ8Cache &c, std::string &err) {
   }
   if (c.num_pages == 0 || c.num_pages > 0x7FFFFFFFu || c.page_size == 0 || c.page_size > (1u << 20) ||
       c.page_size % c.block || c.kv_heads == 0 || c.kv_heads > 32767u ||
-      static_cast<uint64_t>(c.num_pages) * c.page_size > 0xFFFFFFFFull) {
-    err = "the cache needs pages, kv heads, a page_size that is a multiple of block and fewer than 2^32 slots";
+      static_cast<uint64_t>(c.num_pages) * c.page_size > 0x7FFFFFFFull) {
+    err = "the cache needs pages, kv heads, a page_size that is a multiple of block and fewer than 2^31 slots";
     return FNMOE_ERR_SHAPE;
   }
   if (misaligned(c.k_codes, 16) || misaligned(c.v_codes, 16) || misaligned(c.k_scale, 4) ||
