@@ -55,6 +55,12 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int c) {
   if (D == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
   return (c >> 3) * 2048 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
+// The offset 2 st chunks on from one in the first two: the chunk's bits are
+// exclusive-ored, and box st / 4 follows 2048 bytes later.
+template <int D>
+__device__ __forceinline__ uint32_t step_offset(uint32_t off, int st) {
+  return (off ^ ((2 * (st & 3)) << 4)) + (st >> 2) * 2048;
+}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -86,13 +92,13 @@ struct QueryE4M3 {
     q[(2 * s + 1) * 32 + lane] = make_uint2(pair(b.x), pair(b.y));
   }
   static __device__ __forceinline__ void scores(const uint32_t (&at)[2], uint32_t q, float (&s)[2][4]) {
-    const int lane = threadIdx.x & 31, row = lane & 15, half = lane >> 4;
+    const uint32_t off = tile_offset<D>(threadIdx.x & 15, (threadIdx.x >> 4) & 1);
     float c[2][2][4] = {};  // two chains a tile
 #pragma unroll
     for (int st = 0; st < D / 32; ++st) {
       uint32_t w[2][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) ldsm_x4(at[u] + tile_offset<D>(row, 2 * st + half), w[u]);
+      for (int u = 0; u < 2; ++u) ldsm_x4(at[u] + step_offset<D>(off, st), w[u]);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint2 b = lds64(q + (2 * st + k) * 256);
@@ -141,7 +147,7 @@ struct QueryInt8 {
     for (int p = 0; p < 3; ++p) q[(p * (D / 32) + s) * 32 + lane] = make_uint2(plane[p][0], plane[p][1]);
   }
   static __device__ __forceinline__ void scores(const uint32_t (&at)[2], uint32_t q, float (&s)[2][4]) {
-    const int lane = threadIdx.x & 31, row = lane & 15, half = lane >> 4;
+    const uint32_t off = tile_offset<D>(threadIdx.x & 15, (threadIdx.x >> 4) & 1);
     int c[2][3][4] = {};
 #pragma unroll
     for (int st = 0; st < D / 32; ++st) {
@@ -149,7 +155,7 @@ struct QueryInt8 {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t a[4];
-        ldsm_x4(at[u] + tile_offset<D>(row, 2 * st + half), a);
+        ldsm_x4(at[u] + step_offset<D>(off, st), a);
         mma_s8<false>(c[u][0], a[0], a[1], a[2], a[3], b0.x, b0.y);
         mma_s8<false>(c[u][1], a[0], a[1], a[2], a[3], b1.x, b1.y);
         mma_s8<true>(c[u][2], a[0], a[1], a[2], a[3], b2.x, b2.y);
@@ -249,7 +255,6 @@ __device__ Found find_unit(const Q8View &p, int cta, int ctas, long long &start,
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8View p, const __grid_constant__ CUtensorMap kmap,
                                                                                  const __grid_constant__ CUtensorMap vmap, uint32_t *err) {
-  constexpr int KC = D / 64;               // 16-byte pieces of a K row per lane
   constexpr int VC = D == 64 ? 1 : D / 128;  // pieces of a V row per lane
   constexpr int VW = D == 64 ? 2 : 4;      // words of a V piece
   constexpr int MT = D / 16;               // 16-dim tiles of O^T
@@ -321,9 +326,11 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       for (int hh = 0; hh < 2; ++hh) {
         c[hh] = p.scale * kLog2e * __shfl_sync(0xFFFFFFFFu, up, (2 * tq + hh) * 4);
         const int rr = rt * 8 + 2 * tq + hh;
-        lim[hh] = rr < rows ? lim0 + rr / p.gq : -1;
+        lim[hh] = rr < rows ? lim0 + rr / p.gq : 0x7FFFFFFF;  // rows past the end: never written
       }
     }
+
+    const int lim_min = __reduce_min_sync(0xFFFFFFFFu, min(lim[0], lim[1]));
 
     float o[MT][4];
 #pragma unroll
@@ -336,21 +343,22 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
     const int32_t *trow = p.table + static_cast<size_t>(b) * p.width;
     const uint32_t ring = sbase + warp * F::kWarpBytes;
     const uint32_t qat = sbase + F::kOffQ + 8 * lane;
+    // This lane's value bytes of tokens 2t, 2t + 1 (tokens + 8 lie half a box on).
+    const uint32_t v_off[2] = {D == 64 ? tile_offset<D>(2 * tq, g >> 1) + 8 * (g & 1) : tile_offset<D>(2 * tq, g),
+                               D == 64 ? tile_offset<D>(2 * tq + 1, g >> 1) + 8 * (g & 1) : tile_offset<D>(2 * tq + 1, g)};
     const uint32_t kat[2] = {ring, ring + F::kTileBytes}, vat[2] = {ring + 2 * F::kTileBytes, ring + 3 * F::kTileBytes};
     // The two tiles of the step to request next: their pages (looked up a step
     // ahead; -1 where there is none) and the scales that come with their codes.
-    int pg[2];
+    int pg[2], inpage[2], slot[2];
     float ks[2], vs[2];
+    const float *ks_h = p.ks + h, *vs_h = p.vs + h;
     auto look_up = [&](int tt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int pos = tt + 16 * e;
-        pg[e] = pos < t_end ? trow[page_col(p, pos)] : -1;
+        const int pos = tt + 16 * e, cc = page_col(p, pos);
+        inpage[e] = pos - cc * p.page;
+        pg[e] = pos < t_end ? trow[cc] : -1;
       }
-    };
-    auto slot_of = [&](int e, int tt) {  // first slot of a tile, or -1 without a page in the cache
-      const int pos = tt + 16 * e;
-      return static_cast<uint32_t>(pg[e]) < static_cast<uint32_t>(p.pages) ? pg[e] * p.page + (pos - page_col(p, pos) * p.page) : -1;
     };
     auto request = [&](const CUtensorMap &map, const uint32_t (&dst)[2], uint32_t bar, int slot0, int slot1) {
       mbar_expect_tx_u32(bar, ((slot0 >= 0) + (slot1 >= 0)) * F::kTileBytes);
@@ -360,21 +368,21 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
         if (slot1 >= 0) tma_box2d(dst[1] + 2048 * c, &map, h * D + 128 * c, slot1, bar);
       }
     };
-    auto request_k = [&](int tt, bool (&in)[2]) {
+    auto request_k = [&](int tt) {
       if (tt >= t_end) return;
-      const int s0 = slot_of(0, tt), s1 = slot_of(1, tt);
-      in[0] = s0 >= 0;
-      in[1] = s1 >= 0;
-      if (lane == 0 && !dead) request(kmap, kat, kbar, s0, s1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)  // first slot of the tile, or -1 without a page in the cache
+        slot[e] = static_cast<uint32_t>(pg[e]) < static_cast<uint32_t>(p.pages) ? pg[e] * p.page + inpage[e] : -1;
+      if (lane == 0 && !dead) request(kmap, kat, kbar, slot[0], slot[1]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const size_t sc = static_cast<size_t>(max(e ? s1 : s0, 0) >> p.block_shift) * p.Hkv + h;
-        ks[e] = __ldg(p.ks + sc);
-        vs[e] = __ldg(p.vs + sc);
+        const uint64_t sc = static_cast<uint64_t>(static_cast<uint32_t>(max(slot[e], 0)) >> p.block_shift) * static_cast<uint32_t>(p.Hkv);
+        ks[e] = __ldg(ks_h + sc);
+        vs[e] = __ldg(vs_h + sc);
       }
     };
     auto request_v = [&](int tt) {
-      if (tt < t_end && lane == 0 && !dead) request(vmap, vat, vbar, slot_of(0, tt), slot_of(1, tt));
+      if (tt < t_end && lane == 0 && !dead) request(vmap, vat, vbar, slot[0], slot[1]);
     };
     auto arrived = [&](uint32_t bar) {  // bounded: a copy that never lands sets the error word
       uint32_t spins = 0;
@@ -385,14 +393,13 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
         }
       dead = __any_sync(0xFFFFFFFFu, dead);
     };
-    bool in_next[2] = {false, false};
     look_up(t);
-    request_k(t, in_next);
+    request_k(t);
     request_v(t);
     look_up(t + kFewUnit);
     __syncthreads();  // the query rows are in place
     for (; t < t_end; t += kFewUnit) {
-      const bool in[2] = {in_next[0], in_next[1]};
+      const bool in[2] = {slot[0] >= 0, slot[1] >= 0};
       float sc[2][4];  // (token g, row 2 tq), (g, 2 tq + 1), (g + 8, 2 tq), (g + 8, 2 tq + 1)
       arrived(kbar);
       F::Query::scores(kat, qat, sc);
@@ -405,19 +412,28 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
         rv[e] = rcp(v_scale);
       }
       __syncwarp();  // every lane has read its K
-      request_k(t + kFewUnit, in_next);
+      request_k(t + kFewUnit);
 
       // t_j, the running reference, the weights
       float x[2][4];
-      float top[2] = {-INFINITY, -INFINITY};
+      float top[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = t + 16 * e + g + 8 * (k >> 1), hh = k & 1;
-          x[e][k] = in[e] && tok <= lim[hh] ? __fmaf_rn(sc[e][k], c[hh] * k_scale[e], lv[e]) : -INFINITY;
-          top[hh] = fmaxf(top[hh], x[e][k]);
+        for (int hh = 0; hh < 2; ++hh) {
+          const float mul = c[hh] * k_scale[e];
+          x[e][hh] = __fmaf_rn(sc[e][hh], mul, lv[e]);
+          x[e][2 + hh] = __fmaf_rn(sc[e][2 + hh], mul, lv[e]);
         }
+      if (!in[0] || !in[1] || t + 31 > lim_min) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (!in[e] || t + 16 * e + g + 8 * (k >> 1) > lim[k & 1]) x[e][k] = -INFINITY;
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) top[hh] = fmaxf(fmaxf(x[0][hh], x[0][2 + hh]), fmaxf(x[1][hh], x[1][2 + hh]));
       if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
         float al[2];
 #pragma unroll
@@ -456,29 +472,31 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       }
 
       // O^T += V^T P^T.  Slots past the context (or of a page outside the
-      // cache) may hold anything, NaN codes too: their value bytes are zeroed.
+      // cache) may hold anything and weigh 0; e4m3 codes can be NaN, so those
+      // slots' bytes are zeroed.
       arrived(vbar);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int live = in[e] ? min(16, ctx - t - 16 * e) : 0;
+        const bool tail = E4M3 && __any_sync(0xFFFFFFFFu, live < 16);
 #pragma unroll
         for (int i = 0; i < VC; ++i) {
           uint32_t v[4][4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (D == 64) {
-              const uint2 y = lds64(vat[e] + tile_offset<D>(2 * tq + (k & 1) + 8 * (k >> 1), g >> 1) + 8 * (g & 1));
+              const uint2 y = lds64(vat[e] + v_off[k & 1] + (k >> 1) * 512);
               v[k][0] = y.x;
               v[k][1] = y.y;
             } else {
-              const uint4 y = lds128(vat[e] + tile_offset<D>(2 * tq + (k & 1) + 8 * (k >> 1), 8 * i + g));
+              const uint4 y = lds128(vat[e] + v_off[k & 1] + (k >> 1) * 1024 + i * 2048);
               v[k][0] = y.x;
               v[k][1] = y.y;
               v[k][2] = y.z;
               v[k][3] = y.w;
             }
           }
-          if (live < 16) {
+          if (tail) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -486,10 +504,10 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
           }
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
-            const uint32_t la = prmt(v[0][w], v[1][w], 0x5140u), ha = prmt(v[0][w], v[1][w], 0x7362u);
-            const uint32_t lb = prmt(v[2][w], v[3][w], 0x5140u), hb = prmt(v[2][w], v[3][w], 0x7362u);
-            const uint32_t a0[4] = {widen2<E4M3, 0>(la), widen2<E4M3, 1>(la), widen2<E4M3, 0>(lb), widen2<E4M3, 1>(lb)};
-            const uint32_t a1[4] = {widen2<E4M3, 0>(ha), widen2<E4M3, 1>(ha), widen2<E4M3, 0>(hb), widen2<E4M3, 1>(hb)};
+            uint32_t a[4], b4[4];  // [dim of the word]: tokens (2t, 2t+1), tokens (2t+8, 2t+9)
+            widen_pairs<E4M3>(v[0][w], v[1][w], a);
+            widen_pairs<E4M3>(v[2][w], v[3][w], b4);
+            const uint32_t a0[4] = {a[0], a[1], b4[0], b4[1]}, a1[4] = {a[2], a[3], b4[2], b4[3]};
             mma_bf16(o[2 * VW * i + 2 * w], a0, hi[e][0], hi[e][1]);
             mma_bf16(o[2 * VW * i + 2 * w + 1], a1, hi[e][0], hi[e][1]);
             mma_bf16(o[2 * VW * i + 2 * w], a0, lo[e][0], lo[e][1]);

@@ -161,6 +161,29 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
   return d;
 }
 
+// Codes of four dims of two tokens (words w0, w1) as bfloat16 pairs (token 0,
+// token 1), one for each dim.  int8 as in widen2, with the byte that prmt
+// leaves between the two replaced under the mask.
+template <bool E4M3>
+__device__ __forceinline__ void widen_pairs(uint32_t w0, uint32_t w1, uint32_t (&d)[4]) {
+  if (E4M3) {
+    const uint32_t lo = prmt(w0, w1, 0x5140u), hi = prmt(w0, w1, 0x7362u);
+    d[0] = widen2<true, 0>(lo);
+    d[1] = widen2<true, 1>(lo);
+    d[2] = widen2<true, 0>(hi);
+    d[3] = widen2<true, 1>(hi);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t x = prmt(w0, w1, i | (i << 4) | ((4 + i) << 8) | ((4 + i) << 12));
+      uint32_t a, b;  // (x & mask) | 0x43004300
+      asm("lop3.b32 %0, %1, 0x007F007F, 0x43004300, 0xEA;\n" : "=r"(a) : "r"(x));
+      asm("lop3.b32 %0, %1, 0x00800080, 0x43004300, 0xEA;\n" : "=r"(b) : "r"(x));
+      asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(d[i]) : "r"(a), "r"(b));
+    }
+  }
+}
+
 __device__ __forceinline__ uint4 ldg_stream(const void *p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n"
