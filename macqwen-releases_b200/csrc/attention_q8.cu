@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <string>
@@ -30,8 +31,8 @@ namespace {
 //
 // A warp takes 32 tokens at a time, as two tiles of 16 whose chains of
 // dependent instructions overlap.  It fetches them for itself: TMA boxes of
-// 16 tokens x 128 bytes (128-byte swizzle; 64 bytes at D 64) into shared memory
-// of its own, the next step's K as soon as this one's scores are done, the next
+// 16 or 32 tokens x 128 bytes (128-byte swizzle; 64 bytes at D 64) into shared
+// memory of its own, the next step's K as soon as this one's scores are done, the next
 // V when its products are; no warp waits for another inside a piece of work.
 // (Loads by the lanes themselves, to registers or by cp.async, stayed at
 // 3.5 TB/s whatever the occupancy.)
@@ -47,19 +48,19 @@ constexpr int kFewUnit = 128;  // 4 warps x 32 tokens
 constexpr int kFewRows = 16;
 constexpr uint32_t kFewSpin = 1u << 22;  // mbarrier polls before a wait gives up
 
-// Byte offset, in a 16-token tile of codes, of the 16-byte chunk `c` of token
-// `row`: boxes of 16 rows x 128 bytes, chunk c at c ^ (row & 7), or one of 16 x
-// 64 bytes, c at c ^ ((row >> 1) & 3).
+// A step's codes of K (or V): 32 rows of 128 bytes, chunk c of a row at
+// c ^ (row & 7), for each 128-byte piece of D (the boxes' swizzle); at D 64, 32
+// rows of 64 bytes, c at c ^ ((row >> 1) & 3).  Rows 16 and on are the second
+// tile.  tile_offset: where chunk c of the first piece of a tile's row is.
 template <int D>
 __device__ __forceinline__ uint32_t tile_offset(int row, int c) {
-  if (D == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-  return (c >> 3) * 2048 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+  return D == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4) : row * 128 + ((c ^ (row & 7)) << 4);
 }
-// The offset 2 st chunks on from one in the first two: the chunk's bits are
-// exclusive-ored, and box st / 4 follows 2048 bytes later.
+// 2 st chunks on from one of a row's first two: the chunk's bits are
+// exclusive-ored, and the next piece follows 4096 bytes later.
 template <int D>
 __device__ __forceinline__ uint32_t step_offset(uint32_t off, int st) {
-  return (off ^ ((2 * (st & 3)) << 4)) + (st >> 2) * 2048;
+  return (off ^ ((2 * (st & 3)) << 4)) + (st >> 2) * 4096;
 }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
@@ -346,10 +347,11 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
     // This lane's value bytes of tokens 2t, 2t + 1 (tokens + 8 lie half a box on).
     const uint32_t v_off[2] = {D == 64 ? tile_offset<D>(2 * tq, g >> 1) + 8 * (g & 1) : tile_offset<D>(2 * tq, g),
                                D == 64 ? tile_offset<D>(2 * tq + 1, g >> 1) + 8 * (g & 1) : tile_offset<D>(2 * tq + 1, g)};
-    const uint32_t kat[2] = {ring, ring + F::kTileBytes}, vat[2] = {ring + 2 * F::kTileBytes, ring + 3 * F::kTileBytes};
+    constexpr uint32_t kTile1 = D == 64 ? 1024 : 2048;  // from a step's first tile to its second
+    const uint32_t kat[2] = {ring, ring + kTile1}, vat[2] = {ring + 2 * F::kTileBytes, ring + 2 * F::kTileBytes + kTile1};
     // The two tiles of the step to request next: their pages (looked up a step
     // ahead; -1 where there is none) and the scales that come with their codes.
-    int pg[2], inpage[2], slot[2];
+    int pg[2], inpage[2], slot[2] = {-1, -1};
     float ks[2], vs[2];
     const float *ks_h = p.ks + h, *vs_h = p.vs + h;
     auto look_up = [&](int tt) {
@@ -360,12 +362,21 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
         pg[e] = pos < t_end ? trow[cc] : -1;
       }
     };
-    auto request = [&](const CUtensorMap &map, const uint32_t (&dst)[2], uint32_t bar, int slot0, int slot1) {
-      mbar_expect_tx_u32(bar, ((slot0 >= 0) + (slot1 >= 0)) * F::kTileBytes);
+    // Pages of whole steps: one box of 32 rows for both tiles, else one of 16 each.
+    auto request = [&](const CUtensorMap &map, uint32_t dst, uint32_t bar) {
+      const int x = h * D;
+      if (p.pair_boxes) {
+        mbar_expect_tx_u32(bar, slot[0] >= 0 ? 2 * F::kTileBytes : 0);
+        if (slot[0] < 0) return;
 #pragma unroll
-      for (int c = 0; c < (D + 127) / 128; ++c) {
-        if (slot0 >= 0) tma_box2d(dst[0] + 2048 * c, &map, h * D + 128 * c, slot0, bar);
-        if (slot1 >= 0) tma_box2d(dst[1] + 2048 * c, &map, h * D + 128 * c, slot1, bar);
+        for (int c = 0; c < (D + 127) / 128; ++c) tma_box2d(dst + 4096 * c, &map, x + 128 * c, slot[0], bar);
+      } else {
+        mbar_expect_tx_u32(bar, ((slot[0] >= 0) + (slot[1] >= 0)) * F::kTileBytes);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int c = 0; c < (D + 127) / 128; ++c)
+            if (slot[e] >= 0) tma_box2d(dst + kTile1 * e + 4096 * c, &map, x + 128 * c, slot[e], bar);
       }
     };
     auto request_k = [&](int tt) {
@@ -373,7 +384,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
 #pragma unroll
       for (int e = 0; e < 2; ++e)  // first slot of the tile, or -1 without a page in the cache
         slot[e] = static_cast<uint32_t>(pg[e]) < static_cast<uint32_t>(p.pages) ? pg[e] * p.page + inpage[e] : -1;
-      if (lane == 0 && !dead) request(kmap, kat, kbar, slot[0], slot[1]);
+      if (lane == 0 && !dead) request(kmap, kat[0], kbar);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint64_t sc = static_cast<uint64_t>(static_cast<uint32_t>(max(slot[e], 0)) >> p.block_shift) * static_cast<uint32_t>(p.Hkv);
@@ -382,7 +393,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       }
     };
     auto request_v = [&](int tt) {
-      if (tt < t_end && lane == 0 && !dead) request(vmap, vat, vbar, slot[0], slot[1]);
+      if (tt < t_end && lane == 0 && !dead) request(vmap, vat[0], vbar);
     };
     auto arrived = [&](uint32_t bar) {  // bounded: a copy that never lands sets the error word
       uint32_t spins = 0;
@@ -489,7 +500,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
               v[k][0] = y.x;
               v[k][1] = y.y;
             } else {
-              const uint4 y = lds128(vat[e] + v_off[k & 1] + (k >> 1) * 1024 + i * 2048);
+              const uint4 y = lds128(vat[e] + v_off[k & 1] + (k >> 1) * 1024 + i * 4096);
               v[k][0] = y.x;
               v[k][1] = y.y;
               v[k][2] = y.z;
@@ -531,9 +542,15 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
         s_l[warp][2 * tq + hh] = l[hh];
       }
     }
-    if (cur == first && threadIdx.x == 0) {
+    if (threadIdx.x == 0) {
+      const bool cut = cur == first && u0 > 0, done = u0 == 0 && n == u.x;
       const long long a = cur - u0;
-      p.cuts[blockIdx.x] = u0 == 0 ? make_int4(-1, 0, 0, 0) : cut_of(b, h, rt, a, a, a + u.x - 1, f.total, ranges_of(f.total, gridDim.x), blockIdx.x);
+      if (p.by_seg ? cut || done : cur == first) {
+        const int4 c4 = cut ? cut_of(b, h, rt, a, a, a + u.x - 1, f.total, ranges_of(f.total, gridDim.x), blockIdx.x) : make_int4(-1, 0, 0, 0);
+        // by segment: only the first cut in it (or the one CTA that did it all) says so
+        if (!p.by_seg) p.cuts[blockIdx.x] = c4;
+        else if (!cut || c4.x >= 0) p.cuts[(static_cast<size_t>(b) * p.Hkv + h) * p.few_tiles + rt] = make_int4(c4.x, blockIdx.x - 1, c4.z, c4.w);
+      }
     }
     __syncthreads();  // also: every warp is done with its ring
 #pragma unroll
@@ -588,7 +605,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
   if (dead)  // give what is still in flight as long again before the CTA may end
     for (uint32_t spins = 0; spins < kFewSpin && !(mbar_try_wait_u32(kbar, phase) && mbar_try_wait_u32(vbar, phase)); ++spins) {
     }
-  if (first >= end && threadIdx.x == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (first >= end && threadIdx.x == 0 && !p.by_seg) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
   // rows of sequences without a token
   for (int e = blockIdx.x; e < p.B; e += gridDim.x) {
     const int2 u = units_of(p, e);
@@ -600,76 +617,94 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
 }
 
 // Joins the sums of segments that several CTAs worked on, in CTA order.  A CTA
-// takes two of the eight rows of a few-row cut, or 16 of the 128 rows of a
-// many-row cut (four at a time: cut tiles keep four dims of a row together).
-// A CTA's first piece of work is in workspace slot 2c, a later cut one in
-// 2c + 1.
+// takes one of the eight rows of a few-row segment, or four of the 128 rows of
+// a many-row one (cut tiles keep four dims of four rows together).  It finds
+// the cut by the segment where there are fewer of those than CTAs to cut them
+// (by_seg), else by the CTA whose range it begins.  A CTA's first piece of work
+// is in workspace slot 2c, a later cut one in 2c + 1.
 template <int D>
-__global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few_cuts, int many_cuts) {
-  constexpr int L = D / 4, G = 256 / L;
+__global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
+  constexpr int L = D / 4;
   __shared__ float4 s_o[256];
   __shared__ float s_l[256];
   pdl_wait();
-  const bool few = static_cast<int>(blockIdx.x) < 4 * few_cuts;
-  const int at = few ? blockIdx.x : blockIdx.x - 4 * few_cuts;
-  const int c1_cta = few ? at >> 2 : at >> 3;  // the cut is where CTA c1_cta + 1's range begins
-  const int4 cut = few ? p.cuts[c1_cta + 1] : p.tcuts[c1_cta + 1];
+  const bool is_few = static_cast<int>(blockIdx.x) < 8 * few;
+  const int at = is_few ? blockIdx.x >> 3 : (blockIdx.x - 8 * few) >> 5;
+  const int row0 = is_few ? blockIdx.x & 7 : 4 * ((blockIdx.x - 8 * few) & 31);
+  const bool by_seg = is_few ? p.by_seg : p.tby_seg;
+  int4 cut;
+  int c0, h;
+  if (by_seg) {
+    cut = (is_few ? p.cuts : p.tcuts)[at];
+    h = is_few ? at / p.few_tiles % p.Hkv : at % p.Hkv;
+    c0 = cut.y;
+    if (is_few) {  // segments without rows or tokens were not written
+      const int b = at / (p.few_tiles * p.Hkv), rows = rows_of(p, b).y * p.gq;
+      if (tokens_of(p, b) == 0 || rows > p.few_rows || at % p.few_tiles * 8 >= rows) return;
+    } else if (at / p.Hkv >= p.seq_tile[p.B] || p.tiles[at / p.Hkv].z == 0) {
+      return;
+    }
+  } else {
+    cut = (is_few ? p.cuts : p.tcuts)[at + 1];
+    h = cut.y;
+    c0 = at;
+  }
   if (cut.x < 0) return;
-  const int c0 = c1_cta, c1 = cut.w & 0x3FFFFFFF;
+  const int c1 = cut.w & 0x3FFFFFFF;
   const bool late0 = (cut.w >> 30) & 1;
   const int2 qr = rows_of(p, cut.x);
-  const int R = few ? 8 : 128, rows = qr.y * p.gq - cut.z * R;
-  const float2 *ml_all = few ? p.part_ml : p.tpart_ml;
+  const int R = is_few ? 8 : 128, rows = qr.y * p.gq - cut.z * R;
+  if (row0 >= rows) return;
+  // sub: which of the rows taken at once; lane: four dims; every `groups`-th CTA
+  const int per = is_few ? 1 : 4, groups = 256 / (L * per) > 0 ? 256 / (L * per) : 1;
+  const int sub = is_few ? 0 : threadIdx.x & 3;
+  const int lane = is_few ? threadIdx.x % L : (threadIdx.x >> 2) % L;
+  const int grp = threadIdx.x / (L * per), r = row0 + sub;
+  const float2 *ml_all = is_few ? p.part_ml : p.tpart_ml;
   auto slot_of = [&](int c) { return static_cast<size_t>(2 * c + (c == c0 && late0 ? 1 : 0)); };
-  // lane: four dims; sub: which row of those taken at once; grp: every G-th CTA
-  const int per = few ? 1 : 4, groups = G / per > 0 ? G / per : 1;
-  const int sub = few ? 0 : threadIdx.x & 3;
-  const int lane = few ? threadIdx.x % L : (threadIdx.x >> 2) % L;
-  const int grp = few ? threadIdx.x / L : threadIdx.x / (4 * L);
-  const int row_first = few ? 2 * (at & 3) : 16 * (at & 7), row_count = few ? 2 : 16;
-  for (int r0 = row_first; r0 < row_first + row_count && r0 < rows; r0 += per) {
-    const int r = r0 + sub;
-    float mm = -INFINITY;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, ml_all[slot_of(c) * R + r].x);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float ll = 0.0f;
-#pragma unroll 4
-    for (int c = c0 + grp; c <= c1; c += groups) {
-      const size_t s = slot_of(c);
-      const float2 ml = ml_all[s * R + r];
-      const float4 v = few ? *reinterpret_cast<const float4 *>(p.part + (s * 8 + r) * D + 4 * lane)
-                           : reinterpret_cast<const float4 *>(p.tpart)[(s * L + lane) * 128 + r];
-      const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
-      ll += ml.y * w;
-      acc.x += v.x * w;
-      acc.y += v.y * w;
-      acc.z += v.z * w;
-      acc.w += v.w * w;
-    }
-    if (groups > 1) {
-      const int stride = L * per;
-      __syncthreads();
-      s_o[threadIdx.x] = acc;
-      s_l[threadIdx.x] = ll;
-      __syncthreads();
-      if (grp == 0)
-        for (int g = 1; g < groups; ++g) {
-          const float4 v = s_o[threadIdx.x + g * stride];
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
-          ll += s_l[threadIdx.x + g * stride];
-        }
-    }
-    if (grp == 0 && r < rows) {
-      const int rr = cut.z * R + r, qi = rr / p.gq, head = cut.y * p.gq + rr - qi * p.gq;
-      const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
-      *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 4 * lane) =
-          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  float mm = -INFINITY;  // over the CTAs: a lane (or four, one a row) takes every 32nd (8th)
+  const int wl = threadIdx.x & 31;
+  for (int c = c0 + (is_few ? wl : wl >> 2); c <= c1; c += is_few ? 32 : 8) mm = fmaxf(mm, ml_all[slot_of(c) * R + r].x);
+  if (is_few) {
+    mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, 1));
+    mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, 2));
+  }
+#pragma unroll
+  for (int s = 4; s <= 16; s <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, s));
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float ll = 0.0f;
+#pragma unroll 8
+  for (int c = c0 + grp; c <= c1; c += groups) {
+    const size_t s = slot_of(c);
+    const float2 ml = ml_all[s * R + r];
+    const float4 v = is_few ? *reinterpret_cast<const float4 *>(p.part + (s * 8 + r) * D + 4 * lane)
+                            : reinterpret_cast<const float4 *>(p.tpart)[(s * L + lane) * 128 + r];
+    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
+    ll += ml.y * w;
+    acc.x += v.x * w;
+    acc.y += v.y * w;
+    acc.z += v.z * w;
+    acc.w += v.w * w;
+  }
+  if (groups > 1) {
+    s_o[threadIdx.x] = acc;
+    s_l[threadIdx.x] = ll;
+    __syncthreads();
+    if (grp != 0) return;
+    for (int g = 1; g < groups; ++g) {
+      const float4 v = s_o[threadIdx.x + g * L * per];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+      ll += s_l[threadIdx.x + g * L * per];
     }
   }
+  if (r >= rows) return;
+  const int rr = cut.z * R + r, qi = rr / p.gq, head = h * p.gq + rr - qi * p.gq;
+  const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
+  *reinterpret_cast<uint2 *>(p.out + (static_cast<size_t>(qr.x + qi) * p.Hq + head) * D + 4 * lane) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 int check(const FnQ8AttentionArgs *a, std::string &err) {
@@ -754,13 +789,13 @@ EncodeTiledFn q8_encode_fn() {
   return fn;
 }
 
-// Codes as a byte matrix [slots][Hkv * D]: boxes of 16 slots x 128 (or 64) bytes.
-bool make_codes_map(CUtensorMap *map, const void *base, uint64_t slots, uint64_t cols, int D) {
+// Codes as a byte matrix [slots][Hkv * D]: boxes of 16 (pair: 32) slots x 128 (or 64) bytes.
+bool make_codes_map(CUtensorMap *map, const void *base, uint64_t slots, uint64_t cols, int D, bool pair) {
   EncodeTiledFn fn = q8_encode_fn();
   if (fn == nullptr) return false;
   const cuuint64_t dims[2] = {cols, slots};
   const cuuint64_t strides[1] = {cols};
-  const cuuint32_t box[2] = {D == 64 ? 64u : 128u, 16};
+  const cuuint32_t box[2] = {D == 64 ? 64u : 128u, pair ? 32u : 16u};
   const cuuint32_t estr[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
@@ -772,7 +807,7 @@ cudaError_t launch_few(const Q8View &p, bool pdl, cudaStream_t s) {
   using F = Few<D, E4M3>;
   CUtensorMap km, vm;
   const uint64_t slots = static_cast<uint64_t>(p.pages) * p.page, cols = static_cast<uint64_t>(p.Hkv) * D;
-  if (!make_codes_map(&km, p.kc, slots, cols, D) || !make_codes_map(&vm, p.vc, slots, cols, D)) return cudaErrorInvalidValue;
+  if (!make_codes_map(&km, p.kc, slots, cols, D, p.pair_boxes) || !make_codes_map(&vm, p.vc, slots, cols, D, p.pair_boxes)) return cudaErrorInvalidValue;
   // Set for every call: the attribute belongs to the current device.
   const cudaError_t e = cudaFuncSetAttribute(k_q8_few<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
@@ -783,8 +818,8 @@ cudaError_t launch_few(const Q8View &p, bool pdl, cudaStream_t s) {
 }
 
 template <int D>
-cudaError_t launch_joins(const Q8View &p, int few_cuts, int many_cuts, cudaStream_t s) {
-  return launch_pdl(k_q8_join<D>, dim3(4 * few_cuts + 8 * many_cuts), dim3(256), 0, s, p, few_cuts, many_cuts);
+cudaError_t launch_joins(const Q8View &p, int few, int many, cudaStream_t s) {
+  return launch_pdl(k_q8_join<D>, dim3(8 * few + 32 * many), dim3(256), 0, s, p, few, many);
 }
 
 template <int D>
@@ -817,6 +852,7 @@ Q8View view_of(const FnQ8AttentionArgs *a) {
   p.page_magic = static_cast<uint32_t>(((1ull << 32) + c.page_size - 1) / c.page_size);
   p.scale = a->scale;
   p.few_rows = kFewRows;
+  p.pair_boxes = c.page_size % 32 == 0;
   return p;
 }
 
@@ -863,6 +899,12 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
   p.tpart_ml = reinterpret_cast<float2 *>(ws + w.tml);
   p.tpart = reinterpret_cast<float *>(ws + w.tpart);
   const int d = static_cast<int>(a->cache.head_dim);
+  // Segments there can be: the join looks at those where they are fewer than the cuts.
+  p.few_tiles = (std::min(p.few_rows, p.cu ? p.few_rows : p.gq) + 7) / 8;
+  const uint64_t few_segs = static_cast<uint64_t>(p.B) * p.Hkv * p.few_tiles;
+  const uint64_t many_segs = many ? many_tiles(p) * p.Hkv : 0;
+  p.by_seg = few_segs < static_cast<uint64_t>(few_ctas(d) - 1);
+  p.tby_seg = many_segs < static_cast<uint64_t>(many_ctas(d) - 1);
   const bool e4m3 = a->cache.code_type == FNMOE_Q8_E4M3;
   cudaError_t e = cudaSuccess;
   if (many) e = launch_many(p, d, e4m3, s);
@@ -870,7 +912,8 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
     e = d == 64    ? launch_few_d<64>(p, e4m3, many, s)
         : d == 128 ? launch_few_d<128>(p, e4m3, many, s)
                    : launch_few_d<256>(p, e4m3, many, s);
-  const int few_cuts = few ? few_ctas(d) - 1 : 0, many_cuts = many ? many_ctas(d) - 1 : 0;
+  const int few_cuts = !few ? 0 : p.by_seg ? static_cast<int>(few_segs) : few_ctas(d) - 1;
+  const int many_cuts = !many ? 0 : p.tby_seg ? static_cast<int>(many_segs) : many_ctas(d) - 1;
   if (e == cudaSuccess)
     e = d == 64    ? launch_joins<64>(p, few_cuts, many_cuts, s)
         : d == 128 ? launch_joins<128>(p, few_cuts, many_cuts, s)

@@ -45,14 +45,16 @@ struct Q8View {
   float scale;
   int few_rows;         // sequences of more (row, head) pairs per kv head take the many-row kernel
   // workspace of the few-row kernel (8 rows a tile)
-  int4 *cuts;           // [CTAs] where each range begins (Cut)
+  int4 *cuts;           // [CTAs] where each range begins (cut_of), or by_seg: [B][Hkv][few_tiles]
+  int few_tiles;        // tiles of 8 rows that a sequence can have
+  bool by_seg, tby_seg, pair_boxes;
   float *part;          // [2 * CTAs][8][D] unfinished sums
   float2 *part_ml;      // [2 * CTAs][8] their reference and weight sum
   // workspace of the many-row kernel (128 rows a tile)
   int max_tiles;
   int *seq_tile;        // [B + 1] tiles before each sequence
   int4 *tiles;          // [tiles] {sequence, tile of it, units of one kv head, 0}
-  int4 *tcuts;          // [CTAs]
+  int4 *tcuts;          // [CTAs], or tby_seg: [tiles][Hkv]
   long long *tprefix;   // [tiles + 1] units of work before each tile
   float *tpart;         // [2 * CTAs][D / 4][128][4]
   float2 *tpart_ml;     // [2 * CTAs][128]

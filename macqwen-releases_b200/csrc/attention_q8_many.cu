@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
   w.cur = w.first = range_start(total, used, blockIdx.x);
   w.end = range_start(total, used, blockIdx.x + 1);
   if (w.cur >= w.end) {
-    if (tid == 0) p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && !p.tby_seg) p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
     zero_tiles<D>(p, tiles);
     return;
   }
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
     }
     *dead = 0u;
     mbar_init_fence();
-    p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // until the first piece shows a cut
+    if (!p.tby_seg) p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // until the first piece shows a cut
   }
   if (warp == M::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
@@ -409,9 +409,17 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
       const int lim = valid ? p.ctx[q.b] - qr.y + qi : 0x7FFFFFFF;
       const int lim_min = __reduce_min_sync(0xFFFFFFFFu, lim);
       const bool idle = !__any_sync(0xFFFFFFFFu, valid);
-      if (tid == 0 && q.first && q.u0 > 0) {
-        const long long a = w.cur - (kCost + q.u0 + q.n);  // the segment's first unit
-        p.tcuts[blockIdx.x] = cut_of(q.b, q.h, q.mt, a, a + kCost, a + kCost + q.steps - 1, total, used, blockIdx.x);
+      if (tid == 0) {
+        const bool cut = q.first && q.u0 > 0;
+        const long long a = w.cur - (kCost + q.u0 + q.n);  // the segment's first unit, of a piece that does not end it
+        const int4 c4 = cut ? cut_of(q.b, q.h, q.mt, a, a + kCost, a + kCost + q.steps - 1, total, used, blockIdx.x)
+                            : make_int4(-1, 0, 0, 0);
+        if (p.tby_seg) {  // the first cut in a segment, or the CTA that does it all
+          if (c4.x >= 0 || (q.u0 == 0 && q.n == q.steps))
+            p.tcuts[static_cast<size_t>(w.tile) * p.Hkv + q.h] = make_int4(c4.x, blockIdx.x - 1, c4.z, c4.w);
+        } else if (cut) {
+          p.tcuts[blockIdx.x] = c4;
+        }
       }
       // Rows of the warp that this thread moves: row 8 e + lane / 4.
       long long q_at[4], o_at[4];
