@@ -190,44 +190,64 @@ __device__ __forceinline__ int2 units_of(const Q8View &p, int b) {
   return make_int2((tokens_of(p, b) + kFewUnit - 1) / kFewUnit, rows <= p.few_rows ? (rows + 7) / 8 : 0);
 }
 
-// The sequence that holds this CTA's first unit, the units before that
-// sequence and the total.  Every thread gets the result.
-struct Found {
-  int b;
-  long long before, total;
-};
 __device__ __forceinline__ long long seq_units(const Q8View &p, int b) {
   const int2 u = units_of(p, b);
   return static_cast<long long>(u.x) * u.y * p.Hkv;
 }
 
+// The units of all sequences, and the sequence that holds unit begin(cta) of
+// them with the units before it (B, 0 for a CTA without work).  A CTA-wide
+// scan over the sequences, THREADS at a time: once where they are that few.
+struct Found {
+  int b;
+  long long before, total;
+};
 template <int THREADS>
-__device__ Found find_unit(const Q8View &p, int cta, int ctas, long long &start, long long &end) {
-  __shared__ long long s_w[THREADS / 32];
-  __shared__ long long s_before;
-  __shared__ int s_b;
+__device__ Found find_unit(const Q8View &p, int cta, int ctas) {
+  constexpr int W = THREADS / 32;
+  __shared__ long long s_w[W];
+  __shared__ Found s_found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  long long mine = 0;  // units of this thread's first sequence
   long long total = 0;
-  for (int b = tid; b < p.B; b += THREADS) total += seq_units(p, b);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
-  if (lane == 0) s_w[warp] = total;
-  if (tid == 0) {
-    s_b = p.B;
-    s_before = 0;
+  for (int b = tid; b < p.B; b += THREADS) {
+    const long long u = seq_units(p, b);
+    if (b == tid) mine = u;
+    total += u;
   }
-  __syncthreads();
-  total = 0;
+  // Inclusive sums of the first THREADS sequences, and the total.
+  long long v = mine;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) total += s_w[w];
-  const int used = ranges_of(total, ctas);
-  start = range_start(total, used, cta);
-  end = range_start(total, used, cta + 1);
-  long long carry = 0;
-  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long o = __shfl_up_sync(0xFFFFFFFFu, v, off);
+    if (lane >= off) v += o;
+  }
+  if (p.B > THREADS) {
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+    if (lane == 0) s_w[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) total += s_w[w];
+    __syncthreads();
+  }
+  if (lane == 31) s_w[warp] = v;
+  if (tid == 0) s_found = Found{p.B, 0, 0};
+  __syncthreads();
+  long long before = v - mine, carry = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) before += s_w[w];
+    carry += s_w[w];
+  }
+  if (p.B <= THREADS) total = carry;
+  const long long start = Ranges(total, ctas).begin(cta);
+  if (before <= start && start < before + mine) s_found = Found{tid, before, 0};
+  for (int b0 = THREADS; b0 < p.B && carry <= start; b0 += THREADS) {
     const int b = b0 + tid;
-    const long long u = b < p.B ? seq_units(p, b) : 0;
-    long long v = u;
+    mine = b < p.B ? seq_units(p, b) : 0;
+    v = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const long long o = __shfl_up_sync(0xFFFFFFFFu, v, off);
@@ -236,21 +256,16 @@ __device__ Found find_unit(const Q8View &p, int cta, int ctas, long long &start,
     __syncthreads();
     if (lane == 31) s_w[warp] = v;
     __syncthreads();
-    long long before = carry;
+    before = carry + v - mine;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
+    for (int w = 0; w < W; ++w) {
       if (w < warp) before += s_w[w];
       carry += s_w[w];
     }
-    before += v - u;
-    if (b < p.B && before <= start && start < before + u) {
-      s_b = b;
-      s_before = before;
-    }
-    if (carry > start) break;
+    if (before <= start && start < before + mine) s_found = Found{b, before, 0};
   }
   __syncthreads();
-  return Found{s_b, s_before, total};
+  return Found{s_found.b, s_found.before, total};
 }
 
 template <int D, bool E4M3>
@@ -277,9 +292,10 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
   }
   uint32_t phase = 0;  // of both: they complete once a step
   bool dead = false;
-  long long cur, end;
-  const Found f = find_unit<kFewThreads>(p, blockIdx.x, gridDim.x, cur, end);
-  const long long first = cur;
+  const Found f = find_unit<kFewThreads>(p, blockIdx.x, gridDim.x);
+  const Ranges ranges(f.total, gridDim.x);
+  long long cur = ranges.begin(blockIdx.x);
+  const long long first = cur, end = ranges.begin(blockIdx.x + 1);
   int b = f.b;
   long long off = cur - f.before;  // within the sequence
 
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       off -= static_cast<long long>(u.x) * u.y * p.Hkv;
       u = units_of(p, ++b);
     }
-    const int seg = static_cast<int>(off / u.x);
+    const int seg = off <= 0xFFFFFFFFll ? static_cast<uint32_t>(off) / static_cast<uint32_t>(u.x) : static_cast<int>(off / u.x);
     const int u0 = static_cast<int>(off - static_cast<long long>(seg) * u.x);
     const int n = static_cast<int>(min(static_cast<long long>(u.x - u0), end - cur));
     const int h = seg / u.y, rt = seg - h * u.y;
@@ -297,46 +313,6 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
     const int ctx = tokens_of(p, b);
     const int rows = qr.y * p.gq;
     const int lim0 = p.ctx[b] - qr.y;  // last position that row 0 sees
-
-    // ---- this tile's query rows, their scale and the last position each sees ----
-    float c[2];
-    int lim[2];
-    {
-      const int r = rt * 8 + g;
-      const bool live = r < rows;
-      const int qi = live ? r / p.gq : 0;
-      const int head = h * p.gq + (live ? r - qi * p.gq : 0);
-      const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D + 4 * tq;
-      uint2 raw[D / 32][2];
-      uint32_t peak = 0;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          raw[i][e] = live ? *reinterpret_cast<const uint2 *>(src + 32 * i + 16 * e) : make_uint2(0, 0);
-          peak = max(peak, max(max(raw[i][e].x & 0x7FFFu, (raw[i][e].x >> 16) & 0x7FFFu),
-                               max(raw[i][e].y & 0x7FFFu, (raw[i][e].y >> 16) & 0x7FFFu)));
-        }
-      peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 1));
-      peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 2));
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-        if ((i & 3) == warp) F::Query::put(reinterpret_cast<uint2 *>(few_ring + F::kOffQ), i, raw[i][0], raw[i][1], peak);
-      const float up = F::Query::scale_of(peak);
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        c[hh] = p.scale * kLog2e * __shfl_sync(0xFFFFFFFFu, up, (2 * tq + hh) * 4);
-        const int rr = rt * 8 + 2 * tq + hh;
-        lim[hh] = rr < rows ? lim0 + rr / p.gq : 0x7FFFFFFF;  // rows past the end: never written
-      }
-    }
-
-    const int lim_min = __reduce_min_sync(0xFFFFFFFFu, min(lim[0], lim[1]));
-
-    float o[MT][4];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
     // ---- this warp's steps of 32 tokens ----
     const int t_end = min(ctx, (u0 + n) * kFewUnit);
@@ -408,6 +384,47 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
     request_k(t);
     request_v(t);
     look_up(t + kFewUnit);
+
+    // ---- this tile's query rows, their scale and the last position each sees ----
+    float c[2];
+    int lim[2];
+    {
+      const int r = rt * 8 + g;
+      const bool live = r < rows;
+      const int qi = live ? r / p.gq : 0;
+      const int head = h * p.gq + (live ? r - qi * p.gq : 0);
+      const uint16_t *src = p.q + static_cast<uint64_t>(qr.x + qi) * p.q_stride + static_cast<uint64_t>(head) * D + 4 * tq;
+      uint2 raw[D / 32][2];
+      uint32_t peak = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          raw[i][e] = live ? *reinterpret_cast<const uint2 *>(src + 32 * i + 16 * e) : make_uint2(0, 0);
+          peak = max(peak, max(max(raw[i][e].x & 0x7FFFu, (raw[i][e].x >> 16) & 0x7FFFu),
+                               max(raw[i][e].y & 0x7FFFu, (raw[i][e].y >> 16) & 0x7FFFu)));
+        }
+      peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 1));
+      peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 2));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        if ((i & 3) == warp) F::Query::put(reinterpret_cast<uint2 *>(few_ring + F::kOffQ), i, raw[i][0], raw[i][1], peak);
+      const float up = F::Query::scale_of(peak);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        c[hh] = p.scale * kLog2e * __shfl_sync(0xFFFFFFFFu, up, (2 * tq + hh) * 4);
+        const int rr = rt * 8 + 2 * tq + hh;
+        lim[hh] = rr < rows ? lim0 + rr / p.gq : 0x7FFFFFFF;  // rows past the end: never written
+      }
+    }
+
+    const int lim_min = __reduce_min_sync(0xFFFFFFFFu, min(lim[0], lim[1]));
+
+    float o[MT][4];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
     __syncthreads();  // the query rows are in place
     for (; t < t_end; t += kFewUnit) {
       const bool in[2] = {slot[0] >= 0, slot[1] >= 0};
@@ -546,7 +563,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       const bool cut = cur == first && u0 > 0, done = u0 == 0 && n == u.x;
       const long long a = cur - u0;
       if (p.by_seg ? cut || done : cur == first) {
-        const int4 c4 = cut ? cut_of(b, h, rt, a, a, a + u.x - 1, f.total, ranges_of(f.total, gridDim.x), blockIdx.x) : make_int4(-1, 0, 0, 0);
+        const int4 c4 = cut ? cut_of(ranges, b, h, rt, a, a, a + u.x - 1, blockIdx.x) : make_int4(-1, 0, 0, 0);
         // by segment: only the first cut in it (or the one CTA that did it all) says so
         if (!p.by_seg) p.cuts[blockIdx.x] = c4;
         else if (!cut || c4.x >= 0) p.cuts[(static_cast<size_t>(b) * p.Hkv + h) * p.few_tiles + rt] = make_int4(c4.x, blockIdx.x - 1, c4.z, c4.w);
@@ -799,7 +816,9 @@ bool make_codes_map(CUtensorMap *map, const void *base, uint64_t slots, uint64_t
   const cuuint32_t estr[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            // no more than the head's own bytes: its neighbours' are read by others at other times
+            D == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B : D == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, bool E4M3>

@@ -281,7 +281,7 @@ __device__ __forceinline__ bool next_piece(const Q8View &p, Walk &w, Piece &q) {
     q.b = t.x;
     q.mt = t.y;
     q.steps = t.z;
-    q.h = static_cast<int>(w.off / seg);
+    q.h = w.off <= 0xFFFFFFFFll ? static_cast<uint32_t>(w.off) / static_cast<uint32_t>(seg) : static_cast<int>(w.off / seg);
     const int v0 = static_cast<int>(w.off - q.h * seg);
     const int n = static_cast<int>(min(seg - v0, w.end - w.cur));
     q.u0 = max(v0 - kCost, 0);
@@ -334,10 +334,10 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
 
   const int tiles = p.seq_tile[p.B];
   const long long total = p.tprefix[tiles];
-  const int used = ranges_of(total, gridDim.x);
+  const Ranges ranges(total, gridDim.x);
   Walk w;
-  w.cur = w.first = range_start(total, used, blockIdx.x);
-  w.end = range_start(total, used, blockIdx.x + 1);
+  w.cur = w.first = ranges.begin(blockIdx.x);
+  w.end = ranges.begin(blockIdx.x + 1);
   if (w.cur >= w.end) {
     if (tid == 0 && !p.tby_seg) p.tcuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
     zero_tiles<D>(p, tiles);
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
       if (tid == 0) {
         const bool cut = q.first && q.u0 > 0;
         const long long a = w.cur - (kCost + q.u0 + q.n);  // the segment's first unit, of a piece that does not end it
-        const int4 c4 = cut ? cut_of(q.b, q.h, q.mt, a, a + kCost, a + kCost + q.steps - 1, total, used, blockIdx.x)
+        const int4 c4 = cut ? cut_of(ranges, q.b, q.h, q.mt, a, a + kCost, a + kCost + q.steps - 1, blockIdx.x)
                             : make_int4(-1, 0, 0, 0);
         if (p.tby_seg) {  // the first cut in a segment, or the CTA that does it all
           if (c4.x >= 0 || (q.u0 == 0 && q.n == q.steps))
