@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
   __shared__ float s_m[4][8], s_l[4][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tq = lane & 3;
-  pdl_wait();  // launched after the many-row kernel, whose workspace the join reads
+  pdl_wait();
   pdl_trigger();
   const uint32_t kbar = sbase + F::kOffBar + 16 * warp, vbar = kbar + 8;
   if (lane == 0) {
@@ -645,6 +645,7 @@ __global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
   __shared__ float4 s_o[256];
   __shared__ float s_l[256];
   pdl_wait();
+  pdl_trigger();
   const bool is_few = static_cast<int>(blockIdx.x) < 8 * few;
   const int at = is_few ? blockIdx.x >> 3 : (blockIdx.x - 8 * few) >> 5;
   const int row0 = is_few ? blockIdx.x & 7 : 4 * ((blockIdx.x - 8 * few) & 31);
@@ -822,7 +823,7 @@ bool make_codes_map(CUtensorMap *map, const void *base, uint64_t slots, uint64_t
 }
 
 template <int D, bool E4M3>
-cudaError_t launch_few(const Q8View &p, bool pdl, cudaStream_t s) {
+cudaError_t launch_few(const Q8View &p, cudaStream_t s) {
   using F = Few<D, E4M3>;
   CUtensorMap km, vm;
   const uint64_t slots = static_cast<uint64_t>(p.pages) * p.page, cols = static_cast<uint64_t>(p.Hkv) * D;
@@ -830,10 +831,7 @@ cudaError_t launch_few(const Q8View &p, bool pdl, cudaStream_t s) {
   // Set for every call: the attribute belongs to the current device.
   const cudaError_t e = cudaFuncSetAttribute(k_q8_few<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
-  uint32_t *err = device_error_word();
-  if (pdl) return launch_pdl(k_q8_few<D, E4M3>, dim3(F::kMax), dim3(kFewThreads), F::kSmem, s, p, km, vm, err);
-  k_q8_few<D, E4M3><<<F::kMax, kFewThreads, F::kSmem, s>>>(p, km, vm, err);
-  return cudaSuccess;
+  return launch_pdl(k_q8_few<D, E4M3>, dim3(F::kMax), dim3(kFewThreads), F::kSmem, s, p, km, vm, device_error_word());
 }
 
 template <int D>
@@ -842,8 +840,8 @@ cudaError_t launch_joins(const Q8View &p, int few, int many, cudaStream_t s) {
 }
 
 template <int D>
-cudaError_t launch_few_d(const Q8View &p, bool e4m3, bool pdl, cudaStream_t s) {
-  return e4m3 ? launch_few<D, true>(p, pdl, s) : launch_few<D, false>(p, pdl, s);
+cudaError_t launch_few_d(const Q8View &p, bool e4m3, cudaStream_t s) {
+  return e4m3 ? launch_few<D, true>(p, s) : launch_few<D, false>(p, s);
 }
 
 Q8View view_of(const FnQ8AttentionArgs *a) {
@@ -928,9 +926,9 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
   cudaError_t e = cudaSuccess;
   if (many) e = launch_many(p, d, e4m3, s);
   if (e == cudaSuccess && few)
-    e = d == 64    ? launch_few_d<64>(p, e4m3, many, s)
-        : d == 128 ? launch_few_d<128>(p, e4m3, many, s)
-                   : launch_few_d<256>(p, e4m3, many, s);
+    e = d == 64    ? launch_few_d<64>(p, e4m3, s)
+        : d == 128 ? launch_few_d<128>(p, e4m3, s)
+                   : launch_few_d<256>(p, e4m3, s);
   const int few_cuts = !few ? 0 : p.by_seg ? static_cast<int>(few_segs) : few_ctas(d) - 1;
   const int many_cuts = !many ? 0 : p.tby_seg ? static_cast<int>(many_segs) : many_ctas(d) - 1;
   if (e == cudaSuccess)

@@ -210,6 +210,7 @@ __device__ __forceinline__ long long scan1(long long v, long long &carry, long l
 __global__ void __launch_bounds__(kScanThreads) k_q8_tiles(Q8View p) {
   __shared__ long long red[32];
   long long carry = 0;
+  pdl_wait();
   pdl_trigger();
   for (int b0 = 0; b0 < p.B; b0 += kScanThreads) {
     const int b = b0 + threadIdx.x;
@@ -804,7 +805,8 @@ cudaError_t launch(const Q8View &p, cudaStream_t s) {
   // Set for every call: the attribute belongs to the current device.
   cudaError_t e = cudaFuncSetAttribute(k_q8_many<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
   if (e != cudaSuccess) return e;
-  k_q8_tiles<<<1, kScanThreads, 0, s>>>(p);
+  e = launch_pdl(k_q8_tiles, dim3(1), dim3(kScanThreads), 0, s, p);
+  if (e != cudaSuccess) return e;
   return launch_pdl(k_q8_many<D, E4M3>, dim3(M::kMax), dim3(M::kThreads), M::kSmem, s, p, device_error_word());
 }
 
