@@ -828,8 +828,8 @@ cudaError_t launch_few(const Q8View &p, cudaStream_t s) {
   CUtensorMap km, vm;
   const uint64_t slots = static_cast<uint64_t>(p.pages) * p.page, cols = static_cast<uint64_t>(p.Hkv) * D;
   if (!make_codes_map(&km, p.kc, slots, cols, D, p.pair_boxes) || !make_codes_map(&vm, p.vc, slots, cols, D, p.pair_boxes)) return cudaErrorInvalidValue;
-  // Set for every call: the attribute belongs to the current device.
-  const cudaError_t e = cudaFuncSetAttribute(k_q8_few<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+  static SmemLimit limit;
+  const cudaError_t e = limit.set(reinterpret_cast<const void *>(k_q8_few<D, E4M3>), F::kSmem);
   if (e != cudaSuccess) return e;
   return launch_pdl(k_q8_few<D, E4M3>, dim3(F::kMax), dim3(kFewThreads), F::kSmem, s, p, km, vm, device_error_word());
 }

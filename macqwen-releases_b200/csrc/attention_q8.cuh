@@ -23,6 +23,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "async.cuh"
 #include "common.cuh"
 
@@ -253,6 +255,21 @@ __device__ __forceinline__ int4 cut_of(const Ranges &ranges, int b, int h, int t
   const int late = ranges.begin(cta - 1) < seg_begin ? 1 << 30 : 0;
   return make_int4(b, h, tile, ranges.owner(last_unit) | late);
 }
+
+// A kernel's shared-memory limit, set once on each device (the attribute
+// belongs to the device's copy of the kernel).
+struct SmemLimit {
+  std::atomic<uint64_t> done{0};
+  cudaError_t set(const void *kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (e != cudaSuccess || (done.load(std::memory_order_acquire) & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // The many-row kernels (attention_q8_many.cu).
 int many_ctas(int head_dim);

@@ -19,7 +19,7 @@
 //               running reference and sum, P back to TMEM; Q in and the
 //               result out of TMEM, through a shared-memory stage that turns
 //               row-a-thread into coalesced 64-byte pieces;
-//   one warp    issues the MMAs;
+//   one warp    issues the MMAs; another looks the units' scales up;
 //   codes       read K and V codes (16 bytes a thread) one unit ahead in
 //               registers, widen them to bfloat16 and store them to shared
 //               memory as 128B-swizzled tiles, [D / 64][64 tokens][128 bytes]:
@@ -63,7 +63,7 @@ struct Many {
   static constexpr int kCtas = D < 256 ? 2 : 1;  // per SM
   static constexpr int kHalves = D < 256 ? 1 : 2;  // softmax threads a row
   static constexpr int kSoftWarps = 4 * kHalves;
-  static constexpr int kMmaWarp = kSoftWarps;       // the three warps after it only fill its warpgroup
+  static constexpr int kMmaWarp = kSoftWarps;       // then the scales' warp, and two that fill the warpgroup
   static constexpr int kConvWarp0 = kMmaWarp + 4;
   static constexpr int kConvWarps = D < 256 ? 4 : 8;
   static constexpr int kThreads = 32 * (kConvWarp0 + kConvWarps);
@@ -175,7 +175,7 @@ __device__ __forceinline__ int tiles_of(const Q8View &p, int b) {
 // results out, the pipeline's start), which the ranges count: a tile and kv
 // head of n units weighs n + kCost, and its real units are the last n of
 // those.
-constexpr int kCost = 3;
+constexpr int kCost = 6;
 
 constexpr int kScanThreads = 1024;
 
@@ -436,15 +436,17 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
       }
       {  // Q into TMEM; the last piece's products are done (its sums were read)
         const int c0 = half * kDims + 8 * (lane & 3);
+        uint4 x[kDims / 32][4];
 #pragma unroll
-        for (int c = 0; c < kDims / 32; ++c) {
-          uint4 x[4];
+        for (int c = 0; c < kDims / 32; ++c)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            x[e] = q_at[e] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.q + q_at[e] + c0 + 32 * c)) : make_uint4(0, 0, 0, 0);
+            x[c][e] = q_at[e] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.q + q_at[e] + c0 + 32 * c)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < kDims / 32; ++c) {
           __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sts128(other(e), x[e]);
+          for (int e = 0; e < 4; ++e) sts128(other(e), x[c][e]);
           __syncwarp();
           uint32_t v[16];
 #pragma unroll
@@ -582,12 +584,14 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         const int slot = 2 * blockIdx.x + (q.first ? 0 : 1);
         // cut tiles: float4 d of row r at [d][r], so that a warp's stores are contiguous
         float4 *part = reinterpret_cast<float4 *>(p.tpart) + (static_cast<size_t>(slot) * (D / 4) + half * (kDims / 4)) * kTile + row;
-#pragma unroll 1
+        uint32_t vv[2][32];
+        tmem_ld32_nowait(lanes + half * kDims, vv[0]);
+#pragma unroll
         for (int c = 0; c < kDims / 32; ++c) {
-          uint32_t v[32];
+          uint32_t (&v)[32] = vv[c & 1];
           __syncwarp();
-          tmem_ld32_nowait(lanes + half * kDims + 32 * c, v);
           tmem_wait_ld();
+          if (c + 1 < kDims / 32) tmem_ld32_nowait(lanes + half * kDims + 32 * (c + 1), vv[(c + 1) & 1]);
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -678,6 +682,35 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         }
         if (!M::kShared && live) pv(n > 1);
       }
+    } else if (warp == M::kMmaWarp + 1) {
+      // ---------------- the units' scales: a lane for each granule of 16 tokens ----------------
+      uint32_t i = 0;
+      bool live = true;
+      while (live && next_piece(p, w, q)) {
+        const int ctx = tokens_of(p, q.b), bpp = p.page >> p.block_shift;
+        const int32_t *trow = p.table + static_cast<size_t>(q.b) * p.width;
+        for (int u = q.u0; live && u < q.u0 + q.n; ++u, ++i) {
+          const uint32_t slot = i % M::kSlots, ph = (i / M::kSlots) & 1u;
+          const int t = u * kUnit + 16 * (lane & 3);
+          float mul = 1e-37f, add = -INFINITY, inv = 0.0f;  // a granule without a token or page weighs nothing
+          if (t < ctx) {
+            const int c = page_col(p, t), pg = trow[c];
+            if (static_cast<uint32_t>(pg) < static_cast<uint32_t>(p.pages)) {
+              const size_t at = (static_cast<size_t>(pg) * bpp + ((t - c * p.page) >> p.block_shift)) * p.Hkv + q.h;
+              const float v = fmaxf(__ldg(p.vs + at), 0x1p-110f);
+              mul = fmaxf(p.scale * kLog2e * __ldg(p.ks + at), 1e-37f);
+              add = lg2(v);
+              inv = rcp(v);
+            }
+          }
+          // as far ahead as K itself may be, so that the kept units are not overrun
+          live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kKEmpty + slot), ph ^ 1u, dead, err));
+          if (!live) break;
+          if (lane < 4) reinterpret_cast<float4 *>(sm + M::kOffInfo)[(i % kInfo) * 4 + lane] = make_float4(mul, add, inv, 0.0f);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(M::kInfoFull + i % kInfo));
+        }
+      }
     }
     __syncwarp();
   } else {
@@ -693,55 +726,58 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
     const int grp = (ct >> 3) % kGroups, c4 = ct & 3;
     const int row0 = 2 * (ct / (8 * kGroups)) + ((ct >> 2) & 1);
     const uint32_t soff = grp * 8192 + row0 * 128 + (((2 * c4) ^ (row0 & 7)) << 4);  // second half: ^ 16
-    const int bpp = p.page >> p.block_shift;
     const uint32_t row_bytes = static_cast<uint32_t>(p.Hkv) * D;
+    // 16-token granule g of a unit lies in one page: lane g looks its first slot
+    // up, a unit ahead, and the warp shuffles it (a warp's rows of a pass are of
+    // one granule).
+    const int row16 = row0 & 15, g0 = row0 >> 4;
+    constexpr int kGranules = kRowsPass / 16;  // from one pass to the next
     uint32_t i = 0;
     bool live = true;
     while (live && next_piece(p, w, q)) {
       const int ctx = tokens_of(p, q.b);
       const int32_t *trow = p.table + static_cast<size_t>(q.b) * p.width;
       const int last = q.u0 + q.n;
-      const size_t head_off = static_cast<size_t>(q.h) * D + 64 * grp + 16 * c4;
-      const uint8_t *kbase = p.kc + head_off, *vbase = p.vc + head_off;
-      int pg[kPasses];        // page of each pass's token, one unit ahead of the codes
-      uint32_t in[kPasses];   // and the token's place in it
-      uint4 ck[kPasses], cv[kPasses];
-      float ks = 0.0f, vs = 0.0f;  // lanes 0-3 of the first warp: scales of a granule
-      int info_pg = -1, info_in = 0;
-      auto fetch_pages = [&](int u) {
-#pragma unroll
-        for (int k = 0; k < kPasses; ++k) {
-          const int t = u * kUnit + k * kRowsPass + row0;
-          const int c = page_col(p, t);
-          in[k] = t - c * p.page;
-          pg[k] = t < ctx ? trow[c] : -1;
-        }
-        if (ct < 4) {
-          const int t = u * kUnit + 16 * lane;
-          const int c = page_col(p, t);
-          info_in = t - c * p.page;
-          info_pg = t < ctx ? trow[c] : -1;
-        }
+      const size_t off = static_cast<size_t>(row16) * row_bytes + static_cast<size_t>(q.h) * D + 64 * grp + 16 * c4;
+      const uint8_t *kbase = p.kc + off, *vbase = p.vc + off;
+      int slot_next = -1;  // lane g < 4: granule g's first slot, -1 without a token or page
+      int pg_after = -1, in_after = 0;  // of the unit after that: its page, still on its way
+      auto look_up = [&](int u) {
+        const int t = u * kUnit + 16 * (lane & 3), c = page_col(p, t);
+        in_after = t - c * p.page;
+        pg_after = t < ctx ? trow[c] : -1;
       };
+      auto advance = [&]() {
+        slot_next = static_cast<uint32_t>(pg_after) < static_cast<uint32_t>(p.pages) ? pg_after * p.page + in_after : -1;
+      };
+      uint4 ck[kPasses], cv[kPasses];
       auto fetch = [&](const uint8_t *codes, uint4 (&c)[kPasses]) {
 #pragma unroll
         for (int k = 0; k < kPasses; ++k) {
-          c[k] = make_uint4(0, 0, 0, 0);  // tokens past the context or without a page: zero codes
-          if (static_cast<uint32_t>(pg[k]) < static_cast<uint32_t>(p.pages))
-            c[k] = ldg_stream(codes + static_cast<uint64_t>(static_cast<uint32_t>(pg[k]) * static_cast<uint32_t>(p.page) + in[k]) * row_bytes);
+          const int s0 = __shfl_sync(0xFFFFFFFFu, slot_next, g0 + k * kGranules);
+          c[k] = ldg_stream(codes + static_cast<uint64_t>(static_cast<uint32_t>(max(s0, 0))) * row_bytes);
         }
       };
-      auto fetch_scales = [&]() {
-        if (ct >= 4) return;
-        ks = 0.0f;
-        vs = -1.0f;
-        if (static_cast<uint32_t>(info_pg) < static_cast<uint32_t>(p.pages)) {
-          const size_t at = (static_cast<size_t>(info_pg) * bpp + (info_in >> p.block_shift)) * p.Hkv + q.h;
-          ks = __ldg(p.ks + at);
-          vs = fmaxf(__ldg(p.vs + at), 0x1p-110f);
+      // Passes of unit u whose token is past the context or has no page.  They
+      // weigh nothing, but e4m3 codes can be NaN: those are stored as zeros
+      // (when they are stored: touching them before would wait for the loads).
+      auto missing = [&](int u) {
+        uint32_t m = 0;
+        if (E4M3 && (!__all_sync(0xFFFFFFFFu, slot_next >= 0) || (u + 1) * kUnit > ctx)) {
+#pragma unroll
+          for (int k = 0; k < kPasses; ++k) {
+            const int s0 = __shfl_sync(0xFFFFFFFFu, slot_next, g0 + k * kGranules);
+            if (s0 < 0 || u * kUnit + k * kRowsPass + row0 >= ctx) m |= 1u << k;
+          }
         }
+        return m;
       };
-      auto store = [&](uint32_t tile, const uint4 (&c)[kPasses]) {
+      auto store = [&](uint32_t tile, uint4 (&c)[kPasses], uint32_t zero) {
+        if (E4M3 && __any_sync(0xFFFFFFFFu, zero != 0)) {
+#pragma unroll
+          for (int k = 0; k < kPasses; ++k)
+            if ((zero >> k) & 1u) c[k] = make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int k = 0; k < kPasses; ++k) {
           uint4 a, b;
@@ -751,42 +787,38 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
           sts128(at ^ 16u, b);
         }
       };
-      fetch_pages(q.u0);
+      look_up(q.u0);
+      advance();
       fetch(kbase, ck);
       fetch(vbase, cv);
-      fetch_scales();
-      fetch_pages(q.u0 + 1);
+      uint32_t zero = missing(q.u0), zero_next = 0;
+      look_up(q.u0 + 1);
       for (int u = q.u0; u < last; ++u, ++i) {
         const uint32_t slot = i % M::kSlots, ph = (i / M::kSlots) & 1u;
+        advance();
+        look_up(u + 2);
         live = bar_wait(bar(M::kKEmpty + slot), ph ^ 1u, dead, err);
         live = __all_sync(0xFFFFFFFFu, live);
         if (!live) break;
-        store(sbase + slot * M::kSlotBytes, ck);
+        store(sbase + slot * M::kSlotBytes, ck, zero);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(M::kKFull + slot));
-        if (u + 1 < last) fetch(kbase, ck);
-        if (warp == M::kConvWarp0) {
-          if (lane < 4) {
-            const bool ok = vs > 0.0f;
-            reinterpret_cast<float4 *>(sm + M::kOffInfo)[(i % kInfo) * 4 + lane] =
-                make_float4(fmaxf(p.scale * kLog2e * ks, 1e-37f), ok ? __log2f(vs) : -INFINITY, ok ? __frcp_rn(vs) : 0.0f, 0.0f);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(M::kInfoFull + i % kInfo));
-          if (u + 1 < last) fetch_scales();
+        if (u + 1 < last) {
+          fetch(kbase, ck);
+          zero_next = missing(u + 1);
         }
         live = bar_wait(bar(M::kVEmpty + slot), ph ^ 1u, dead, err);
         live = __all_sync(0xFFFFFFFFu, live);
         if (!live) break;
-        store(sbase + M::kOffV + slot * M::kSlotBytes, cv);
+        store(sbase + M::kOffV + slot * M::kSlotBytes, cv, zero);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(M::kVFull + slot));
         if (u + 1 < last) {
           fetch(vbase, cv);
-          fetch_pages(u + 2);
         }
+        zero = zero_next;
       }
     }
   }
@@ -802,8 +834,8 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
 template <int D, bool E4M3>
 cudaError_t launch(const Q8View &p, cudaStream_t s) {
   using M = Many<D>;
-  // Set for every call: the attribute belongs to the current device.
-  cudaError_t e = cudaFuncSetAttribute(k_q8_many<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
+  static SmemLimit limit;
+  cudaError_t e = limit.set(reinterpret_cast<const void *>(k_q8_many<D, E4M3>), M::kSmem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(k_q8_tiles, dim3(1), dim3(kScanThreads), 0, s, p);
   if (e != cudaSuccess) return e;

@@ -82,28 +82,38 @@ def _rows(t, heads, dim, what):
 
 
 def _cache(k_cache, v_cache, k_scale, v_scale):
-    dtype = k_cache.dtype
-    code = _CODES.get(dtype)
-    if code is None:
-        raise TypeError("k_cache must be an int8 or float8_e4m3fn tensor")
-    shape, scales = k_cache.shape, k_scale.shape
+    """FnQ8Cache of the four tensors, and (kv_heads, head_dim)."""
+    dtype, shape, scales = k_cache.dtype, k_cache.shape, k_scale.shape
     if len(shape) != 4 or len(scales) != 3:
         raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] and scales "
                          "[pages, page_size / block, kv_heads]")
     pages, page, heads, dim = shape
     blocks = scales[1]
+    if (k_scale.dtype is v_scale.dtype is torch.float32 and v_cache.dtype is dtype and dtype in _CODES
+            and v_cache.shape == shape and v_scale.shape == scales and scales[0] == pages and scales[2] == heads
+            and blocks and page % blocks == 0 and k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda
+            and v_scale.is_cuda and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        return _lib.FnQ8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                              pages, page, page // blocks, heads, dim, _CODES[dtype]), heads, dim
+    # say which
+    if dtype not in _CODES:
+        raise TypeError("k_cache must be an int8 or float8_e4m3fn tensor")
     if blocks == 0 or page % blocks:
         raise ValueError("a page must hold a whole number of scale blocks")
     ss, f32 = (pages, blocks, heads), torch.float32
-    return _lib.FnQ8Cache(_want(k_cache, dtype, shape, "k_cache"), _want(v_cache, dtype, shape, "v_cache"),
-                          _want(k_scale, f32, ss, "k_scale"), _want(v_scale, f32, ss, "v_scale"),
-                          pages, page, page // blocks, heads, dim, code)
+    for t, d, x, what in ((k_cache, dtype, shape, "k_cache"), (v_cache, dtype, shape, "v_cache"),
+                          (k_scale, f32, ss, "k_scale"), (v_scale, f32, ss, "v_scale")):
+        _want(t, d, x, what)
+    raise AssertionError("unreachable")
 
 
 def _ready(t):
     """The library and the current stream of the current device, which must be ``t``'s."""
-    lib = _lib.ensure_device_of(t.get_device())
-    return lib, torch._C._cuda_getCurrentRawStream(t.get_device())
+    index = t.get_device()
+    if torch._C._cuda_getDevice() != index or not _lib._available.get(index):
+        _lib.ensure_device_of(index)  # refuses, or starts the library up
+    return _lib._handle, torch._C._cuda_getCurrentRawStream(index)
 
 
 def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size: int, max_tokens: int,
@@ -126,7 +136,7 @@ def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size
     width, max_tokens = block_table.shape[1], int(max_tokens)
     if batch == 0 or width == 0 or max_tokens <= 0:
         raise ValueError("page_plan needs sequences, table columns and max_tokens > 0")
-    one, cells, two = (batch,), (batch, width), (2,)
+    one, cells, two = seq_lens.shape, block_table.shape, (2,)
     ins = (_want(seq_lens, i32, one, "seq_lens"), _want(new_lens, i32, one, "new_lens"),
            None if release is None else _want(release, i32, one, "release"),
            _want(block_table, i32, cells, "block_table"), _want(free_pages, i32, (free_pages.numel(),), "free_pages"),
@@ -160,9 +170,9 @@ def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
     ascending slots, as :func:`page_plan` maps them; slots outside the cache
     (-1) are skipped.  Infinities store the largest code, NaN stores 0.
     """
-    c = _cache(k_cache, v_cache, k_scale, v_scale)
-    kp, ks = _rows(k, c.kv_heads, c.head_dim, "k")
-    vp, vs = _rows(v, c.kv_heads, c.head_dim, "v")
+    c, heads, dim = _cache(k_cache, v_cache, k_scale, v_scale)
+    kp, ks = _rows(k, heads, dim, "k")
+    vp, vs = _rows(v, heads, dim, "v")
     tokens = k.shape[0]
     if v.shape[0] != tokens:
         raise ValueError("k and v must have the same number of rows")
@@ -175,14 +185,18 @@ def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
 def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
     """The values ``(k, v)`` that ``slots`` [n] int64 hold, bfloat16
     [n, kv_heads, head_dim]; slots outside the cache (-1) read as zeros."""
-    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    c, heads, dim = _cache(k_cache, v_cache, k_scale, v_scale)
     n = slots.shape[0]
-    shape = (n, c.kv_heads, c.head_dim)
+    at = _want(slots, torch.int64, (n,), "slots")
     if out is None:
-        out = (torch.empty(shape, dtype=torch.bfloat16, device=slots.device),
-               torch.empty(shape, dtype=torch.bfloat16, device=slots.device))
-    a = _lib.FnQ8ReadArgs(_lib.ABI_VERSION, n, c, _want(slots, torch.int64, (n,), "slots"),
-                          _want(out[0], torch.bfloat16, shape, "out[0]"), _want(out[1], torch.bfloat16, shape, "out[1]"))
+        both = k_scale.new_empty((2, n, heads, dim), dtype=torch.bfloat16)
+        ko = both.data_ptr()
+        vo = ko + 2 * n * heads * dim
+        out = both.unbind()
+    else:
+        shape = (n, heads, dim)
+        ko, vo = _want(out[0], torch.bfloat16, shape, "out[0]"), _want(out[1], torch.bfloat16, shape, "out[1]")
+    a = _lib.FnQ8ReadArgs(_lib.ABI_VERSION, n, c, at, ko, vo)
     lib, stream = _ready(slots)
     _lib.check(lib.fnmoe_kv_read_q8(ctypes.byref(a), stream), "kv_read_q8")
     return out
@@ -200,24 +214,27 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
     ``fnmoe_paged_attention_q8_workspace_size`` reports, or None for one that
     is kept for the current stream.
     """
-    c = _cache(k_cache, v_cache, k_scale, v_scale)
-    if q.dim() != 3:
+    c, _, head_dim = _cache(k_cache, v_cache, k_scale, v_scale)
+    shape, table = q.shape, block_table.shape
+    if len(shape) != 3:
         raise ValueError("q must be [rows, q_heads, head_dim]")
-    rows, heads, dim = q.shape
-    if dim != c.head_dim:
+    rows, heads, dim = shape
+    if dim != head_dim:
         raise ValueError("cache head_dim differs from q")
     qp, qs = _rows(q, heads, dim, "q")
-    if block_table.dim() != 2:
+    if len(table) != 2:
         raise ValueError("block_table must be [batch, max_pages]")
-    batch, width = block_table.shape
+    batch, width = table
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device=q.device)
+        out = k_scale.new_empty(shape, dtype=torch.bfloat16)
+        op = out.data_ptr()
+    else:
+        op = _want(out, torch.bfloat16, shape, "out")
     i32 = torch.int32
     a = _lib.FnQ8AttentionArgs(
         _lib.ABI_VERSION, batch, rows, heads, width, float(scale), c, qp, qs,
-        _want(block_table, i32, (batch, width), "block_table"), _want(context_lens, i32, (batch,), "context_lens"),
-        None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q"),
-        _want(out, torch.bfloat16, (rows, heads, dim), "out"))
+        _want(block_table, i32, table, "block_table"), _want(context_lens, i32, (batch,), "context_lens"),
+        None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q"), op)
     lib, stream = _ready(q)
     ref = ctypes.byref(a)
     kept = workspace if workspace is not None else _workspaces.get((q.get_device(), stream))
