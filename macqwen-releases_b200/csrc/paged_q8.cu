@@ -297,6 +297,23 @@ __device__ __forceinline__ uint32_t peak8(uint4 v) {
   return m;
 }
 
+// The codes of rows row0, row0 + step, ... below `rows` (eight each, at `a`,
+// `pitch` bytes from row to row) rounded again to a scale 1 / shrink times as large.
+template <int D, bool E4M3>
+__device__ __forceinline__ void requantise(uint8_t *a, uint64_t pitch, int row0, int step, int rows, float shrink) {
+  for (int r = row0; r < rows; r += step) {
+    uint2 *at = reinterpret_cast<uint2 *>(a + static_cast<uint64_t>(r) * pitch);
+    const uint2 q = *at;
+    float f[8];
+    Q8Code<E4M3>::decode4(q.x, f);
+    Q8Code<E4M3>::decode4(q.y, f + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // a slot that was never written may hold a NaN code
+      f[e] = f[e] != f[e] ? 0.0f : clamp_top(__fmul_rn(f[e], shrink), Q8Code<E4M3>::kTop);
+    *at = make_uint2(Q8Code<E4M3>::encode4(f), Q8Code<E4M3>::encode4(f + 4));
+  }
+}
+
 // D: head dim; NP: passes of the CTA over a block's rows.
 template <int D, int NP, bool E4M3>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append_q8(Q8Store p) {
@@ -382,20 +399,82 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append_q8(Q8Store p) {
         if (r < len) *at(first + r) = encode_row8<E4M3>(v[i], inv);
       }
       if (first > 0 && scale != old) {
-        const float shrink = __fdiv_rn(old, scale);
-        for (int r = row; r < first; r += kRows) {
-          uint2 *a = at(r);
-          const uint2 q = *a;
-          float f[8];
-          Q8Code<E4M3>::decode4(q.x, f);
-          Q8Code<E4M3>::decode4(q.y, f + 4);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)  // a slot that was never written may hold a NaN code
-            f[e] = f[e] != f[e] ? 0.0f : clamp_top(__fmul_rn(f[e], shrink), kTop);
-          *a = make_uint2(Q8Code<E4M3>::encode4(f), Q8Code<E4M3>::encode4(f + 4));
-        }
+        requantise<D, E4M3>(codes + (static_cast<uint64_t>(slot0) * p.Hkv + h) * D + col, static_cast<uint64_t>(p.Hkv) * D, row,
+                            kRows, first, __fdiv_rn(old, scale));
       }
       if (tid == 0) *sp = scale;  // every thread has read the old one (two barriers ago)
+    }
+  }
+}
+
+// Small blocks (at most 4,096 values a head): a warp takes a run's rows of one
+// kv head, of K or of V, so that neither a barrier nor shared memory stands
+// between its loads, its maximum and its stores; the CTA's warps take
+// different heads.  With a CTA a run, 13,000 rows of 8 heads of 128 in blocks
+// of 16 took 53 us; this takes KKK us.
+template <int D, int NP, bool E4M3>
+__global__ void __launch_bounds__(256) k_kv_append_q8_small(Q8Store p) {
+  constexpr int kTpr = D / 8, kRows = 32 / kTpr;  // lanes per row, rows per pass
+  constexpr float kTop = Q8Code<E4M3>::kTop;
+  __shared__ int64_t s_slot[1 + 2 * kMaxBlock];
+  const int lane = threadIdx.x & 31, item = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk);
+  for (int i = threadIdx.x; i < 1 + p.chunk + p.block; i += blockDim.x) {
+    const int t = t0 - 1 + i;
+    s_slot[i] = t >= 0 && t < p.tokens ? p.slots[t] : -1;
+  }
+  __syncthreads();
+  if (item >= 2 * p.Hkv) return;
+  const int side = item & 1, h = item >> 1;
+  const uint16_t *x = p.x[side];
+  const uint64_t stride = p.stride[side];
+  float *scales = p.scale[side];
+  const int row = lane / kTpr, col = (lane % kTpr) * 8;
+  const uint32_t bmask = static_cast<uint32_t>(p.block - 1);
+  for (int c0 = t0; c0 < t1; c0 += 32) {
+    const int tl = c0 + lane;
+    bool begins = false;
+    if (tl < t1) {
+      const int64_t s = s_slot[tl - t0 + 1], before = s_slot[tl - t0];
+      begins = s >= 0 && s < p.n_slots &&
+               !((static_cast<uint32_t>(s) & bmask) != 0 && before >= 0 && before == s - 1);
+    }
+    uint32_t runs = __ballot_sync(0xFFFFFFFFu, begins);
+    while (runs) {
+      const int t = c0 + __ffs(runs) - 1;
+      runs &= runs - 1;
+      const int64_t slot = s_slot[t - t0 + 1];
+      const int first = static_cast<int>(static_cast<uint32_t>(slot) & bmask);
+      float *sp = scales + (slot >> p.block_shift) * p.Hkv + h;
+      const float old = first > 0 ? *sp : 0.0f;
+      const int most = min(p.block - first, p.tokens - t);
+      const uint16_t *src = x + static_cast<uint64_t>(t) * stride + static_cast<uint64_t>(h) * D + col;
+      uint4 v[NP];
+      uint32_t peak = 0, here = 0;  // bit i: pass i's row is of the run
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int r = i * kRows + row;
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (r < most && s_slot[t - t0 + 1 + r] == slot + r) {  // slots ascend: a run has no gap
+          here |= 1u << i;
+          v[i] = __ldg(reinterpret_cast<const uint4 *>(src + static_cast<uint64_t>(r) * stride));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) peak = max(peak, peak8(v[i]));
+      peak = __reduce_max_sync(0xFFFFFFFFu, peak);
+      const float mag = fmaxf(bf16_to_f32(static_cast<uint16_t>(peak)), kQ8Tiny);
+      const float scale = fmaxf(old, __fdiv_rn(mag, kTop));
+      const float inv = __fdiv_rn(1.0f, scale);
+      uint8_t *dst = p.codes[side] + (static_cast<uint64_t>(slot - first) * p.Hkv + h) * D + col;
+      const uint64_t pitch = static_cast<uint64_t>(p.Hkv) * D;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if ((here >> i) & 1u)
+          *reinterpret_cast<uint2 *>(dst + static_cast<uint64_t>(first + i * kRows + row) * pitch) = encode_row8<E4M3>(v[i], inv);
+      if (first > 0 && scale != old) requantise<D, E4M3>(dst, pitch, row, kRows, first, __fdiv_rn(old, scale));
+      __syncwarp();  // every lane has read the old scale
+      if (lane == 0) *sp = scale;
     }
   }
 }
@@ -465,12 +544,35 @@ void launch_append(const Q8Store &p, dim3 grid, bool e4m3, cudaStream_t s) {
     k_kv_append_q8<D, NP, false><<<grid, kAppendThreads, 0, s>>>(p);
 }
 
+template <int D, int NP>
+void launch_append_small(const Q8Store &p, dim3 grid, int warps, bool e4m3, cudaStream_t s) {
+  if (e4m3)
+    k_kv_append_q8_small<D, NP, true><<<grid, 32 * warps, 0, s>>>(p);
+  else
+    k_kv_append_q8_small<D, NP, false><<<grid, 32 * warps, 0, s>>>(p);
+}
+
 template <int D>
-void launch_append_d(const Q8Store &p, dim3 grid, bool e4m3, cudaStream_t s) {
+void launch_append_d(Q8Store p, bool e4m3, cudaStream_t s) {
+  const int items = 2 * p.Hkv, values = p.block * D;
+  const bool small = values <= 4096;
+  const int warps = std::min(items, 8);
+  const unsigned across = small ? (items + warps - 1) / warps : items;
+  // Chunks of one token while that gives every SM its eight CTAs, of a block at most.
+  const uint64_t ctas = static_cast<uint64_t>(p.tokens) * across / (148 * 8);
+  p.chunk = static_cast<int>(std::min<uint64_t>(std::max<uint64_t>(ctas, 1), p.block));
+  const dim3 grid((p.tokens + p.chunk - 1) / p.chunk, across);
+  if (small) {
+    if constexpr (D == 64) {
+      if (p.block == 16) return launch_append_small<D, 4>(p, grid, warps, e4m3, s);
+    }
+    if constexpr (D <= 128) {
+      if (values == 2048) return launch_append_small<D, 8>(p, grid, warps, e4m3, s);
+    }
+    return launch_append_small<D, 16>(p, grid, warps, e4m3, s);
+  }
   constexpr int kRows = kAppendThreads / (D / 8);
   const int np = (p.block + kRows - 1) / kRows;
-  if (np <= 1) return launch_append<D, 1>(p, grid, e4m3, s);
-  if (np <= 2) return launch_append<D, 2>(p, grid, e4m3, s);
   if (np <= 4) return launch_append<D, 4>(p, grid, e4m3, s);
   if constexpr (D >= 128) {
     if (np <= 8) return launch_append<D, 8>(p, grid, e4m3, s);
@@ -611,14 +713,11 @@ int kv_append_q8(const FnQ8AppendArgs *a, cudaStream_t s, std::string &err) {
   p.block = static_cast<int>(c.block);
   p.block_shift = shift_of(c.block);
   p.Hkv = static_cast<int>(c.kv_heads);
-  const uint64_t ctas = static_cast<uint64_t>(a->tokens) * c.kv_heads * 2 / (148 * 8);
-  p.chunk = static_cast<int>(std::min<uint64_t>(std::max<uint64_t>(ctas, 1), c.block));
-  const dim3 grid((a->tokens + p.chunk - 1) / p.chunk, 2 * c.kv_heads);
   const bool e4m3 = c.code_type == FNMOE_Q8_E4M3;
   switch (c.head_dim) {
-    case 64: launch_append_d<64>(p, grid, e4m3, s); break;
-    case 128: launch_append_d<128>(p, grid, e4m3, s); break;
-    default: launch_append_d<256>(p, grid, e4m3, s); break;
+    case 64: launch_append_d<64>(p, e4m3, s); break;
+    case 128: launch_append_d<128>(p, e4m3, s); break;
+    default: launch_append_d<256>(p, e4m3, s); break;
   }
   return launched("kv append", err);
 }
