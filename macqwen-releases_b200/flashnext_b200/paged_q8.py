@@ -249,3 +249,76 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
         code = lib.fnmoe_paged_attention_q8(ref, stream)
     _lib.check(code, "paged_attention_q8")
     return out
+
+
+class PagedKVCacheQ8:
+    """Pages, scales, block tables and free ring of one attention layer's
+    8-bit cache, and a serving step over them:
+
+        plan = cache.plan(new_lens, release)   # tables and slots on the device
+        cache.append(k, v)                     # the step's packed rows
+        out = cache.attention(q, scale)        # causal, packed like k and v
+
+    ``batch`` rows of at most ``max_pages_per_seq`` pages; ``max_tokens`` new
+    tokens a step.  Nothing is read on the host: a sequence that does not fit
+    has ``plan.admitted`` 0 and takes no part in the step, so its rows must not
+    be among those packed (``plan.cu_new`` counts them as none).  Tables and
+    lengths alternate between two sets of buffers; a captured CUDA graph
+    therefore holds an even number of plans.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_pages_per_seq: int,
+                 batch: int, max_tokens: int, block: int | None = None, codes=torch.int8, device="cuda"):
+        if codes not in _CODES:
+            raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn")
+        block = block or next((b for b in reversed(BLOCKS) if page_size % b == 0), 0)
+        if block not in BLOCKS or page_size % block:
+            raise ValueError(f"page_size must be a multiple of a block of {BLOCKS} tokens")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
+        i32 = torch.int32
+        # zeros: e4m3 slots that are never written stay finite
+        self.k, self.v = (torch.zeros((num_pages, page_size, kv_heads, head_dim), dtype=torch.uint8, device=device).view(codes)
+                          for _ in range(2))
+        self.k_scale, self.v_scale = (torch.zeros((num_pages, page_size // block, kv_heads), device=device) for _ in range(2))
+        self.free_pages = torch.arange(num_pages, dtype=i32, device=device)
+        self.page_size, self.max_tokens = page_size, int(max_tokens)
+
+        def buffers():
+            return PagePlan(torch.full((batch, max_pages_per_seq), -1, dtype=i32, device=device),
+                            torch.zeros(batch, dtype=i32, device=device), self.free_pages,
+                            torch.tensor([0, num_pages], dtype=i32, device=device),
+                            torch.full((self.max_tokens,), -1, dtype=torch.int64, device=device),
+                            *(torch.full((self.max_tokens,), -1, dtype=i32, device=device) for _ in range(2)),
+                            torch.zeros(batch + 1, dtype=i32, device=device),
+                            torch.ones(batch, dtype=i32, device=device))
+
+        self.last, self._other = buffers(), buffers()
+
+    @property
+    def tensors(self):
+        """(k, v, k_scale, v_scale), as the functions of this module take them."""
+        return self.k, self.v, self.k_scale, self.v_scale
+
+    def plan(self, new_lens, release=None) -> PagePlan:
+        """Give every row ``new_lens[b]`` more tokens (rows with ``release`` set start over)."""
+        was = self.last
+        self.last = page_plan(was.seq_lens, new_lens, was.block_table, self.free_pages, was.free_state, self.page_size,
+                              self.max_tokens, release=release, out=self._other)
+        self._other = was
+        return self.last
+
+    def append(self, k, v) -> None:
+        """Store the last plan's packed rows [tokens, kv_heads, head_dim]."""
+        kv_append_q8(k, v, self.last.slot_map[: k.shape[0]], *self.tensors)
+
+    def attention(self, q, scale: float, one_row: bool = False, out=None):
+        """Attention of the last plan's packed rows [tokens, q_heads, head_dim];
+        ``one_row``: every row of the table has exactly one (a decode step)."""
+        p = self.last
+        return paged_attention_q8(q, *self.tensors, p.block_table, p.seq_lens, scale,
+                                  cu_q=None if one_row else p.cu_new, out=out)
+
+    def read(self, slots):
+        """The bfloat16 (k, v) that slots hold (:func:`kv_read_q8`)."""
+        return kv_read_q8(slots, *self.tensors)

@@ -626,3 +626,125 @@ def test_offsets_past_32_bits(cuda_lib):
         seen = np.arange(n)[None] <= (n - rows + np.arange(rows))[:, None]
         want, mag = oq8.attention(q.float().numpy(), k, v, seen, 0.0625)
         assert (np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * mag).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_serving_steps_match_attention_over_the_values_held(cuda_lib, kind):
+    """Prompts, decodes, a verify step and a released row through
+    PagedKVCacheQ8: after each step the attention equals float64 attention
+    over the values that the cache then holds, read back by slot."""
+    import torch
+    from flashnext_b200.paged_q8 import PagedKVCacheQ8
+
+    codes = torch.int8 if kind == "int8" else torch.float8_e4m3fn
+    batch, kv, group, dim, page = 4, 2, 4, 64, 32
+    cache = PagedKVCacheQ8(40, page, kv, dim, 10, batch, 512, block=16, codes=codes)
+    rng = np.random.default_rng(12)
+    lens = [0] * batch
+    steps = [([70, 1, 0, 33], None), ([1, 1, 1, 1], None), ([4, 0, 7, 1], None), ([1, 1, 1, 50], [1, 0, 0, 0]),
+             ([1, 1, 1, 1], None)]
+    scale = 0.17
+    for new, gone in steps:
+        dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+        plan = cache.plan(dev(new), None if gone is None else dev(gone))
+        lens = [(0 if gone and gone[b] else lens[b]) + new[b] for b in range(batch)]
+        n = sum(new)
+        assert plan.seq_lens.tolist() == lens and plan.admitted.tolist() == [1] * batch
+        x = [_bf16(rng.standard_normal((n, h, dim))).cuda() for h in (kv, kv, kv * group)]
+        cache.append(x[0], x[1])
+        out = cache.attention(x[2], scale, one_row=new == [1] * batch).float().cpu().numpy()
+        q, table, at = x[2].float().cpu().numpy(), plan.block_table.cpu().numpy(), 0
+        for b in range(batch):
+            if new[b]:
+                slots = torch.from_numpy(_slots(table, b, 0, lens[b], page)).cuda()
+                c = [t.float().view(-1, kv, dim)[slots].cpu().numpy() for t in (cache.k, cache.v)]
+                s = [t.view(-1, kv)[slots // 16].cpu().numpy()[:, :, None] for t in (cache.k_scale, cache.v_scale)]
+                seen = np.arange(lens[b])[None] <= (lens[b] - new[b] + np.arange(new[b]))[:, None]
+                want, mag = oq8.attention(q[at:at + new[b]], c[0] * s[0], c[1] * s[1], seen, scale)
+                off = np.abs(out[at:at + new[b]] - want)
+                assert (off <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * mag + 1e-30).all(), (b, new[b], lens[b])
+                back = cache.read(slots)
+                for i in range(2):
+                    assert torch.equal(back[i].cpu().float(), _bf16(c[i] * s[i]).float())
+            at += new[b]
+
+
+@pytest.mark.gpu
+def test_a_decode_step_replays_from_a_graph(cuda_lib):
+    """Two steps (the two sets of buffers) captured and replayed: lengths grow
+    on the device and the outputs equal those of eager calls."""
+    import torch
+    from flashnext_b200.paged_q8 import PagedKVCacheQ8
+
+    def fresh():
+        c = PagedKVCacheQ8(24, 32, 1, 128, 8, 3, 256)
+        c.plan(torch.tensor([40, 7, 100], dtype=torch.int32, device="cuda"))
+        g = torch.Generator(device="cuda")
+        g.manual_seed(3)
+        r = torch.randn(147, 1, 128, device="cuda", generator=g).bfloat16()
+        c.append(r, 2 * r)
+        return c
+
+    one = torch.ones(3, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    k, q = torch.randn(3, 1, 128, device="cuda", generator=g).bfloat16(), torch.randn(3, 4, 128, device="cuda", generator=g).bfloat16()
+    out = torch.empty(2, 3, 4, 128, dtype=torch.bfloat16, device="cuda")
+
+    def two(c):
+        for i in range(2):
+            c.plan(one)
+            c.append(k, k)
+            c.attention(q, 0.09, one_row=True, out=out[i])
+
+    eager = fresh()
+    want = []
+    for _ in range(3):
+        two(eager)
+        want.append(out.clone())
+    c = fresh()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        two(c)  # warm-up: the stream's workspace
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(out, want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        two(c)
+    for i in (1, 2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+    assert c.last.seq_lens.tolist() == [46, 13, 106]
+
+
+def test_cache_class_refuses_geometries():
+    from flashnext_b200.paged_q8 import PagedKVCacheQ8
+
+    import torch
+    for kw, err in (({"page_size": 24}, ValueError), ({"block": 48}, ValueError), ({"head_dim": 96}, ValueError),
+                    ({"codes": torch.uint8}, TypeError)):
+        args = dict(num_pages=2, page_size=64, kv_heads=1, head_dim=64, max_pages_per_seq=1, batch=1, max_tokens=8,
+                    device="cpu") | kw
+        with pytest.raises(err):
+            PagedKVCacheQ8(**args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,most", [("int8", 0.03), ("e4m3", 0.08)])
+def test_the_serving_example_stays_near_unquantised_attention(cuda_lib, kind, most):
+    """The example's own comparison.  A code's rounding is uniform within half
+    a code of the block's largest magnitude (about 4.5 of normal rows: 4.5 /
+    127 / sqrt(12) = 1% of a value for int8; e4m3 keeps 4 bits, 2^-4 / sqrt(12)
+    / 1.4 = 1.3% to 2.6% of each); keys and values each contribute, and the bound is
+    about twice their sum."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "macqwen-releases_b200" / "examples" / "serve_q8.py"
+    spec = importlib.util.spec_from_file_location("serve_q8", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(["--steps", "24", "--codes", kind]) < most
