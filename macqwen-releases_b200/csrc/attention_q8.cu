@@ -646,9 +646,9 @@ __global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
   __shared__ float s_l[256];
   pdl_wait();
   pdl_trigger();
-  const bool is_few = static_cast<int>(blockIdx.x) < 8 * few;
-  const int at = is_few ? blockIdx.x >> 3 : (blockIdx.x - 8 * few) >> 5;
-  const int row0 = is_few ? blockIdx.x & 7 : 4 * ((blockIdx.x - 8 * few) & 31);
+  const bool is_few = static_cast<int>(blockIdx.x) < p.join_rows * few;
+  const int at = is_few ? blockIdx.x / p.join_rows : (blockIdx.x - p.join_rows * few) >> 5;
+  const int row0 = is_few ? blockIdx.x % p.join_rows : 4 * ((blockIdx.x - p.join_rows * few) & 31);
   const bool by_seg = is_few ? p.by_seg : p.tby_seg;
   int4 cut;
   int c0, h;
@@ -836,7 +836,7 @@ cudaError_t launch_few(const Q8View &p, cudaStream_t s) {
 
 template <int D>
 cudaError_t launch_joins(const Q8View &p, int few, int many, cudaStream_t s) {
-  return launch_pdl(k_q8_join<D>, dim3(8 * few + 32 * many), dim3(256), 0, s, p, few, many);
+  return launch_pdl(k_q8_join<D>, dim3(p.join_rows * few + 32 * many), dim3(256), 0, s, p, few, many);
 }
 
 template <int D>
@@ -918,6 +918,7 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
   const int d = static_cast<int>(a->cache.head_dim);
   // Segments there can be: the join looks at those where they are fewer than the cuts.
   p.few_tiles = (std::min(p.few_rows, p.cu ? p.few_rows : p.gq) + 7) / 8;
+  p.join_rows = p.cu ? 8 : std::min(p.gq, 8);
   const uint64_t few_segs = static_cast<uint64_t>(p.B) * p.Hkv * p.few_tiles;
   const uint64_t many_segs = many ? many_tiles(p) * p.Hkv : 0;
   p.by_seg = few_segs < static_cast<uint64_t>(few_ctas(d) - 1);

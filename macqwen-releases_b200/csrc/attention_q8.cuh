@@ -49,6 +49,7 @@ struct Q8View {
   // workspace of the few-row kernel (8 rows a tile)
   int4 *cuts;           // [CTAs] where each range begins (cut_of), or by_seg: [B][Hkv][few_tiles]
   int few_tiles;        // tiles of 8 rows that a sequence can have
+  int join_rows;        // rows that such a tile can have
   bool by_seg, tby_seg, pair_boxes;
   float *part;          // [2 * CTAs][8][D] unfinished sums
   float2 *part_ml;      // [2 * CTAs][8] their reference and weight sum
