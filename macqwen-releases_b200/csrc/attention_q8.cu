@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint64_t sc = static_cast<uint64_t>(static_cast<uint32_t>(max(slot[e], 0)) >> p.block_shift) * static_cast<uint32_t>(p.Hkv);
-        ks[e] = __ldg(ks_h + sc);
-        vs[e] = __ldg(vs_h + sc);
+        ks[e] = __ldcg(ks_h + sc);
+        vs[e] = __ldcg(vs_h + sc);
       }
     };
     auto request_v = [&](int tt) {

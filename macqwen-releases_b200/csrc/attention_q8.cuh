@@ -189,16 +189,13 @@ __device__ __forceinline__ void widen_pairs(uint32_t w0, uint32_t w1, uint32_t (
   }
 }
 
+// 16 bytes from L2.  The kernels may be resident while an earlier one of the
+// stream still writes (programmatic dependent launch), so nothing that such a
+// kernel produced -- queries, codes, scales -- is read through the non-coherent
+// path.
 __device__ __forceinline__ uint4 ldg_stream(const void *p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 

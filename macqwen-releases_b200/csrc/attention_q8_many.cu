@@ -32,8 +32,8 @@
 // unit's Q K^T runs while this one's P is made.  At D 64 and 128 P takes S's
 // columns and a CTA needs 256 of the 512: two CTAs share an SM and fill each
 // other's waits.
-// Measured: a 5,000-token prefill chunk (16/2 heads, D 256, 205 GFLOP) 376 us,
-// 0.54 PFLOP/s, about 4,000 clocks a unit.  What bounds it now is the chain
+// Measured: a 5,000-token prefill chunk (16/2 heads, D 256, 205 GFLOP) 356 us,
+// 0.58 PFLOP/s, about 3,800 clocks a unit.  What bounds it now is the chain
 // softmax -> P V and the issue slots that widening takes beside it (IPC 2.0);
 // the MMAs alone take about 1,700 clocks a unit (N 64 and two terms of P).
 // Every wait is bounded: a timeout sets the device error word and marks the
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         for (int c = 0; c < kDims / 32; ++c)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            x[c][e] = q_at[e] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.q + q_at[e] + c0 + 32 * c)) : make_uint4(0, 0, 0, 0);
+            x[c][e] = q_at[e] >= 0 ? __ldcg(reinterpret_cast<const uint4 *>(p.q + q_at[e] + c0 + 32 * c)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int c = 0; c < kDims / 32; ++c) {
           __syncwarp();
@@ -701,8 +701,8 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
             const int c = page_col(p, t), pg = trow[c];
             if (static_cast<uint32_t>(pg) < static_cast<uint32_t>(p.pages)) {
               const size_t at = (static_cast<size_t>(pg) * bpp + ((t - c * p.page) >> p.block_shift)) * p.Hkv + q.h;
-              const float v = fmaxf(__ldg(p.vs + at), 0x1p-110f);
-              mul = fmaxf(p.scale * kLog2e * __ldg(p.ks + at), 1e-37f);
+              const float v = fmaxf(__ldcg(p.vs + at), 0x1p-110f);
+              mul = fmaxf(p.scale * kLog2e * __ldcg(p.ks + at), 1e-37f);
               add = lg2(v);
               inv = rcp(v);
             }
