@@ -32,8 +32,8 @@
 // unit's Q K^T runs while this one's P is made.  At D 64 and 128 P takes S's
 // columns and a CTA needs 256 of the 512: two CTAs share an SM and fill each
 // other's waits.
-// Measured: a 5,000-token prefill chunk (16/2 heads, D 256, 205 GFLOP) 356 us,
-// 0.58 PFLOP/s, about 3,800 clocks a unit.  What bounds it now is the chain
+// Measured: a 5,000-token prefill chunk (16/2 heads, D 256, 205 GFLOP) 375 us,
+// 0.55 PFLOP/s, about 4,000 clocks a unit.  What bounds it now is the chain
 // softmax -> P V and the issue slots that widening takes beside it (IPC 2.0);
 // the MMAs alone take about 1,700 clocks a unit (N 64 and two terms of P).
 // Every wait is bounded: a timeout sets the device error word and marks the
