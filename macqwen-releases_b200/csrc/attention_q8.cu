@@ -433,6 +433,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
 #pragma unroll
     for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float v_top = 0.0f;  // the largest value scale so far
 
     __syncthreads();  // the query rows are in place
     for (; t < t_end; t += kFewUnit) {
@@ -441,12 +442,16 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       arrived(kbar);
       F::Query::scores(kat, qat, sc);
       const float k_scale[2] = {ks[0], ks[1]};
-      float lv[2], rv[2];
+      float lv[2], rv[2], fold[2];
+      v_top = fmaxf(v_top, fmaxf(in[0] ? vs[0] : 0.0f, in[1] ? vs[1] : 0.0f));
+      const float v_least = fmaxf(v_top * kScaleSpan, kScaleLeast);
+      const bool folds = (in[0] && vs[0] < v_least) || (in[1] && vs[1] < v_least);  // of the whole warp
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float v_scale = fmaxf(vs[e], 0x1p-110f);
+        const float v_scale = fmaxf(vs[e], v_least);
         lv[e] = lg2(v_scale);
         rv[e] = rcp(v_scale);
+        fold[e] = vs[e] < v_least ? vs[e] * rv[e] : 1.0f;
       }
       __syncwarp();  // every lane has read its K
       request_k(t + kFewUnit);
@@ -480,8 +485,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
           for (int s = 4; s <= 16; s <<= 1) cm = fmaxf(cm, __shfl_xor_sync(0xFFFFFFFFu, cm, s));
           cm = fmaxf(cm, m[hh]);
           al[hh] = cm == -INFINITY ? 1.0f : ex2(m[hh] - cm);
+          if (cm != -INFINITY) l[hh] = times_ex2(l[hh], m[hh] - cm);
           m[hh] = cm;
-          l[hh] *= al[hh];
         }
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
@@ -495,10 +500,16 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
       uint32_t hi[2][2], lo[2][2];  // [tile][tokens g | g + 8 transposed]
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float p0 = ex2(x[e][0] - ref[0]), p1 = ex2(x[e][1] - ref[1]);
-        const float p2 = ex2(x[e][2] - ref[0]), p3 = ex2(x[e][3] - ref[1]);
+        float p0 = ex2(x[e][0] - ref[0]), p1 = ex2(x[e][1] - ref[1]);
+        float p2 = ex2(x[e][2] - ref[0]), p3 = ex2(x[e][3] - ref[1]);
         l[0] = __fmaf_rn(p0 + p2, rv[e], l[0]);
         l[1] = __fmaf_rn(p1 + p3, rv[e], l[1]);
+        if (folds) {
+          p0 *= fold[e];
+          p1 *= fold[e];
+          p2 *= fold[e];
+          p3 *= fold[e];
+        }
         split_bf16x2(p0, p1, hi[e][0], lo[e][0]);
         split_bf16x2(p2, p3, hi[e][1], lo[e][1]);
 #pragma unroll
@@ -611,7 +622,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
         s.y += v.y;
         s.z += v.z;
         s.w += v.w;
-        if (s_m[w][r] != -INFINITY) ll += s_l[w][r] * ex2(s_m[w][r] - mm);
+        if (s_m[w][r] != -INFINITY) ll += times_ex2(s_l[w][r], s_m[w][r] - mm);
       }
       if (whole) {
         const float inv = ll > 0.0f ? __frcp_rn(ll) : 0.0f;
@@ -700,18 +711,32 @@ __global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
   for (int s = 4; s <= 16; s <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, s));
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float ll = 0.0f;
-#pragma unroll 8
-  for (int c = c0 + grp; c <= c1; c += groups) {
-    const size_t s = slot_of(c);
-    const float2 ml = ml_all[s * R + r];
-    const float4 v = is_few ? *reinterpret_cast<const float4 *>(p.part + (s * 8 + r) * D + 4 * lane)
-                            : reinterpret_cast<const float4 *>(p.tpart)[(s * L + lane) * 128 + r];
-    const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
-    ll += ml.y * w;
-    acc.x += v.x * w;
-    acc.y += v.y * w;
-    acc.z += v.z * w;
-    acc.w += v.w * w;
+  // CTAs whose sums are asked for at once.  (1: verify of 16 sequences 91 us, prefill chunk 368;
+  // 2: 89 and 368; 4: 88 and 373; 8: 91 and 393.)
+  constexpr int kAhead = 2;
+  for (int c = c0 + grp; c <= c1; c += kAhead * groups) {
+    float2 ml[kAhead];
+    float4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.0f);
+      v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (c + k * groups <= c1) {
+        const size_t s = slot_of(c + k * groups);
+        ml[k] = ml_all[s * R + r];
+        v[k] = is_few ? *reinterpret_cast<const float4 *>(p.part + (s * 8 + r) * D + 4 * lane)
+                      : reinterpret_cast<const float4 *>(p.tpart)[(s * L + lane) * 128 + r];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float half = ml[k].x == -INFINITY ? 0.0f : ex2(0.5f * (ml[k].x - mm)), w = half * half;
+      ll += ml[k].y * half * half;  // as times_ex2
+      acc.x += v[k].x * w;
+      acc.y += v[k].y * w;
+      acc.z += v[k].z * w;
+      acc.w += v[k].w * w;
+    }
   }
   if (groups > 1) {
     s_o[threadIdx.x] = acc;

@@ -12,7 +12,16 @@
 //   t_j = (scale * log2 e * ks) (q . kcode_j) + log2 vs,   u_j = 2^(t_j - m),
 // m a running reference of the t_j,
 //   out = sum_j u_j vcode_j / sum_blocks (1 / vs) sum_(j in block) u_j :
-// the value scale rides in the exponent.  The weights enter the second product
+// the value scale rides in the exponent.  The sums hold t_j within 2^126 of the
+// reference, so a block whose vs is far below its neighbours' would drop out of
+// the denominator, where its tokens count in full whatever their values: a block
+// of zeros has vs = 2^-107.  Its vs is therefore raised to vs' = 2^-64 of the
+// largest that the warp (or tile) has met in its piece of work, which leaves
+// weights down to 2^-62 of the largest in the denominator, and its weights go
+// into the second product as u_j vs / vs', at least 2^-62 of the largest weight
+// where the scales lie within 2^128 of each other; beyond that the values of the
+// smaller blocks fade.  vs' is at least 2^-90, so that no denominator overflows.
+//   The weights enter the second product
 // as two bfloat16 terms, u = hi + lo with 16 bits: one term alone would cost
 // up to 2^-9 of an output (as much as its final rounding), and float16 loses
 // weights below 2^-24 of the largest, which are all that is left of an output
@@ -32,6 +41,7 @@ namespace fnmoe {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;  // a reference may fall this far (log2) below the largest t
+constexpr float kScaleSpan = 0x1p-64f, kScaleLeast = 0x1p-90f;  // vs' >= vs of the largest block * span, and >= least
 
 constexpr int kUnit = 64;  // tokens of a unit of work
 
@@ -78,6 +88,12 @@ __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+// x 2^d where 2^d alone may be too small for a float: a denominator's sum can be
+// as large as 2^90 of its weights.
+__device__ __forceinline__ float times_ex2(float x, float d) {
+  const float h = ex2(0.5f * d);
+  return x * h * h;
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t d;

@@ -43,6 +43,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_q8.cuh"
 #include "moe_kernels.cuh"
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
           float tm = -INFINITY;
 #pragma unroll
           for (int g = 0; g < kTok / 16; ++g) {
-            f[g] = info[g];  // scale * log2 e * ks, log2 vs, 1 / vs
+            f[g] = info[g];  // scale * log2 e * ks, log2 vs', 1 / vs', vs / vs'
             float a = s[16 * g], b = s[16 * g + 1];
 #pragma unroll
             for (int e = 2; e < 16; e += 2) {
@@ -513,8 +514,8 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
           if (__any_sync(0xFFFFFFFFu, tm > m + kLazy)) {
             const float mn = fmaxf(m, tm);
             const float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
+            if (mn != -INFINITY) l = times_ex2(l, m - mn);
             m = mn;
-            l *= al;
             if (j > 0) {
               live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err));
               tc_fence_after();
@@ -534,25 +535,32 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
 #pragma unroll
           for (int h2 = 0; h2 < kTok / 32; ++h2) {
             uint32_t hi[16], lo[16];
+            auto weigh = [&](auto folds) {
 #pragma unroll
-            for (int g2 = 0; g2 < 2; ++g2) {
-              const int g = 2 * h2 + g2;
-              const float2 mul = make_float2(f[g].x, f[g].x), add = make_float2(f[g].y - ref, f[g].y - ref);
-              float2 sum = make_float2(0.0f, 0.0f);
+              for (int g2 = 0; g2 < 2; ++g2) {
+                const int g = 2 * h2 + g2;
+                const float2 mul = make_float2(f[g].x, f[g].x), add = make_float2(f[g].y - ref, f[g].y - ref);
+                float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const float2 x = fma2(make_float2(s[16 * g + e], s[16 * g + e + 1]), mul, add);
-                const float2 u = make_float2(ex2(x.x), ex2(x.y));
-                sum = add2(sum, u);
-                // hi: the upper 16 bits of each; lo: what is left, rounded
-                const uint32_t a0 = __float_as_uint(u.x), a1 = __float_as_uint(u.y);
-                hi[8 * g2 + e / 2] = prmt(a0, a1, 0x7632u);
-                const float2 left = add2(u, make_float2(__uint_as_float((a0 & 0xFFFF0000u) ^ 0x80000000u),
-                                                        __uint_as_float((a1 & 0xFFFF0000u) ^ 0x80000000u)));
-                lo[8 * g2 + e / 2] = pack_bf16x2(left.x, left.y);
+                for (int e = 0; e < 16; e += 2) {
+                  const float2 x = fma2(make_float2(s[16 * g + e], s[16 * g + e + 1]), mul, add);
+                  float2 u = make_float2(ex2(x.x), ex2(x.y));
+                  sum = add2(sum, u);
+                  if constexpr (decltype(folds)::value) u = make_float2(u.x * f[g].w, u.y * f[g].w);
+                  // hi: the upper 16 bits of each; lo: what is left, rounded
+                  const uint32_t a0 = __float_as_uint(u.x), a1 = __float_as_uint(u.y);
+                  hi[8 * g2 + e / 2] = prmt(a0, a1, 0x7632u);
+                  const float2 left = add2(u, make_float2(__uint_as_float((a0 & 0xFFFF0000u) ^ 0x80000000u),
+                                                          __uint_as_float((a1 & 0xFFFF0000u) ^ 0x80000000u)));
+                  lo[8 * g2 + e / 2] = pack_bf16x2(left.x, left.y);
+                }
+                l = __fmaf_rn(sum.x + sum.y, f[g].z, l);
               }
-              l = __fmaf_rn(sum.x + sum.y, f[g].z, l);
-            }
+            };
+            if (f[2 * h2].w == 1.0f && f[2 * h2 + 1].w == 1.0f)  // alike in all threads of the warp
+              weigh(std::false_type{});
+            else
+              weigh(std::true_type{});
             if (h2 == 0) {  // P may be written once the last unit's P V is done
               live = live && bar_wait(bar(M::kPEmpty), (i & 1u) ^ 1u, dead, err);
               live = __all_sync(0xFFFFFFFFu, live);
@@ -693,24 +701,32 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
       while (live && next_piece(p, w, q)) {
         const int ctx = tokens_of(p, q.b), bpp = p.page >> p.block_shift;
         const int32_t *trow = p.table + static_cast<size_t>(q.b) * p.width;
+        float v_top = 0.0f;  // the largest value scale of the piece so far
         for (int u = q.u0; live && u < q.u0 + q.n; ++u, ++i) {
           const uint32_t slot = i % M::kSlots, ph = (i / M::kSlots) & 1u;
           const int t = u * kUnit + 16 * (lane & 3);
-          float mul = 1e-37f, add = -INFINITY, inv = 0.0f;  // a granule without a token or page weighs nothing
+          float mul = 1e-37f, add = -INFINITY, inv = 0.0f, fold = 1.0f;  // a granule without a token or page weighs nothing
+          float v = -1.0f;
           if (t < ctx) {
             const int c = page_col(p, t), pg = trow[c];
             if (static_cast<uint32_t>(pg) < static_cast<uint32_t>(p.pages)) {
               const size_t at = (static_cast<size_t>(pg) * bpp + ((t - c * p.page) >> p.block_shift)) * p.Hkv + q.h;
-              const float v = fmaxf(__ldcg(p.vs + at), 0x1p-110f);
+              v = fmaxf(__ldcg(p.vs + at), 0.0f);
               mul = fmaxf(p.scale * kLog2e * __ldcg(p.ks + at), 1e-37f);
-              add = lg2(v);
-              inv = rcp(v);
             }
+          }
+          // bits of numbers that are not negative order as the numbers do
+          v_top = fmaxf(v_top, __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fmaxf(v, 0.0f)))));
+          if (v >= 0.0f) {
+            const float v_least = fmaxf(v_top * kScaleSpan, kScaleLeast), v_scale = fmaxf(v, v_least);
+            add = lg2(v_scale);
+            inv = rcp(v_scale);
+            if (v < v_least) fold = v * inv;
           }
           // as far ahead as K itself may be, so that the kept units are not overrun
           live = __all_sync(0xFFFFFFFFu, bar_wait(bar(M::kKEmpty + slot), ph ^ 1u, dead, err));
           if (!live) break;
-          if (lane < 4) reinterpret_cast<float4 *>(sm + M::kOffInfo)[(i % kInfo) * 4 + lane] = make_float4(mul, add, inv, 0.0f);
+          if (lane < 4) reinterpret_cast<float4 *>(sm + M::kOffInfo)[(i % kInfo) * 4 + lane] = make_float4(mul, add, inv, fold);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(M::kInfoFull + i % kInfo));
         }

@@ -1,0 +1,140 @@
+"""The paged 8-bit KV cache at its edges: value scales far apart.
+
+Attention is held to this: an output is the bfloat16 rounding of a number within
+2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
+That covers the float32 arithmetic: a weight enters the second product as two
+bfloat16 terms, together within 2^-16; a score of magnitude below 64 (in log2)
+is a few float32 roundings of 2^-24 off, 2^-16 of its weight; ex2, lg2 and the
+reciprocal are within 2^-21; and a float32 sum of up to 5,000 terms of the matrix
+instructions, 16 at a time and two for each, is within 700 * 2^-23 < 2^-13.5 in
+the worst case.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from flashnext_b200 import _lib
+from oracle import paged_q8 as oq8
+from test_paged_q8 import KINDS, _bf16, _empty_cache, _place, _slots
+
+C_MAG = 2.0 ** -13
+
+
+def _outside(out, want, mag, c=C_MAG):
+    """How many of the bfloat16 values `out` are not the rounding of a float32
+    within c * mag of `want` (rounding is monotonic)."""
+    low, high = (_bf16((want + s * c * mag).astype(np.float32)).float().numpy() for s in (-1, 1))
+    return int(((out < low) | (out > high) | np.isnan(out)).sum())
+
+
+def _dev(a):
+    import torch
+
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+def _cache_of(table, pages, page, block, kind, k, ks, v, vs):
+    """Device cache whose slots hold the code values k, v [slots, heads, dim]
+    and whose blocks have the scales ks, vs [blocks, heads]."""
+    import torch
+
+    cache = _empty_cache(pages, page, block, k.shape[1], k.shape[2], kind)
+    for i, (c, s) in enumerate(((k, ks), (v, vs))):
+        cache[i].copy_(torch.from_numpy(c).to(cache[i].dtype).view(cache[i].shape).cuda())
+        cache[2 + i].copy_(torch.from_numpy(s).view(cache[2 + i].shape))
+    return cache
+
+
+def _wrong(out, q, table, held, new, host, page, block, scale):
+    """Outputs of all rows that are outside the bound."""
+    (k, ks), (v, vs) = host
+    at = wrong = 0
+    for b, (h, n) in enumerate(zip(held, new)):
+        if n == 0:
+            continue
+        slot = _slots(table, b, 0, h, page)
+        kk, vv = (c[slot].astype(np.float64) * s[slot // block][:, :, None] for c, s in ((k, ks), (v, vs)))
+        seen = np.arange(h)[None] <= (h - n + np.arange(n))[:, None]
+        want, mag = oq8.attention(q[at:at + n], kk, vv, seen, scale)
+        wrong += _outside(out[at:at + n], want, mag)
+        at += n
+    return wrong
+
+
+FORMS = [None, [1, 40, 30], [64, 60, 70]]  # one row each; packed; packed rows of the many-row kernel alone
+
+
+# ---- value scales far apart ----
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", FORMS)
+@pytest.mark.parametrize("big", [-5.0, 20.0, 60.0])
+@pytest.mark.parametrize("zeros_first", [True, False])
+def test_blocks_of_zero_values_keep_their_share_of_the_weights(cuda_lib, kind, dim, new, big, zeros_first):
+    """Half the blocks hold values of scale 2^big, half hold zeros (whose scale
+    is the least that an append makes); every token scores about the same, so
+    the zeros take half of the softmax."""
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    page, block, kv, group = 16, 16, 1, 8
+    held = [64, 352, 1024]
+    rng = np.random.default_rng(dim + int(big) + 100)
+    table, pages = _place(rng, held, page)
+    n = pages * page
+    k = np.ones((n, kv, dim), np.float32)
+    k[:, :, 1:] = 0
+    ks = np.ones((pages, kv), np.float32)
+    v = rng.integers(1, 100, (n, kv, dim)).astype(np.float32)
+    if kind == "e4m3":
+        v = oq8.e4m3_round(v)
+    vs = np.full((pages, kv), 2.0 ** big, np.float32)
+    for row, h in zip(table, held):
+        mine = row[: h // page]
+        none = mine[: len(mine) // 2] if zeros_first else mine[1::2]
+        vs[none] = oq8.TINY / oq8.TOP[kind]
+        v.reshape(pages, -1)[none] = 0
+    cache = _cache_of(table, pages, page, block, kind, k, ks, v, vs)
+    rows = new or [1] * 3
+    q = _bf16(rng.standard_normal((sum(rows), kv * group, dim)))
+    cu = None if new is None else _dev(np.concatenate([[0], np.cumsum(new)]))
+    out = paged_attention_q8(q.cuda(), *cache, _dev(table), _dev(held), 0.25, cu_q=cu).float().cpu().numpy()
+    assert _wrong(out, q.float().numpy(), table, held, rows, ((k, ks), (v, vs)), page, block, 0.25) == 0
+    assert _lib.read_device_errors() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [None, [33]])
+def test_many_light_tokens_of_zero_values_add_up(cuda_lib, kind, new):
+    """One block of values of scale 8, then 65,584 zeros of 2^-17 the weight of
+    its tokens each: together they take 3% of the softmax."""
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    page = block = 16
+    dim, held = 64, [65600]
+    rng = np.random.default_rng(3)
+    table, pages = _place(rng, held, page)
+    first = table[0, 0]
+    k = np.zeros((pages * page, 1, dim), np.float32)
+    k[:, 0, 0] = 48
+    k.reshape(pages, page, dim)[first, :, 0] = 64
+    ks = np.ones((pages, 1), np.float32)
+    v = np.zeros_like(k)
+    v.reshape(pages, page, dim)[first] = 96
+    vs = np.full((pages, 1), oq8.TINY / oq8.TOP[kind], np.float32)
+    vs[first] = 8.0
+    cache = _cache_of(table, pages, page, block, kind, k, ks, v, vs)
+    rows = new or [1]
+    q = np.zeros((sum(rows), 2, dim), np.float32)
+    q[:, :, 0] = 1.0
+    scale = 17.0 / 16.0 / np.log2(np.e)
+    cu = None if new is None else _dev([0, rows[0]])
+    out = paged_attention_q8(_bf16(q).cuda(), *cache, _dev(table), _dev(held), scale, cu_q=cu).float().cpu().numpy()
+    # float32 sums of 65,600 equal weights, 64 or 128 at a time: within 1,025 * 2^-24, inside the bound
+    share = 16 / (16 + (held[0] - 16 - np.arange(rows[0])[::-1]) * 2.0 ** -17)
+    want = 768.0 * share[:, None, None] * np.ones_like(out)
+    assert _outside(out, want, want) == 0, (out[0, 0, 0], want[0, 0, 0])
