@@ -368,8 +368,9 @@ typedef struct FnQ8ReadArgs {
  * its last n tokens: row i is at position context_lens[b] - n + i and sees the
  * positions up to its own (cu_q NULL: one row per sequence, seeing the whole
  * context).  Positions whose page is outside the cache or past the table row
- * are not seen.  A row that sees nothing is 0.  Softmax statistics and sums
- * are float32; rows of q outside cu_q are not written. */
+ * are not seen.  A row that sees nothing is 0, and so is a row of no sequence
+ * (before cu_q[0] or from cu_q[batch] on: a padded batch, or tokens that were
+ * not admitted).  Softmax statistics and sums are float32. */
 typedef struct FnQ8AttentionArgs {
   uint32_t abi_version;
   uint32_t batch;

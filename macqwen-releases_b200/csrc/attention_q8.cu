@@ -651,6 +651,15 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, E4M3>::kCtas) k_q8_few(Q8V
     uint2 *dst = reinterpret_cast<uint2 *>(p.out + static_cast<size_t>(qr.x) * p.Hq * D);
     for (int i = threadIdx.x; i < qr.y * p.Hq * (D / 4); i += kFewThreads) dst[i] = make_uint2(0, 0);
   }
+  if (p.cu == nullptr) return;
+  // rows of no sequence: before the first one's and past the last one's
+  const uint64_t row = static_cast<uint64_t>(p.Hq) * (D / 8);
+  const uint64_t ahead = row * static_cast<uint64_t>(min(max(p.cu[0], 0), p.rows));
+  const uint64_t after = row * static_cast<uint64_t>(min(max(p.cu[p.B], 0), p.rows)), all = row * static_cast<uint64_t>(p.rows);
+  uint4 *dst = reinterpret_cast<uint4 *>(p.out);
+  const uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kFewThreads + threadIdx.x, step = static_cast<uint64_t>(gridDim.x) * kFewThreads;
+  for (uint64_t i = i0; i < ahead; i += step) dst[i] = make_uint4(0, 0, 0, 0);
+  for (uint64_t i = after + i0; i < all; i += step) dst[i] = make_uint4(0, 0, 0, 0);
 }
 
 // Joins the sums of segments that several CTAs worked on, in CTA order.  A CTA

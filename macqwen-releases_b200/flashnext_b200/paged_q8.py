@@ -210,7 +210,7 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
     With ``cu_q`` [batch + 1] int32, rows ``cu_q[b] .. cu_q[b + 1]`` are the
     last tokens of sequence b's ``context_lens[b]``, each seeing the positions
     up to its own; without it, row b sees all of sequence b's context.  A row
-    that sees nothing is 0.  ``workspace``: a uint8 tensor of as many bytes as
+    that sees nothing is 0, as are rows past ``cu_q[batch]``.  ``workspace``: a uint8 tensor of as many bytes as
     ``fnmoe_paged_attention_q8_workspace_size`` reports, or None for one that
     is kept for the current stream.
     """

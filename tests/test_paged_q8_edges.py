@@ -1,4 +1,5 @@
-"""The paged 8-bit KV cache at its edges: value scales far apart.
+"""The paged 8-bit KV cache at its edges: value scales far apart, rows of no
+sequence.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -138,3 +139,53 @@ def test_many_light_tokens_of_zero_values_add_up(cuda_lib, kind, new):
     share = 16 / (16 + (held[0] - 16 - np.arange(rows[0])[::-1]) * 2.0 ** -17)
     want = 768.0 * share[:, None, None] * np.ones_like(out)
     assert _outside(out, want, want) == 0, (out[0, 0, 0], want[0, 0, 0])
+
+
+# ---- rows of no sequence ----
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [[1, 0, 2], [0, 0, 0], [3, 90, 1], [64, 60, 70]])
+@pytest.mark.parametrize("extra", [1, 13, 700])
+def test_rows_of_no_sequence_are_zero(cuda_lib, dim, new, extra):
+    """A padded batch: q has more rows than cu_q counts."""
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    page, block, kv, group, held = 32, 16, 2, 4, [70, 95, 128]
+    rng = np.random.default_rng(dim + extra + sum(new))
+    table, pages = _place(rng, held, page)
+    n, blocks = pages * page, pages * page // block
+    k, v = (rng.integers(-100, 100, (n, kv, dim)).astype(np.float32) for _ in range(2))
+    ks, vs = (np.exp(rng.standard_normal((blocks, kv))).astype(np.float32) / 50 for _ in range(2))
+    cache = _cache_of(table, pages, page, block, "int8", k, ks, v, vs)
+    q = _bf16(rng.standard_normal((sum(new) + extra, kv * group, dim)))
+    cu = _dev(np.concatenate([[0], np.cumsum(new)]))
+    out = torch.full(q.shape, float("nan"), dtype=torch.bfloat16, device="cuda")
+    paged_attention_q8(q.cuda(), *cache, _dev(table), _dev(held), dim ** -0.5, cu_q=cu, out=out)
+    out = out.float().cpu().numpy()
+    assert (out[sum(new):] == 0).all()
+    assert _wrong(out, q.float().numpy(), table, held, new, ((k, ks), (v, vs)), page, block, dim ** -0.5) == 0
+    cu += 5  # the first sequence begins at row 5
+    out = torch.full((q.shape[0] + 5, *q.shape[1:]), float("nan"), dtype=torch.bfloat16, device="cuda")
+    q5 = torch.cat([torch.ones_like(q[:1]).expand(5, -1, -1), q])
+    paged_attention_q8(q5.cuda(), *cache, _dev(table), _dev(held), dim ** -0.5, cu_q=cu, out=out)
+    out = out.float().cpu().numpy()
+    assert (out[:5] == 0).all() and (out[5 + sum(new):] == 0).all()
+    assert _wrong(out[5:], q.float().numpy(), table, held, new, ((k, ks), (v, vs)), page, block, dim ** -0.5) == 0
+
+
+@pytest.mark.gpu
+def test_a_padded_step_of_the_cache_class_has_zero_rows(cuda_lib):
+    import torch
+    from flashnext_b200.paged_q8 import PagedKVCacheQ8
+
+    junk = torch.full((1 << 22,), float("nan"), device="cuda")  # what the allocator hands out next
+    del junk
+    cache = PagedKVCacheQ8(8, 32, 1, 64, 4, 3, 64)
+    cache.plan(_dev([7, 0, 20]))
+    x = torch.randn(64, 1, 64, device="cuda").bfloat16()  # 27 tokens, padded to 64
+    cache.append(x, x)
+    out = cache.attention(x.expand(-1, 4, -1).contiguous(), 0.125)
+    assert torch.isfinite(out).all() and bool((out[27:] == 0).all()) and bool((out[:27] != 0).any())
