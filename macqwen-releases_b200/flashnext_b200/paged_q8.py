@@ -23,6 +23,7 @@ host, so a step can be captured in a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass
 from typing import Any
 
@@ -33,7 +34,6 @@ from . import _lib
 BLOCKS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
 _CODES = {torch.int8: _lib.Q8_INT8, torch.float8_e4m3fn: _lib.Q8_E4M3}
-_workspaces: dict[tuple[int, int], Any] = {}  # (device, stream) -> scratch, so that streams do not share one
 
 
 @dataclass(slots=True)
@@ -202,6 +202,23 @@ def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
     return out
 
 
+class _Scratch(threading.local):
+    """Attention scratch that a thread keeps for each (device, stream).
+
+    A thread's calls on one stream follow one another there and may share it.
+    Two threads may not (a call is several launches, which interleave), nor may
+    graphs: a captured call gets memory of its own from the graph's pool, which
+    lives as long as the graph, and never the kept one, which is dropped when a
+    later call needs more.
+    """
+
+    def __init__(self):
+        self.kept = {}
+
+
+_scratch = _Scratch()
+
+
 def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, scale: float, cu_q=None,
                        out=None, workspace=None):
     """Causal attention of bfloat16 rows ``q`` [rows, q_heads, head_dim]
@@ -210,9 +227,11 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
     With ``cu_q`` [batch + 1] int32, rows ``cu_q[b] .. cu_q[b + 1]`` are the
     last tokens of sequence b's ``context_lens[b]``, each seeing the positions
     up to its own; without it, row b sees all of sequence b's context.  A row
-    that sees nothing is 0, as are rows past ``cu_q[batch]``.  ``workspace``: a uint8 tensor of as many bytes as
-    ``fnmoe_paged_attention_q8_workspace_size`` reports, or None for one that
-    is kept for the current stream.
+    that sees nothing is 0, as are rows past ``cu_q[batch]``.  ``workspace``:
+    a uint8 tensor of as many bytes as
+    ``fnmoe_paged_attention_q8_workspace_size`` reports, which no other call
+    uses at the same time; or None for one that this module keeps for the
+    calling thread and stream (in a CUDA graph's capture: one of the graph's own).
     """
     c, _, head_dim = _cache(k_cache, v_cache, k_scale, v_scale)
     shape, table = q.shape, block_table.shape
@@ -237,15 +256,20 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
         None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q"), op)
     lib, stream = _ready(q)
     ref = ctypes.byref(a)
-    kept = workspace if workspace is not None else _workspaces.get((q.get_device(), stream))
-    if kept is not None:
-        a.workspace, a.workspace_bytes = kept.data_ptr(), kept.numel()
+    capturing = workspace is None and torch.cuda.is_current_stream_capturing()
+    given = workspace
+    if given is None and not capturing:
+        given = _scratch.kept.get((q.get_device(), stream))
+    if given is not None:
+        a.workspace, a.workspace_bytes = given.data_ptr(), given.numel()
     code = lib.fnmoe_paged_attention_q8(ref, stream)
-    if code == _lib.ERR_WORKSPACE and workspace is None:  # none kept for this stream yet, or too small a one
+    if code == _lib.ERR_WORKSPACE and workspace is None:  # none yet, or too small a one
         need = ctypes.c_uint64(0)
         _lib.check(lib.fnmoe_paged_attention_q8_workspace_size(ref, ctypes.byref(need)), "paged attention q8 workspace")
-        kept = _workspaces[(q.get_device(), stream)] = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = kept.data_ptr(), kept.numel()
+        given = k_scale.new_empty((need.value,), dtype=torch.uint8)
+        if not capturing:
+            _scratch.kept[(q.get_device(), stream)] = given
+        a.workspace, a.workspace_bytes = given.data_ptr(), given.numel()
         code = lib.fnmoe_paged_attention_q8(ref, stream)
     _lib.check(code, "paged_attention_q8")
     return out

@@ -1,5 +1,5 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
-sequence.
+sequence, scratch under graphs and threads.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -11,6 +11,8 @@ instructions, 16 at a time and two for each, is within 700 * 2^-23 < 2^-13.5 in
 the worst case.
 """
 from __future__ import annotations
+
+import threading
 
 import numpy as np
 import pytest
@@ -189,3 +191,213 @@ def test_a_padded_step_of_the_cache_class_has_zero_rows(cuda_lib):
     cache.append(x, x)
     out = cache.attention(x.expand(-1, 4, -1).contiguous(), 0.125)
     assert torch.isfinite(out).all() and bool((out[27:] == 0).all()) and bool((out[:27] != 0).any())
+
+
+# ---- scratch ----
+
+
+class _Cuda:
+    """A CPU tensor that says that it is on CUDA device `index`."""
+
+    is_cuda = True
+
+    def __init__(self, *shape, dtype, index=0):
+        import torch
+
+        self.real, self.index = torch.zeros(shape, dtype=dtype), index
+
+    def get_device(self):
+        return self.index
+
+    def __getattr__(self, name):
+        return getattr(self.real, name)
+
+
+class _Library:
+    """Stands in for the C library: says what scratch a call needs and sees what it was given."""
+
+    def __init__(self, seen=lambda args: None):
+        self.seen = seen
+
+    def fnmoe_paged_attention_q8_workspace_size(self, ref, need):
+        need._obj.value = 4096 * ref._obj.q_rows
+        return _lib.OK
+
+    def fnmoe_paged_attention_q8(self, ref, stream):
+        a = ref._obj
+        if not a.workspace or a.workspace_bytes < 4096 * a.q_rows:
+            return _lib.ERR_WORKSPACE
+        self.seen(a)
+        return _lib.OK
+
+
+def _fake_attention(rows):
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    cache = [_Cuda(4, 32, 2, 64, dtype=torch.int8) for _ in range(2)] + [_Cuda(4, 2, 2, dtype=torch.float32) for _ in range(2)]
+    paged_attention_q8(_Cuda(rows, 4, 64, dtype=torch.bfloat16), *cache, _Cuda(rows, 2, dtype=torch.int32),
+                       _Cuda(rows, dtype=torch.int32), 0.125)
+
+
+def test_calls_of_two_threads_on_one_stream_have_scratch_of_their_own(monkeypatch):
+    import torch
+    from flashnext_b200 import paged_q8
+
+    inside, given = threading.Barrier(2), []
+    lib = _Library()
+    monkeypatch.setattr(paged_q8, "_ready", lambda t: (lib, 7))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    _fake_attention(3)  # whatever an earlier call may leave behind
+
+    def seen(a):
+        given.append((a.workspace, a.workspace_bytes))
+        inside.wait(10)  # both calls are in the library
+
+    lib.seen = seen
+    threads = [threading.Thread(target=_fake_attention, args=(rows,)) for rows in (2, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(20)
+    (a, n), (b, m) = sorted(given)
+    assert a + n <= b, "two calls in flight were given the same scratch"
+
+
+def test_a_captured_call_has_scratch_of_the_graphs_own(monkeypatch):
+    """Allocated in the capture, by each call, and neither kept nor given to another."""
+    import torch
+    from flashnext_b200 import paged_q8
+
+    made, used, capturing = [], [], [False]
+    empty, new_empty = torch.empty, torch.Tensor.new_empty
+
+    def note(t):
+        made.append((t.data_ptr(), t.numel() * t.element_size(), t))  # the graph's pool keeps it
+        return t
+
+    lib = _Library(lambda a: used.append((a.workspace, a.workspace_bytes)))
+    monkeypatch.setattr(paged_q8, "_ready", lambda t: (lib, 7))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: note(empty(*a, **k)))
+    monkeypatch.setattr(torch.Tensor, "new_empty", lambda *a, **k: note(new_empty(*a, **k)))
+    of_graphs = []
+    for captured, rows in ((False, 3), (True, 3), (False, 2), (True, 2), (False, 5), (True, 5), (False, 5)):
+        before, capturing[0] = len(made), captured
+        _fake_attention(rows)
+        at, n = used[-1]
+        assert n >= 4096 * rows
+        assert all(at + n <= p or p + m <= at for p, m in of_graphs), "a graph's scratch was given to another call"
+        if captured:
+            assert any(p <= at and at + n <= p + m for p, m, _ in made[before:]), "not the graph's own"
+            of_graphs.append((at, n))
+
+
+def _served(batch, held, dim=256, kv=2, seed=1):
+    """A cache holding `held` tokens a sequence of random rows, by its own append."""
+    import torch
+    from flashnext_b200.paged_q8 import PagedKVCacheQ8
+
+    page = 64
+    cache = PagedKVCacheQ8(batch * (held // page + 4), page, kv, dim, held // page + 4, batch, batch * held)
+    cache.plan(_dev([held] * batch))
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    r = torch.randn(2, batch * held, kv, dim, device="cuda", generator=g).bfloat16()
+    cache.append(r[0], r[1])
+    return cache
+
+
+@pytest.mark.gpu
+def test_a_captured_step_outlives_larger_calls_on_its_stream(cuda_lib):
+    """Capture a decode, run a prefill that needs more scratch on the same
+    stream, fill new tensors, replay: the outputs are those of an eager call and
+    the tensors keep their values."""
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    cache = _served(4, 2000)
+    p = cache.last
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    q = torch.randn(4, 16, 256, device="cuda", generator=g).bfloat16()
+    long = torch.randn(4 * 700, 16, 256, device="cuda", generator=g).bfloat16()
+    cu = _dev(700 * np.arange(5))
+    args = (*cache.tensors, p.block_table, p.seq_lens, 0.0625)
+    want = paged_attention_q8(q, *args)
+    want_long = paged_attention_q8(long, *args, cu_q=cu)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    out = torch.empty_like(q)
+    with torch.cuda.stream(s):
+        paged_attention_q8(q, *args, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            paged_attention_q8(q, *args, out=out)
+        assert torch.equal(paged_attention_q8(long, *args, cu_q=cu), want_long)
+        torch.cuda.synchronize()
+        fresh = [torch.full((n,), 7, dtype=torch.uint8, device="cuda") for n in [1 << 20] * 16 + [1 << 22] * 8 + [1 << 25] * 4]
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+            assert torch.equal(paged_attention_q8(long, *args, cu_q=cu), want_long)
+        torch.cuda.synchronize()
+        assert all(bool((t == 7).all()) for t in fresh)
+
+
+@pytest.mark.gpu
+def test_two_graphs_of_one_stream_may_replay_at_once(cuda_lib):
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    cache = _served(4, 3000)
+    p = cache.last
+    args = (*cache.tensors, p.block_table, p.seq_lens, 0.0625)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    qs = [torch.randn(4, 16, 256, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    wants = [paged_attention_q8(q, *args) for q in qs]
+    s, outs, graphs = torch.cuda.Stream(), [torch.empty_like(q) for q in qs], []
+    torch.cuda.synchronize()
+    for q, out in zip(qs, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            paged_attention_q8(q, *args, out=out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for t, graph in zip(streams, graphs):
+            with torch.cuda.stream(t):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+
+
+@pytest.mark.gpu
+def test_two_threads_on_one_stream(cuda_lib):
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    jobs = []
+    for i, (batch, held, rows) in enumerate(((3, 900, 60), (7, 300, 21))):
+        cache = _served(batch, held, seed=10 + i)
+        q = torch.randn(batch * rows, 16, 256, device="cuda").bfloat16()
+        args = (q, *cache.tensors, cache.last.block_table, cache.last.seq_lens, 0.0625)
+        cu = _dev(rows * np.arange(batch + 1))
+        jobs.append((args, cu, paged_attention_q8(*args, cu_q=cu)))
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(2)
+
+    def work(args, cu, want):
+        start.wait(10)
+        got = [paged_attention_q8(*args, cu_q=cu) for _ in range(50)]
+        torch.cuda.synchronize()
+        wrong.append(sum(not torch.equal(o, want) for o in got))
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [0, 0] and _lib.read_device_errors() == 0
