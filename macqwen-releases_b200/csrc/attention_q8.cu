@@ -696,12 +696,14 @@ __global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
     h = cut.y;
     c0 = at;
   }
-  if (cut.x < 0) return;
-  const int c1 = cut.w & 0x3FFFFFFF;
+  // Not cut; or never written, where a kernel gave up a wait (its device error is set).
+  if (!cut_fits(cut, c0, h, p.B, p.Hkv, is_few ? p.ctas : p.tctas)) return;
+  const int c1 = last_cta(cut);
   const bool late0 = (cut.w >> 30) & 1;
   const int2 qr = rows_of(p, cut.x);
-  const int R = is_few ? 8 : 128, rows = qr.y * p.gq - cut.z * R;
-  if (row0 >= rows) return;
+  const int R = is_few ? 8 : 128;
+  if (static_cast<long long>(cut.z) * R + row0 >= static_cast<long long>(qr.y) * p.gq) return;
+  const int rows = qr.y * p.gq - cut.z * R;
   // sub: which of the rows taken at once; lane: four dims; every `groups`-th CTA
   const int per = is_few ? 1 : 4, groups = 256 / (L * per) > 0 ? 256 / (L * per) : 1;
   const int sub = is_few ? 0 : threadIdx.x & 3;
@@ -964,6 +966,8 @@ int paged_attention_q8(const FnQ8AttentionArgs *a, cudaStream_t s, std::string &
   p.join_rows = p.cu ? 8 : std::min(p.gq, 8);
   const uint64_t few_segs = static_cast<uint64_t>(p.B) * p.Hkv * p.few_tiles;
   const uint64_t many_segs = many ? many_tiles(p) * p.Hkv : 0;
+  p.ctas = few_ctas(d);
+  p.tctas = many_ctas(d);
   p.by_seg = few_segs < static_cast<uint64_t>(few_ctas(d) - 1);
   p.tby_seg = many_segs < static_cast<uint64_t>(many_ctas(d) - 1);
   const bool e4m3 = a->cache.code_type == FNMOE_Q8_E4M3;

@@ -36,6 +36,7 @@
 
 #include "async.cuh"
 #include "common.cuh"
+#include "q8_ranges.cuh"
 
 namespace fnmoe {
 
@@ -60,6 +61,7 @@ struct Q8View {
   int4 *cuts;           // [CTAs] where each range begins (cut_of), or by_seg: [B][Hkv][few_tiles]
   int few_tiles;        // tiles of 8 rows that a sequence can have
   int join_rows;        // rows that such a tile can have
+  int ctas, tctas;      // CTAs of the few-row and the many-row kernel
   bool by_seg, tby_seg, pair_boxes;
   float *part;          // [2 * CTAs][8][D] unfinished sums
   float2 *part_ml;      // [2 * CTAs][8] their reference and weight sum
@@ -231,44 +233,6 @@ __device__ __forceinline__ int page_col(const Q8View &p, int pos) {
 // Tokens of sequence b that the cache can hold.
 __device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
   return max(0, min(p.ctx[b], p.width * p.page));
-}
-
-// Equal contiguous ranges of `total` units for the CTAs: CTA i takes
-// [begin(i), begin(i + 1)), the first `more` CTAs one unit more than the
-// others.  At most a CTA per unit is used, so that no range between two others
-// is empty.
-struct Ranges {
-  long long total, per;
-  int used, more;
-  __device__ __forceinline__ Ranges(long long units, int ctas) : total(units) {
-    used = static_cast<int>(min(static_cast<long long>(ctas), max(units, 1ll)));
-    per = units <= 0xFFFFFFFFll ? static_cast<uint32_t>(units) / static_cast<uint32_t>(used) : units / used;
-    more = static_cast<int>(units - per * used);
-  }
-  __device__ __forceinline__ long long begin(int i) const {
-    i = min(i, used);
-    return per * i + min(i, more);
-  }
-  // The CTA whose range holds `unit`.
-  __device__ __forceinline__ int owner(long long unit) const {
-    const long long big = (per + 1) * more;
-    const long long rest = unit < big ? unit : unit - big, n = unit < big ? per + 1 : per;
-    const int q = rest <= 0xFFFFFFFFll && n <= 0xFFFFFFFFll ? static_cast<uint32_t>(rest) / static_cast<uint32_t>(n)
-                                                            : static_cast<int>(rest / n);
-    return unit < big ? q : more + q;
-  }
-};
-
-// Where a CTA's range begins.  When that is the first cut inside a segment
-// (work of one sequence, kv head and tile that several CTAs share), the join
-// finds here all it needs: {sequence, kv head, tile, last CTA of the segment,
-// with bit 30 set when the CTA before, the segment's first, began earlier than
-// the segment}; otherwise the sequence is -1.
-__device__ __forceinline__ int4 cut_of(const Ranges &ranges, int b, int h, int tile, long long seg_begin,
-                                       long long first_unit, long long last_unit, int cta) {
-  if (ranges.owner(first_unit) != cta - 1) return make_int4(-1, 0, 0, 0);
-  const int late = ranges.begin(cta - 1) < seg_begin ? 1 << 30 : 0;
-  return make_int4(b, h, tile, ranges.owner(last_unit) | late);
 }
 
 // A kernel's shared-memory limit, set once on each device (the attribute

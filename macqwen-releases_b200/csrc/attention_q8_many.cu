@@ -37,7 +37,8 @@
 // softmax -> P V and the issue slots that widening takes beside it (IPC 2.0);
 // the MMAs alone take about 1,700 clocks a unit (N 64 and two terms of P).
 // Every wait is bounded: a timeout sets the device error word and marks the
-// CTA dead, whereupon every role runs to the end.
+// CTA dead, whereupon every role leaves its loop.  The join then finds parts that
+// were not written, but no descriptor that leads outside its arrays (cut_fits).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -249,6 +250,9 @@ __global__ void __launch_bounds__(kScanThreads) k_q8_tiles(Q8View p) {
     if (t < tiles) p.tprefix[t] = s - units;
   }
   if (threadIdx.x == 0) p.tprefix[tiles] = carry;
+  // No cut, until the CTA that makes one says so.  (Not by segment: k_q8_many does this.)
+  if (p.tby_seg)
+    for (int i = threadIdx.x; i < p.max_tiles * p.Hkv; i += kScanThreads) p.tcuts[i] = make_int4(-1, 0, 0, 0);
 }
 
 // The last of `tiles` tiles that begins at or before `unit`; a whole warp.
@@ -694,6 +698,15 @@ __global__ void __launch_bounds__(Many<D>::kThreads, Many<D>::kCtas) k_q8_many(Q
         }
         if (!M::kShared && live) pv(n > 1);
       }
+      // Products may still be under way when another role gave up: they end (or a
+      // bounded wait does) before the TMEM that they write is freed.
+      auto settle = [&](int i, uint32_t units) {
+        if (units > 0)
+          for (uint32_t spins = 0; spins < kSpin && !mbar_try_wait_u32(bar(i), (units - 1) & 1u); ++spins) {
+          }
+      };
+      settle(M::kSFull, nk);
+      settle(M::kPEmpty, nv);
     } else if (warp == M::kMmaWarp + 1) {
       // ---------------- the units' scales: a lane for each granule of 16 tokens ----------------
       uint32_t i = 0;

@@ -1,5 +1,5 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
-sequence, scratch under graphs and threads.
+sequence, scratch under graphs and threads, descriptors of cut work.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -401,3 +401,102 @@ def test_two_threads_on_one_stream(cuda_lib):
     for t in threads:
         t.join()
     assert wrong == [0, 0] and _lib.read_device_errors() == 0
+
+
+# ---- descriptors of cut work ----
+
+RANGES_CHECK = r"""
+#include <cstdio>
+#include <cstring>
+#include <random>
+#include <vector>
+#include "q8_ranges.cuh"
+using namespace fnmoe;
+#define CHECK(x) if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; }
+int main() {
+  std::mt19937_64 rng(1);
+  auto pick = [&](long long lo, long long hi) { return lo + static_cast<long long>(rng() % (hi - lo + 1)); };
+  // Segments laid end to end (the last `real` units of each are work, as the join sees it),
+  // dealt to CTAs: each segment that several CTAs share is described exactly once, rightly.
+  for (int round = 0; round < 3000; ++round) {
+    const int segs = pick(1, 40), ctas = pick(1, 60), cost = round & 1 ? 6 : 0;
+    std::vector<long long> begin(segs + 1);
+    for (int s = 0; s < segs; ++s) begin[s + 1] = begin[s] + pick(1, pick(1, 50)) + cost;
+    const Ranges r(begin[segs], ctas);
+    CHECK(r.begin(0) == 0 && r.begin(ctas) == begin[segs]);
+    std::vector<int> said(segs);
+    for (int c = 0; c < ctas; ++c) {
+      const long long at = r.begin(c);
+      CHECK(r.begin(c + 1) >= at);
+      if (r.begin(c + 1) == at) continue;
+      CHECK(r.owner(at) == c && r.owner(r.begin(c + 1) - 1) == c);
+      int s = 0;
+      while (begin[s + 1] <= at) ++s;
+      if (at <= begin[s] + cost) continue;  // not inside the segment's work
+      const int4 cut = cut_of(r, s, 0, 3, begin[s], begin[s] + cost, begin[s + 1] - 1, c);
+      if (cut.x < 0) continue;
+      ++said[s];
+      CHECK(cut.x == s && cut.z == 3 && cut_fits(cut, c - 1, cut.y, segs, 1, ctas));
+      CHECK(last_cta(cut) == r.owner(begin[s + 1] - 1) && r.owner(begin[s] + cost) == c - 1);
+      CHECK((cut.w >> 30 & 1) == (r.begin(c - 1) < begin[s]));
+    }
+    for (int s = 0; s < segs; ++s) CHECK(said[s] == (r.owner(begin[s] + cost) != r.owner(begin[s + 1] - 1)));
+  }
+  // Anything else is refused, or stays inside the arrays.
+  const int batch = 5, heads = 3, ctas = 148;
+  const unsigned fills[] = {0u, ~0u, 0x5A5A5A5Au, 0x7FFFFFFFu, 0x80000000u, 0x3FFFFFFFu, 0x40000000u, 1u};
+  for (unsigned f : fills) {
+    int4 cut;
+    const unsigned w[4] = {f, f, f, f};
+    std::memcpy(&cut, w, 16);
+    CHECK(!cut_fits(cut, cut.y, 0, batch, heads, ctas) && !cut_fits(cut, 0, cut.y, batch, heads, ctas) || f == 1u);
+  }
+  for (int i = 0; i < 2000000; ++i) {
+    const int bits = pick(1, 32);
+    auto any = [&] { return static_cast<int>(static_cast<unsigned>(rng()) >> (32 - bits)) * (rng() & 1 ? 1 : -1); };
+    const int4 cut = make_int4(any(), any(), any(), any());
+    const int c0 = any(), h = any();
+    if (!cut_fits(cut, c0, h, batch, heads, ctas)) continue;
+    CHECK(cut.x >= 0 && cut.x < batch && h >= 0 && h < heads && cut.z >= 0);
+    CHECK(c0 >= 0 && c0 < last_cta(cut) && last_cta(cut) < ctas);
+  }
+  return 0;
+}
+"""
+
+
+def _run_host_code(tmp_path, text):
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    csrc = Path(__file__).resolve().parents[1] / "macqwen-releases_b200" / "csrc"
+    src, exe = tmp_path / "check.cu", tmp_path / "check"
+    src.write_text(text)
+    subprocess.run([nvcc, "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a", "-I", str(csrc), str(src), "-o",
+                    str(exe)], check=True)
+    got = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout + got.stderr
+
+
+def test_descriptors_of_cut_work_are_right_and_wild_ones_are_refused(tmp_path):
+    """Host code: every shared segment is described once, and memory that no
+    kernel wrote (one that gave up a wait) is no descriptor that can be followed."""
+    _run_host_code(tmp_path, RANGES_CHECK)
+
+
+@pytest.mark.gpu
+def test_every_descriptor_by_segment_is_set_before_the_join(cuda_lib):
+    """Three tiles of work where the workspace has room for six: the other
+    descriptors say "no cut", not what the workspace held."""
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    cache = _served(3, 512, dim=128)
+    q = torch.randn(3 * 16, 16, 128, device="cuda").bfloat16()
+    ws = torch.full((64 << 20,), 0x5A, dtype=torch.uint8, device="cuda")
+    paged_attention_q8(q, *cache.tensors, cache.last.block_table, cache.last.seq_lens, 0.09, cu_q=_dev([0, 16, 32, 48]),
+                       workspace=ws)
+    none = torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device="cuda")
+    assert int((ws.view(torch.int32).view(-1, 4) == none).all(1).sum()) >= 6  # (6 - 3) tiles x 2 kv heads
