@@ -697,7 +697,9 @@ __global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
     c0 = at;
   }
   // Not cut; or never written, where a kernel gave up a wait (its device error is set).
-  if (!cut_fits(cut, c0, h, p.B, p.Hkv, is_few ? p.ctas : p.tctas)) return;
+  // (By segment h is in range; its divisions are still under way, and waiting for them here
+  // costs 64 ragged sequences 1.3 us.)
+  if (!cut_fits(cut, c0, by_seg ? 0 : h, p.B, p.Hkv, is_few ? p.ctas : p.tctas)) return;
   const int c1 = last_cta(cut);
   const bool late0 = (cut.w >> 30) & 1;
   const int2 qr = rows_of(p, cut.x);
