@@ -51,25 +51,33 @@ class PagePlan:
     admitted: Any     # [batch] int32: 0 where pages, tokens or table columns ran out
 
 
-def _refuse(t, dtype, shape, what):
+def _elsewhere(t, index, what):
+    raise ValueError(f"{what} is on device {t.get_device()}, the call's other tensors are on device {index}")
+
+
+def _refuse(t, dtype, shape, what, index):
     if t.dtype != dtype or not t.is_cuda:
         raise TypeError(f"{what} must be a {dtype} CUDA tensor")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    if t.get_device() != index:
+        _elsewhere(t, index, what)
     raise ValueError(f"{what} must be contiguous")
 
 
-def _want(t, dtype, shape, what):
-    """Pointer of a contiguous CUDA tensor of this type and shape."""
-    if t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous():
+def _want(t, dtype, shape, what, index):
+    """Pointer of a contiguous tensor of this type and shape on CUDA device ``index``."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index >= 0 and t.is_contiguous():
         return t.data_ptr()
-    _refuse(t, dtype, shape, what)
+    _refuse(t, dtype, shape, what, index)
 
 
-def _rows(t, heads, dim, what):
+def _rows(t, heads, dim, what, index):
     """Pointer and token stride of bfloat16 rows [n, heads, dim]; a row is contiguous, rows may be apart."""
     if t.dtype is not torch.bfloat16 or not t.is_cuda:
         raise TypeError(f"{what} must be a bfloat16 CUDA tensor")
+    if t.get_device() != index:
+        _elsewhere(t, index, what)
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
         raise ValueError(f"{what} must be [tokens, {heads}, {dim}], not {tuple(shape)}")
@@ -82,8 +90,8 @@ def _rows(t, heads, dim, what):
 
 
 def _cache(k_cache, v_cache, k_scale, v_scale):
-    """FnQ8Cache of the four tensors, and (kv_heads, head_dim)."""
-    dtype, shape, scales = k_cache.dtype, k_cache.shape, k_scale.shape
+    """FnQ8Cache of the four tensors, (kv_heads, head_dim) and their device."""
+    dtype, shape, scales, index = k_cache.dtype, k_cache.shape, k_scale.shape, k_cache.get_device()
     if len(shape) != 4 or len(scales) != 3:
         raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] and scales "
                          "[pages, page_size / block, kv_heads]")
@@ -91,11 +99,11 @@ def _cache(k_cache, v_cache, k_scale, v_scale):
     blocks = scales[1]
     if (k_scale.dtype is v_scale.dtype is torch.float32 and v_cache.dtype is dtype and dtype in _CODES
             and v_cache.shape == shape and v_scale.shape == scales and scales[0] == pages and scales[2] == heads
-            and blocks and page % blocks == 0 and k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda
-            and v_scale.is_cuda and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
-            and v_scale.is_contiguous()):
+            and blocks and page % blocks == 0 and 0 <= index == v_cache.get_device() == k_scale.get_device()
+            and index == v_scale.get_device() and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_scale.is_contiguous() and v_scale.is_contiguous()):
         return _lib.FnQ8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                              pages, page, page // blocks, heads, dim, _CODES[dtype]), heads, dim
+                              pages, page, page // blocks, heads, dim, _CODES[dtype]), heads, dim, index
     # say which
     if dtype not in _CODES:
         raise TypeError("k_cache must be an int8 or float8_e4m3fn tensor")
@@ -104,7 +112,7 @@ def _cache(k_cache, v_cache, k_scale, v_scale):
     ss, f32 = (pages, blocks, heads), torch.float32
     for t, d, x, what in ((k_cache, dtype, shape, "k_cache"), (v_cache, dtype, shape, "v_cache"),
                           (k_scale, f32, ss, "k_scale"), (v_scale, f32, ss, "v_scale")):
-        _want(t, d, x, what)
+        _want(t, d, x, what, index)
     raise AssertionError("unreachable")
 
 
@@ -136,11 +144,11 @@ def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size
     width, max_tokens = block_table.shape[1], int(max_tokens)
     if batch == 0 or width == 0 or max_tokens <= 0:
         raise ValueError("page_plan needs sequences, table columns and max_tokens > 0")
-    one, cells, two = seq_lens.shape, block_table.shape, (2,)
-    ins = (_want(seq_lens, i32, one, "seq_lens"), _want(new_lens, i32, one, "new_lens"),
-           None if release is None else _want(release, i32, one, "release"),
-           _want(block_table, i32, cells, "block_table"), _want(free_pages, i32, (free_pages.numel(),), "free_pages"),
-           _want(free_state, i32, two, "free_state"))
+    one, cells, two, at = seq_lens.shape, block_table.shape, (2,), seq_lens.get_device()
+    ins = (_want(seq_lens, i32, one, "seq_lens", at), _want(new_lens, i32, one, "new_lens", at),
+           None if release is None else _want(release, i32, one, "release", at),
+           _want(block_table, i32, cells, "block_table", at),
+           _want(free_pages, i32, (free_pages.numel(),), "free_pages", at), _want(free_state, i32, two, "free_state", at))
     if out is None:
         dev = seq_lens.device
         words = torch.empty(batch * (width + 3) + 1 + 2 + 2 * max_tokens, dtype=i32, device=dev)
@@ -150,10 +158,10 @@ def page_plan(seq_lens, new_lens, block_table, free_pages, free_state, page_size
     tok = (max_tokens,)
     a = _lib.FnPagePlanArgs(
         _lib.ABI_VERSION, batch, int(page_size), width, free_pages.shape[0], max_tokens, *ins,
-        _want(out.block_table, i32, cells, "out.block_table"), _want(out.seq_lens, i32, one, "out.seq_lens"),
-        _want(out.free_state, i32, two, "out.free_state"), _want(out.slot_map, torch.int64, tok, "out.slot_map"),
-        _want(out.token_seq, i32, tok, "out.token_seq"), _want(out.positions, i32, tok, "out.positions"),
-        _want(out.cu_new, i32, (batch + 1,), "out.cu_new"), _want(out.admitted, i32, one, "out.admitted"))
+        _want(out.block_table, i32, cells, "out.block_table", at), _want(out.seq_lens, i32, one, "out.seq_lens", at),
+        _want(out.free_state, i32, two, "out.free_state", at), _want(out.slot_map, torch.int64, tok, "out.slot_map", at),
+        _want(out.token_seq, i32, tok, "out.token_seq", at), _want(out.positions, i32, tok, "out.positions", at),
+        _want(out.cu_new, i32, (batch + 1,), "out.cu_new", at), _want(out.admitted, i32, one, "out.admitted", at))
     lib, stream = _ready(seq_lens)
     _lib.check(lib.fnmoe_page_plan(ctypes.byref(a), stream), "page_plan")
     out.free_pages = free_pages
@@ -170,14 +178,14 @@ def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
     ascending slots, as :func:`page_plan` maps them; slots outside the cache
     (-1) are skipped.  Infinities store the largest code, NaN stores 0.
     """
-    c, heads, dim = _cache(k_cache, v_cache, k_scale, v_scale)
-    kp, ks = _rows(k, heads, dim, "k")
-    vp, vs = _rows(v, heads, dim, "v")
+    c, heads, dim, index = _cache(k_cache, v_cache, k_scale, v_scale)
+    kp, ks = _rows(k, heads, dim, "k", index)
+    vp, vs = _rows(v, heads, dim, "v", index)
     tokens = k.shape[0]
     if v.shape[0] != tokens:
         raise ValueError("k and v must have the same number of rows")
     a = _lib.FnQ8AppendArgs(_lib.ABI_VERSION, tokens, c, kp, vp, ks, vs,
-                            _want(slot_map, torch.int64, (tokens,), "slot_map"))
+                            _want(slot_map, torch.int64, (tokens,), "slot_map", index))
     lib, stream = _ready(k)
     _lib.check(lib.fnmoe_kv_append_q8(ctypes.byref(a), stream), "kv_append_q8")
 
@@ -185,9 +193,9 @@ def kv_append_q8(k, v, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
 def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
     """The values ``(k, v)`` that ``slots`` [n] int64 hold, bfloat16
     [n, kv_heads, head_dim]; slots outside the cache (-1) read as zeros."""
-    c, heads, dim = _cache(k_cache, v_cache, k_scale, v_scale)
+    c, heads, dim, index = _cache(k_cache, v_cache, k_scale, v_scale)
     n = slots.shape[0]
-    at = _want(slots, torch.int64, (n,), "slots")
+    at = _want(slots, torch.int64, (n,), "slots", index)
     if out is None:
         both = k_scale.new_empty((2, n, heads, dim), dtype=torch.bfloat16)
         ko = both.data_ptr()
@@ -195,7 +203,7 @@ def kv_read_q8(slots, k_cache, v_cache, k_scale, v_scale, out=None):
         out = both.unbind()
     else:
         shape = (n, heads, dim)
-        ko, vo = _want(out[0], torch.bfloat16, shape, "out[0]"), _want(out[1], torch.bfloat16, shape, "out[1]")
+        ko, vo = (_want(t, torch.bfloat16, shape, f"out[{i}]", index) for i, t in enumerate(out))
     a = _lib.FnQ8ReadArgs(_lib.ABI_VERSION, n, c, at, ko, vo)
     lib, stream = _ready(slots)
     _lib.check(lib.fnmoe_kv_read_q8(ctypes.byref(a), stream), "kv_read_q8")
@@ -233,14 +241,14 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
     uses at the same time; or None for one that this module keeps for the
     calling thread and stream (in a CUDA graph's capture: one of the graph's own).
     """
-    c, _, head_dim = _cache(k_cache, v_cache, k_scale, v_scale)
+    c, _, head_dim, index = _cache(k_cache, v_cache, k_scale, v_scale)
     shape, table = q.shape, block_table.shape
     if len(shape) != 3:
         raise ValueError("q must be [rows, q_heads, head_dim]")
     rows, heads, dim = shape
     if dim != head_dim:
         raise ValueError("cache head_dim differs from q")
-    qp, qs = _rows(q, heads, dim, "q")
+    qp, qs = _rows(q, heads, dim, "q", index)
     if len(table) != 2:
         raise ValueError("block_table must be [batch, max_pages]")
     batch, width = table
@@ -248,18 +256,20 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
         out = k_scale.new_empty(shape, dtype=torch.bfloat16)
         op = out.data_ptr()
     else:
-        op = _want(out, torch.bfloat16, shape, "out")
+        op = _want(out, torch.bfloat16, shape, "out", index)
+    if workspace is not None:
+        _want(workspace, torch.uint8, workspace.shape, "workspace", index)
     i32 = torch.int32
     a = _lib.FnQ8AttentionArgs(
         _lib.ABI_VERSION, batch, rows, heads, width, float(scale), c, qp, qs,
-        _want(block_table, i32, table, "block_table"), _want(context_lens, i32, (batch,), "context_lens"),
-        None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q"), op)
+        _want(block_table, i32, table, "block_table", index), _want(context_lens, i32, (batch,), "context_lens", index),
+        None if cu_q is None else _want(cu_q, i32, (batch + 1,), "cu_q", index), op)
     lib, stream = _ready(q)
     ref = ctypes.byref(a)
     capturing = workspace is None and torch.cuda.is_current_stream_capturing()
     given = workspace
     if given is None and not capturing:
-        given = _scratch.kept.get((q.get_device(), stream))
+        given = _scratch.kept.get((index, stream))
     if given is not None:
         a.workspace, a.workspace_bytes = given.data_ptr(), given.numel()
     code = lib.fnmoe_paged_attention_q8(ref, stream)
@@ -268,7 +278,7 @@ def paged_attention_q8(q, k_cache, v_cache, k_scale, v_scale, block_table, conte
         _lib.check(lib.fnmoe_paged_attention_q8_workspace_size(ref, ctypes.byref(need)), "paged attention q8 workspace")
         given = k_scale.new_empty((need.value,), dtype=torch.uint8)
         if not capturing:
-            _scratch.kept[(q.get_device(), stream)] = given
+            _scratch.kept[(index, stream)] = given
         a.workspace, a.workspace_bytes = given.data_ptr(), given.numel()
         code = lib.fnmoe_paged_attention_q8(ref, stream)
     _lib.check(code, "paged_attention_q8")

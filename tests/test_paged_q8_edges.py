@@ -1,5 +1,6 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
-sequence, scratch under graphs and threads, descriptors of cut work.
+sequence, scratch under graphs and threads, descriptors of cut work,
+tensors of another device.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -500,3 +501,90 @@ def test_every_descriptor_by_segment_is_set_before_the_join(cuda_lib):
                        workspace=ws)
     none = torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device="cuda")
     assert int((ws.view(torch.int32).view(-1, 4) == none).all(1).sum()) >= 6  # (6 - 3) tiles x 2 kv heads
+
+
+# ---- tensors of another device ----
+
+
+def _calls(place):
+    """Every call of the module on stand-in tensors; place(name) says where the named one is."""
+    import torch
+    from flashnext_b200 import paged_q8 as m
+
+    def t(name, *shape, dtype=torch.int32):
+        index = place(name)
+        real = torch.zeros(shape, dtype=dtype)
+        return real if index < 0 else _Cuda(*shape, dtype=dtype, index=index)
+
+    def cache():
+        return [t(n, 4, 32, 2, 64, dtype=torch.int8) for n in ("k_cache", "v_cache")] + \
+            [t(n, 4, 2, 2, dtype=torch.float32) for n in ("k_scale", "v_scale")]
+
+    def rows(name, heads=2):
+        return t(name, 3, heads, 64, dtype=torch.bfloat16)
+
+    def plan(names=("seq_lens", "new_lens", "release", "block_table", "free_pages", "free_state")):
+        shapes = {"block_table": (3, 5), "free_pages": (9,), "free_state": (2,)}
+        seq, new, gone, table, ring, state = (t(n, *shapes.get(n, (3,))) for n in names)
+        out = m.PagePlan(t("out.block_table", 3, 5), t("out.seq_lens", 3), ring, t("out.free_state", 2),
+                         t("out.slot_map", 8, dtype=torch.int64), t("out.token_seq", 8), t("out.positions", 8),
+                         t("out.cu_new", 4), t("out.admitted", 3))
+        return m.page_plan(seq, new, table, ring, state, 32, 8, release=gone, out=out)
+
+    return {
+        "plan": plan,
+        "append": lambda: m.kv_append_q8(rows("k"), rows("v"), t("slot_map", 3, dtype=torch.int64), *cache()),
+        "read": lambda: m.kv_read_q8(t("slots", 3, dtype=torch.int64), *cache(), out=(rows("out[0]"), rows("out[1]"))),
+        "attention": lambda: m.paged_attention_q8(
+            rows("q", 4), *cache(), t("block_table", 2, 5), t("context_lens", 2), 0.1, cu_q=t("cu_q", 3),
+            out=rows("out", 4), workspace=t("workspace", 1 << 16, dtype=torch.uint8)),
+    }
+
+
+CACHE = ("k_cache", "v_cache", "k_scale", "v_scale")
+TENSORS = {
+    "plan": ("seq_lens", "new_lens", "release", "block_table", "free_pages", "free_state", "out.block_table", "out.seq_lens",
+             "out.free_state", "out.slot_map", "out.token_seq", "out.positions", "out.cu_new", "out.admitted"),
+    "append": ("k", "v", "slot_map", *CACHE),
+    "read": ("slots", "out[0]", "out[1]", *CACHE),
+    "attention": ("q", "block_table", "context_lens", "cu_q", "out", "workspace", *CACHE),
+}
+
+
+class _Accepts:
+    """A library that takes every call."""
+
+    def __getattr__(self, name):
+        return lambda *a: _lib.OK
+
+
+@pytest.mark.parametrize("call", list(TENSORS))
+def test_calls_refuse_tensors_of_another_device_or_the_host(monkeypatch, call):
+    from flashnext_b200 import paged_q8
+
+    started = []
+    monkeypatch.setattr(paged_q8, "_ready", lambda t: started.append(t) or (_Accepts(), 7))
+    _calls(lambda name: 0)[call]()
+    assert len(started) == 1
+    for name in TENSORS[call]:
+        for index, error in ((1, ValueError), (-1, TypeError)):
+            with pytest.raises(error):
+                _calls(lambda n: index if n == name else 0)[call]()
+    assert len(started) == 1, "a call with a misplaced tensor reached the library"
+
+
+def test_a_workspace_is_checked(monkeypatch):
+    import torch
+    from flashnext_b200 import paged_q8
+
+    monkeypatch.setattr(paged_q8, "_ready", lambda t: (_Accepts(), 7))
+    cache = [_Cuda(4, 32, 2, 64, dtype=torch.int8) for _ in range(2)] + [_Cuda(4, 2, 2, dtype=torch.float32) for _ in range(2)]
+    args = (_Cuda(3, 4, 64, dtype=torch.bfloat16), *cache, _Cuda(3, 2, dtype=torch.int32), _Cuda(3, dtype=torch.int32), 0.1)
+    good = _Cuda(1 << 16, dtype=torch.uint8)
+    paged_q8.paged_attention_q8(*args, workspace=good)
+    with pytest.raises(TypeError):
+        paged_q8.paged_attention_q8(*args, workspace=_Cuda(1 << 14, dtype=torch.float32))
+    strided = _Cuda(1 << 16, dtype=torch.uint8)
+    strided.real = strided.real[::2]
+    with pytest.raises(ValueError):
+        paged_q8.paged_attention_q8(*args, workspace=strided)
