@@ -305,7 +305,8 @@ typedef struct FnQ8Cache {
  * not gets neither pages nor slots and keeps its length; the caller sees
  * admitted[b] == 0.  Pages come from the head of the free ring in order;
  * pages of released rows join its end (in order of sequence and column) and
- * can be given from the next call on.  Unused table cells hold -1. */
+ * can be given from the next call on.  Unused table cells hold -1.  Arrays
+ * are aligned as their elements. */
 typedef struct FnPagePlanArgs {
   uint32_t abi_version;
   uint32_t batch;              /* sequences (table rows), at most 8192 */
@@ -381,7 +382,7 @@ typedef struct FnQ8AttentionArgs {
   FnQ8Cache cache;
   const void *q;               /* [q_rows, q_heads, head_dim] bf16, heads contiguous, 16-byte aligned */
   uint64_t q_stride;           /* elements from one row to the next, a multiple of 8 */
-  const int32_t *block_table;  /* [batch, max_pages] */
+  const int32_t *block_table;  /* [batch, max_pages]; like the next two 4-byte aligned */
   const int32_t *context_lens; /* [batch] */
   const int32_t *cu_q;         /* [batch + 1] ascending from 0, at most q_rows; or NULL */
   void *out;                   /* [q_rows, q_heads, head_dim] bf16, 16-byte aligned */

@@ -803,6 +803,11 @@ int check(const FnQ8AttentionArgs *a, std::string &err) {
     err = "q and out must be 16-byte aligned and q_stride a multiple of 8 values";
     return FNMOE_ERR_VALUE;
   }
+  if ((reinterpret_cast<uintptr_t>(a->block_table) | reinterpret_cast<uintptr_t>(a->context_lens) |
+       reinterpret_cast<uintptr_t>(a->cu_q)) & 3u) {
+    err = "block_table, context_lens and cu_q must be 4-byte aligned";
+    return FNMOE_ERR_VALUE;
+  }
   return FNMOE_OK;
 }
 

@@ -648,6 +648,16 @@ int page_plan(const FnPagePlanArgs *a, cudaStream_t s, std::string &err) {
     err = "at most " + std::to_string(kPlanMaxBatch) + " sequences";
     return FNMOE_ERR_SHAPE;
   }
+  for (const void *at : {static_cast<const void *>(a->seq_lens), static_cast<const void *>(a->new_lens),
+                         static_cast<const void *>(a->release), static_cast<const void *>(a->block_table),
+                         static_cast<const void *>(a->free_pages), static_cast<const void *>(a->free_state),
+                         static_cast<const void *>(a->block_table_out), static_cast<const void *>(a->seq_lens_out),
+                         static_cast<const void *>(a->free_state_out), static_cast<const void *>(a->token_seq),
+                         static_cast<const void *>(a->positions), static_cast<const void *>(a->cu_new),
+                         static_cast<const void *>(a->admitted)}) {
+    if (misaligned(at, 4)) { err = "the int32 arrays must be 4-byte aligned"; return FNMOE_ERR_VALUE; }
+  }
+  if (misaligned(a->slot_map, 8)) { err = "slot_map must be 8-byte aligned"; return FNMOE_ERR_VALUE; }
   if (a->seq_lens_out == a->seq_lens || a->free_state_out == a->free_state) {
     err = "seq_lens_out and free_state_out must not be the inputs (other CTAs still read those)";
     return FNMOE_ERR_VALUE;

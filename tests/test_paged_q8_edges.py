@@ -1,6 +1,6 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
 sequence, scratch under graphs and threads, descriptors of cut work,
-tensors of another device.
+tensors of another device, arrays off their alignment.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -13,6 +13,7 @@ the worst case.
 """
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import numpy as np
@@ -20,7 +21,7 @@ import pytest
 
 from flashnext_b200 import _lib
 from oracle import paged_q8 as oq8
-from test_paged_q8 import KINDS, _bf16, _empty_cache, _place, _slots
+from test_paged_q8 import KINDS, _attention_args, _bf16, _empty_cache, _place, _plan_args, _set, _slots
 
 C_MAG = 2.0 ** -13
 
@@ -588,3 +589,20 @@ def test_a_workspace_is_checked(monkeypatch):
     strided.real = strided.real[::2]
     with pytest.raises(ValueError):
         paged_q8.paged_attention_q8(*args, workspace=strided)
+
+
+# ---- arrays off their alignment ----
+
+
+@pytest.mark.parametrize("entry,make,names,off", [
+    ("fnmoe_page_plan", _plan_args, TENSORS["plan"], 2), ("fnmoe_page_plan", _plan_args, ("out.slot_map",), 4),
+    ("fnmoe_paged_attention_q8", _attention_args, ("block_table", "context_lens", "cu_q"), 2)])
+def test_entry_points_refuse_arrays_off_their_alignment(entry, make, names, off):
+    fields = {"out.block_table": "block_table_out", "out.seq_lens": "seq_lens_out", "out.free_state": "free_state_out"}
+    fn = getattr(_lib.load(), entry)
+    for name in names:
+        field = fields.get(name, name.removeprefix("out."))
+        args = make()
+        args = _set(args, field, (getattr(args, field) or 0x90000) + off)
+        assert fn(ctypes.byref(args), None) == _lib.ERR_VALUE, name
+        assert "aligned" in _lib.last_error()
