@@ -377,7 +377,7 @@ typedef struct FnQ8AttentionArgs {
   uint32_t batch;
   uint32_t q_rows;             /* rows of q and out (batch when cu_q is NULL); 0 is a no-op */
   uint32_t q_heads;            /* multiple of kv_heads, at most 32 per kv head */
-  uint32_t max_pages;
+  uint32_t max_pages;          /* max_pages * page_size at most 2^31 - 1024 */
   float scale;                 /* finite, > 0 */
   FnQ8Cache cache;
   const void *q;               /* [q_rows, q_heads, head_dim] bf16, heads contiguous, 16-byte aligned */

@@ -772,15 +772,18 @@ __global__ void __launch_bounds__(256) k_q8_join(Q8View p, int few, int many) {
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
+// Tokens of a table row: positions are ints, and the kernels look up to three steps of 128 ahead.
+constexpr uint64_t kMostTokens = (1ull << 31) - 1024;
+
 int check(const FnQ8AttentionArgs *a, std::string &err) {
   if (a == nullptr) { err = "args is NULL"; return FNMOE_ERR_NULL; }
   if (a->abi_version != FNMOE_ABI_VERSION) { err = "abi_version mismatch"; return FNMOE_ERR_ABI; }
   if (const int rc = check_q8_cache(a->cache, err)) return rc;
   const FnQ8Cache &c = a->cache;
   if (a->batch == 0 || a->batch > 0x7FFFFFFFu || a->max_pages == 0 || a->q_rows > 0x7FFFFFFFu || a->q_heads == 0 ||
-      a->q_heads % c.kv_heads || static_cast<uint64_t>(a->max_pages) * c.page_size > 0x7FFFFFFFull ||
+      a->q_heads % c.kv_heads || static_cast<uint64_t>(a->max_pages) * c.page_size > kMostTokens ||
       (a->cu_q == nullptr && a->q_rows != a->batch)) {
-    err = "attention needs sequences, a table row below 2^31 tokens, q_heads a multiple of kv_heads and, "
+    err = "attention needs sequences, a table row of at most 2^31 - 1024 tokens, q_heads a multiple of kv_heads and, "
           "without cu_q, one row per sequence";
     return FNMOE_ERR_SHAPE;
   }

@@ -1,6 +1,7 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
 sequence, scratch under graphs and threads, descriptors of cut work,
-tensors of another device, arrays off their alignment.
+tensors of another device, arrays off their alignment,
+positions near 2^31.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -21,7 +22,7 @@ import pytest
 
 from flashnext_b200 import _lib
 from oracle import paged_q8 as oq8
-from test_paged_q8 import KINDS, _attention_args, _bf16, _empty_cache, _place, _plan_args, _set, _slots
+from test_paged_q8 import KINDS, _attention_args, _bf16, _cache_struct, _empty_cache, _place, _plan_args, _set, _slots
 
 C_MAG = 2.0 ** -13
 
@@ -606,3 +607,15 @@ def test_entry_points_refuse_arrays_off_their_alignment(entry, make, names, off)
         args = _set(args, field, (getattr(args, field) or 0x90000) + off)
         assert fn(ctypes.byref(args), None) == _lib.ERR_VALUE, name
         assert "aligned" in _lib.last_error()
+
+
+# ---- positions near 2^31 ----
+
+
+@pytest.mark.parametrize("page", [16, 48, 128, 1 << 20, 786432])
+def test_attention_refuses_table_rows_whose_lookahead_would_pass_2_31(page):
+    """The kernels step and look ahead in ints past a row's end."""
+    fn, most = _lib.load().fnmoe_paged_attention_q8, ((1 << 31) - 1024) // page
+    for pages, code in ((most, _lib.ERR_WORKSPACE), (most + 1, _lib.ERR_SHAPE)):  # the first lacks a workspace only
+        a = _set(_set(_attention_args(), "cache", _cache_struct(page_size=page, block=16)), "max_pages", pages)
+        assert fn(ctypes.byref(a), None) == code
