@@ -94,6 +94,11 @@ __device__ __forceinline__ Sum3 block_scan(Sum3 v, Sum3 &carry, long long *red) 
   return v;
 }
 
+// Pages of `tokens` tokens; both are ints, their sum may not be one.
+__device__ __forceinline__ int pages_of(int tokens, int page) {
+  return static_cast<int>((static_cast<uint32_t>(tokens) + static_cast<uint32_t>(page) - 1u) / static_cast<uint32_t>(page));
+}
+
 __global__ void __launch_bounds__(kPlanThreads) k_page_plan(PlanView p) {
   extern __shared__ int32_t plan_sm[];
   __shared__ long long red[3 * (kPlanThreads / 32)];
@@ -159,8 +164,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_page_plan(PlanView p) {
   const int gwarp = blockIdx.x * (kPlanThreads / 32) + (tid >> 5), warps = gridDim.x * (kPlanThreads / 32);
   for (int b = gwarp; b < B; b += warps) {
     const int held = s_held[b], n = s_cu[b + 1] - s_cu[b];
-    const int pages0 = (held + p.page - 1) / p.page;
-    const int pages1 = (held + n + p.page - 1) / p.page;
+    const int pages0 = pages_of(held, p.page), pages1 = pages_of(held + n, p.page);
     const int back0 = s_back[b], back = s_back[b + 1] - back0;
     const bool gone = p.release != nullptr && p.release[b] != 0;
     const size_t row = static_cast<size_t>(b) * p.width;
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_page_plan(PlanView p) {
       seq = lo;
       pos = s_held[seq] + t - s_cu[seq];
       const int c = pos / p.page;
-      const int pages0 = (s_held[seq] + p.page - 1) / p.page;
+      const int pages0 = pages_of(s_held[seq], p.page);
       const int page = c < pages0 ? p.table[static_cast<size_t>(seq) * p.width + c]
                                   : p.ring[(head + s_start[seq] + (c - pages0)) % num];
       slot = page < 0 ? -1 : static_cast<long long>(page) * p.page + (pos - c * p.page);

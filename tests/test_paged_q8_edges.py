@@ -619,3 +619,20 @@ def test_attention_refuses_table_rows_whose_lookahead_would_pass_2_31(page):
     for pages, code in ((most, _lib.ERR_WORKSPACE), (most + 1, _lib.ERR_SHAPE)):  # the first lacks a workspace only
         a = _set(_set(_attention_args(), "cache", _cache_struct(page_size=page, block=16)), "max_pages", pages)
         assert fn(ctypes.byref(a), None) == code
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,held,new", [((1 << 30) - 1, (1 << 31) - 4, 2), ((1 << 30) - 1, (1 << 31) - 3, 0),
+                                           (715827882, (1 << 31) - 4, 2), ((1 << 31) - 1, 9, 4), ((1 << 31) - 1, 0, 4)])
+def test_page_plan_of_lengths_near_2_31(cuda_lib, page, held, new):
+    from flashnext_b200.paged_q8 import page_plan
+
+    width = ((1 << 31) - 1) // page
+    lens, add = [held, 0], [new, 1]
+    table = np.full((2, width), -1)
+    table[0, : -(-held // page)] = 3 + np.arange(-(-held // page))
+    ring = [8, 7, 6, 9, 10]
+    want = oq8.page_plan(lens, add, None, table.tolist(), ring, 4, 3, page, 8)
+    got = page_plan(_dev(lens), _dev(add), _dev(table), _dev(ring), _dev([4, 3]), page, 8)
+    for name in want:
+        np.testing.assert_array_equal(getattr(got, name).cpu().numpy(), np.asarray(want[name]), err_msg=name)
