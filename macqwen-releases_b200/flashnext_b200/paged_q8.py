@@ -296,7 +296,8 @@ class PagedKVCacheQ8:
     ``batch`` rows of at most ``max_pages_per_seq`` pages; ``max_tokens`` new
     tokens a step.  Nothing is read on the host: a sequence that does not fit
     has ``plan.admitted`` 0 and takes no part in the step, so its rows must not
-    be among those packed (``plan.cu_new`` counts them as none).  Tables and
+    be among those packed (``plan.cu_new`` counts them as none): where that can
+    happen, :meth:`pack` takes them out on the device.  Tables and
     lengths alternate between two sets of buffers; a captured CUDA graph
     therefore holds an even number of plans.
     """
@@ -341,6 +342,18 @@ class PagedKVCacheQ8:
                               self.max_tokens, release=release, out=self._other)
         self._other = was
         return self.last
+
+    def pack(self, x, first):
+        """The last plan's rows among ``x`` [n, ...], in which each row of the
+        table has its ``new_lens[b]`` rows from ``first[b]`` on ([batch] int32),
+        whether or not it was admitted.  -> [min(n, max_tokens), ...]: the
+        admitted rows as :meth:`append` and :meth:`attention` want them; those
+        past ``plan.cu_new[batch]`` repeat others, are stored nowhere and come
+        back from the attention as zeros."""
+        p, n = self.last, min(x.shape[0], self.max_tokens)
+        seq = p.token_seq[:n].clamp(min=0).long()
+        at = first[seq] + torch.arange(n, device=x.device) - p.cu_new[seq]
+        return x[at.clamp(0, max(x.shape[0] - 1, 0))]
 
     def append(self, k, v) -> None:
         """Store the last plan's packed rows [tokens, kv_heads, head_dim]."""

@@ -1,7 +1,7 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
 sequence, scratch under graphs and threads, descriptors of cut work,
 tensors of another device, arrays off their alignment,
-positions near 2^31.
+positions near 2^31, steps in which a request is refused.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -636,3 +636,52 @@ def test_page_plan_of_lengths_near_2_31(cuda_lib, page, held, new):
     got = page_plan(_dev(lens), _dev(add), _dev(table), _dev(ring), _dev([4, 3]), page, 8)
     for name in want:
         np.testing.assert_array_equal(getattr(got, name).cpu().numpy(), np.asarray(want[name]), err_msg=name)
+
+
+# ---- steps in which a request is refused ----
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("refused", ["pages", "columns", "tokens"])
+def test_rows_of_a_step_with_a_refused_request_line_up(cuda_lib, refused):
+    """The rows of all requests go in; those of the admitted ones are stored
+    and attended as if the refused one had not been there."""
+    import torch
+    from flashnext_b200.paged_q8 import PagedKVCacheQ8
+
+    # the sums that decide over pages and tokens count a refused request too, if it fits its row
+    pages, columns, most, admitted = {"pages": (12, 12, 400, [1, 0, 0, 1]), "columns": (40, 5, 400, [1, 0, 1, 1]),
+                                      "tokens": (40, 12, 150, [1, 0, 0, 0])}[refused]
+    page, batch, kv, group, dim = 32, 4, 2, 4, 64
+    cache = PagedKVCacheQ8(pages, page, kv, dim, columns, batch, most, block=32)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    held, rows = [0] * batch, [[] for _ in range(batch)]
+    for step, new in enumerate(([20, 33, 7, 1], [3, 330, 60, 2], [1, 5, 1, 1])):
+        k, v, q = (torch.randn(sum(new), h, dim, device="cuda", generator=g).bfloat16() for h in (kv, kv, kv * group))
+        first = np.concatenate([[0], np.cumsum(new)])
+        plan = cache.plan(_dev(new))
+        cache.append(cache.pack(k, _dev(first[:-1])), cache.pack(v, _dev(first[:-1])))
+        out = cache.attention(cache.pack(q, _dev(first[:-1])), 0.125).float().cpu().numpy()
+        ok = plan.admitted.tolist()
+        assert ok == (admitted if step == 1 else [1] * 4)
+        at = 0
+        for b in range(batch):
+            if not ok[b]:
+                continue
+            n, span = new[b], slice(int(first[b]), int(first[b + 1]))
+            held[b] += n
+            rows[b].append((k[span], v[span]))
+            # the cache holds the request's own rows, to within half a code of their block's largest
+            slots = torch.from_numpy(_slots(plan.block_table.cpu().numpy(), b, 0, held[b], page)).cuda()
+            back = cache.read(slots)
+            for i in range(2):
+                mine = torch.cat([r[i] for r in rows[b]]).float()
+                assert float((back[i].float() - mine).abs().max()) <= float(mine.abs().max()) * (1.5 / 127 + 2.0 ** -8)
+            kk, vv = (c.float().view(-1, kv, dim)[slots].cpu().numpy() * s.view(-1, kv)[slots // 32].cpu().numpy()[:, :, None]
+                      for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+            seen = np.arange(held[b])[None] <= (held[b] - n + np.arange(n))[:, None]
+            want, mag = oq8.attention(q[span].float().cpu().numpy(), kk, vv, seen, 0.125)
+            assert _outside(out[at:at + n], want, mag) == 0
+            at += n
+        assert (out[at:] == 0).all()
