@@ -1,7 +1,7 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
 sequence, scratch under graphs and threads, descriptors of cut work,
 tensors of another device, arrays off their alignment,
-positions near 2^31, steps in which a request is refused.
+positions near 2^31, steps in which a request is refused, large batches.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -685,3 +685,41 @@ def test_rows_of_a_step_with_a_refused_request_line_up(cuda_lib, refused):
             assert _outside(out[at:at + n], want, mag) == 0
             at += n
         assert (out[at:] == 0).all()
+
+
+# ---- large batches ----
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,batch", [(256, 170), (128, 210), (64, 300)])
+@pytest.mark.parametrize("rows", [None, (0, 3), (9, 20), (0, 30)])
+def test_large_batches_are_scanned_and_joined_by_cuts(cuda_lib, kind, dim, batch, rows):
+    """More sequences than a CTA has threads, and more segments (sequence, kv
+    head, tile) than CTAs to cut them, so that the join goes by the cuts: rows of
+    the few-row kernel, of the many-row kernel and of both."""
+    import torch
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    page, block, kv, group = 32, 32, 4, 2
+    rng = np.random.default_rng(dim + batch + (rows or (7, 7))[1])
+    held = rng.integers(0, 200, batch)
+    held[rng.integers(0, batch, 12)] = rng.integers(700, 3000, 12)
+    held[[0, 5, batch - 1]] = 0, 1, 0
+    new = [1] * batch if rows is None else rng.integers(rows[0], rows[1] + 1, batch).tolist()
+    held = held.tolist()
+    table, pages = _place(rng, held, page)
+    n = pages * page
+    k, v = (np.clip(np.rint(rng.standard_normal((n, kv, dim)) * 40), -127, 127).astype(np.float32) for _ in range(2))
+    if kind == "e4m3":
+        k, v = oq8.e4m3_round(k), oq8.e4m3_round(v)
+    ks, vs = ((np.exp(0.5 * rng.standard_normal((n // block, kv))) / 40).astype(np.float32) for _ in range(2))
+    cache = _cache_of(table, pages, page, block, kind, k, ks, v, vs)
+    q = _bf16(rng.standard_normal((sum(new), kv * group, dim)))
+    cu = None if rows is None else _dev(np.concatenate([[0], np.cumsum(new)]))
+    args = (q.cuda(), *cache, _dev(table), _dev(held), dim ** -0.5)
+    out = paged_attention_q8(*args, cu_q=cu)
+    assert torch.equal(out, paged_attention_q8(*args, cu_q=cu))
+    out = out.float().cpu().numpy()
+    assert _wrong(out, q.float().numpy(), table, held, new, ((k, ks), (v, vs)), page, block, dim ** -0.5) == 0
+    assert _lib.read_device_errors() == 0
