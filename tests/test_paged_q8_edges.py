@@ -1,7 +1,7 @@
 """The paged 8-bit KV cache at its edges: value scales far apart, rows of no
 sequence, scratch under graphs and threads, descriptors of cut work,
 tensors of another device, arrays off their alignment,
-positions near 2^31, steps in which a request is refused, large batches.
+positions near 2^31, steps in which a request is refused, large batches, the weights' low terms.
 
 Attention is held to this: an output is the bfloat16 rounding of a number within
 2^-13 mean|v| of the truth, with mean|v| the weighted mean of the magnitudes.
@@ -723,3 +723,74 @@ def test_large_batches_are_scanned_and_joined_by_cuts(cuda_lib, kind, dim, batch
     out = out.float().cpu().numpy()
     assert _wrong(out, q.float().numpy(), table, held, new, ((k, ks), (v, vs)), page, block, dim ** -0.5) == 0
     assert _lib.read_device_errors() == 0
+
+
+# ---- the weights' low terms ----
+
+
+def _opposed(dim, lengths, kind, page=16, seed=7):
+    """Even tokens hold values +v with one score, odd ones -v with another a
+    little lower, so an output is a small difference of large sums: (1 - w) / (1 + w)
+    of v for w near 1, while mean|v| is v.  A weight that is off by 2^-10 shows."""
+    rng = np.random.default_rng(seed + dim)
+    table, pages = _place(rng, lengths, page)
+    n = pages * page
+    k, sign = np.zeros((n, 1, dim), np.float32), np.ones((n, 1, 1), np.float32)
+    k[:, :, 1:] = np.rint(rng.standard_normal(dim - 1) * 3)  # alike for all tokens
+    for b, length in enumerate(lengths):
+        slot = _slots(table, b, 0, length, page)
+        k[slot, 0, 0] = np.where(np.arange(length) % 2, 60, 64)
+        sign[slot, 0, 0] = np.where(np.arange(length) % 2, -1, 1)
+    v = (sign * 96 * rng.choice([-1, 1], (1, 1, dim))).astype(np.float32)
+    one = np.ones((pages, 1), np.float32)
+    return table, pages, ((k, one), (v, one / 32)), rng
+
+
+def _queries(rng, rows, group, dim):
+    q = np.zeros((rows, group, dim), np.float32)
+    q[:, :, 0] = rng.uniform(0.5, 4.0, (rows, group))
+    return _bf16(q)
+
+
+def _bf16_of(x, up):
+    """float32 to bfloat16 and back: to nearest, or (up False) toward zero."""
+    return _bf16(x).float().numpy() if up else (np.ascontiguousarray(x, np.float32).view(np.uint32) & 0xFFFF0000).view(np.float32)
+
+
+@pytest.mark.parametrize("up", [True, False])
+def test_the_bound_on_opposed_values_tells_one_term_of_a_weight_from_two(up):
+    """The test below, with the weights' rounding planted in the oracle: with
+    both terms every output is inside the bound, with the high term alone some
+    rows of every length have outputs outside."""
+    dim, lengths, scale = 64, [2, 17, 64, 333, 1000, 5000], 1 / 64
+    table, _, ((k, _), (v, vs)), rng = _opposed(dim, lengths, "int8")
+    q = _queries(rng, len(lengths), 16, dim).float().numpy()
+    for b, length in enumerate(lengths):
+        slot = _slots(table, b, 0, length, 16)
+        kk, vv = k[slot].astype(np.float64), v[slot].astype(np.float64) * vs[0, 0]
+        want, mag = oq8.attention(q[b:b + 1], kk, vv, np.ones((1, length), bool), scale)
+        t = (q[b].astype(np.float64) @ kk[:, 0].T) * scale * np.log2(np.e)
+        u = np.exp2(t - t.max(1, keepdims=True)).astype(np.float32)
+        hi = _bf16_of(u, up)
+        for terms, w in ((2, hi.astype(np.float64) + _bf16_of(u - hi, True)), (1, hi.astype(np.float64))):
+            out = _bf16((w @ vv[:, 0] / u.sum(1, dtype=np.float64, keepdims=True)).astype(np.float32)).float().numpy()
+            off = [_outside(out[h], want[0, h], mag[0, h]) > 0 for h in range(16)]
+            assert (sum(off) == 0) if terms == 2 else (sum(off) > 0), (length, terms, sum(off))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [None, 1, 2, 9])
+def test_small_differences_of_large_sums(cuda_lib, kind, dim, rows):
+    from flashnext_b200.paged_q8 import paged_attention_q8
+
+    lengths, group, page = [2, 17, 64, 333, 1000, 5000], 16, 16
+    table, pages, host, rng = _opposed(dim, lengths, kind)
+    (k, ks), (v, vs) = host
+    cache = _cache_of(table, pages, page, page, kind, k, ks, v, vs)
+    new = [min(rows or 1, h) for h in lengths]
+    q = _queries(rng, sum(new), group, dim)
+    cu = None if rows is None else _dev(np.concatenate([[0], np.cumsum(new)]))
+    out = paged_attention_q8(q.cuda(), *cache, _dev(table), _dev(lengths), 1 / 64, cu_q=cu).float().cpu().numpy()
+    assert _wrong(out, q.float().numpy(), table, lengths, new, host, page, page, 1 / 64) == 0
