@@ -43,9 +43,9 @@ namespace {
 //     tokens' bytes with prmt.
 // 16 tokens lie in one page and one scale block.
 //
-// Measured: 16 sequences of 1k-32k tokens (16/2 heads, D 256; 290 MB) 67 us with
-// the join, 4.3 TB/s; 16 x 131,072 tokens 6.1 TB/s (94% of a measured copy) at D
-// 256 and 128, 4.6 TB/s at D 64, whose rows are 64-byte pieces.  The rest is a
+// Measured: 16 sequences of 1k-32k tokens (16/2 heads, D 256; 290 MB) 66 us with
+// the join, 4.4 TB/s; 16 x 131,072 tokens 6.1 TB/s (94% of a measured copy) at D
+// 256 and 128, 4.6 TB/s at D 64 (64-byte pieces; the kernel also spills).  The rest is a
 // fixed 20 us: launch, finding the range, the first copies, joining warps and
 // CTAs.
 

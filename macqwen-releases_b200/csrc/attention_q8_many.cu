@@ -11,8 +11,8 @@
 //
 // Per unit, S = Q K^T (M128 N64, K = D) and O += P V (M128 N = D, K = 64, for
 // each of the two terms of P) run on the tensor cores with Q and P as TMEM
-// operands, S and O as TMEM accumulators: 6 D * 128 * 64 multiply-adds where
-// the formula has 4, which bounds the kernel (1,536 clocks a unit at D 256).
+// operands, S and O as TMEM accumulators: 3 D * 128 * 64 multiply-adds where
+// the formula has 2, at least 1,536 clocks a unit at D 256.
 // Roles:
 //   softmax     a row a thread (at D 256 two threads, 32 tokens each, which
 //               exchange their maxima through shared memory): S from TMEM,
@@ -32,8 +32,9 @@
 // unit's Q K^T runs while this one's P is made.  At D 64 and 128 P takes S's
 // columns and a CTA needs 256 of the 512: two CTAs share an SM and fill each
 // other's waits.
-// Measured: a 5,000-token prefill chunk (16/2 heads, D 256, 205 GFLOP) 375 us,
-// 0.55 PFLOP/s, about 4,000 clocks a unit.  What bounds it now is the chain
+// Measured: a 5,000-token prefill chunk (16/2 heads, D 256, 205 GFLOP) 368 us,
+// 0.56 PFLOP/s, about 4,000 clocks a unit; at D 128 290 us and at D 64 235 us of
+// half and a quarter of the work (these spill at 80 registers).  What bounds it now is the chain
 // softmax -> P V and the issue slots that widening takes beside it (IPC 2.0);
 // the MMAs alone take about 1,700 clocks a unit (N 64 and two terms of P).
 // Every wait is bounded: a timeout sets the device error word and marks the

@@ -32,8 +32,10 @@ namespace {
 //
 // Bytes: the table read and written once (8 B a cell), 16 B a token, the
 // lengths once per CTA (from L2).  Measured: 8.3 us for 16 rows of 512 columns,
-// 8.4 us for 512 rows of 256 columns and 26,000 tokens; a chain of latencies
-// (lengths, sums, columns), below the 11 us that a call costs the host.
+// 8.4 us for 512 rows of 256 columns and 26,000 tokens; a chain of latencies:
+// lengths, sums, and up to `width` / 32 rounds of load and store over the columns,
+// which stay in order since the table may be updated in place.  Below the 11 us
+// that a call costs the host.
 
 constexpr int kPlanThreads = 256;
 constexpr int kPlanMaxBatch = 8192;
@@ -217,8 +219,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_page_plan(PlanView p) {
 // Grid: chunks of `chunk` tokens x (kv head, K or V); a CTA handles the runs
 // that begin in its chunk.  The host picks the chunk from the token count so
 // that a decode batch gets a CTA per row and a prefill chunk does not launch
-// a CTA per token.  Measured: 5,000 rows of 2 heads of 256, 14 us (15 MB;
-// 2.2 us at HBM rate): a CTA's chain of slots, rows, maximum and codes.
+// a CTA per token.  Measured: 5,000 rows of 2 heads of 256, 12.5 us (15 MB;
+// 2.4 us at HBM rate): a CTA's chain of slots, rows, maximum and codes.
 
 constexpr int kAppendThreads = 256;
 constexpr int kMaxBlock = 128;
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append_q8(Q8Store p) {
 // kv head, of K or of V, so that neither a barrier nor shared memory stands
 // between its loads, its maximum and its stores; the CTA's warps take
 // different heads.  With a CTA a run, 13,000 rows of 8 heads of 128 in blocks
-// of 16 took 53 us; this takes 36 us.
+// of 16 took 53 us; this takes 36 us (10,500 rows: 29 us, 65 MB).
 template <int D, int NP, bool E4M3>
 __global__ void __launch_bounds__(256) k_kv_append_q8_small(Q8Store p) {
   constexpr int kTpr = D / 8, kRows = 32 / kTpr;  // lanes per row, rows per pass
@@ -489,8 +491,8 @@ __global__ void __launch_bounds__(256) k_kv_append_q8_small(Q8Store p) {
 // ---- read-back --------------------------------------------------------------
 //
 // A thread takes 16 codes of K and the same 16 of V of one slot: two 16-byte
-// loads, four 16-byte stores.  Bound by HBM: 3 bytes a value moved.  32,768
-// slots of 2 heads of 256: 22.8 us, 4.4 TB/s (8 codes a thread 25 us, two or four
+// loads, four 16-byte stores.  3 bytes a value moved.  32,768 slots of 2 heads
+// of 256: 23 us, 4.4 TB/s, two thirds of HBM (8 codes a thread 25 us, two or four
 // such pieces a thread 23 and 25 us).
 
 struct Q8Load {
