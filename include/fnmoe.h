@@ -413,6 +413,118 @@ typedef struct FnRowsArgs {
   void *out;                   /* [count, dims] bf16, 16-byte aligned */
 } FnRowsArgs;
 
+/* ---- The dense steps around the block ----
+ * Rows of hidden states (norms, 8-bit rows), matrix products with their
+ * epilogue and the draw of a token from logits.  Element types: FNMOE_DTYPE_*
+ * where a dtype is asked for, FNMOE_Q8_* codes.  Strides are in elements and
+ * from row to row; a row's elements are adjacent.  No call needs a workspace. */
+
+#define FNMOE_NORM_UNIT_OFFSET 0x1u      /* the weight is kept as w - 1: rows are multiplied by 1 + weight */
+#define FNMOE_NORM_ROWS_AS_THEY_ARE 0x2u /* no norm and no weight: x (+ residual) to codes or another place */
+
+/* s = x + residual; y = s / sqrt(mean(s^2) + eps) * weight; codes of y with one
+ * scale a row, max(max|y|, 2^-100) / top (top 127 or 448).  A row that is not
+ * finite gets a scale that is not a number and codes of 0 (int8 and e4m3). */
+typedef struct FnNormArgs {
+  uint32_t abi_version;
+  uint32_t flags;              /* FNMOE_NORM_* */
+  uint32_t rows;
+  uint32_t dim;                /* 1..16384 */
+  uint32_t x_dtype;            /* of x and y */
+  uint32_t residual_dtype;     /* of residual and residual_out */
+  uint32_t weight_dtype;
+  uint32_t code_type;          /* FNMOE_Q8_* of codes */
+  float eps;                   /* finite, >= 0 */
+  uint32_t reserved;
+  const void *x;               /* [rows, dim], x_stride apart */
+  uint64_t x_stride;
+  const void *residual;        /* [rows, dim], residual_stride apart; NULL: none */
+  uint64_t residual_stride;
+  const void *weight;          /* [dim] */
+  void *y;                     /* [rows, dim] or NULL */
+  void *residual_out;          /* [rows, dim]: s, rounded; NULL: not kept.  May be residual where its rows are adjacent */
+  void *codes;                 /* [rows, dim] or NULL */
+  float *scales;               /* [rows], with codes */
+} FnNormArgs;
+
+/* out[r, c] = codes[r, c] * scales[r]. */
+typedef struct FnRowCodesArgs {
+  uint32_t abi_version;
+  uint32_t rows;
+  uint32_t dim;
+  uint32_t code_type;          /* FNMOE_Q8_* */
+  uint32_t out_dtype;
+  uint32_t reserved;
+  const void *codes;           /* [rows, dim] */
+  const float *scales;         /* [rows] */
+  void *out;                   /* [rows, dim] */
+} FnRowCodesArgs;
+
+#define FNMOE_LINEAR_BF16 0u   /* bfloat16 x and weight, float32 sums */
+#define FNMOE_LINEAR_INT8 1u   /* int8 codes and a scale a row of both, exact int32 sums */
+#define FNMOE_LINEAR_E4M3 2u   /* float8 e4m3 codes and a scale a row of both, float32 sums */
+
+#define FNMOE_ACT_NONE 0u
+#define FNMOE_ACT_SILU 1u      /* a / (1 + exp(-a)) */
+#define FNMOE_ACT_GELU 2u      /* a (1 + erf(a / sqrt 2)) / 2 */
+#define FNMOE_ACT_RELU 3u
+
+/* out = act(x_scale weight_scale (x weight^T) + bias) + residual. */
+typedef struct FnLinearArgs {
+  uint32_t abi_version;
+  uint32_t type;               /* FNMOE_LINEAR_* */
+  uint32_t rows;               /* of x and out */
+  uint32_t in_width;           /* columns of x and weight; at most 131072 */
+  uint32_t out_width;          /* rows of weight, columns of out */
+  uint32_t activation;         /* FNMOE_ACT_* */
+  uint32_t bias_dtype;
+  uint32_t residual_dtype;
+  uint32_t out_dtype;
+  uint32_t reserved;
+  const void *x;               /* [rows, in_width]; start and rows on 16-byte boundaries */
+  uint64_t x_stride;
+  const void *weight;          /* [out_width, in_width]; start and rows on 16-byte boundaries */
+  uint64_t weight_stride;
+  const float *x_scale;        /* [rows], 8-bit types */
+  const float *weight_scale;   /* [out_width], 8-bit types */
+  const void *bias;            /* [out_width] or NULL */
+  const void *residual;        /* [rows, out_width] or NULL; may be out where types and strides are the same */
+  uint64_t residual_stride;
+  void *out;                   /* [rows, out_width], rows adjacent */
+} FnLinearArgs;
+
+#define FNMOE_SAMPLE_MAX_VOCAB 262144u
+
+/* One token a row.  Weights are exp((l - max l) / temperature); tokens are
+ * ranked by falling logit, equal ones by rising index, and kept while they are
+ * among the first top_k, while the weight ranked before them is below top_p of
+ * the top_k's, and while their own weight is at least min_p.  The token is the
+ * first, by index, at which the kept weights up to and with it exceed uniform
+ * times their total.  Each setting is an array [rows] or, where that is NULL,
+ * the value beside it.  Off: top_k <= 0, top_p >= 1, min_p <= 0.  temperature
+ * <= 0 (or not a number), top_k 1 and top_p <= 0 take the largest logit.
+ * Logits of -infinity and NaN are never taken; a row of nothing else has token
+ * -1 and log-probability 0. */
+typedef struct FnSampleArgs {
+  uint32_t abi_version;
+  uint32_t rows;
+  uint32_t vocab;              /* 1..FNMOE_SAMPLE_MAX_VOCAB */
+  uint32_t logits_dtype;
+  const void *logits;          /* [rows, vocab], logits_stride apart */
+  uint64_t logits_stride;
+  const float *uniform;        /* [rows] in [0, 1) */
+  const float *temperatures;   /* [rows] or NULL */
+  const int32_t *top_ks;       /* [rows] or NULL */
+  const float *top_ps;         /* [rows] or NULL */
+  const float *min_ps;         /* [rows] or NULL */
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+  int64_t *tokens;             /* [rows] */
+  float *logprobs;             /* [rows] or NULL: the token's log-probability among the kept */
+} FnSampleArgs;
+
 /* 1 when an sm_100 device is current and the library initialised, else 0.
  * Replaces flashnext_native_available (metal_runtime_native.mm:196-201). */
 FNMOE_API int fnmoe_available(void);
@@ -563,6 +675,14 @@ FNMOE_API int fnmoe_paged_attention_q8(const FnQ8AttentionArgs *args, void *stre
  * StreamingShardedEmbedding._direct_rows (ngram.py:160-185); the input
  * embedding's streamed rows use the same class (loader.py:266-283). */
 FNMOE_API int fnmoe_rows_dequantize(const FnRowsArgs *args, void *stream);
+
+/* The dense steps around the block (see FnNormArgs, FnRowCodesArgs,
+ * FnLinearArgs, FnSampleArgs).  The reference leaves these to mlx (mx.fast.rms_norm,
+ * nn.Linear, the sampler of its generation loop); no file of its own. */
+FNMOE_API int fnmoe_add_rms_norm(const FnNormArgs *args, void *stream);
+FNMOE_API int fnmoe_dequantize_rows(const FnRowCodesArgs *args, void *stream);
+FNMOE_API int fnmoe_linear(const FnLinearArgs *args, void *stream);
+FNMOE_API int fnmoe_sample(const FnSampleArgs *args, void *stream);
 
 /* ---- Expert-parallel exchange over NVLink peer memory ----
  * No reference counterpart: the reference runs on one device.  One process

@@ -17,6 +17,7 @@
 
 #include "../../include/fnmoe.h"
 #include "attention.cuh"
+#include "dense.cuh"
 #include "paged_q8.cuh"
 #include "rows.cuh"
 #include "common.cuh"
@@ -1074,6 +1075,22 @@ int fnmoe_kv_append_q8(const FnQ8AppendArgs *args, void *stream) {
 
 int fnmoe_kv_read_q8(const FnQ8ReadArgs *args, void *stream) {
   return kv_read_q8(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_add_rms_norm(const FnNormArgs *args, void *stream) {
+  return add_rms_norm(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_dequantize_rows(const FnRowCodesArgs *args, void *stream) {
+  return dequantize_rows(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_linear(const FnLinearArgs *args, void *stream) {
+  return linear(args, static_cast<cudaStream_t>(stream), g_last_error);
+}
+
+int fnmoe_sample(const FnSampleArgs *args, void *stream) {
+  return sample(args, static_cast<cudaStream_t>(stream), g_last_error);
 }
 
 int fnmoe_paged_attention_q8_workspace_size(const FnQ8AttentionArgs *args, uint64_t *bytes) {

@@ -186,6 +186,55 @@ class FnRowsArgs(ctypes.Structure):
     ]
 
 
+NORM_UNIT_OFFSET = 0x1
+NORM_ROWS_AS_THEY_ARE = 0x2
+
+
+class FnNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("flags", _u32), ("rows", _u32), ("dim", _u32),
+        ("x_dtype", _u32), ("residual_dtype", _u32), ("weight_dtype", _u32), ("code_type", _u32),
+        ("eps", ctypes.c_float), ("reserved", _u32),
+        ("x", _vp), ("x_stride", _u64), ("residual", _vp), ("residual_stride", _u64), ("weight", _vp),
+        ("y", _vp), ("residual_out", _vp), ("codes", _vp), ("scales", _vp),
+    ]
+
+
+class FnRowCodesArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("rows", _u32), ("dim", _u32), ("code_type", _u32), ("out_dtype", _u32),
+        ("reserved", _u32), ("codes", _vp), ("scales", _vp), ("out", _vp),
+    ]
+
+
+LINEAR_BF16 = 0
+LINEAR_INT8 = 1
+LINEAR_E4M3 = 2
+
+
+class FnLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("type", _u32), ("rows", _u32), ("in_width", _u32), ("out_width", _u32),
+        ("activation", _u32), ("bias_dtype", _u32), ("residual_dtype", _u32), ("out_dtype", _u32), ("reserved", _u32),
+        ("x", _vp), ("x_stride", _u64), ("weight", _vp), ("weight_stride", _u64),
+        ("x_scale", _vp), ("weight_scale", _vp), ("bias", _vp), ("residual", _vp), ("residual_stride", _u64),
+        ("out", _vp),
+    ]
+
+
+SAMPLE_MAX_VOCAB = 262144
+
+
+class FnSampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _u32), ("rows", _u32), ("vocab", _u32), ("logits_dtype", _u32),
+        ("logits", _vp), ("logits_stride", _u64), ("uniform", _vp),
+        ("temperatures", _vp), ("top_ks", _vp), ("top_ps", _vp), ("min_ps", _vp),
+        ("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float), ("tokens", _vp), ("logprobs", _vp),
+    ]
+
+
 EP_IPC_BYTES = 64
 
 
@@ -237,6 +286,10 @@ SIGNATURES = {
                                                 ctypes.c_int),
     "fnmoe_paged_attention_q8": ([ctypes.POINTER(FnQ8AttentionArgs), _vp], ctypes.c_int),
     "fnmoe_rows_dequantize": ([ctypes.POINTER(FnRowsArgs), _vp], ctypes.c_int),
+    "fnmoe_add_rms_norm": ([ctypes.POINTER(FnNormArgs), _vp], ctypes.c_int),
+    "fnmoe_dequantize_rows": ([ctypes.POINTER(FnRowCodesArgs), _vp], ctypes.c_int),
+    "fnmoe_linear": ([ctypes.POINTER(FnLinearArgs), _vp], ctypes.c_int),
+    "fnmoe_sample": ([ctypes.POINTER(FnSampleArgs), _vp], ctypes.c_int),
     "fnmoe_read_device_errors": ([ctypes.POINTER(_u32), ctypes.c_int], ctypes.c_int),
     "fnmoe_profile_enable": ([ctypes.c_int], ctypes.c_int),
     "fnmoe_ep_create": ([ctypes.POINTER(FnEpConfig), ctypes.POINTER(_vp)], ctypes.c_int),

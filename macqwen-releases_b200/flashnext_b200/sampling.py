@@ -1,0 +1,76 @@
+"""The draw of a token from logits (:func:`sample`)."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .dense import _float, _matrix
+from .paged_q8 import _ready, _want
+
+MAX_VOCAB = _lib.SAMPLE_MAX_VOCAB
+
+
+def _setting(v, dtype, rows, what, index):
+    """(pointer of a [rows] tensor, or None; value where it is a number)."""
+    if isinstance(v, torch.Tensor):
+        return _want(v, dtype, (rows,), what, index), 0
+    return None, v
+
+
+def _number(v, what):
+    v = float(v)
+    if not math.isfinite(v):
+        raise ValueError(f"{what} must be finite")
+    return v
+
+
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token a row of ``logits`` [rows, vocab] (bfloat16 or float32; rows may
+    be slices of wider ones) from ``uniform`` [rows] float32 in [0, 1)
+    -> ``(tokens [rows] int64, logprobs [rows] float32)``.
+
+    Weights are ``exp((l - max l) / temperature)``.  Tokens are ranked by falling
+    logit, equal ones by rising index, and kept while they are among the first
+    ``top_k``, while the weight ranked before them is below ``top_p`` of the
+    top-k's, and while their own weight is at least ``min_p`` (of the largest
+    token's).  The token is the first, by index, at which the kept weights, it
+    included, exceed ``uniform`` times their total; its log-probability is that
+    among the kept.
+
+    Each setting is a number or a [rows] tensor (float32; top_k int32), for
+    requests with settings of their own.  ``top_k`` <= 0, ``top_p`` >= 1 and
+    ``min_p`` <= 0 keep everything; ``temperature`` 0, ``top_k`` 1 or ``top_p``
+    0 take the largest logit (log-probability 0).  Logits of -infinity and NaN
+    are never taken; a row of nothing else has token -1.  The result does not
+    depend on how the work is divided: weights are summed as exact integers.
+    ``vocab`` is at most 262144.
+    """
+    index = logits.get_device()
+    dtype = _float(logits, "logits")
+    lp, rows, vocab, stride = _matrix(logits, "logits", index)
+    f32 = torch.float32
+    tp, t = _setting(temperature, f32, rows, "temperature", index)
+    kp, k = _setting(top_k, torch.int32, rows, "top_k", index)
+    pp, p = _setting(top_p, f32, rows, "top_p", index)
+    mp, m = _setting(min_p, f32, rows, "min_p", index)
+    if tp is None and _number(t, "temperature") < 0:
+        raise ValueError("temperature must not be negative")
+    if kp is None and not -2 ** 31 <= k < 2 ** 31:
+        raise ValueError("top_k must fit 32 bits")
+    if pp is None and _number(p, "top_p") < 0:
+        raise ValueError("top_p must not be negative")
+    if mp is None and not 0 <= _number(m, "min_p") <= 1:
+        raise ValueError("min_p must be between 0 and 1")
+    up = _want(uniform, f32, (rows,), "uniform", index)
+    tokens = logits.new_empty((rows,), dtype=torch.int64)
+    logprobs = logits.new_empty((rows,), dtype=f32)
+    lib, stream = _ready(logits)
+    a = _lib.FnSampleArgs(_lib.ABI_VERSION, rows, vocab, dtype, lp, stride, up, tp, kp, pp, mp, t, k, p, m,
+                          tokens.data_ptr(), logprobs.data_ptr())
+    code = lib.fnmoe_sample(ctypes.byref(a), stream)
+    if code:
+        _lib.check(code, "sample")
+    return tokens, logprobs
