@@ -33,13 +33,20 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
-constexpr int kList = 1024;       // tokens that are ranked against one another
+constexpr int kList = 512;        // tokens of a range that are ranked against one another
+constexpr int kFew = 384;         // kept tokens that one CTA finishes by itself
+constexpr int kGroups = 256;      // groups of tokens whose maxima bound the top-k ..
+constexpr int kByGroups = 190;    // .. up to this k: about 256 ln(1 / (1 - k / 256)) tokens lie above the bound
+constexpr int kBlock = 512;       // adjacent tokens whose weights are summed together for the draw
+constexpr int kMaxBlocks = 128;
+constexpr int kMaxCtas = 16;
+constexpr int kRoots = 512;
 constexpr int kIndexBits = 18;    // FNMOE_SAMPLE_MAX_VOCAB
 constexpr int kPlaceBits = 32 + kIndexBits;
 constexpr uint64_t kAll = ~0ull;  // past every place
 constexpr uint64_t kOne = 1ull << 44;  // the largest weight
-constexpr int kRoots = 128;
 constexpr float kMinusInf = -__builtin_inff();
+constexpr int kEvery = 0x7FFFFFFF;
 
 struct SampleView {
   const void *logits;
@@ -54,25 +61,48 @@ struct SampleView {
   int32_t top_k;
 };
 
-// What the CTAs of a cluster tell one another, each in its own copy.
+// A CTA's working memory.  What other CTAs have to know is written into their
+// copies before a cluster barrier, so that it is read near by after it.
 struct Shared {
-  uint32_t count[kBins];                   // this CTA's histogram
-  uint32_t mass_lo[kBins], mass_hi[kBins]; // and its weights
-  uint64_t list_at[kList], list_w[kList];  // (rank 0) gathered tokens: places and weights
-  double root[kRoots];                     // 2^(j / kRoots)
+  union {
+    struct {
+      uint32_t count[kBins];                     // this CTA's histogram (read by the others)
+      uint32_t mass_lo[kBins], mass_hi[kBins];   // and its weights
+    };
+    struct {
+      uint64_t pulled[kList], pulled_w[kList];   // (rank 0) the cluster's gathered tokens, and their weights
+    };
+  };
+  union {
+    struct {
+      uint32_t count[kBins];                     // the cluster's histogram
+      uint64_t mass[kBins];
+    } sum;
+    struct {
+      uint64_t at[kList], w[kList];              // gathered tokens: places and weights (read by rank 0)
+    } list;
+    float pack[kWarps][kBlock / 2];              // the draw: a warp's kept logits
+  };
+  double root[kRoots];                           // 2^(j / kRoots)
+  uint64_t block_mass[kMaxBlocks];
+  float own_group[kGroups], group[kGroups];      // largest logits of groups: this CTA's, the cluster's
   uint64_t warp_sum[kWarps];
   uint32_t warp_count[kWarps];
   float warp_max[kWarps], warp_min[kWarps];
-  float row_max, row_min;                  // of this CTA's part
-  uint64_t part_mass;                      // of this CTA's kept tokens
-  uint32_t list_n;                         // (rank 0)
-  uint32_t best;                           // this CTA's lowest index of the largest logit
+  float rank_max[kMaxCtas], rank_min[kMaxCtas];
+  uint64_t rank_mass[kMaxCtas];
+  uint32_t rank_list[kMaxCtas];
+  uint32_t list_n;
+  uint32_t best;                                 // (rank 0) lowest index of the largest logit
+  float bound;                                   // no more than the top_k-th largest logit
   // the range in which the place falls
   uint32_t hit_bin, hit_count, hit_before_count;
   uint64_t hit_before_mass;
-  uint64_t place;                          // the last kept token (written to every copy by rank 0)
+  uint64_t place;                                // the last kept token (written to every copy by rank 0)
 };
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -113,38 +143,31 @@ struct Weights {
   __device__ __forceinline__ double exponent(float l) const {
     return (static_cast<double>(l) - static_cast<double>(top)) * per;
   }
-  // 2^y for -46 < y <= 0, to 2^-49 of itself: y = k + j / 128 + r, 2^r by its
-  // series up to r^4 (the next term is below 2^-49), 2^(j / 128) from the
-  // table, 2^(k + 44) in the exponent; adding 2^52 leaves the nearest whole
-  // number in the low bits.  (CUDA's exp would be three times the float64
-  // operations.)
-  __device__ __forceinline__ uint64_t power(double y) const {
-    constexpr double kRound = 0x1.8p45;  // its last bit is 2^-7
-    const double t = __dadd_rn(y, kRound), r = __dadd_rn(y, -__dadd_rn(t, -kRound));
+  // The weight of a logit in (low, top]: 2^y, y = (l - top) per = k + j / 512 + r,
+  // to 2^-46 of itself: 2^r by its series up to r^3, 2^(j / 512) from the table,
+  // 2^(k + 44) in the exponent; adding 2^52 leaves the nearest whole number in
+  // the low bits.  Eight float64 operations; CUDA's exp takes three times that.
+  __device__ __forceinline__ uint64_t of(float l) const {
+    constexpr double kRound = 0x1.8p43;  // its last bit is 2^-9
+    const double d = l == top ? 0.0 : static_cast<double>(l) - static_cast<double>(top);
+    const double t = fma(d, per, kRound);
+    const double r = fma(d, per, -__dadd_rn(t, -kRound));
     const int m = __double2loint(t);
-    double q = fma(r, 0x1.3b2ab6fba4e77p-7, 0x1.c6b08d704a0c0p-5);  // ln(2)^4 / 24, ln(2)^3 / 6
-    q = fma(r, q, 0x1.ebfbdff82c58fp-3);                            // ln(2)^2 / 2
+    double q = fma(r, 0x1.c6b08d704a0c0p-5, 0x1.ebfbdff82c58fp-3);  // ln(2)^3 / 6, ln(2)^2 / 2
     q = fma(r, q, 0x1.62e42fefa39efp-1);                            // ln(2)
     q = fma(r, q, 1.0);
     const double s = root[m & (kRoots - 1)];
-    const double scaled = __hiloint2double(__double2hiint(s) + (((m >> 7) + 44) << 20), __double2loint(s));
+    const double scaled = __hiloint2double(__double2hiint(s) + (((m >> 9) + 44) << 20), __double2loint(s));
     return static_cast<uint64_t>(__double_as_longlong(fma(q, scaled, 0x1p52))) & ((1ull << 52) - 1ull);
   }
-  __device__ __forceinline__ uint64_t of(float l) const {
-    if (l == top) return kOne;
-    return l > low ? power(exponent(l)) : 0ull;
-  }
-  // Four at once, whose chains of float64 operations overlap; 0 where `on` is
-  // false or log2 of the weight (of the largest) is below `least`.
-  __device__ __forceinline__ void of4(const float (&l)[4], const bool (&on)[4], double least, uint64_t (&w)[4]) const {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool some = on[e] && (l[e] > low || l[e] == top);
-      const double y = l[e] == top ? 0.0 : exponent(l[e]);
-      w[e] = power(some ? y : 0.0);
-      if (!some || y < least) w[e] = 0ull;
-    }
-  }
+  __device__ __forceinline__ uint64_t any(float l) const { return l > low || l == top ? of(l) : 0ull; }
+};
+
+// What is kept: logits above `l`, and those equal to it up to index `index`.
+struct Cut {
+  float l;
+  int index;
+  __device__ __forceinline__ bool keeps(float x, int i) const { return x > l || (x == l && i <= index); }
 };
 
 // Exclusive prefix over the CTA's threads of (count, mass), and their totals.
@@ -176,20 +199,6 @@ __device__ __forceinline__ void scan(uint32_t &count, uint64_t &mass, uint32_t &
   mass = before_m + m - mass;
 }
 
-// Sorts s.list_at[0 .. len), a power of two up to kList, upwards.
-__device__ void sort_list(Shared &s, int len) {
-  for (int size = 2; size <= len; size <<= 1)
-    for (int gap = size >> 1; gap > 0; gap >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < len / 2; i += kThreads) {
-        const int a = 2 * i - (i & (gap - 1)), b = a + gap;  // a: the pairs' first ones, gap bit clear
-        const uint64_t x = s.list_at[a], y = s.list_at[b];
-        if ((x > y) == ((a & size) == 0)) s.list_at[a] = y, s.list_at[b] = x;
-      }
-    }
-  __syncthreads();
-}
-
 struct Settings {
   float t, top_p, min_p, u;
   int top_k;  // 0: off
@@ -201,76 +210,57 @@ __device__ __forceinline__ uint64_t drawn_at(float u, uint64_t all) {
   const double want = u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0;
   return min(all - uint64_t{1}, static_cast<uint64_t>(fmin(want, 0x1p63)));
 }
+// The units that the weights before a kept token stay below, for top-p of `all`.
+__device__ __forceinline__ uint64_t share_of(float top_p, uint64_t all) {
+  return max(uint64_t{1}, static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(all))));
+}
 
 __device__ __forceinline__ void write_row(const SampleView &p, int row, uint32_t index, float l, const Weights &weights,
-                                          float t, uint64_t all) {
+                                          uint64_t all) {
   p.tokens[row] = static_cast<int64_t>(index);
   if (p.logprobs) {
-    const double x = l == weights.top ? 0.0 : (static_cast<double>(l) - static_cast<double>(weights.top)) / static_cast<double>(t);
+    const double x = l == weights.top ? 0.0 : weights.exponent(l) * 0.6931471805599453094;
     p.logprobs[row] = static_cast<float>(x - log(static_cast<double>(all) * (1.0 / kOne)));
   }
 }
 
-// The rest of a row whose every token that may be kept is in rank 0's list, by
-// that CTA.  by_count: the list holds the first top_k, and more; else what may
-// be kept by top-p, the weights before a kept token staying below `target`.
+// The rest of a row whose every token that may be kept is among rank 0's n
+// pulled ones (n <= kFew), by that CTA, a thread a token.  by_count: they hold the
+// first top_k, and more; else what may be kept by top-p, the weights before a
+// kept token staying below `target`.  The two orders that this needs, by rank
+// for the filters and by index for the draw, come from counting what lies before.
 __device__ void draw_from_list(const SampleView &p, int row, const Settings &set, const Weights &weights, double least,
-                               bool by_count, uint64_t target, Shared &s) {
-  const int tid = threadIdx.x, n = static_cast<int>(s.list_n);
-  int len = 2;
-  while (len < n) len <<= 1;
-  for (int i = n + tid; i < len; i += kThreads) s.list_at[i] = kAll;
-  sort_list(s, len);
-  // threads take two adjacent tokens by rank
-  const int kept_n = by_count ? min(set.top_k, n) : n;
-  uint64_t at[2], w[2];
-  float l[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = 2 * tid + j;
-    at[j] = e < kept_n ? s.list_at[e] : kAll;
-    l[j] = logit_at(at[j]);
-    w[j] = e < kept_n ? weights.of(l[j]) : 0ull;
-  }
-  uint32_t none = 0, none_total;
-  uint64_t before = w[0] + w[1], total;
-  scan(none, before, none_total, total, s);
-  if (by_count)
-    target = set.top_p < 1.0f ? max(uint64_t{1}, static_cast<uint64_t>(ceil(static_cast<double>(set.top_p) * static_cast<double>(total)))) : kAll;
-  uint64_t kept[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const bool keep = before < target && (l[j] == weights.top || weights.exponent(l[j]) >= least);
-    before += w[j];
-    const int e = 2 * tid + j;
-    if (!keep) w[j] = 0ull;
-    // by index now, with the rank behind it; tokens of no weight are not drawn
-    kept[j] = w[j] != 0ull ? (static_cast<uint64_t>(index_at(at[j])) << 10) | static_cast<uint64_t>(e) : kAll;
-    if (e < len) s.list_at[e] = kept[j], s.list_w[e] = w[j];  // list_at[e] was read by this thread alone since the sort
-  }
-  sort_list(s, len);
-  uint64_t key[2], v[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = 2 * tid + j;
-    key[j] = e < len ? s.list_at[e] : kAll;
-    v[j] = key[j] != kAll ? s.list_w[key[j] & (kList - 1)] : 0ull;
-  }
-  before = v[0] + v[1];
-  scan(none, before, none_total, total, s);
-  const uint64_t drawn = drawn_at(set.u, total);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (before <= drawn && drawn < before + v[j]) {
-      s.hit_bin = static_cast<uint32_t>(key[j]) & (kList - 1);
-    }
-    before += v[j];
+                               bool by_count, uint64_t target, int n, Shared &s) {
+  const int tid = threadIdx.x;
+  if (tid < n) {
+    const uint64_t mine = s.pulled[tid];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) r += s.pulled[j] < mine;
+    s.list.at[r] = mine;
   }
   __syncthreads();
-  // the drawn token's logit, by the thread that had it by rank
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (s.hit_bin == static_cast<uint32_t>(2 * tid + j)) write_row(p, row, index_at(at[j]), l[j], weights, set.t, total);
+  const int kept_n = by_count ? min(set.top_k, n) : n;
+  const uint64_t at = tid < kept_n ? s.list.at[tid] : kAll;
+  const float l = logit_at(at);
+  uint64_t w = tid < kept_n ? weights.any(l) : 0ull;
+  uint32_t none = 0, none_total;
+  uint64_t before = w, total;
+  scan(none, before, none_total, total, s);
+  if (by_count) target = set.top_p < 1.0f ? share_of(set.top_p, total) : kAll;
+  if (!(before < target && (l == weights.top || weights.exponent(l) >= least))) w = 0ull;
+  // list.at[tid] was read by this thread alone since it was written
+  if (tid < n) s.list.at[tid] = index_at(at), s.list.w[tid] = w;
+  uint64_t sum = w;
+  scan(none, sum, none_total, total, s);
+  const uint64_t drawn = drawn_at(set.u, total);
+  if (w != 0ull) {
+    const uint32_t index = index_at(at);
+    uint64_t lower = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) lower += s.list.at[j] < index ? s.list.w[j] : 0ull;
+    if (lower <= drawn && drawn < lower + w) write_row(p, row, index, l, weights, total);
+  }
 }
 
 // One row, in a cluster of p.ctas CTAs.
@@ -283,10 +273,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
   const uint32_t rank = blockIdx.x % p.ctas;
   const uint32_t begin = rank * static_cast<uint32_t>(p.slice);
   const int n = max(0, min(p.slice, p.vocab - static_cast<int>(begin)));
-  if (tid < kRoots) s.root[tid] = exp2(static_cast<double>(tid) / kRoots);
+  static_assert(kRoots == kThreads, "a root a thread");
+  s.root[tid] = exp2(static_cast<double>(tid) / kRoots);
   if (tid == 0) s.list_n = 0u, s.best = 0xFFFFFFFFu;
+  cluster_arrive();  // this CTA is here: the others wait for it before they write into its memory
   pdl_wait();
   pdl_trigger();
+  // the row's settings
+  Settings set;
+  set.t = p.temperatures ? p.temperatures[row] : p.temperature;
+  set.top_k = p.top_ks ? p.top_ks[row] : p.top_k;
+  set.top_p = p.top_ps ? p.top_ps[row] : p.top_p;
+  set.min_p = p.min_ps ? p.min_ps[row] : p.min_p;
+  set.u = p.uniform[row];
 
   // ---- the CTA's part of the row into shared memory, with its largest and least logit ----
   constexpr int kVec = 16 / sizeof(T);
@@ -298,10 +297,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
     hi = fmaxf(hi, l);
     if (l > kMinusInf) lo = fminf(lo, l);
   };
-  const int head = min(n, (kVec - skew) % kVec), vecs = (n - head) / kVec;
-  for (int i = tid; i < head; i += kThreads) {
-    data[i] = src[i];
-    meet(logit<T>(src + i));
+  const int head = min(n, (kVec - skew) % kVec), vecs = (n - head) / kVec, tail = head + vecs * kVec;
+  if (tid < head) {
+    data[tid] = src[tid];
+    meet(logit<T>(src + tid));
   }
   const uint4 *src4 = reinterpret_cast<const uint4 *>(src + head);
   uint4 *data4 = reinterpret_cast<uint4 *>(data + head);
@@ -331,9 +330,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
     for (int j = 0; j < 4; ++j) take(v[j], v0 + j * kThreads);
   }
   for (; v0 < vecs; v0 += kThreads) take(src4[v0], v0);
-  for (int i = head + vecs * kVec + tid; i < n; i += kThreads) {
-    data[i] = src[i];
-    meet(logit<T>(src + i));
+  if (tail + tid < n) {
+    data[tail + tid] = src[tail + tid];
+    meet(logit<T>(src + tail + tid));
   }
   // every token of the part, from shared memory: f(four logits, index of the
   // first in the part); places without a token hold -infinity
@@ -352,83 +351,108 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
         f(l4, head + i * kVec + g);
       }
     }
-    const int tail = head + vecs * kVec;
     if (tail + tid < n) one(tail + tid);
   };
-  auto each = [&](auto &&f) {
-    each4([&](const float (&l)[4], int i) {
+  // groups of 2 ctas threads, so that a cluster has kGroups of them
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f(l[e], i + e);
-    });
-  };
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = 1; o < 32; o <<= 1) {
     hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
     lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+    if (o == p.ctas && lane % (2 * o) == 0) s.own_group[tid / (2 * o)] = hi;
   }
   if (lane == 0) s.warp_max[warp] = hi, s.warp_min[warp] = lo;
-  // the row's settings
-  Settings set;
-  set.t = p.temperatures ? p.temperatures[row] : p.temperature;
-  set.top_k = p.top_ks ? p.top_ks[row] : p.top_k;
-  set.top_p = p.top_ps ? p.top_ps[row] : p.top_p;
-  set.min_p = p.min_ps ? p.min_ps[row] : p.min_p;
-  set.u = p.uniform[row];
-  if (set.top_k < 0 || set.top_k >= p.vocab) set.top_k = p.vocab == 1 ? 1 : 0;
+  if (set.top_k < 0 || set.top_k >= p.vocab) set.top_k = 0;
+  const bool by_groups = set.top_k > 1 && set.top_k <= kByGroups;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kWarps; ++i) hi = fmaxf(hi, s.warp_max[i]), lo = fminf(lo, s.warp_min[i]);
-    s.row_max = hi;
-    s.row_min = lo;
+  cluster_wait();
+  if (by_groups && tid < kGroups) {
+    const int each = kGroups / p.ctas;
+    at_rank(&s, tid / each)->group[rank * each + tid % each] = s.own_group[tid % each];
+  }
+  if (warp == 0) {
+    hi = s.warp_max[lane % kWarps], lo = s.warp_min[lane % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+      lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+    }
+    if (lane < p.ctas) {
+      Shared *o = at_rank(&s, lane);
+      o->rank_max[rank] = hi;
+      o->rank_min[rank] = lo;
+    }
   }
   cluster_barrier();
   hi = kMinusInf, lo = -kMinusInf;
   for (int r = 0; r < p.ctas; ++r) {
-    hi = fmaxf(hi, at_rank(&s, r)->row_max);
-    lo = fminf(lo, at_rank(&s, r)->row_min);
+    hi = fmaxf(hi, s.rank_max[r]);
+    lo = fminf(lo, s.rank_min[r]);
   }
-  const Weights weights{hi, __fsub_rd(hi, __fmul_ru(set.t, 31.54f)), 1.4426950408889634074 / static_cast<double>(set.t), s.root};
   // the largest logit: asked for, or all that there is
   if (!(set.t > 0.0f) || set.top_k == 1 || !(set.top_p > 0.0f) || !(hi > kMinusInf)) {
     uint32_t best = 0xFFFFFFFFu;
     if (hi > kMinusInf)
-      each([&](float l, int i) {
-        if (l == hi) best = min(best, begin + static_cast<uint32_t>(i));
+      each4([&](const float (&l)[4], int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (l[e] == hi) best = min(best, begin + static_cast<uint32_t>(i + e));
       });
     best = __reduce_min_sync(0xFFFFFFFFu, best);
-    if (lane == 0 && best != 0xFFFFFFFFu) atomicMin(&s.best, best);
+    if (lane == 0 && best != 0xFFFFFFFFu) atomicMin(&at_rank(&s, 0)->best, best);
     cluster_barrier();
     if (rank == 0 && tid == 0) {
-      for (int r = 0; r < p.ctas; ++r) best = min(best, at_rank(&s, r)->best);
-      p.tokens[row] = best == 0xFFFFFFFFu ? -1 : static_cast<int64_t>(best);
+      p.tokens[row] = s.best == 0xFFFFFFFFu ? -1 : static_cast<int64_t>(s.best);
       if (p.logprobs) p.logprobs[row] = 0.0f;
     }
-    cluster_barrier();
     return;
   }
+  const Weights weights{hi, hi < -kMinusInf ? __fsub_rd(hi, __fmul_ru(set.t, 31.54f)) : hi, 1.4426950408889634074 / static_cast<double>(set.t), s.root};
   const double least = set.min_p > 0.0f ? log2(static_cast<double>(fminf(set.min_p, 1.0f))) : -1e300;
 
   // ---- the place of the last kept token ----
-  float cut = kMinusInf;  // its logit and its index: so far every token that is not masked
-  int cut_index = -1;
-  auto kept = [&](float l, int i) { return l > cut || (l == cut && static_cast<int>(begin) + i <= cut_index); };
-  // Tokens up to there: the first set.top_k of them, or (by_mass)
-  // those before whose place less than set.top_p of their weights lies.  True:
-  // every token that may be kept went to rank 0's list instead.
+  Cut cut{kMinusInf, -1};  // so far every token that is not masked
+  // of the tokens that `c` keeps, those that weigh something
+  auto weighing = [&](Cut c) {
+    if (weights.low >= hi) return c.l < hi ? Cut{hi, kEvery} : c;
+    return weights.low >= c.l ? Cut{weights.low, -1} : c;
+  };
+  auto append = [&](uint64_t at, uint64_t w) {
+    const uint32_t k = atomicAdd(&s.list_n, 1u);
+    if (k < kList) s.list.at[k] = at, s.list.w[k] = w;
+  };
+  // The number of tokens in the cluster's lists.
+  auto listed = [&]() {
+    __syncthreads();
+    if (tid < p.ctas) at_rank(&s, tid)->rank_list[rank] = s.list_n;
+    cluster_barrier();
+    uint32_t all = 0;
+    for (int r = 0; r < p.ctas; ++r) all += s.rank_list[r];
+    return all;
+  };
+  // Rank 0 takes them, up to kList.
+  auto pull = [&]() {
+    int from = 0, r = 0;
+    for (int i = tid; i < kList; i += kThreads) {
+      while (r < p.ctas && i >= from + static_cast<int>(s.rank_list[r])) from += static_cast<int>(s.rank_list[r++]);
+      if (r == p.ctas) break;
+      const Shared *o = at_rank(&s, r);
+      s.pulled[i] = o->list.at[i - from];
+      s.pulled_w[i] = o->list.w[i - from];
+    }
+    __syncthreads();
+  };
+  // Tokens up to there: the first set.top_k of them, or (by_mass) those before
+  // whose place less than set.top_p of their weights lies.  Not 0: every token
+  // that may be kept is in the cluster's lists instead, so many of them.
   auto narrow = [&](const bool by_mass, uint64_t &target) {
     const uint32_t want = static_cast<uint32_t>(set.top_k);
+    const Cut among = by_mass ? weighing(cut) : cut;
     // ranges of the first round: equal parts of the logits that can matter
     float span = __fsub_rn(hi, lo);
     if (by_mass) span = fminf(span, __fsub_rn(hi, weights.low));
     const float per = span > 0.0f ? __fdiv_rn(static_cast<float>(kBins), span) : 0.0f;
     auto range_of = [&](float l) {  // rises (weakly) with falling logits
-      const int b = static_cast<int>(__fmul_rn(__fsub_rn(hi, l), per));
-      return static_cast<uint32_t>(min(max(b, 0), kBins - 1));
-    };
-    auto append = [&](uint64_t at, uint64_t w) {
-      Shared *o = at_rank(&s, 0);
-      const uint32_t k = atomicAdd(&o->list_n, 1u);
-      if (k < kList) o->list_at[k] = at, o->list_w[k] = w;
+      return static_cast<uint32_t>(min(max(static_cast<int>(__fmul_rn(__fsub_rn(hi, l), per)), 0), kBins - 1));
     };
     uint32_t range = 0;   // chosen in the first round
     uint64_t prefix = 0;  // of (logit, index), chosen in later rounds
@@ -447,54 +471,67 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
       for (int b = tid; b < kBins; b += kThreads) s.count[b] = 0u, s.mass_lo[b] = 0u, s.mass_hi[b] = 0u;
       __syncthreads();
       each4([&](const float (&l)[4], int i) {
-        bool on[4];
         uint32_t b[4];
+        uint64_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          on[e] = kept(l[e], i + e);
-          b[e] = on[e] ? bin_of(l[e], i + e) : kBins;
-          on[e] = b[e] < kBins;
+          b[e] = among.keeps(l[e], static_cast<int>(begin) + i + e) ? bin_of(l[e], i + e) : kBins;
+          if (by_mass) w[e] = weights.of(b[e] < kBins ? l[e] : hi);
         }
-        if (by_mass) {
-          uint64_t w[4];
-          weights.of4(l, on, -1e300, w);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (w[e] == 0ull) continue;
-            atomicAdd(&s.count[b[e]], 1u);
+        for (int e = 0; e < 4; ++e) {
+          if (b[e] >= kBins) continue;
+          atomicAdd(&s.count[b[e]], 1u);
+          if (by_mass) {
             const uint32_t low = static_cast<uint32_t>(w[e]), was = atomicAdd(&s.mass_lo[b[e]], low);
             const uint32_t high = static_cast<uint32_t>(w[e] >> 32) + (was + low < was ? 1u : 0u);
             if (high) atomicAdd(&s.mass_hi[b[e]], high);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (on[e]) atomicAdd(&s.count[b[e]], 1u);
         }
       });
-      cluster_barrier();
-      // the cluster's histogram, two bins a thread, summed by every CTA for itself
-      uint32_t c[2] = {0u, 0u};
-      uint64_t m[2] = {0ull, 0ull};
-      for (int r = 0; r < p.ctas; ++r) {
-        const Shared *o = at_rank(&s, r);
-        const uint2 k = reinterpret_cast<const uint2 *>(o->count)[tid];
-        c[0] += k.x, c[1] += k.y;
-        if (by_mass) {
-          const uint2 a = reinterpret_cast<const uint2 *>(o->mass_lo)[tid], b = reinterpret_cast<const uint2 *>(o->mass_hi)[tid];
-          m[0] += a.x + (static_cast<uint64_t>(b.x) << 32), m[1] += a.y + (static_cast<uint64_t>(b.y) << 32);
+      // The cluster's histogram, two bins a thread.  Each CTA sums its share of
+      // the bins, ctas / 2 threads a bin and two CTAs a thread, and writes the
+      // sums to all (every CTA reading all bins of all took 3 to 9 us at 16 CTAs).
+      uint32_t c[2];
+      uint64_t m[2];
+      if (p.ctas == 1) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          c[j] = s.count[2 * tid + j];
+          m[j] = s.mass_lo[2 * tid + j] + (static_cast<uint64_t>(s.mass_hi[2 * tid + j]) << 32);
         }
+      } else {
+        cluster_barrier();
+        const int team = p.ctas / 2, bin = static_cast<int>(rank) * (kBins / p.ctas) + tid / team, r0 = tid % team * 2;
+        uint32_t sum_c = 0;
+        uint64_t sum_m = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const Shared *o = at_rank(&s, r0 + j);
+          sum_c += o->count[bin];
+          if (by_mass) sum_m += o->mass_lo[bin] + (static_cast<uint64_t>(o->mass_hi[bin]) << 32);
+        }
+        for (int o = 1; o < team; o <<= 1) {
+          sum_c += __shfl_xor_sync(0xFFFFFFFFu, sum_c, o);
+          sum_m += __shfl_xor_sync(0xFFFFFFFFu, sum_m, o);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          Shared *o = at_rank(&s, r0 + j);
+          o->sum.count[bin] = sum_c;
+          o->sum.mass[bin] = sum_m;
+        }
+        cluster_barrier();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c[j] = s.sum.count[2 * tid + j], m[j] = s.sum.mass[2 * tid + j];
       }
       uint32_t cum_c = c[0] + c[1], all_c;
       uint64_t cum_m = m[0] + m[1], all_m;
       scan(cum_c, cum_m, all_c, all_m, s);
       if (round == 0) {
-        if (!by_mass && all_c <= want) {
-          cluster_barrier();  // the histograms are read before they are cleared again
-          return false;       // no more tokens than that: all stay
-        }
-        // mass before < top_p * all, in whole units: < ceil(top_p * all); at least one token
-        if (by_mass) target = max(uint64_t{1}, static_cast<uint64_t>(ceil(static_cast<double>(set.top_p) * static_cast<double>(all_m))));
+        if (!by_mass && all_c <= want) return 0;  // no more tokens than that: all stay
+        if (by_mass) target = share_of(set.top_p, all_m);
       }
       cum_c += before_count;
       cum_m += before_mass;
@@ -513,110 +550,176 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
       const uint32_t bin = s.hit_bin, inside = s.hit_count;
       before_count = s.hit_before_count;
       before_mass = s.hit_before_mass;
-      if (round == 0 && before_count + inside <= kList) {
-        each([&](float l, int i) {
-          if (kept(l, i) && range_of(l) <= bin && (!by_mass || weights.of(l) != 0ull))
-            append(place_of(l, begin + static_cast<uint32_t>(i)), 0ull);
+      const bool all_of_it = round == 0 && before_count + inside <= kFew;  // the ranges above as well
+      if (all_of_it || inside <= kList) {
+        each4([&](const float (&l)[4], int i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (!among.keeps(l[e], static_cast<int>(begin) + i + e)) continue;
+            if (all_of_it ? range_of(l[e]) > bin : bin_of(l[e], i + e) != bin) continue;
+            append(place_of(l[e], begin + static_cast<uint32_t>(i + e)), by_mass && !all_of_it ? weights.of(l[e]) : 0ull);
+          }
         });
-        cluster_barrier();
-        return true;
-      }
-      if (inside <= kList) {
-        each([&](float l, int i) {
-          if (!kept(l, i) || bin_of(l, i) != bin) return;
-          const uint64_t w = by_mass ? weights.of(l) : 0ull;
-          if (!by_mass || w != 0ull) append(place_of(l, begin + static_cast<uint32_t>(i)), w);
-        });
-        cluster_barrier();
+        const int all = static_cast<int>(listed());
+        if (all_of_it) return all;
         if (rank == 0) {
-          const int len = static_cast<int>(min(s.list_n, static_cast<uint32_t>(kList)));
-          for (int i = tid; i < len; i += kThreads) {
-            const uint64_t at = s.list_at[i], w = s.list_w[i];
+          pull();
+          if (tid < all) {
+            const uint64_t at = s.pulled[tid], w = s.pulled_w[tid];
             uint32_t c0 = before_count;
             uint64_t m0 = before_mass;
-            for (int j = 0; j < len; ++j)
-              if (s.list_at[j] < at) ++c0, m0 += s.list_w[j];
+            for (int j = 0; j < all; ++j)
+              if (s.pulled[j] < at) ++c0, m0 += s.pulled_w[j];
             if (by_mass ? (m0 < target && target <= m0 + w) : (c0 + 1u == want))
               for (int r = 0; r < p.ctas; ++r) at_rank(&s, r)->place = at;
           }
-          __syncthreads();
-          if (tid == 0) s.list_n = 0u;
         }
+        if (tid == 0) s.list_n = 0u;
         cluster_barrier();
-        cut = logit_at(s.place);
-        cut_index = static_cast<int>(index_at(s.place));
-        return false;
+        cut = Cut{logit_at(s.place), static_cast<int>(index_at(s.place))};
+        return 0;
       }
-      cluster_barrier();  // the histograms are read before they are cleared again
+      __syncthreads();  // hit_bin was read
       if (round == 0) range = bin, prefix = 0;
       else prefix = (prefix << 10) | bin;
     }
   };
   uint64_t target = 0;
-  const bool by_count = set.top_k > 0 && narrow(false, target);
-  if (by_count || (set.top_p < 1.0f && narrow(true, target))) {
-    if (rank == 0) draw_from_list(p, row, set, weights, least, by_count, target, s);
-    return;  // nobody reads the others' shared memory any more
+  int few = 0;
+  bool by_count = set.top_k > 0;
+  if (by_groups) {
+    // The top_k-th largest of the groups' maxima is at most the top_k-th largest
+    // logit: what is no less holds the first top_k, and seldom many more.
+    if (tid < kGroups) {
+      const float v = s.group[tid];
+      int above = 0;
+#pragma unroll 8
+      for (int j = 0; j < kGroups; ++j) {
+        const float o = s.group[j];
+        above += o > v || (o == v && j < tid);
+      }
+      if (above == set.top_k - 1) s.bound = v;
+    }
+    __syncthreads();
+    const float bound = s.bound;
+    if (bound > kMinusInf) {
+      each4([&](const float (&l)[4], int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (l[e] >= bound) append(place_of(l[e], begin + static_cast<uint32_t>(i + e)), 0ull);
+      });
+      const uint32_t all = listed();
+      if (all <= kFew) few = static_cast<int>(all);
+      else if (tid == 0) s.list_n = 0u;
+    }
+  }
+  if (few == 0 && by_count) few = narrow(false, target);
+  if (few == 0 && set.top_p < 1.0f) by_count = false, few = narrow(true, target);
+  if (few != 0) {
+    if (rank != 0) {
+      cluster_barrier();  // rank 0 has read this CTA's list
+      return;
+    }
+    pull();
+    cluster_arrive();
+    draw_from_list(p, row, set, weights, least, by_count, target, few, s);
+    cluster_wait();
+    return;
   }
 
-  // ---- the draw: weights of adjacent tokens, walked by index ----
-  const int per = ((n + kThreads - 1) / kThreads) | 1;  // odd: threads start in different banks
-  const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
-  auto weigh = [&](int i, uint64_t (&w)[4]) {  // four tokens from i on, none from i1 on
-    float l[4];
-    bool on[4], some = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      l[e] = i + e < i1 ? logit<T>(data + i + e) : kMinusInf;
-      on[e] = kept(l[e], i + e);
-      some |= on[e];
-      w[e] = 0ull;
+  // ---- the draw: kept weights summed block by block, and walked by index in the block drawn ----
+  if (set.min_p > 0.0f) {
+    // the least logit whose weight is min_p or more: by the formula's inverse,
+    // then exactly among its neighbours
+    const float guess = static_cast<float>(static_cast<double>(hi) + least / weights.per);
+    float l = hi;
+#pragma unroll 1
+    for (int step = 4; step >= -4; --step) {
+      const uint32_t up = static_cast<uint32_t>(~(place_of(guess, 0) >> kIndexBits)) + static_cast<uint32_t>(step);
+      const float x = __uint_as_float((up & 0x80000000u) ? up & 0x7FFFFFFFu : ~up);
+      if (x <= hi && weights.exponent(x) >= least) l = fminf(l, x);
     }
-    if (some) weights.of4(l, on, least, w);
-  };
-  uint64_t sum = 0, w4[4];
-  for (int i = i0; i < i1; i += 4) {
-    weigh(i, w4);
-    sum += (w4[0] + w4[1]) + (w4[2] + w4[3]);
+    if (l > cut.l) cut = Cut{l, kEvery};
   }
+  const Cut kept = weighing(cut);
+  const int blocks = (n + kBlock - 1) / kBlock;
+  for (int b = warp; b < blocks; b += kWarps) {
+    uint64_t sum = 0;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      // the kept logits side by side, in any order, so that every lane has work
+      const int i0 = b * kBlock + part * (kBlock / 2) + lane;
+      float *pack = s.pack[warp];
+      int m = 0;
+#pragma unroll
+      for (int e = 0; e < kBlock / 64; ++e) {
+        const int i = i0 + 32 * e;
+        const float l = i < n ? logit<T>(data + i) : kMinusInf;
+        const bool on = kept.keeps(l, static_cast<int>(begin) + i);
+        const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
+        if (on) pack[m + __popc(who & ((1u << lane) - 1u))] = l;
+        m += __popc(who);
+      }
+      __syncwarp();
+      for (int j = lane; j < m; j += 128) {
+        uint64_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = weights.of(j + 32 * e < m ? pack[j + 32 * e] : hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += j + 32 * e < m ? w[e] : 0ull;
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == 0) s.block_mass[b] = sum;
+  }
+  __syncthreads();
+  const uint64_t mine = tid < blocks ? s.block_mass[tid] : 0ull;
   uint32_t none = 0, none_total;
-  uint64_t before = sum, total;
+  uint64_t before = mine, total;
   scan(none, before, none_total, total, s);
-  if (tid == 0) s.part_mass = total;
+  if (tid < p.ctas) at_rank(&s, tid)->rank_mass[rank] = total;
   cluster_barrier();
   uint64_t all = 0, base = 0;
   for (int r = 0; r < p.ctas; ++r) {
     if (r == static_cast<int>(rank)) base = all;
-    all += at_rank(&s, r)->part_mass;
+    all += s.rank_mass[r];
   }
   const uint64_t drawn = drawn_at(set.u, all);
+  if (drawn < base || drawn >= base + total) return;
   before += base;
-  if (before <= drawn && drawn < before + sum) {
-    for (int i = i0; i < i1 && before <= drawn; i += 4) {
-      weigh(i, w4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (before <= drawn && drawn < before + w4[e])
-          write_row(p, row, begin + static_cast<uint32_t>(i + e), logit<T>(data + i + e), weights, set.t, all);
-        before += w4[e];
-      }
-    }
-  }
-  cluster_barrier();  // no CTA ends while another reads its sums
+  if (before <= drawn && drawn < before + mine) s.hit_bin = static_cast<uint32_t>(tid), s.hit_before_mass = before;
+  __syncthreads();
+  const int i = static_cast<int>(s.hit_bin) * kBlock + tid;  // a token a thread
+  static_assert(kBlock == kThreads, "the block drawn is walked a token a thread");
+  const float l = i < n ? logit<T>(data + i) : kMinusInf;
+  const bool on = kept.keeps(l, static_cast<int>(begin) + i);
+  const uint64_t w = on ? weights.of(l) : 0ull, first = s.hit_before_mass;
+  before = w;
+  scan(none, before, none_total, total, s);
+  before += first;
+  if (before <= drawn && drawn < before + w) write_row(p, row, begin + static_cast<uint32_t>(i), l, weights, all);
 }
 
 template <typename T>
 cudaError_t launch(SampleView p, int rows, int sms, cudaStream_t s) {
-  // A row's part in a CTA's shared memory lets two CTAs share an SM, down to
-  // 4096 tokens a CTA while there are SMs without one.
-  constexpr int kMost = 96 * 1024 / sizeof(T);
-  p.ctas = 1;
-  while (p.ctas < 8 && ((p.vocab + p.ctas - 1) / p.ctas > kMost ||
-                        (static_cast<int64_t>(rows) * p.ctas < 2 * sms && p.vocab / p.ctas >= 2 * 4096)))
-    p.ctas *= 2;
+  // CTAs of a row: as many as finish soonest, by rounds over the SMs (two CTAs
+  // each) times a CTA's tokens and about 8000 tokens' time for its barriers.
+  constexpr int kMost = 72 * 1024 / sizeof(T);  // tokens that leave room for a second CTA
+  constexpr int64_t kFixed = 8000;
+  int64_t least = INT64_MAX;
+  for (int c = 1; c <= kMaxCtas; c *= 2) {
+    const int64_t slice = (p.vocab + c - 1) / c;
+    if (slice > kMaxBlocks * kBlock || slice * sizeof(T) > 160 * 1024) continue;
+    const int64_t slots = static_cast<int64_t>(sms) * (slice > kMost ? 1 : 2);
+    const int64_t time = (static_cast<int64_t>(rows) * c + slots - 1) / slots * (slice + kFixed);
+    if (time < least) least = time, p.ctas = c;
+  }
   p.slice = (p.vocab + p.ctas - 1) / p.ctas;
   const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + 16 + static_cast<size_t>(p.slice) * sizeof(T);
   cudaError_t e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess && p.ctas > 8) e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * static_cast<unsigned>(p.ctas));
