@@ -12,6 +12,9 @@
 // are float32; y and the carried residual are rounded once, from float32 (the
 // norm sees the unrounded sum, so rounding the carried residual costs it
 // nothing).
+//
+// Bound by HBM, and by the latency of a row's chain (load, sum, store): CTAs stay
+// on their SM and ask for the rows two rounds ahead.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
@@ -21,6 +24,7 @@
 
 #include "common.cuh"
 #include "dense.cuh"
+#include "moe_kernels.cuh"
 
 namespace fnmoe {
 namespace {
@@ -38,15 +42,17 @@ struct NormView {
   int64_t rows;
   int dim;
   float eps, offset;  // offset: 1 where the weight is kept as w - 1
-  bool w_f32, norm, e4m3;
+  bool w_f32, w_vec, norm, e4m3;  // w_vec: the weight starts on a 16-byte boundary
 };
 
-// 8 values of a row.  VEC: columns 8 (c G + t) .. + 7 in one or two 16-byte
-// accesses; else columns (8 c + e) G + t, one by one but coalesced.
-template <bool VEC>
-__device__ __forceinline__ int column(int c, int e, int G, int t) {
-  return VEC ? (c * G + t) * 8 + e : (c * 8 + e) * G + t;
-}
+// How a row's values are dealt to its G threads, 8 to a thread's chunk:
+//   kEven  columns 8 q .. + 7 of chunk q, in 16-byte accesses: rows and widths on
+//          boundaries of 8 values;
+//   kFlat  the same over the rows laid end to end, for rows of any width that
+//          are contiguous: chunk q starts on the boundary of 8 at or below the
+//          row's start, chunks that reach into a neighbour's row are masked;
+//   kOdd   columns (8 c + e) G + t, one value at a time: any stride and start.
+enum Deal { kEven, kFlat, kOdd };
 
 template <typename T>
 __device__ __forceinline__ float widen(T v);
@@ -61,252 +67,461 @@ __device__ __forceinline__ uint16_t narrow<uint16_t>(float v) { return f32_to_bf
 template <>
 __device__ __forceinline__ float narrow<float>(float v) { return v; }
 
-template <bool VEC, typename T>
-__device__ __forceinline__ void load8(const T *row, int c, int G, int t, int dim, float (&v)[8]) {
-  if constexpr (VEC) {
-    const int at = column<true>(c, 0, G, t);
-    if (at >= dim) {
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 8 adjacent values to a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_eight(T *to, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4 *>(to) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  } else {
+    reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// Codes of four values whose magnitudes are at most 127 (448): int8 by adding
+// 1.5 2^23, whose last bit is 1, so that the sum's low byte is the nearest whole
+// number (ties to even) in two's complement.
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, bool e4m3) {
+  if (e4m3) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(d), "f"(c));
+    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+  }
+  constexpr float kWhole = 0x1.8p23f;
+  const uint32_t ab = __byte_perm(__float_as_uint(__fadd_rn(a, kWhole)), __float_as_uint(__fadd_rn(b, kWhole)), 0x0040);
+  const uint32_t cd = __byte_perm(__float_as_uint(__fadd_rn(c, kWhole)), __float_as_uint(__fadd_rn(d, kWhole)), 0x0040);
+  return __byte_perm(ab, cd, 0x5410);
+}
+
+// A row's values and where this thread's chunks of them lie.
+struct RowAt {
+  int64_t row;
+  int skew;  // kFlat: values before the row in its first chunk
+};
+struct Columns {
+  int G, t, dim;
+  int64_t total;  // values of all rows
+  template <Deal D>
+  __device__ __forceinline__ RowAt at(int64_t row) const {
+    return RowAt{row, D == kFlat ? static_cast<int>(static_cast<uint64_t>(row) * static_cast<uint32_t>(dim) & 7u) : 0};
+  }
+  // the column of value e of chunk c; below 0 or from dim on where there is none
+  template <Deal D>
+  __device__ __forceinline__ int column(const RowAt &r, int c, int e) const {
+    return D == kOdd ? (c * 8 + e) * G + t : (c * G + t) * 8 + e - r.skew;
+  }
+  // whether chunk c lies in the row whole; whether any of it does
+  template <Deal D>
+  __device__ __forceinline__ bool whole(const RowAt &r, int c) const {
+    const int first = column<D>(r, c, 0);
+    return first >= 0 && first + 8 <= dim;
+  }
+  template <Deal D>
+  __device__ __forceinline__ bool some(const RowAt &r, int c) const { return column<D>(r, c, 0) < dim; }
+};
+
+// 8 values as they were loaded.
+template <Deal D, typename T>
+struct Raw8 {
+  union {
+    uint4 q[sizeof(T) / 2];
+    T v[8];
+  };
+  __device__ __forceinline__ void load(const T *x, uint64_t stride, const Columns &k, const RowAt &r, int c) {
+    const T *row = x + r.row * stride;
+    if constexpr (D == kOdd) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      for (int e = 0; e < 8; ++e) {
+        const int at = k.column<D>(r, c, e);
+        v[e] = at < k.dim ? row[at] : T(0);
+      }
+    } else {
+      const int first = k.column<D>(r, c, 0);
+      if (first < k.dim && (D == kEven || r.row * k.dim + first + 8 <= k.total)) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) q[i] = reinterpret_cast<const uint4 *>(row + first)[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) q[i] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (D == kFlat) {  // the last values of all
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (first + e < k.dim) put(e, row[first + e]);
+        }
+      }
+      if constexpr (D == kFlat) {
+        if (!k.whole<D>(r, c)) {  // a neighbour's values do not count
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (first + e < 0 || first + e >= k.dim) put(e, T(0));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(int e, T x) {
+    uint32_t *w = &q[sizeof(T) == 2 ? 0 : e / 4].x;
+    if constexpr (sizeof(T) == 4) {
+      w[e % 4] = __float_as_uint(x);
+    } else {
+      w[e / 2] = (e & 1) ? (w[e / 2] & 0xFFFFu) | (static_cast<uint32_t>(x) << 16) : (w[e / 2] & 0xFFFF0000u) | x;
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (D == kOdd) {
+      return widen<T>(v[e]);
     } else if constexpr (sizeof(T) == 2) {
-      const uint4 q = *reinterpret_cast<const uint4 *>(row + at);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float((e & 1) ? (w[e / 2] & 0xFFFF0000u) : (w[e / 2] << 16));
+      const uint32_t w = e < 2 ? q[0].x : e < 4 ? q[0].y : e < 6 ? q[0].z : q[0].w;
+      return __uint_as_float((e & 1) ? (w & 0xFFFF0000u) : (w << 16));
     } else {
-      const float4 a = *reinterpret_cast<const float4 *>(row + at), b = *reinterpret_cast<const float4 *>(row + at + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      const uint4 w = q[e / 4];
+      return __uint_as_float(e % 4 == 0 ? w.x : e % 4 == 1 ? w.y : e % 4 == 2 ? w.z : w.w);
     }
-  } else {
+  }
+};
+
+// 8 values of chunk c to contiguous rows at `to`.
+template <Deal D, typename T>
+__device__ __forceinline__ void store8(T *to, const Columns &k, const RowAt &r, int c, const float (&v)[8]) {
+  T *row = to + r.row * k.dim;
+  if (D != kOdd && k.whole<D>(r, c)) {
+    store_eight(row + k.column<D>(r, c, 0), v);
+  } else if (D != kEven) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int at = column<false>(c, e, G, t);
-      v[e] = at < dim ? widen<T>(row[at]) : 0.0f;
+      const int at = k.column<D>(r, c, e);
+      if (at >= 0 && at < k.dim) row[at] = narrow<T>(v[e]);
     }
   }
 }
 
-template <bool VEC, typename T>
-__device__ __forceinline__ void store8(T *row, int c, int G, int t, int dim, const float (&v)[8]) {
-  if constexpr (VEC) {
-    const int at = column<true>(c, 0, G, t);
-    if (at >= dim) return;
-    if constexpr (sizeof(T) == 2) {
-      uint32_t w[4];
+template <Deal D>
+__device__ __forceinline__ void store_codes(uint8_t *to, const Columns &k, const RowAt &r, int c, const float (&v)[8],
+                                            bool bad, bool e4m3) {
+  if (!k.some<D>(r, c)) return;
+  uint8_t *row = to + r.row * k.dim;
+  uint32_t w[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = static_cast<uint32_t>(f32_to_bf16(v[2 * e])) | (static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16);
-      *reinterpret_cast<uint4 *>(row + at) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      *reinterpret_cast<float4 *>(row + at) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4 *>(row + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  } else {
+  for (int h = 0; h < 2; ++h) w[h] = bad ? 0u : four_codes(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3], e4m3);
+  if (D != kOdd && k.whole<D>(r, c)) {
+    *reinterpret_cast<uint2 *>(row + k.column<D>(r, c, 0)) = make_uint2(w[0], w[1]);
+  } else if (D != kEven) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int at = column<false>(c, e, G, t);
-      if (at < dim) row[at] = narrow<T>(v[e]);
+      const int at = k.column<D>(r, c, e);
+      if (at >= 0 && at < k.dim) row[at] = static_cast<uint8_t>(w[e / 4] >> (8 * (e % 4)));
     }
   }
 }
 
-__device__ __forceinline__ uint8_t code_of(float v, bool e4m3) {
-  if (e4m3) return static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
-  return static_cast<uint8_t>(max(-127, min(127, __float2int_rn(v))));
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t *row, int c, int G, int t, int dim, const float (&v)[8], bool e4m3) {
-  if constexpr (VEC) {
-    const int at = column<true>(c, 0, G, t);
-    if (at >= dim) return;
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e / 4] |= static_cast<uint32_t>(code_of(v[e], e4m3)) << (8 * (e & 3));
-    *reinterpret_cast<uint2 *>(row + at) = make_uint2(w[0], w[1]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = column<false>(c, e, G, t);
-      if (at < dim) row[at] = code_of(v[e], e4m3);
-    }
-  }
-}
-
-// Sum of `sum` and maximum of `top` over the G threads of a row (all threads
-// of the CTA call it together; `part` has two words a warp).
-__device__ __forceinline__ void reduce_row(float &sum, uint32_t &top, int G, float2 *part) {
+// Sum of `sum` and maximum of `top` (which is not negative) over the G threads of
+// a row: a warp, or the CTA, whose warps meet in `part` (two of them in turn, so
+// that one barrier is enough).
+__device__ __forceinline__ void reduce_row(float &sum, float &top, int G, float2 *part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
   if (G == 32) return;
-  const int warp = threadIdx.x >> 5, per = G >> 5, first = warp / per * per;
-  __syncthreads();  // a second reduction does not overtake the first one's reads
-  if ((threadIdx.x & 31) == 0) part[warp] = make_float2(sum, __uint_as_float(top));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(sum, top);
   __syncthreads();
   sum = 0.0f;
-  top = 0u;
-  for (int i = first; i < first + per; ++i) {
-    sum += part[i].x;
-    top = max(top, __float_as_uint(part[i].y));
+#pragma unroll 4
+  for (int i = 0; i < G >> 5; ++i) {
+    const float2 o = part[i];
+    sum += o.x;
+    top = fmaxf(top, o.y);
   }
 }
 
-// One row per G threads; a CTA holds blockDim.x / G rows.  TR void: no residual.
-template <bool VEC, int VPT, typename TX, typename TR>
-__global__ void __launch_bounds__(512) k_norm(NormView p, int G) {
-  __shared__ float2 part[16];
-  const int t = threadIdx.x % G;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / G) + threadIdx.x / G;
-  const bool live = row < p.rows;  // threads past the last row only keep the barriers company
+// Rows by G threads each: a warp (four of them a CTA) or a CTA.  TR void: no residual.
+template <Deal D, int VPT, typename TX, typename TR>
+__global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int G) {
+  constexpr bool kRes = !std::is_void_v<TR>;
+  constexpr int kAhead = VPT == 1 && D != kOdd ? 2 : 1;  // rows whose loads are under way
+  using R = std::conditional_t<kRes, TR, TX>;
+  __shared__ float2 part[2][16];
+  extern __shared__ __align__(16) float weight[];
+  const Columns k{G, static_cast<int>(threadIdx.x) % G, p.dim, p.rows * p.dim};
+  const int rows_here = blockDim.x / G;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * rows_here;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * rows_here + threadIdx.x / G;
   pdl_wait();
   pdl_trigger();
-  float s[VPT][8];
+  Raw8<D, TX> x[kAhead][VPT];
+  Raw8<D, R> r[kAhead][kRes ? VPT : 1];
+  auto ask = [&](int a, int64_t at) {
+    if (at >= p.rows) return;
+    const RowAt ra = k.at<D>(at);
 #pragma unroll
-  for (int c = 0; c < VPT; ++c)
+    for (int c = 0; c < VPT; ++c) x[a][c].load(static_cast<const TX *>(p.x), p.x_stride, k, ra, c);
+    if constexpr (kRes) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[c][e] = 0.0f;
-  if (live) {
-    const TX *x = static_cast<const TX *>(p.x) + row * p.x_stride;
+      for (int c = 0; c < VPT; ++c) r[a][c].load(static_cast<const R *>(p.res), p.res_stride, k, ra, c);
+    }
+  };
 #pragma unroll
-    for (int c = 0; c < VPT; ++c) load8<VEC>(x, c, G, t, p.dim, s[c]);
-    if constexpr (!std::is_void_v<TR>) {
-      const TR *r = static_cast<const TR *>(p.res) + row * p.res_stride;
-      float add[VPT][8];
+  for (int a = 0; a < kAhead; ++a) ask(a, row + a * step);
+  // Weights.  kEven: a thread's columns are the same in every row, so it reads
+  // them each time, from L1.  Otherwise from shared memory; kFlat: value i at
+  // (i % 8) pitch + i / 8, so that threads that read value e of adjacent chunks
+  // read adjacent words whatever the skew.
+  const int pitch = p.dim / 8 + 1;
+  auto weight_at = [&](int i) {
+    return __fadd_rn(p.w_f32 ? static_cast<const float *>(p.w)[i] : bf16_to_f32(static_cast<const uint16_t *>(p.w)[i]), p.offset);
+  };
+  if (D != kEven && p.norm) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.dim; i += blockDim.x) weight[D == kFlat ? (i & 7) * pitch + (i >> 3) : i] = weight_at(i);
+    __syncthreads();
+  }
+  // this thread's weights of chunk c (where there is no value: anything, it counts as 0)
+  auto weights = [&](const RowAt &ra, int c, float (&w)[8]) {
+    if (!p.norm) {
 #pragma unroll
-      for (int c = 0; c < VPT; ++c) load8<VEC>(r, c, G, t, p.dim, add[c]);
+      for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+    } else if constexpr (D == kEven) {
+      const int at = min(k.column<D>(ra, c, 0), p.dim - 8);
+      if (!p.w_vec) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = weight_at(at + e);
+      } else if (p.w_f32) {
+        const float4 *g = reinterpret_cast<const float4 *>(static_cast<const float *>(p.w) + at);
+        const float4 a = g[0], b = g[1];
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+      } else {
+        const uint4 q = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.w) + at);
+        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __uint_as_float((e & 1) ? (v[e / 2] & 0xFFFF0000u) : (v[e / 2] << 16));
+      }
+      if (p.w_vec && p.offset != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __fadd_rn(w[e], p.offset);
+      }
+    } else if constexpr (D == kFlat) {
+      const float *at = weight + min(c * G + k.t, pitch - 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = at[((e - ra.skew) & 7) * pitch - (e < ra.skew ? 1 : 0)];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = weight[min(k.column<D>(ra, c, e), p.dim - 1)];
+    }
+  };
+  const float limit = p.e4m3 ? 448.0f : 127.0f, per_dim = 1.0f / static_cast<float>(p.dim);
+  int turn = 0;
+  while (row < p.rows) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a, row += step) {
+      if (row >= p.rows) break;  // the whole row's threads
+      const RowAt ra = k.at<D>(row);
+      float s[VPT][8], sum = 0.0f, top = 0.0f;
 #pragma unroll
       for (int c = 0; c < VPT; ++c) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[c][e] = __fadd_rn(s[c][e], add[c][e]);
-        if (p.res_out) store8<VEC>(static_cast<TR *>(p.res_out) + row * p.dim, c, G, t, p.dim, s[c]);
+        for (int e = 0; e < 8; ++e) {
+          s[c][e] = x[a][c].get(e);
+          if constexpr (kRes) s[c][e] = __fadd_rn(s[c][e], r[a][c].get(e));
+        }
       }
-    }
-  }
-  float sum = 0.0f, w[VPT][8];
-  uint32_t top = 0u;
+      ask(a, row + kAhead * step);
 #pragma unroll
-  for (int c = 0; c < VPT; ++c) {
-    if (p.norm && live) {
-      if (p.w_f32) load8<VEC>(static_cast<const float *>(p.w), c, G, t, p.dim, w[c]);
-      else load8<VEC>(static_cast<const uint16_t *>(p.w), c, G, t, p.dim, w[c]);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[c][e] = p.norm && live ? __fadd_rn(w[c][e], p.offset) : 1.0f;
-      sum = fmaf(s[c][e], s[c][e], sum);
-      top = max(top, __float_as_uint(s[c][e] * w[c][e]) & 0x7FFFFFFFu);
-    }
-  }
-  reduce_row(sum, top, G, part);
-  float gain = 1.0f;
-  if (p.norm) {
-    const float n = static_cast<float>(p.dim);
-    // Rows whose squares or products leave float32's range (or lose bits below
-    // it) are scaled by a power of two first.  Every thread of the CTA takes
-    // part, so that rows that share a CTA may differ.
-    const bool far = !(sum <= 0x1p120f) || top > 0x7E000000u || (sum < 0x1p-80f && p.eps < 0x1p-80f);
-    float rms_eps = p.eps;
-    if (__syncthreads_or(far)) {
-      uint32_t most = 0u;
-      float none = 0.0f;
-#pragma unroll
-      for (int c = 0; c < VPT; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(s[c][e]) & 0x7FFFFFFFu);
-      reduce_row(none, most, G, part);
-      // by 2^-e with 2^e about the larger of max |s| and sqrt(eps); by 1 where that is 0 or not finite
-      int e2 = 0;
-      if (far && most != 0u && most < kInfBits) {
-        e2 = max(-126, min(126, ilogbf(__uint_as_float(most))));
-        if (p.eps > 0.0f) e2 = max(e2, ilogbf(p.eps) / 2);
-      }
-      const float down = ldexpf(1.0f, -e2);
-      rms_eps = ldexpf(ldexpf(p.eps, -e2), -e2);
-      sum = 0.0f;
-      top = 0u;
-#pragma unroll
-      for (int c = 0; c < VPT; ++c)
+      for (int c = 0; c < VPT; ++c) {
+        float w[8];
+        weights(ra, c, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          s[c][e] *= down;
           sum = fmaf(s[c][e], s[c][e], sum);
-          top = max(top, __float_as_uint(s[c][e] * w[c][e]) & 0x7FFFFFFFu);
+          top = fmaxf(top, fabsf(s[c][e] * w[e]));  // NaN is left to the sum
         }
-      reduce_row(sum, top, G, part);
-    }
-    gain = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, n), rms_eps)));
-  }
-  if (!live) return;
+        if constexpr (kRes)
+          if (p.res_out) store8<D>(static_cast<R *>(p.res_out), k, ra, c, s[c]);
+      }
+      reduce_row(sum, top, G, part[turn ^= 1]);
+      bool bad = sum != sum;  // not a number somewhere
+      float gain = 1.0f;
+      if (p.norm) {
+        float rms_eps = p.eps;
+        // Rows whose squares or products leave float32's range (or lose bits
+        // below it) are scaled by a power of two first.
+        if (!(sum <= 0x1p120f) || !(top <= 0x1p125f) || (sum < 0x1p-80f && p.eps < 0x1p-80f)) {
+          float most = 0.0f, none = 0.0f;
 #pragma unroll
-  for (int c = 0; c < VPT; ++c)
+          for (int c = 0; c < VPT; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[c][e] = s[c][e] * gain * w[c][e];
-  if (p.y)
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[c][e]));
+          reduce_row(none, most, G, part[turn ^= 1]);
+          // by 2^-e with 2^e about the larger of max |s| and sqrt(eps); by 1 where that is 0 or not finite
+          int e2 = 0;
+          if (most != 0.0f && most < __uint_as_float(kInfBits)) {
+            e2 = max(-126, min(126, ilogbf(most)));
+            if (p.eps > 0.0f) e2 = max(e2, ilogbf(p.eps) / 2);
+          }
+          const float down = ldexpf(1.0f, -e2);
+          rms_eps = ldexpf(ldexpf(p.eps, -e2), -e2);
+          sum = 0.0f;
+          top = 0.0f;
 #pragma unroll
-    for (int c = 0; c < VPT; ++c) store8<VEC>(static_cast<TX *>(p.y) + row * p.dim, c, G, t, p.dim, s[c]);
-  if (p.codes) {
-    const float limit = p.e4m3 ? 448.0f : 127.0f;
-    const float most = __uint_as_float(top) * gain;
-    // a row that is not finite has a scale that is not a number, and codes of 0
-    const bool bad = !(most < __uint_as_float(kInfBits));
-    const float held = fmaxf(most, kTiny);
-    const float inv = bad ? 0.0f : __fdiv_rn(limit, held);
-    if (t == 0) p.scales[row] = bad ? __uint_as_float(0x7FC00000u) : __fdiv_rn(held, limit);
+          for (int c = 0; c < VPT; ++c) {
+            float w[8];
+            weights(ra, c, w);
 #pragma unroll
-    for (int c = 0; c < VPT; ++c) {
+            for (int e = 0; e < 8; ++e) {
+              s[c][e] *= down;
+              sum = fmaf(s[c][e], s[c][e], sum);
+              top = fmaxf(top, fabsf(s[c][e] * w[e]));
+            }
+          }
+          reduce_row(sum, top, G, part[turn ^= 1]);
+        }
+        gain = rsqrtf(fmaf(sum, per_dim, rms_eps));  // to 2^-22
+      }
+      float inv = 0.0f;
+      if (p.codes) {
+        const float most = top * gain, held = fmaxf(most, kTiny);
+        // a row that is not finite has a scale that is not a number, and codes of 0
+        bad |= !(most < __uint_as_float(kInfBits));
+        inv = __fdividef(limit, held);
+        if (k.t == 0) p.scales[row] = bad ? __uint_as_float(0x7FC00000u) : __fdiv_rn(held, limit);
+      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[c][e] = bad ? 0.0f : s[c][e] * inv;
-      store_codes<VEC>(p.codes + row * p.dim, c, G, t, p.dim, s[c], p.e4m3);
+      for (int c = 0; c < VPT; ++c) {
+        float w[8];
+        weights(ra, c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[c][e] = s[c][e] * gain * w[e];
+        if (p.y) store8<D>(static_cast<TX *>(p.y), k, ra, c, s[c]);
+        if (p.codes) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[c][e] *= inv;
+          store_codes<D>(p.codes, k, ra, c, s[c], bad, p.e4m3);
+        }
+      }
     }
   }
 }
 
-// Values of codes: a unit of U codes (one access) per thread.
-template <int U, typename T>
+// Four codes' values, whole numbers of int8 (from a byte b ^ 128 below 2^23: 2^23
+// + b + 128 less that much) or e4m3 (by way of float16, exact).
+__device__ __forceinline__ void four_values(uint32_t c, bool e4m3, float *v) {
+  if (e4m3) {
+    uint32_t lo, hi;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(lo) : "h"(static_cast<uint16_t>(c)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(hi) : "h"(static_cast<uint16_t>(c >> 16)));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&lo)), b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  } else {
+    c ^= 0x80808080u;
+    constexpr uint32_t kSelect[4] = {0x7440, 0x7441, 0x7442, 0x7443};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(__byte_perm(c, 0x4B000000u, kSelect[e])) - (0x1p23f + 128.0f);
+  }
+}
+
+// Values of codes, 16 adjacent ones a thread whatever rows they lie in (codes
+// and values are contiguous), the last few one by one.  VEC: both start on
+// 16-byte boundaries.
+template <bool VEC, typename T>
 __global__ void __launch_bounds__(256) k_dequantize_rows(const uint8_t *codes, const float *scales, T *out,
-                                                         uint64_t units, uint32_t per_row, bool e4m3) {
+                                                         uint64_t count, uint32_t dim, bool e4m3) {
+  constexpr int U = 16;
   pdl_wait();
   pdl_trigger();
+  const uint64_t units = (count + U - 1) / U;
   for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < units;
        i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
-    const uint64_t row = (units >> 32) ? i / per_row : static_cast<uint32_t>(i) / per_row;
-    const float scale = scales[row];
-    uint8_t c[U];
-    if constexpr (U == 8) *reinterpret_cast<uint2 *>(c) = *reinterpret_cast<const uint2 *>(codes + 8 * i);
-    else c[0] = codes[i];
+    const uint64_t first = U * i;
+    const int n = static_cast<int>(min(count - first, static_cast<uint64_t>(U)));
+    const bool vec = VEC && n == U;
+    uint32_t c[U / 4] = {};
+    if (vec) {
+      const uint4 q = *reinterpret_cast<const uint4 *>(codes + first);
+      c[0] = q.x, c[1] = q.y, c[2] = q.z, c[3] = q.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < U; ++e)
+        if (e < n) c[e / 4] |= static_cast<uint32_t>(codes[first + e]) << (8 * (e % 4));
+    }
+    uint64_t row = (count >> 32) ? first / dim : static_cast<uint32_t>(first) / dim;
+    const uint64_t left = (row + 1) * dim - first;  // codes of this row from here on
     float v[U];
 #pragma unroll
-    for (int e = 0; e < U; ++e) {
-      const float q = e4m3 ? __half2float(__nv_cvt_fp8_to_halfraw(c[e], __NV_E4M3))
-                           : static_cast<float>(static_cast<int8_t>(c[e]));
-      v[e] = __fmul_rn(q, scale);
+    for (int e = 0; e < U; e += 4) four_values(c[e / 4], e4m3, v + e);
+    float scale = scales[row];
+    if (left >= static_cast<uint64_t>(n)) {
+#pragma unroll
+      for (int e = 0; e < U; ++e) v[e] = __fmul_rn(v[e], scale);
+    } else {
+      uint32_t until = static_cast<uint32_t>(left);
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        if (static_cast<uint32_t>(e) == until && e < n) scale = scales[++row], until += dim;
+        v[e] = __fmul_rn(v[e], scale);
+      }
     }
-    if constexpr (U == 8) store8<true>(out + 8 * i, 0, 1, 0, 8, v);
-    else out[i] = narrow<T>(v[0]);
+    if (vec) {
+#pragma unroll
+      for (int h = 0; h < U; h += 8) {
+        const float eight[8] = {v[h], v[h + 1], v[h + 2], v[h + 3], v[h + 4], v[h + 5], v[h + 6], v[h + 7]};
+        store_eight(out + first + h, eight);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < U; ++e)
+        if (e < n) out[first + e] = narrow<T>(v[e]);
+    }
   }
 }
 
 bool misaligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
-template <bool VEC, int VPT, typename TX>
-cudaError_t launch_res(const NormView &p, uint32_t res_dtype, dim3 grid, int threads, int G, cudaStream_t s) {
-  if (!p.res) return launch_pdl(k_norm<VEC, VPT, TX, void>, grid, dim3(threads), 0, s, p, G);
-  if (res_dtype == FNMOE_DTYPE_F32) return launch_pdl(k_norm<VEC, VPT, TX, float>, grid, dim3(threads), 0, s, p, G);
-  return launch_pdl(k_norm<VEC, VPT, TX, uint16_t>, grid, dim3(threads), 0, s, p, G);
+template <Deal D, int VPT, typename TX, typename TR>
+cudaError_t launch_k(const NormView &p, int per, int G, cudaStream_t s) {
+  const size_t smem = p.norm && D != kEven ? (static_cast<size_t>(p.dim) / 8 + 1) * 8 * sizeof(float) : 0;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(k_norm<D, VPT, TX, TR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  // as many CTAs as stay on the SMs: 1024 threads (512 where a thread holds more of a row)
+  const int ctas = std::max(1, (VPT <= 2 ? 1024 : 512) / (per * G));
+  const int64_t most = static_cast<int64_t>(device_info().sms) * ctas, need = (p.rows + per - 1) / per;
+  return launch_pdl(k_norm<D, VPT, TX, TR>, dim3(static_cast<unsigned>(std::min(need, most))), dim3(per * G), smem, s, p, G);
 }
 
-template <bool VEC, typename TX>
+template <Deal D, typename TX>
 cudaError_t launch_norm(const NormView &p, uint32_t res_dtype, cudaStream_t s) {
-  const int chunks = (p.dim + 7) / 8;
-  int vpt = chunks > 1024 ? 4 : chunks > 512 ? 2 : 1;
-  const int G = (chunks + 32 * vpt - 1) / (32 * vpt) * 32;
-  const int per = std::max(1, 128 / G);  // rows of a CTA
-  const dim3 grid(static_cast<unsigned>((p.rows + per - 1) / per));
-  switch (vpt) {
-    case 1: return launch_res<VEC, 1, TX>(p, res_dtype, grid, per * G, G, s);
-    case 2: return launch_res<VEC, 2, TX>(p, res_dtype, grid, per * G, G, s);
-    default: return launch_res<VEC, 4, TX>(p, res_dtype, grid, per * G, G, s);
+  const int chunks = (p.dim + 7) / 8 + (D == kFlat && p.dim % 8 != 0 ? 1 : 0);  // a row off its boundary touches one more
+  // A thread's chunks: one, so that few rows wait least for one another's sums,
+  // or, from two rows an SM on, two where they fit the registers: the
+  // sums' steps and the row's root and quotient cost a thread as much as a chunk.
+  const bool wide = p.res && (sizeof(TX) == 4 || res_dtype == FNMOE_DTYPE_F32);
+  const int many = p.rows >= 2 * device_info().sms && !wide ? 2 : 1;
+  const int vpt = std::max(many, chunks > 1024 ? 4 : chunks > 512 ? 2 : 1);
+  const int G = (chunks + 32 * vpt - 1) / (32 * vpt) * 32, per = G == 32 ? 4 : 1;
+  auto go = [&](auto residual) {
+    using TR = typename decltype(residual)::type;
+    switch (vpt) {
+      case 1: return launch_k<D, 1, TX, TR>(p, per, G, s);
+      case 2: return launch_k<D, 2, TX, TR>(p, per, G, s);
+      default: return launch_k<D, 4, TX, TR>(p, per, G, s);
+    }
+  };
+  if (!p.res) return go(std::common_type<void>{});
+  if (res_dtype == FNMOE_DTYPE_F32) return go(std::common_type<float>{});
+  return go(std::common_type<uint16_t>{});
+}
+
+template <typename TX>
+cudaError_t launch_deal(const NormView &p, Deal d, uint32_t res_dtype, cudaStream_t s) {
+  switch (d) {
+    case kEven: return launch_norm<kEven, TX>(p, res_dtype, s);
+    case kFlat: return launch_norm<kFlat, TX>(p, res_dtype, s);
+    default: return launch_norm<kOdd, TX>(p, res_dtype, s);
   }
 }
 
@@ -367,16 +582,18 @@ int add_rms_norm(const FnNormArgs *a, cudaStream_t s, std::string &err) {
   p.eps = a->eps;
   p.offset = (a->flags & FNMOE_NORM_UNIT_OFFSET) ? 1.0f : 0.0f;
   p.w_f32 = a->weight_dtype == FNMOE_DTYPE_F32;
+  p.w_vec = !misaligned(a->weight, 16);
   p.norm = norm;
   p.e4m3 = a->code_type == FNMOE_Q8_E4M3;
-  // 16-byte accesses where every row of every array allows them
-  const bool vec = a->dim % 8 == 0 && !misaligned(a->x, 16) && !misaligned(a->residual, 16) &&
-                   !(norm && misaligned(a->weight, 16)) && !misaligned(a->y, 16) && !misaligned(a->residual_out, 16) &&
-                   !misaligned(a->codes, 8) && (a->rows == 1 || (a->x_stride * xs % 16 == 0 &&
-                   (!a->residual || a->residual_stride * rs % 16 == 0)));
-  cudaError_t e;
-  if (a->x_dtype == FNMOE_DTYPE_F32) e = vec ? launch_norm<true, float>(p, a->residual_dtype, s) : launch_norm<false, float>(p, a->residual_dtype, s);
-  else e = vec ? launch_norm<true, uint16_t>(p, a->residual_dtype, s) : launch_norm<false, uint16_t>(p, a->residual_dtype, s);
+  const bool starts = !misaligned(a->x, 16) && !misaligned(a->residual, 16) && !misaligned(a->y, 16) &&
+                      !misaligned(a->residual_out, 16) && !misaligned(a->codes, 8);
+  const bool even = a->dim % 8 == 0 && (a->rows == 1 || (a->x_stride * xs % 16 == 0 &&
+                    (!a->residual || a->residual_stride * rs % 16 == 0)));
+  const bool contiguous = a->rows == 1 || (a->x_stride == a->dim && (!a->residual || a->residual_stride == a->dim));
+  // (kFlat holds up to 16376 columns: its rows may touch one chunk more)
+  const Deal d = starts && even ? kEven : starts && contiguous && a->dim <= kMaxDim - 8 ? kFlat : kOdd;
+  const cudaError_t e = a->x_dtype == FNMOE_DTYPE_F32 ? launch_deal<float>(p, d, a->residual_dtype, s)
+                                                      : launch_deal<uint16_t>(p, d, a->residual_dtype, s);
   return done(e, "add_rms_norm", err);
 }
 
@@ -395,20 +612,19 @@ int dequantize_rows(const FnRowCodesArgs *a, cudaStream_t s, std::string &err) {
     err = "scales and out must be aligned to their elements";
     return FNMOE_ERR_VALUE;
   }
-  const bool vec = a->dim % 8 == 0 && !misaligned(a->codes, 8) && !misaligned(a->out, 16);
-  const uint32_t per_row = vec ? a->dim / 8 : a->dim;
-  const uint64_t units = static_cast<uint64_t>(a->rows) * per_row;
-  const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((units + 255) / 256, 1u << 20)));
+  const bool vec = !misaligned(a->codes, 16) && !misaligned(a->out, 16);
+  const uint64_t count = static_cast<uint64_t>(a->rows) * a->dim;
+  const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((count + 4095) / 4096, 1u << 20)));
   const uint8_t *c = static_cast<const uint8_t *>(a->codes);
   cudaError_t e;
   if (f32) {
     float *o = static_cast<float *>(a->out);
-    e = vec ? launch_pdl(k_dequantize_rows<8, float>, grid, dim3(256), 0, s, c, a->scales, o, units, per_row, e4m3)
-            : launch_pdl(k_dequantize_rows<1, float>, grid, dim3(256), 0, s, c, a->scales, o, units, per_row, e4m3);
+    e = vec ? launch_pdl(k_dequantize_rows<true, float>, grid, dim3(256), 0, s, c, a->scales, o, count, a->dim, e4m3)
+            : launch_pdl(k_dequantize_rows<false, float>, grid, dim3(256), 0, s, c, a->scales, o, count, a->dim, e4m3);
   } else {
     uint16_t *o = static_cast<uint16_t *>(a->out);
-    e = vec ? launch_pdl(k_dequantize_rows<8, uint16_t>, grid, dim3(256), 0, s, c, a->scales, o, units, per_row, e4m3)
-            : launch_pdl(k_dequantize_rows<1, uint16_t>, grid, dim3(256), 0, s, c, a->scales, o, units, per_row, e4m3);
+    e = vec ? launch_pdl(k_dequantize_rows<true, uint16_t>, grid, dim3(256), 0, s, c, a->scales, o, count, a->dim, e4m3)
+            : launch_pdl(k_dequantize_rows<false, uint16_t>, grid, dim3(256), 0, s, c, a->scales, o, count, a->dim, e4m3);
   }
   return done(e, "dequantize_rows", err);
 }

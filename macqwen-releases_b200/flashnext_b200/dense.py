@@ -49,26 +49,35 @@ def _float(t, what):
 def _matrix(t, what, index):
     """Pointer, rows, columns and row stride of a matrix on CUDA device ``index`` whose rows are contiguous."""
     shape = t.shape
+    if len(shape) == 2 and t.get_device() == index >= 0:
+        rows, dim = shape
+        if t.is_contiguous():
+            return t.data_ptr(), rows, dim, dim
+        s0, s1 = t.stride()
+        if (s1 == 1 or dim < 2) and (s0 >= dim or rows < 2):
+            return t.data_ptr(), rows, dim, s0 if rows > 1 else dim
+    # say what is wrong
     if len(shape) != 2:
         raise ValueError(f"{what} must have two dimensions, not {tuple(shape)}")
     if not t.is_cuda:
         raise TypeError(f"{what} must be a CUDA tensor")
     if t.get_device() != index:
         _elsewhere(t, index, what)
-    rows, dim = shape
-    s0, s1 = t.stride()
     if s1 != 1 and dim > 1:
         raise ValueError(f"{what}'s rows must be contiguous")
-    if s0 < dim and rows > 1:
-        raise ValueError(f"{what}'s rows overlap")
-    return t.data_ptr(), rows, dim, s0 if rows > 1 else dim
+    raise ValueError(f"{what}'s rows overlap")
 
 
-def _same(t, shape, what, index):
-    p, rows, dim, stride = _matrix(t, what, index)
-    if (rows, dim) != shape:
-        raise ValueError(f"{what} has shape {(rows, dim)}, not {shape}")
+def _same(t, rows, dim, what, index):
+    p, r, d, stride = _matrix(t, what, index)
+    if r != rows or d != dim:
+        raise ValueError(f"{what} has shape {(r, d)}, not {(rows, dim)}")
     return p, stride
+
+
+def _new(rows, dim, dtype, like):
+    """A new contiguous matrix on ``like``'s device (the cheapest of torch's ways to make one)."""
+    return torch.empty_strided((rows, dim), (dim, 1), dtype=dtype, device=like.device)
 
 
 def add_rms_norm(x, weight, residual=None, eps: float = 1e-6, *, unit_offset: bool = False, codes=None,
@@ -97,29 +106,30 @@ def add_rms_norm(x, weight, residual=None, eps: float = 1e-6, *, unit_offset: bo
 
 
 def _norm(x, xd, xp, rows, dim, xs, weight, wp, residual, eps, flags, codes, keep, residual_out, index, what):
-    y = x.new_empty((rows, dim)) if keep else None
-    q = scales = None
-    ct = 0
+    y = q = scales = yp = qp = sp = rp = op = None
+    ct = rs = rd = 0
+    lib, stream = _ready(x)
+    if residual is not None:
+        rd = _float(residual, "residual")
+        rp, rs = _same(residual, rows, dim, "residual", index)
+        if residual_out is None:
+            residual_out = _new(rows, dim, residual.dtype, x)
+            op = residual_out.data_ptr()
+        else:
+            op = _want(residual_out, residual.dtype, (rows, dim), "residual_out", index)
+    elif residual_out is not None:
+        raise ValueError("residual_out needs residual")
+    if keep:
+        y = _new(rows, dim, x.dtype, x)
+        yp = y.data_ptr()
     if codes is not None:
         ct = _CODES.get(codes)
         if ct is None:
             raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn")
-        q, scales = x.new_empty((rows, dim), dtype=codes), x.new_empty((rows,), dtype=torch.float32)
-    rp, rs, rd = None, 0, 0
-    if residual is not None:
-        rd = _float(residual, "residual")
-        rp, rs = _same(residual, (rows, dim), "residual", index)
-        if residual_out is None:
-            residual_out = residual.new_empty((rows, dim))
-        else:
-            _want(residual_out, residual.dtype, (rows, dim), "residual_out", index)
-    elif residual_out is not None:
-        raise ValueError("residual_out needs residual")
-    lib, stream = _ready(x)
-    a = _lib.FnNormArgs(
-        _lib.ABI_VERSION, flags, rows, dim, xd, rd, 0 if weight is None else _float(weight, "weight"), ct, eps, 0, xp, xs,
-        rp, rs, wp, None if y is None else y.data_ptr(), None if residual_out is None else residual_out.data_ptr(),
-        None if q is None else q.data_ptr(), None if q is None else scales.data_ptr())
+        q, scales = _new(rows, dim, codes, x), torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device)
+        qp, sp = q.data_ptr(), scales.data_ptr()
+    a = _lib.FnNormArgs(_lib.ABI_VERSION, flags, rows, dim, xd, rd, 0 if weight is None else _float(weight, "weight"), ct,
+                        eps, 0, xp, xs, rp, rs, wp, yp, op, qp, sp)
     code = lib.fnmoe_add_rms_norm(ctypes.byref(a), stream)
     if code:
         _lib.check(code, what)
@@ -150,12 +160,13 @@ def dequantize_rows(codes, scales, out_dtype=torch.bfloat16, out=None):
     if len(shape) != 2:
         raise ValueError(f"codes must have two dimensions, not {tuple(shape)}")
     cp, sp = _want(codes, codes.dtype, shape, "codes", index), _want(scales, torch.float32, (shape[0],), "scales", index)
-    if out is None:
-        out = scales.new_empty(shape, dtype=out_dtype)
-    od = _float(out, "out")
-    a = _lib.FnRowCodesArgs(_lib.ABI_VERSION, shape[0], shape[1], ct, od, 0, cp, sp,
-                            _want(out, out.dtype, shape, "out", index))
     lib, stream = _ready(codes)
+    if out is None:
+        out = _new(shape[0], shape[1], out_dtype, codes)
+        op = out.data_ptr()
+    else:
+        op = _want(out, out.dtype, shape, "out", index)
+    a = _lib.FnRowCodesArgs(_lib.ABI_VERSION, shape[0], shape[1], ct, _float(out, "out"), 0, cp, sp, op)
     code = lib.fnmoe_dequantize_rows(ctypes.byref(a), stream)
     if code:
         _lib.check(code, "dequantize_rows")
@@ -201,14 +212,17 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
         bd, bp = _float(bias, "bias"), _want(bias, bias.dtype, (n,), "bias", index)
     if residual is not None:
         rd = _float(residual, "residual")
-        rp, rs = _same(residual, (rows, n), "residual", index)
+        rp, rs = _same(residual, rows, n, "residual", index)
+    lib, stream = _ready(x)
     if out is None:
-        out = x.new_empty((rows, n), dtype=torch.bfloat16 if out_dtype is None else out_dtype)
+        out = _new(rows, n, torch.bfloat16 if out_dtype is None else out_dtype, x)
+        op = out.data_ptr()
     elif out_dtype is not None and out.dtype is not out_dtype:
         raise TypeError(f"out is {out.dtype}, out_dtype {out_dtype}")
-    lib, stream = _ready(x)
+    else:
+        op = _want(out, out.dtype, (rows, n), "out", index)
     a = _lib.FnLinearArgs(_lib.ABI_VERSION, kind, rows, k, n, act, bd, rd, _float(out, "out"), 0, xp, xs, wp, ws, xsp, wsp,
-                          bp, rp, rs, _want(out, out.dtype, (rows, n), "out", index))
+                          bp, rp, rs, op)
     code = lib.fnmoe_linear(ctypes.byref(a), stream)
     if code:
         _lib.check(code, "linear")

@@ -65,9 +65,10 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if mp is None and not 0 <= _number(m, "min_p") <= 1:
         raise ValueError("min_p must be between 0 and 1")
     up = _want(uniform, f32, (rows,), "uniform", index)
-    tokens = logits.new_empty((rows,), dtype=torch.int64)
-    logprobs = logits.new_empty((rows,), dtype=f32)
     lib, stream = _ready(logits)
+    device = logits.device
+    tokens = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)
+    logprobs = torch.empty_strided((rows,), (1,), dtype=f32, device=device)
     a = _lib.FnSampleArgs(_lib.ABI_VERSION, rows, vocab, dtype, lp, stride, up, tp, kp, pp, mp, t, k, p, m,
                           tokens.data_ptr(), logprobs.data_ptr())
     code = lib.fnmoe_sample(ctypes.byref(a), stream)
