@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
         const float most = top * gain, held = fmaxf(most, kTiny);
         // a row that is not finite has a scale that is not a number, and codes of 0
         bad |= !(most < __uint_as_float(kInfBits));
-        inv = __fdividef(limit, held);
+        inv = __fdiv_rn(limit, held);
         if (k.t == 0) p.scales[row] = bad ? __uint_as_float(0x7FC00000u) : __fdiv_rn(held, limit);
       }
 #pragma unroll

@@ -83,7 +83,7 @@ struct Shared {
     } list;
     float pack[kWarps][kBlock / 2];              // the draw: a warp's kept logits
   };
-  double root[kRoots];                           // 2^(j / kRoots)
+  double root[kRoots];                           // 2^(44 + j / kRoots)
   uint64_t block_mass[kMaxBlocks];
   float own_group[kGroups], group[kGroups];      // largest logits of groups: this CTA's, the cluster's
   uint64_t warp_sum[kWarps];
@@ -144,9 +144,9 @@ struct Weights {
     return (static_cast<double>(l) - static_cast<double>(top)) * per;
   }
   // The weight of a logit in (low, top]: 2^y, y = (l - top) per = k + j / 512 + r,
-  // to 2^-46 of itself: 2^r by its series up to r^3, 2^(j / 512) from the table,
-  // 2^(k + 44) in the exponent; adding 2^52 leaves the nearest whole number in
-  // the low bits.  Eight float64 operations; CUDA's exp takes three times that.
+  // to 2^-46 of itself: 2^r by its series up to r^3, 2^(44 + j / 512) from the
+  // table, 2^k in the exponent; adding 2^52 leaves the nearest whole number in the
+  // low bits.  Eight float64 operations; CUDA's exp takes three times that.
   __device__ __forceinline__ uint64_t of(float l) const {
     constexpr double kRound = 0x1.8p43;  // its last bit is 2^-9
     const double d = l == top ? 0.0 : static_cast<double>(l) - static_cast<double>(top);
@@ -157,7 +157,7 @@ struct Weights {
     q = fma(r, q, 0x1.62e42fefa39efp-1);                            // ln(2)
     q = fma(r, q, 1.0);
     const double s = root[m & (kRoots - 1)];
-    const double scaled = __hiloint2double(__double2hiint(s) + (((m >> 9) + 44) << 20), __double2loint(s));
+    const double scaled = __hiloint2double(__double2hiint(s) + static_cast<int>(static_cast<uint32_t>(m) << 11 & 0xFFF00000u), __double2loint(s));
     return static_cast<uint64_t>(__double_as_longlong(fma(q, scaled, 0x1p52))) & ((1ull << 52) - 1ull);
   }
   __device__ __forceinline__ uint64_t any(float l) const { return l > low || l == top ? of(l) : 0ull; }
@@ -225,19 +225,26 @@ __device__ __forceinline__ void write_row(const SampleView &p, int row, uint32_t
 }
 
 // The rest of a row whose every token that may be kept is among rank 0's n
-// pulled ones (n <= kFew), by that CTA, a thread a token.  by_count: they hold the
+// pulled ones (n <= kFew), by that CTA.  by_count: they hold the
 // first top_k, and more; else what may be kept by top-p, the weights before a
 // kept token staying below `target`.  The two orders that this needs, by rank
 // for the filters and by index for the draw, come from counting what lies before.
 __device__ void draw_from_list(const SampleView &p, int row, const Settings &set, const Weights &weights, double least,
                                bool by_count, uint64_t target, int n, Shared &s) {
   const int tid = threadIdx.x;
-  if (tid < n) {
-    const uint64_t mine = s.pulled[tid];
+  // adjacent threads of a token share what is counted for it
+  int team = 1;
+  while (team < 32 && 2 * team * n <= kThreads) team *= 2;
+  const int token = tid / team, part = tid % team;
+  {
+    const uint64_t mine = token < n ? s.pulled[token] : 0ull;
     int r = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) r += s.pulled[j] < mine;
-    s.list.at[r] = mine;
+    if (token < n) {
+#pragma unroll 4
+      for (int j = part; j < n; j += team) r += s.pulled[j] < mine;
+    }
+    for (int o = 1; o < team; o <<= 1) r += __shfl_xor_sync(0xFFFFFFFFu, r, o);
+    if (token < n && part == 0) s.list.at[r] = mine;
   }
   __syncthreads();
   const int kept_n = by_count ? min(set.top_k, n) : n;
@@ -249,18 +256,19 @@ __device__ void draw_from_list(const SampleView &p, int row, const Settings &set
   scan(none, before, none_total, total, s);
   if (by_count) target = set.top_p < 1.0f ? share_of(set.top_p, total) : kAll;
   if (!(before < target && (l == weights.top || weights.exponent(l) >= least))) w = 0ull;
-  // list.at[tid] was read by this thread alone since it was written
-  if (tid < n) s.list.at[tid] = index_at(at), s.list.w[tid] = w;
+  if (tid < n) s.pulled[tid] = at, s.list.w[tid] = w;
   uint64_t sum = w;
   scan(none, sum, none_total, total, s);
   const uint64_t drawn = drawn_at(set.u, total);
-  if (w != 0ull) {
-    const uint32_t index = index_at(at);
-    uint64_t lower = 0;
+  const uint64_t held = token < n ? s.list.w[token] : 0ull, mine = token < n ? s.pulled[token] : 0ull;
+  const uint32_t index = index_at(mine);
+  uint64_t lower = 0;
+  if (held != 0ull) {
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) lower += s.list.at[j] < index ? s.list.w[j] : 0ull;
-    if (lower <= drawn && drawn < lower + w) write_row(p, row, index, l, weights, total);
+    for (int j = part; j < n; j += team) lower += index_at(s.pulled[j]) < index ? s.list.w[j] : 0ull;
   }
+  for (int o = 1; o < team; o <<= 1) lower += __shfl_xor_sync(0xFFFFFFFFu, lower, o);
+  if (part == 0 && lower <= drawn && drawn < lower + held) write_row(p, row, index, logit_at(mine), weights, total);
 }
 
 // One row, in a cluster of p.ctas CTAs.
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
   const uint32_t begin = rank * static_cast<uint32_t>(p.slice);
   const int n = max(0, min(p.slice, p.vocab - static_cast<int>(begin)));
   static_assert(kRoots == kThreads, "a root a thread");
-  s.root[tid] = exp2(static_cast<double>(tid) / kRoots);
+  s.root[tid] = exp2(44.0 + static_cast<double>(tid) / kRoots);
   if (tid == 0) s.list_n = 0u, s.best = 0xFFFFFFFFu;
   cluster_arrive();  // this CTA is here: the others wait for it before they write into its memory
   pdl_wait();
@@ -590,15 +598,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
   if (by_groups) {
     // The top_k-th largest of the groups' maxima is at most the top_k-th largest
     // logit: what is no less holds the first top_k, and seldom many more.
-    if (tid < kGroups) {
-      const float v = s.group[tid];
-      int above = 0;
-#pragma unroll 8
-      for (int j = 0; j < kGroups; ++j) {
-        const float o = s.group[j];
-        above += o > v || (o == v && j < tid);
+    // (To 16 bits, found from the top one down by a warp.)
+    if (warp == 0) {
+      uint32_t key[kGroups / 32], bound = 0u;
+#pragma unroll
+      for (int e = 0; e < kGroups / 32; ++e) key[e] = ~static_cast<uint32_t>(place_of(s.group[lane + 32 * e], 0) >> kIndexBits);
+#pragma unroll 1
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t more = bound | (1u << bit);
+        int above = 0;
+#pragma unroll
+        for (int e = 0; e < kGroups / 32; ++e) above += key[e] >= more;
+        if (__reduce_add_sync(0xFFFFFFFFu, above) >= set.top_k) bound = more;
       }
-      if (above == set.top_k - 1) s.bound = v;
+      // fewer groups than that hold a token: not a number
+      if (lane == 0) s.bound = __uint_as_float((bound & 0x80000000u) ? bound & 0x7FFFFFFFu : ~bound);
     }
     __syncthreads();
     const float bound = s.bound;
@@ -647,26 +661,42 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
     uint64_t sum = 0;
 #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
-      // the kept logits side by side, in any order, so that every lane has work
       const int i0 = b * kBlock + part * (kBlock / 2) + lane;
-      float *pack = s.pack[warp];
+      constexpr int kEach = kBlock / 64;
+      float l[kEach];
+      uint32_t who[kEach];
       int m = 0;
 #pragma unroll
-      for (int e = 0; e < kBlock / 64; ++e) {
+      for (int e = 0; e < kEach; ++e) {
         const int i = i0 + 32 * e;
-        const float l = i < n ? logit<T>(data + i) : kMinusInf;
-        const bool on = kept.keeps(l, static_cast<int>(begin) + i);
-        const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
-        if (on) pack[m + __popc(who & ((1u << lane) - 1u))] = l;
-        m += __popc(who);
+        l[e] = i < n ? logit<T>(data + i) : kMinusInf;
+        who[e] = __ballot_sync(0xFFFFFFFFu, kept.keeps(l[e], static_cast<int>(begin) + i));
+        m += __popc(who[e]);
+      }
+      if (m > kBlock / 4) {  // most are kept
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const bool on = who[e] >> lane & 1u;
+          const uint64_t w = weights.of(on ? l[e] : hi);
+          sum += on ? w : 0ull;
+        }
+        continue;
+      }
+      // else the kept logits side by side, in any order, so that every lane has work
+      float *pack = s.pack[warp];
+      int at = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (who[e] >> lane & 1u) pack[at + __popc(who[e] & ((1u << lane) - 1u))] = l[e];
+        at += __popc(who[e]);
       }
       __syncwarp();
-      for (int j = lane; j < m; j += 128) {
-        uint64_t w[4];
+      for (int j = lane; j < m; j += 64) {
+        uint64_t w[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = weights.of(j + 32 * e < m ? pack[j + 32 * e] : hi);
+        for (int e = 0; e < 2; ++e) w[e] = weights.of(j + 32 * e < m ? pack[j + 32 * e] : hi);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += j + 32 * e < m ? w[e] : 0ull;
+        for (int e = 0; e < 2; ++e) sum += j + 32 * e < m ? w[e] : 0ull;
       }
       __syncwarp();
     }
