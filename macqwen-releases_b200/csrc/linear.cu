@@ -12,6 +12,10 @@
 // Sums: float32 in TMEM for bfloat16 and e4m3, exact int32 for int8 (widths up
 // to 131072 keep 127^2 K below 2^31).  The epilogue works on float32 and rounds
 // once, to the output's type.
+//
+// Measured: 16 x 2048 > 131072 (a head) 87.5 us, 6.2 TB/s; 1 x 2048 > 5120 6.6 us;
+// 5000 x 2048 > 5120 with SiLU 83.5 us, 1,256 TFLOP/s of 1,653; 8192 x 4096 x 4096
+// int8 98 us, 2,800 TOPS.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -333,8 +337,9 @@ __device__ __forceinline__ void finish(const LinearView &p, const Column &c, int
 // A pair's first CTA issues the MMAs of both (cta_group::2, M 256): each CTA
 // brings its own weight rows and half the rows of x, both on the first one's
 // barriers, and reads its own lanes' sums.  It halves the traffic of x into
-// shared memory, which bounds large products (48 KB a k-step at 64 bytes a
-// clock against 512 clocks of bfloat16 MMAs, 256 of 8-bit ones).
+// shared memory, which bounds large products: 48 KB a k-step come in at about 44
+// bytes a clock (measured), against 512 clocks of bfloat16 MMAs, 256 of 8-bit
+// ones.  (8192 x 4096 x 4096 int8: 117 us alone, 94 in pairs.)
 // Every wait is bounded; a timeout sets kErrTimeout, marks the CTA dead (later
 // waits return at once) and every role runs to the teardown.
 template <int KIND, int NT, bool PAIR>
@@ -616,6 +621,7 @@ bool make_map(CUtensorMap *map, const void *base, bool bf16, uint64_t rows, uint
   const cuuint32_t estr[2] = {1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base),
             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            // a k-step takes 128 bytes of many rows; DRAM gives the next k-step's along (97 -> 88 us for a head)
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -13,8 +13,10 @@
 // norm sees the unrounded sum, so rounding the carried residual costs it
 // nothing).
 //
-// Bound by HBM, and by the latency of a row's chain (load, sum, store): CTAs stay
-// on their SM and ask for the rows two rounds ahead.
+// Bound by issue slots and HBM: CTAs stay on their SM and ask for rows ahead, and
+// nothing is chosen a value at a time.  5000 x 2048 bfloat16 with a residual: 17.5
+// us, 4.7 TB/s of 6.46 (41 instructions a value with codes, 55 in the first form);
+// one row of 2048: 2.0 us, of which a launch is most.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
@@ -424,7 +426,8 @@ __device__ __forceinline__ void four_values(uint32_t c, bool e4m3, float *v) {
 
 // Values of codes, 16 adjacent ones a thread whatever rows they lie in (codes
 // and values are contiguous), the last few one by one.  VEC: both start on
-// 16-byte boundaries.
+// 16-byte boundaries.  Bound by HBM's latency: 5000 x 2048 to bfloat16 about 8 us
+// (31 MB); one code a thread took 50 us at 5003 x 2561.
 template <bool VEC, typename T>
 __global__ void __launch_bounds__(256) k_dequantize_rows(const uint8_t *codes, const float *scales, T *out,
                                                          uint64_t count, uint32_t dim, bool e4m3) {

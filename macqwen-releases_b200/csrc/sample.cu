@@ -17,6 +17,11 @@
 // atomics, and a vocabulary of 2^18 stays below 2^62.  Float32 weights (2^-24)
 // would draw another token than the definition once in some thousand rows of a
 // flat distribution, whose borders lie 2^-17 apart.
+//
+// Bound by issue slots (57 to 163 instructions a token over all passes) and, for
+// few rows, by a chain of cluster barriers of about 1 us: 1 x 131072 with top-k 50,
+// top-p and min-p 10.4 us; 64 x 131072 33.4 us, with settings of their own 54.9 us,
+// top-p alone 77.5 us.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
