@@ -648,16 +648,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
 
   // ---- the draw: kept weights summed block by block, and walked by index in the block drawn ----
   if (set.min_p > 0.0f) {
-    // the least logit whose weight is min_p or more: by the formula's inverse,
-    // then exactly among its neighbours
-    const float guess = static_cast<float>(static_cast<double>(hi) + least / weights.per);
-    float l = hi;
+    // The least float whose weight is min_p or more, by its bits in rising order,
+    // five at a time: a lane a candidate.  (The formula's inverse is not near
+    // enough where it comes out next to 0.)
+    const uint32_t most = ~static_cast<uint32_t>(place_of(hi, 0) >> kIndexBits);
+    uint32_t below = 0u;  // the largest that weighs less, as far as it is known
 #pragma unroll 1
-    for (int step = 4; step >= -4; --step) {
-      const uint32_t up = static_cast<uint32_t>(~(place_of(guess, 0) >> kIndexBits)) + static_cast<uint32_t>(step);
-      const float x = __uint_as_float((up & 0x80000000u) ? up & 0x7FFFFFFFu : ~up);
-      if (x <= hi && weights.exponent(x) >= least) l = fminf(l, x);
+    for (int shift = 27; shift > -5; shift -= 5) {
+      const uint32_t key = below | (shift >= 0 ? static_cast<uint32_t>(lane) << shift : static_cast<uint32_t>(lane) >> -shift);
+      const float x = __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
+      const uint32_t less = __ballot_sync(0xFFFFFFFFu, !(key >= most || weights.exponent(x) >= least));
+      const int last = 31 - __clz(less);  // lane 0 always weighs less
+      below = __shfl_sync(0xFFFFFFFFu, key, last);
     }
+    const uint32_t first = below + 1u;
+    const float l = __uint_as_float((first & 0x80000000u) ? first & 0x7FFFFFFFu : ~first);
     if (l > cut.l) cut = Cut{l, kEvery};
   }
   const Cut kept = weighing(cut);

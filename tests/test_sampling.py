@@ -288,3 +288,23 @@ def test_streams_graphs_and_refusals(cuda_lib):
                  lambda: sampling.sample(x, u, top_k=t), lambda: sampling.sample(x.half(), u), lambda: sampling.sample(x, u.cpu())):
         with pytest.raises(TypeError):
             call()
+
+
+@gpu
+@pytest.mark.parametrize("sign", [1, -1])
+def test_min_p_whose_logit_lies_next_to_zero(cuda_lib, sign):
+    """The least kept logit, max l + T ln(min_p), within 1e-9 of 0: floats lie 1e-16 apart there and less, closer than
+    any sum of the larger terms, and what lies well above it has to stay."""
+    import torch
+
+    temps = np.float32(0.9) + np.arange(2000, dtype=np.float32) * np.float32(2.0 ** -24)
+    mins = np.float32(0.01) + np.arange(2000, dtype=np.float32) * np.float32(2.0 ** -30)
+    hi = np.float32(-np.log(np.float64(mins[0])) * np.float64(temps[0]))
+    least = np.float64(hi) + np.outer(temps.astype(np.float64), np.log(mins.astype(np.float64)))
+    least = np.where(sign * least > 0, np.abs(least), np.inf)
+    order = np.argsort(least, axis=None)[:48]
+    i, j = np.unravel_index(order, least.shape)
+    assert least[i, j].max() < 1e-8  # 1e-10 for the nearest
+    x = torch.tensor([[float(hi), 3.0, 2.0, 1.0, 0.5, 0.0, -0.5, -1.0, 1e-20, -1e-20] * 400], device="cuda").repeat(48, 1)
+    u = (torch.arange(48, device="cuda", dtype=torch.float32) + 0.5) / 48
+    _check(x.contiguous(), u, torch.from_numpy(temps[i]).cuda(), 0, 1.0, torch.from_numpy(mins[j]).cuda())
