@@ -474,7 +474,7 @@ typedef struct FnLinearArgs {
   uint32_t abi_version;
   uint32_t type;               /* FNMOE_LINEAR_* */
   uint32_t rows;               /* of x and out */
-  uint32_t in_width;           /* columns of x and weight; at most 131072 */
+  uint32_t in_width;           /* columns of x and weight; at most 131071 */
   uint32_t out_width;          /* rows of weight, columns of out */
   uint32_t activation;         /* FNMOE_ACT_* */
   uint32_t bias_dtype;

@@ -10,6 +10,16 @@
 
 namespace fnmoe {
 
+// Bytes of a caller's array, for refusing outputs that overlap inputs.
+struct Span {
+  const void *at;
+  uint64_t bytes;
+  bool meets(const Span &o) const {
+    const uint64_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+    return at != nullptr && o.at != nullptr && a < b + o.bytes && b < a + bytes;
+  }
+};
+
 int add_rms_norm(const FnNormArgs *a, cudaStream_t s, std::string &err);
 int dequantize_rows(const FnRowCodesArgs *a, cudaStream_t s, std::string &err);
 int linear(const FnLinearArgs *a, cudaStream_t s, std::string &err);

@@ -10,7 +10,7 @@
 // ragged sizes need no masks before the stores.
 //
 // Sums: float32 in TMEM for bfloat16 and e4m3, exact int32 for int8 (widths up
-// to 131072 keep 127^2 K below 2^31).  The epilogue works on float32 and rounds
+// to 131071 keep 128^2 K below 2^31).  The epilogue works on float32 and rounds
 // once, to the output's type.
 //
 // Measured: 16 x 2048 > 131072 (a head) 87.5 us, 6.2 TB/s; 1 x 2048 > 5120 6.6 us;
@@ -35,7 +35,7 @@ namespace {
 constexpr int kLanes = 128;            // weight rows of a tile
 constexpr int kBoxW = kLanes * 128;    // bytes of a k-step's weight box
 constexpr uint32_t kSpin = 1u << 20;   // polls before a wait gives up
-constexpr uint32_t kMaxWidth = 131072;
+constexpr uint32_t kMaxWidth = 131071;
 
 enum Kind { kBf16 = FNMOE_LINEAR_BF16, kInt8 = FNMOE_LINEAR_INT8, kE4m3 = FNMOE_LINEAR_E4M3 };
 
@@ -757,6 +757,17 @@ int linear(const FnLinearArgs *a, cudaStream_t s, std::string &err) {
   if (misaligned(a->x_scale, 4) || misaligned(a->weight_scale, 4) || misaligned(a->bias, bytes(a->bias_dtype)) ||
       misaligned(a->residual, bytes(a->residual_dtype)) || misaligned(a->out, bytes(a->out_dtype))) {
     err = "arrays must be aligned to their elements";
+    return FNMOE_ERR_VALUE;
+  }
+  const uint64_t rows = a->rows, width = a->out_width, rs = bytes(a->residual_dtype), os = bytes(a->out_dtype);
+  const Span out{a->out, rows * width * os};
+  const bool in_place = a->out == a->residual && a->out_dtype == a->residual_dtype && (rows == 1 || a->residual_stride == width);
+  if (out.meets(Span{a->x, ((rows - 1) * a->x_stride + a->in_width) * size}) ||
+      out.meets(Span{a->weight, ((width - 1) * a->weight_stride + a->in_width) * size}) ||
+      out.meets(Span{a->x_scale, rows * 4}) || out.meets(Span{a->weight_scale, width * 4}) ||
+      out.meets(Span{a->bias, width * bytes(a->bias_dtype)}) ||
+      (!in_place && out.meets(Span{a->residual, ((rows - 1) * a->residual_stride + width) * rs}))) {
+    err = "out overlaps an input (it may be residual where types and strides are the same)";
     return FNMOE_ERR_VALUE;
   }
   LinearView p{};

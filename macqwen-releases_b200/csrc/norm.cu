@@ -221,6 +221,13 @@ __device__ __forceinline__ void store_codes(uint8_t *to, const Columns &k, const
   }
 }
 
+// The larger of two magnitudes; not a number where either is not.
+__device__ __forceinline__ float larger(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 // Sum of `sum` and maximum of `top` (which is not negative) over the G threads of
 // a row: a warp, or the CTA, whose warps meet in `part` (two of them in turn, so
 // that one barrier is enough).
@@ -236,7 +243,7 @@ __device__ __forceinline__ void reduce_row(float &sum, float &top, int G, float2
   for (int i = 0; i < G >> 5; ++i) {
     const float2 o = part[i];
     sum += o.x;
-    top = fmaxf(top, o.y);
+    top = larger(top, o.y);
   }
 }
 
@@ -338,13 +345,12 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           sum = fmaf(s[c][e], s[c][e], sum);
-          top = fmaxf(top, fabsf(s[c][e] * w[e]));  // NaN is left to the sum
+          top = larger(top, fabsf(s[c][e] * w[e]));
         }
         if constexpr (kRes)
           if (p.res_out) store8<D>(static_cast<R *>(p.res_out), k, ra, c, s[c]);
       }
       reduce_row(sum, top, G, part[turn ^= 1]);
-      bool bad = sum != sum;  // not a number somewhere
       float gain = 1.0f;
       if (p.norm) {
         float rms_eps = p.eps;
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
             for (int e = 0; e < 8; ++e) {
               s[c][e] *= down;
               sum = fmaf(s[c][e], s[c][e], sum);
-              top = fmaxf(top, fabsf(s[c][e] * w[e]));
+              top = larger(top, fabsf(s[c][e] * w[e]));
             }
           }
           reduce_row(sum, top, G, part[turn ^= 1]);
@@ -383,10 +389,12 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
         gain = rsqrtf(fmaf(sum, per_dim, rms_eps));  // to 2^-22
       }
       float inv = 0.0f;
+      bool codes_are_0 = false;
       if (p.codes) {
         const float most = top * gain, held = fmaxf(most, kTiny);
         // a row that is not finite has a scale that is not a number, and codes of 0
-        bad |= !(most < __uint_as_float(kInfBits));
+        const bool bad = !(top < __uint_as_float(kInfBits)) || !(most < __uint_as_float(kInfBits));
+        codes_are_0 = bad;
         inv = __fdiv_rn(limit, held);
         if (k.t == 0) p.scales[row] = bad ? __uint_as_float(0x7FC00000u) : __fdiv_rn(held, limit);
       }
@@ -400,7 +408,7 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
         if (p.codes) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[c][e] *= inv;
-          store_codes<D>(p.codes, k, ra, c, s[c], bad, p.e4m3);
+          store_codes<D>(p.codes, k, ra, c, s[c], codes_are_0, p.e4m3);
         }
       }
     }
@@ -568,6 +576,19 @@ int add_rms_norm(const FnNormArgs *a, cudaStream_t s, std::string &err) {
   if (misaligned(a->x, xs) || misaligned(a->y, xs) || misaligned(a->residual, rs) || misaligned(a->residual_out, rs) ||
       (norm && misaligned(a->weight, ws)) || misaligned(a->scales, 4)) {
     err = "arrays must be aligned to their elements";
+    return FNMOE_ERR_VALUE;
+  }
+  const uint64_t rows = a->rows, n = rows * a->dim;
+  const Span x{a->x, ((rows - 1) * a->x_stride + a->dim) * xs}, res{a->residual, ((rows - 1) * a->residual_stride + a->dim) * rs},
+      w{norm ? a->weight : nullptr, a->dim * ws}, y{a->y, n * xs}, out{a->residual_out, n * rs}, codes{a->codes, n},
+      scales{a->scales, rows * 4};
+  // in place: the same rows in the same place
+  const bool y_in_x = a->y == a->x && (rows == 1 || a->x_stride == a->dim),
+             out_in_res = a->residual_out == a->residual && (rows == 1 || a->residual_stride == a->dim);
+  if ((!y_in_x && y.meets(x)) || y.meets(res) || y.meets(w) || y.meets(out) || out.meets(x) || (!out_in_res && out.meets(res)) ||
+      out.meets(w) || codes.meets(x) || codes.meets(res) || codes.meets(w) || codes.meets(y) || codes.meets(out) ||
+      scales.meets(x) || scales.meets(res) || scales.meets(w) || scales.meets(y) || scales.meets(out) || scales.meets(codes)) {
+    err = "outputs overlap inputs or one another (residual_out may be residual, y may be x, where rows are adjacent)";
     return FNMOE_ERR_VALUE;
   }
   NormView p{};

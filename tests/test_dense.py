@@ -81,7 +81,7 @@ def test_linear_refuses_before_any_device_call():
                      ({"activation": 4}, _lib.ERR_UNSUPPORTED), ({"bias_dtype": 2}, _lib.ERR_UNSUPPORTED),
                      ({"out_dtype": 2}, _lib.ERR_UNSUPPORTED), ({"residual_dtype": 2}, _lib.ERR_UNSUPPORTED),
                      ({"in_width": 0}, _lib.ERR_SHAPE), ({"out_width": 0}, _lib.ERR_SHAPE),
-                     ({"in_width": 131073}, _lib.ERR_SHAPE), ({"rows": 0x7FFFFF01}, _lib.ERR_SHAPE),
+                     ({"in_width": 131072}, _lib.ERR_SHAPE), ({"rows": 0x7FFFFF01}, _lib.ERR_SHAPE),
                      ({"x": None}, _lib.ERR_NULL), ({"weight": None}, _lib.ERR_NULL), ({"out": None}, _lib.ERR_NULL),
                      ({"x_scale": 0x8000}, _lib.ERR_NULL), (dict(q, x_scale=None), _lib.ERR_NULL),
                      (dict(q, weight_scale=None), _lib.ERR_NULL), ({"x_stride": 56}, _lib.ERR_SHAPE),
@@ -470,3 +470,47 @@ def test_other_streams_and_graphs(cuda_lib):
             held.zero_()
             gr.replay()
             assert not torch.equal(out, y)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 65])
+def test_weights_that_are_not_finite_show_in_the_scales(cuda_lib, kind, dim):
+    import torch
+
+    from flashnext_b200 import dense
+
+    x = torch.randn(400, dim, device="cuda")
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        w = torch.ones(dim, device="cuda")
+        w[dim - 2] = bad
+        r = dense.add_rms_norm(x, w, codes=_types()[kind], keep=True)
+        assert torch.isnan(r.scales).all() and (r.codes.float() == 0).all() and not torch.isfinite(r.y[:, dim - 2]).any()
+
+
+def test_outputs_that_overlap_inputs_are_refused():
+    lib = _lib.load()
+    a = _lib.FnLinearArgs(_lib.ABI_VERSION, _lib.LINEAR_BF16, 4, 64, 64, 0, 0, 0, 0, 0, 0x1000, 64, 0x2000, 64, None, None,
+                          None, 0x8000, 64, 0x9000)
+    run = lambda **kw: lib.fnmoe_linear(ctypes.byref(_set(a, **kw)), None)  # noqa: E731
+    # x, the weight, a residual one row on, a residual of another type or stride in the same place
+    for kw in ({"out": 0x1000}, {"out": 0x11F0}, {"out": 0x2100}, {"residual": 0x9080}, {"residual": 0x8FF0},
+               {"residual": 0x9000, "residual_dtype": 1}, {"residual": 0x9000, "residual_stride": 72}):
+        assert run(**kw) == _lib.ERR_VALUE, kw
+        assert "overlap" in _lib.last_error(lib)
+    n = _lib.FnNormArgs(_lib.ABI_VERSION, 0, 4, 64, 0, 0, 0, 0, 1e-6, 0, 0x10000, 64, 0x20000, 64, 0x30000, 0x40000, 0x50000,
+                        0x60000, 0x70000)
+    run = lambda **kw: lib.fnmoe_add_rms_norm(ctypes.byref(_set(n, **kw)), None)  # noqa: E731
+    for kw in ({"residual_out": 0x20080}, {"residual_out": 0x10080}, {"y": 0x20100}, {"y": 0x10002}, {"codes": 0x10000},
+               {"y": 0x50000}, {"codes": 0x40010}, {"scales": 0x60000}, {"y": 0x30000},
+               {"residual_out": 0x20000, "residual_stride": 72}, {"y": 0x10000, "x_stride": 72}):
+        assert run(**kw) == _lib.ERR_VALUE, kw
+        assert "overlap" in _lib.last_error(lib)
+
+
+def test_int8_widths_whose_sums_pass_32_bits_are_refused():
+    """128^2 x 131072 is 2^31: rows of -128, which no quantiser here makes, would wrap."""
+    lib = _lib.load()
+    a = _lib.FnLinearArgs(_lib.ABI_VERSION, _lib.LINEAR_INT8, 1, 131072, 1, 0, 0, 0, 0, 0, 0x100000, 131072, 0x200000, 131072,
+                          0x1000, 0x2000, None, None, 0, 0x3000)
+    assert lib.fnmoe_linear(ctypes.byref(a), None) == _lib.ERR_SHAPE
