@@ -9,6 +9,7 @@ loaded or no sm_100 device is present, every op raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -302,6 +303,23 @@ SIGNATURES = {
     "fnmoe_profile_read": ([ctypes.c_char_p, _u32, ctypes.c_int], ctypes.c_int),
 }
 
+_FORMATS = {_vp: "Q", _u32: "I", _u64: "Q", ctypes.c_float: "f", ctypes.c_int32: "i"}
+
+
+def _packer(cls):
+    """Packs the fields of an args structure (0 for NULL) into bytes laid out like it, in half the time that
+    ctypes takes to build one."""
+    packed = struct.Struct("@" + "".join(_FORMATS[kind] for _, kind in cls._fields_))
+    assert packed.size == ctypes.sizeof(cls)
+    return packed.pack
+
+
+# Entry points called as (packed args, stream).
+pack_norm, pack_row_codes, pack_linear, pack_sample = (
+    _packer(c) for c in (FnNormArgs, FnRowCodesArgs, FnLinearArgs, FnSampleArgs))
+PACKED = ("fnmoe_add_rms_norm", "fnmoe_dequantize_rows", "fnmoe_linear", "fnmoe_sample")
+packed: dict = {}
+
 _lock = threading.Lock()
 _handle: ctypes.CDLL | None = None
 
@@ -326,6 +344,8 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
         if lib.fnmoe_abi_version() != ABI_VERSION:
             raise RuntimeError("libfnmoe ABI version mismatch")
         if path is None:
+            call = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, _vp)
+            packed.update((name, call((name, lib))) for name in PACKED)
             _handle = lib
         return lib
 

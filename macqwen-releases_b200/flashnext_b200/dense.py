@@ -15,17 +15,17 @@ be captured in a CUDA graph.  Rows may be slices of wider ones.  Forward only.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Any, NamedTuple
 
 import torch
 
 from . import _lib
-from .paged_q8 import _elsewhere, _ready, _want
+from .paged_q8 import _elsewhere, _want
 
 _FLOATS = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 _CODES = {torch.int8: _lib.Q8_INT8, torch.float8_e4m3fn: _lib.Q8_E4M3}
 _LINEAR = {torch.bfloat16: _lib.LINEAR_BF16, torch.int8: _lib.LINEAR_INT8, torch.float8_e4m3fn: _lib.LINEAR_E4M3}
+_FLT_MAX = 3.4028234663852886e38
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 
 
@@ -80,6 +80,13 @@ def _new(rows, dim, dtype, like):
     return torch.empty_strided((rows, dim), (dim, 1), dtype=dtype, device=like.device)
 
 
+def _ready_stream(index):
+    """The current stream of CUDA device ``index``, which must be the current one, with the library started up."""
+    if torch._C._cuda_getDevice() != index or not _lib._available.get(index):
+        _lib.ensure_device_of(index)  # refuses, or starts the library up
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def add_rms_norm(x, weight, residual=None, eps: float = 1e-6, *, unit_offset: bool = False, codes=None,
                  keep: bool | None = None, residual_out=None) -> NormedRows:
     """``y = s / sqrt(mean(s^2) + eps) * weight`` with ``s = x + residual``, row by row.
@@ -94,21 +101,24 @@ def add_rms_norm(x, weight, residual=None, eps: float = 1e-6, *, unit_offset: bo
     asked for).  A row that is not finite gets NaN as its scale.  ``dim`` is at
     most 16384.
     """
-    index = x.get_device()
-    xd = _float(x, "x")
+    index, dtype = x.get_device(), x.dtype
+    xd = _FLOATS.get(dtype)
+    if xd is None:
+        xd = _float(x, "x")
     xp, rows, dim, xs = _matrix(x, "x", index)
+    wd = _FLOATS.get(weight.dtype)
+    if wd is None:
+        wd = _float(weight, "weight")
     wp = _want(weight, weight.dtype, (dim,), "weight", index)
-    keep = codes is None if keep is None else keep
+    if keep is None:
+        keep = codes is None
     if codes is None and not keep:
         raise ValueError("neither y nor codes are asked for")
-    return _norm(x, xd, xp, rows, dim, xs, weight, wp, residual, eps, _lib.NORM_UNIT_OFFSET if unit_offset else 0, codes,
-                 keep, residual_out, index, "add_rms_norm")
-
-
-def _norm(x, xd, xp, rows, dim, xs, weight, wp, residual, eps, flags, codes, keep, residual_out, index, what):
-    y = q = scales = yp = qp = sp = rp = op = None
-    ct = rs = rd = 0
-    lib, stream = _ready(x)
+    if not 0.0 <= eps <= _FLT_MAX:
+        raise ValueError("eps must be finite and not negative")
+    y = q = scales = None
+    rp = op = yp = qp = sp = rs = rd = ct = 0
+    stream = _ready_stream(index)
     if residual is not None:
         rd = _float(residual, "residual")
         rp, rs = _same(residual, rows, dim, "residual", index)
@@ -120,20 +130,26 @@ def _norm(x, xd, xp, rows, dim, xs, weight, wp, residual, eps, flags, codes, kee
     elif residual_out is not None:
         raise ValueError("residual_out needs residual")
     if keep:
-        y = _new(rows, dim, x.dtype, x)
+        y = _new(rows, dim, dtype, x)
         yp = y.data_ptr()
     if codes is not None:
-        ct = _CODES.get(codes)
-        if ct is None:
-            raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn")
-        q, scales = _new(rows, dim, codes, x), torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device)
-        qp, sp = q.data_ptr(), scales.data_ptr()
-    a = _lib.FnNormArgs(_lib.ABI_VERSION, flags, rows, dim, xd, rd, 0 if weight is None else _float(weight, "weight"), ct,
-                        eps, 0, xp, xs, rp, rs, wp, yp, op, qp, sp)
-    code = lib.fnmoe_add_rms_norm(ctypes.byref(a), stream)
+        ct, q, qp, scales, sp = _code_rows(rows, dim, codes, x)
+    code = _lib.packed["fnmoe_add_rms_norm"](_lib.pack_norm(
+        _lib.ABI_VERSION, _lib.NORM_UNIT_OFFSET if unit_offset else 0, rows, dim, xd, rd, wd, ct, eps, 0, xp, xs, rp, rs, wp,
+        yp, op, qp, sp), stream)
     if code:
-        _lib.check(code, what)
+        _lib.check(code, "add_rms_norm")
     return NormedRows(y, residual_out, q, scales)
+
+
+def _code_rows(rows, dim, codes, like):
+    """New codes and scales: (code type, codes, their pointer, scales, their pointer)."""
+    ct = _CODES.get(codes)
+    if ct is None:
+        raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn")
+    q = _new(rows, dim, codes, like)
+    scales = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=like.device)
+    return ct, q, q.data_ptr(), scales, scales.data_ptr()
 
 
 def quantize_rows(x, codes=torch.int8):
@@ -144,11 +160,13 @@ def quantize_rows(x, codes=torch.int8):
     index = x.get_device()
     xd = _float(x, "x")
     xp, rows, dim, xs = _matrix(x, "x", index)
-    if codes is None:
-        raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn")
-    r = _norm(x, xd, xp, rows, dim, xs, None, None, None, 0.0, _lib.NORM_ROWS_AS_THEY_ARE, codes, False, None, index,
-              "quantize_rows")
-    return r.codes, r.scales
+    stream = _ready_stream(index)
+    ct, q, qp, scales, sp = _code_rows(rows, dim, codes, x)
+    code = _lib.packed["fnmoe_add_rms_norm"](_lib.pack_norm(
+        _lib.ABI_VERSION, _lib.NORM_ROWS_AS_THEY_ARE, rows, dim, xd, 0, 0, ct, 0.0, 0, xp, xs, 0, 0, 0, 0, 0, qp, sp), stream)
+    if code:
+        _lib.check(code, "quantize_rows")
+    return q, scales
 
 
 def dequantize_rows(codes, scales, out_dtype=torch.bfloat16, out=None):
@@ -160,14 +178,14 @@ def dequantize_rows(codes, scales, out_dtype=torch.bfloat16, out=None):
     if len(shape) != 2:
         raise ValueError(f"codes must have two dimensions, not {tuple(shape)}")
     cp, sp = _want(codes, codes.dtype, shape, "codes", index), _want(scales, torch.float32, (shape[0],), "scales", index)
-    lib, stream = _ready(codes)
+    stream = _ready_stream(index)
     if out is None:
         out = _new(shape[0], shape[1], out_dtype, codes)
         op = out.data_ptr()
     else:
         op = _want(out, out.dtype, shape, "out", index)
-    a = _lib.FnRowCodesArgs(_lib.ABI_VERSION, shape[0], shape[1], ct, _float(out, "out"), 0, cp, sp, op)
-    code = lib.fnmoe_dequantize_rows(ctypes.byref(a), stream)
+    code = _lib.packed["fnmoe_dequantize_rows"](_lib.pack_row_codes(
+        _lib.ABI_VERSION, shape[0], shape[1], ct, _float(out, "out"), 0, cp, sp, op), stream)
     if code:
         _lib.check(code, "dequantize_rows")
     return out
@@ -199,8 +217,7 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(map(str, ACTIVATIONS))}, not {activation!r}")
-    xsp = wsp = bp = rp = None
-    bd = rd = rs = 0
+    xsp = wsp = bp = rp = bd = rd = rs = 0
     if kind:
         if x_scale is None or weight_scale is None:
             raise ValueError("8-bit x and weight need x_scale and weight_scale")
@@ -213,7 +230,7 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     if residual is not None:
         rd = _float(residual, "residual")
         rp, rs = _same(residual, rows, n, "residual", index)
-    lib, stream = _ready(x)
+    stream = _ready_stream(index)
     if out is None:
         out = _new(rows, n, torch.bfloat16 if out_dtype is None else out_dtype, x)
         op = out.data_ptr()
@@ -221,9 +238,11 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
         raise TypeError(f"out is {out.dtype}, out_dtype {out_dtype}")
     else:
         op = _want(out, out.dtype, (rows, n), "out", index)
-    a = _lib.FnLinearArgs(_lib.ABI_VERSION, kind, rows, k, n, act, bd, rd, _float(out, "out"), 0, xp, xs, wp, ws, xsp, wsp,
-                          bp, rp, rs, op)
-    code = lib.fnmoe_linear(ctypes.byref(a), stream)
+    od = _FLOATS.get(out.dtype)
+    if od is None:
+        od = _float(out, "out")
+    code = _lib.packed["fnmoe_linear"](_lib.pack_linear(
+        _lib.ABI_VERSION, kind, rows, k, n, act, bd, rd, od, 0, xp, xs, wp, ws, xsp, wsp, bp, rp, rs, op), stream)
     if code:
         _lib.check(code, "linear")
     return out

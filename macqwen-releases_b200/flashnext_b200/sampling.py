@@ -1,30 +1,22 @@
 """The draw of a token from logits (:func:`sample`)."""
 from __future__ import annotations
 
-import ctypes
-import math
+import operator
 
 import torch
 
 from . import _lib
-from .dense import _float, _matrix
-from .paged_q8 import _ready, _want
+from .dense import _FLT_MAX, _float, _matrix, _ready_stream
+from .paged_q8 import _want
 
 MAX_VOCAB = _lib.SAMPLE_MAX_VOCAB
 
 
 def _setting(v, dtype, rows, what, index):
-    """(pointer of a [rows] tensor, or None; value where it is a number)."""
+    """(pointer of a [rows] tensor, or 0; value where it is a number)."""
     if isinstance(v, torch.Tensor):
         return _want(v, dtype, (rows,), what, index), 0
-    return None, v
-
-
-def _number(v, what):
-    v = float(v)
-    if not math.isfinite(v):
-        raise ValueError(f"{what} must be finite")
-    return v
+    return 0, v
 
 
 def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -56,22 +48,22 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     kp, k = _setting(top_k, torch.int32, rows, "top_k", index)
     pp, p = _setting(top_p, f32, rows, "top_p", index)
     mp, m = _setting(min_p, f32, rows, "min_p", index)
-    if tp is None and _number(t, "temperature") < 0:
-        raise ValueError("temperature must not be negative")
-    if kp is None and not -2 ** 31 <= k < 2 ** 31:
+    if not tp and not 0.0 <= t <= _FLT_MAX:
+        raise ValueError("temperature must be finite and not negative")
+    if not kp and not -2 ** 31 <= operator.index(k) < 2 ** 31:
         raise ValueError("top_k must fit 32 bits")
-    if pp is None and _number(p, "top_p") < 0:
-        raise ValueError("top_p must not be negative")
-    if mp is None and not 0 <= _number(m, "min_p") <= 1:
+    if not pp and not 0.0 <= p <= _FLT_MAX:
+        raise ValueError("top_p must be finite and not negative")
+    if not mp and not 0.0 <= m <= 1.0:
         raise ValueError("min_p must be between 0 and 1")
     up = _want(uniform, f32, (rows,), "uniform", index)
-    lib, stream = _ready(logits)
+    stream = _ready_stream(index)
     device = logits.device
     tokens = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)
     logprobs = torch.empty_strided((rows,), (1,), dtype=f32, device=device)
-    a = _lib.FnSampleArgs(_lib.ABI_VERSION, rows, vocab, dtype, lp, stride, up, tp, kp, pp, mp, t, k, p, m,
-                          tokens.data_ptr(), logprobs.data_ptr())
-    code = lib.fnmoe_sample(ctypes.byref(a), stream)
+    code = _lib.packed["fnmoe_sample"](_lib.pack_sample(
+        _lib.ABI_VERSION, rows, vocab, dtype, lp, stride, up, tp, kp, pp, mp, t, k, p, m, tokens.data_ptr(),
+        logprobs.data_ptr()), stream)
     if code:
         _lib.check(code, "sample")
     return tokens, logprobs
