@@ -276,6 +276,25 @@ __device__ void draw_from_list(const SampleView &p, int row, const Settings &set
   if (part == 0 && lower <= drawn && drawn < lower + held) write_row(p, row, index, logit_at(mine), weights, total);
 }
 
+// The least float, in the order of place_of, at or below `most` for which `above`
+// holds; `above` rises with it and holds for `most`.  By its bits, five at a time:
+// a lane a candidate (a whole warp calls it).
+template <typename F>
+__device__ __forceinline__ float least_float(float most, F &&above) {
+  const uint32_t lane = threadIdx.x & 31, end = ~static_cast<uint32_t>(place_of(most, 0) >> kIndexBits);
+  uint32_t below = 0u;  // the largest for which it does not hold, as far as it is known
+#pragma unroll 1
+  for (int shift = 27; shift > -5; shift -= 5) {
+    const uint32_t key = below | (shift >= 0 ? lane << shift : lane >> -shift);
+    const float x = __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
+    // what is not a number sorts below -infinity: no; above infinity: past `most`
+    const uint32_t less = __ballot_sync(0xFFFFFFFFu, !(key >= end || (x >= kMinusInf && above(x))));
+    below = __shfl_sync(0xFFFFFFFFu, key, 31 - __clz(less));  // lane 0 is always among them
+  }
+  const uint32_t first = below + 1u;
+  return __uint_as_float((first & 0x80000000u) ? first & 0x7FFFFFFFu : ~first);
+}
+
 // One row, in a cluster of p.ctas CTAs.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
@@ -461,12 +480,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
     const uint32_t want = static_cast<uint32_t>(set.top_k);
     const Cut among = by_mass ? weighing(cut) : cut;
     // ranges of the first round: equal parts of the logits that can matter
-    float span = __fsub_rn(hi, lo);
+    float span = fminf(__fsub_rn(hi, lo), 0x1p127f);
     if (by_mass) span = fminf(span, __fsub_rn(hi, weights.low));
-    const float per = span > 0.0f ? __fdiv_rn(static_cast<float>(kBins), span) : 0.0f;
-    auto range_of = [&](float l) {  // rises (weakly) with falling logits
-      return static_cast<uint32_t>(min(max(static_cast<int>(__fmul_rn(__fsub_rn(hi, l), per)), 0), kBins - 1));
-    };
+    const float per = span > 0.0f ? __fdiv_rn(static_cast<float>(kBins - 1), span) : 0.0f;
+    // 2^23 and the range, the nearest whole number, which rises (weakly) with
+    // falling logits; where the largest is infinite all are in the last one
+    auto spot = [&](float l) { return fmaf(fminf(__fsub_rn(hi, l), span), per, 0x1p23f); };
+    auto range_of = [&](float l) { return __float_as_uint(spot(l)) & (kBins - 1); };
     uint32_t range = 0;   // chosen in the first round
     uint64_t prefix = 0;  // of (logit, index), chosen in later rounds
     uint32_t before_count = 0;
@@ -565,11 +585,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
       before_mass = s.hit_before_mass;
       const bool all_of_it = round == 0 && before_count + inside <= kFew;  // the ranges above as well
       if (all_of_it || inside <= kList) {
+        // the first round's ranges by their ends: two comparisons instead of the range of every logit
+        const float at_bin = 0x1p23f + static_cast<float>(bin), none = -kMinusInf;
+        const float from = least_float(hi, [&](float x) { return spot(x) <= at_bin; });
+        const float until = all_of_it || bin == 0u || hi == none ? none : least_float(hi, [&](float x) { return spot(x) < at_bin; });
         each4([&](const float (&l)[4], int i) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
+            if (round == 0) {
+              if (!(l[e] >= from && (l[e] < until || until == none))) continue;
+            } else if (bin_of(l[e], i + e) != bin) {
+              continue;
+            }
             if (!among.keeps(l[e], static_cast<int>(begin) + i + e)) continue;
-            if (all_of_it ? range_of(l[e]) > bin : bin_of(l[e], i + e) != bin) continue;
             append(place_of(l[e], begin + static_cast<uint32_t>(i + e)), by_mass && !all_of_it ? weights.of(l[e]) : 0ull);
           }
         });
@@ -648,21 +676,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
 
   // ---- the draw: kept weights summed block by block, and walked by index in the block drawn ----
   if (set.min_p > 0.0f) {
-    // The least float whose weight is min_p or more, by its bits in rising order,
-    // five at a time: a lane a candidate.  (The formula's inverse is not near
-    // enough where it comes out next to 0.)
-    const uint32_t most = ~static_cast<uint32_t>(place_of(hi, 0) >> kIndexBits);
-    uint32_t below = 0u;  // the largest that weighs less, as far as it is known
-#pragma unroll 1
-    for (int shift = 27; shift > -5; shift -= 5) {
-      const uint32_t key = below | (shift >= 0 ? static_cast<uint32_t>(lane) << shift : static_cast<uint32_t>(lane) >> -shift);
-      const float x = __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
-      const uint32_t less = __ballot_sync(0xFFFFFFFFu, !(key >= most || weights.exponent(x) >= least));
-      const int last = 31 - __clz(less);  // lane 0 always weighs less
-      below = __shfl_sync(0xFFFFFFFFu, key, last);
-    }
-    const uint32_t first = below + 1u;
-    const float l = __uint_as_float((first & 0x80000000u) ? first & 0x7FFFFFFFu : ~first);
+    // (The formula's inverse is not near enough where it comes out next to 0.)
+    const float l = least_float(hi, [&](float x) { return weights.exponent(x) >= least; });
     if (l > cut.l) cut = Cut{l, kEvery};
   }
   const Cut kept = weighing(cut);

@@ -308,3 +308,19 @@ def test_min_p_whose_logit_lies_next_to_zero(cuda_lib, sign):
     x = torch.tensor([[float(hi), 3.0, 2.0, 1.0, 0.5, 0.0, -0.5, -1.0, 1e-20, -1e-20] * 400], device="cuda").repeat(48, 1)
     u = (torch.arange(48, device="cuda", dtype=torch.float32) + 0.5) / 48
     _check(x.contiguous(), u, torch.from_numpy(temps[i]).cuda(), 0, 1.0, torch.from_numpy(mins[j]).cuda())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_many_infinite_and_far_apart_logits(cuda_lib, dtype, form):
+    """More infinities than a list holds, and logits whose distance from the largest is past float32's range."""
+    import torch
+
+    x, u = _rows(4, 7001, getattr(torch, dtype), 50 + form)
+    x[0, ::15] = INF                      # 467 of them
+    x[1, ::3] = INF                       # 2334
+    x[2, 4000:] = torch.finfo(x.dtype).min
+    x[2, ::11] = torch.finfo(x.dtype).max
+    x[3] *= 1e37
+    _check(x, u, **FORMS[form])
