@@ -284,8 +284,12 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
     return __fadd_rn(p.w_f32 ? static_cast<const float *>(p.w)[i] : bf16_to_f32(static_cast<const uint16_t *>(p.w)[i]), p.offset);
   };
   if (D != kEven && p.norm) {
+    // kFlat: zeros where there is no column, which masked values are multiplied by
+    const int slots = D == kFlat ? 8 * pitch : p.dim;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < p.dim; i += blockDim.x) weight[D == kFlat ? (i & 7) * pitch + (i >> 3) : i] = weight_at(i);
+    for (int i = threadIdx.x; i < slots; i += blockDim.x)
+      weight[D == kFlat ? (i & 7) * pitch + (i >> 3) : i] = i < p.dim ? weight_at(i) : 0.0f;
+    if (D == kFlat && threadIdx.x == 0) weight[slots] = 0.0f;
     __syncthreads();
   }
   // this thread's weights of chunk c (where there is no value: anything, it counts as 0)
@@ -313,7 +317,8 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
         for (int e = 0; e < 8; ++e) w[e] = __fadd_rn(w[e], p.offset);
       }
     } else if constexpr (D == kFlat) {
-      const float *at = weight + min(c * G + k.t, pitch - 1);
+      // (a row's last chunk may be one past dim / 8; only values before its skew count there)
+      const float *at = weight + min(c * G + k.t, pitch);
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = at[((e - ra.skew) & 7) * pitch - (e < ra.skew ? 1 : 0)];
     } else {
@@ -492,7 +497,7 @@ bool misaligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t
 
 template <Deal D, int VPT, typename TX, typename TR>
 cudaError_t launch_k(const NormView &p, int per, int G, cudaStream_t s) {
-  const size_t smem = p.norm && D != kEven ? (static_cast<size_t>(p.dim) / 8 + 1) * 8 * sizeof(float) : 0;
+  const size_t smem = p.norm && D != kEven ? ((static_cast<size_t>(p.dim) / 8 + 1) * 8 + 1) * sizeof(float) : 0;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(k_norm<D, VPT, TX, TR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(smem));

@@ -514,3 +514,27 @@ def test_int8_widths_whose_sums_pass_32_bits_are_refused():
     a = _lib.FnLinearArgs(_lib.ABI_VERSION, _lib.LINEAR_INT8, 1, 131072, 1, 0, 0, 0, 0, 0, 0x100000, 131072, 0x200000, 131072,
                           0x1000, 0x2000, None, None, 0, 0x3000)
     assert lib.fnmoe_linear(ctypes.byref(a), None) == _lib.ERR_SHAPE
+
+
+@gpu
+@pytest.mark.parametrize("rows", [9, 700])
+@pytest.mark.parametrize("dim", [*range(1, 42), 252, 253, 255, 1021, 2053, 2559, 4101, 8189, 16373, 16375, 16376])
+def test_norm_of_contiguous_rows_of_any_width(cuda_lib, rows, dim):
+    """Rows laid end to end start at every offset from a boundary of eight and end at every other."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    if rows * dim > 2_000_000:
+        rows = 17
+    t, g = _types(), _gen(dim)
+    w = torch.randn(dim, device="cuda", generator=g)
+    for xd, rd in (("bf16", None), ("f32", None), ("bf16", "bf16"), ("f32", "bf16")):
+        x = torch.randn(rows, dim, device="cuda", generator=g).to(t[xd])
+        res = None if rd is None else torch.randn(rows, dim, device="cuda", generator=g).to(t[rd])
+        got = dense.add_rms_norm(x, w, res, 1e-5, codes=torch.int8, keep=True)
+        y, s = od.add_rms_norm(_np(x), _np(w), None if res is None else _np(res), 1e-5)
+        assert (np.abs(_np(got.y) - y) <= np.abs(y) * (HALF[xd] + 2.0 ** -18) + 1e-37).all()
+        if rd:
+            assert (np.abs(_np(got.residual) - s) <= np.abs(s) * (HALF[rd] + 2.0 ** -23) + 1e-37).all()
+        _held(got.codes, got.scales, y, "int8")
