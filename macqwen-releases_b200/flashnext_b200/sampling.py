@@ -37,7 +37,10 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     ``min_p`` <= 0 keep everything; ``temperature`` 0, ``top_k`` 1 or ``top_p``
     0 take the largest logit (log-probability 0).  Logits of -infinity and NaN
     are never taken; a row of nothing else has token -1.  The result does not
-    depend on how the work is divided: weights are summed as exact integers.
+    depend on how the work is divided: weights are summed as exact integers,
+    in units of 2^-44 of the largest token's.  So a log-probability is off by at
+    most 2^-44 a kept token besides its rounding to float32: that of a token
+    with almost all of the weight, itself near 0, has fewer significant digits.
     ``vocab`` is at most 262144.
     """
     index = logits.get_device()
