@@ -482,7 +482,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
     // ranges of the first round: equal parts of the logits that can matter
     float span = fminf(__fsub_rn(hi, lo), 0x1p127f);
     if (by_mass) span = fminf(span, __fsub_rn(hi, weights.low));
-    const float per = span > 0.0f ? __fdiv_rn(static_cast<float>(kBins - 1), span) : 0.0f;
+    // (Logits that lie closer than 2^-100 share a range, and the digits divide
+    // it: the quotient stays finite, so that ranges always rise.)
+    span = fmaxf(span, 0x1p-100f);
+    const float per = __fdiv_rn(static_cast<float>(kBins - 1), span);
     // 2^23 and the range, the nearest whole number, which rises (weakly) with
     // falling logits; where the largest is infinite all are in the last one
     auto spot = [&](float l) { return fmaf(fminf(__fsub_rn(hi, l), span), per, 0x1p23f); };

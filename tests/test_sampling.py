@@ -324,3 +324,44 @@ def test_many_infinite_and_far_apart_logits(cuda_lib, dtype, form):
     x[2, ::11] = torch.finfo(x.dtype).max
     x[3] *= 1e37
     _check(x, u, **FORMS[form])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("vocab", [300, 500, 3000, 20000])
+@pytest.mark.parametrize("spread", [1e-45, 1e-41, 1e-38, 2.9e-36, 1e-35, 1e-30])
+def test_close_logits(cuda_lib, dtype, vocab, spread):
+    """Logits that differ by so little that a range of them, or the ranges in one of their differences, is no float."""
+    import torch
+
+    step = max(spread, 2.0 ** -133) if dtype == "bfloat16" else spread  # the least bfloat16
+    x = torch.zeros(6, vocab, device="cuda")
+    x[0, ::2] = step
+    x[1, vocab // 3] = step
+    x[2] = torch.randint(0, 8, (vocab,), device="cuda", generator=_gen(vocab)).float() * step
+    x[3, : 2 * vocab // 3] = -step
+    x[4] = 1.0
+    x[5, 1::3] = -step
+    x[5, ::400] = -INF
+    x = x.to(getattr(torch, dtype))
+    u = torch.tensor([0.0, 0.999, 0.4321, 0.77, 0.5, 0.123], device="cuda")
+    for form in ({"top_k": 250}, {"top_k": 300, "top_p": 0.7}, {"top_p": 0.5}, {"top_p": 0.99, "min_p": 0.5},
+                 {"temperature": 1e-38, "top_p": 0.6}, {"temperature": 1e-38, "top_k": 280}):
+        _check(x, u, **form)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("ties", [100, 385, 450, 512, 600, 2500])
+@pytest.mark.parametrize("temperature", [1e-45, 1e-40, 1e-38, 9e-38, 1e-37, 1e-30])
+def test_small_temperatures(cuda_lib, dtype, ties, temperature):
+    """The largest logit, 0, many times over: it alone weighs something, however far below the others lie."""
+    import torch
+
+    x = torch.full((3, 3000), -1.0, device="cuda")
+    x[:, 7:7 + ties] = 0.0
+    x[1, 2700:] = -1e-38
+    x[2, ::5] = -2e-38
+    u = torch.tensor([0.999, 0.3, 0.65], device="cuda")
+    for form in ({"top_p": 0.5}, {"top_p": 0.97}, {"top_k": 400, "top_p": 0.8}, {"top_k": 2000}):
+        _check(x.to(getattr(torch, dtype)), u, temperature=temperature, **form)
