@@ -360,8 +360,10 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
       if (p.norm) {
         float rms_eps = p.eps;
         // Rows whose squares or products leave float32's range (or lose bits
-        // below it) are scaled by a power of two first.
-        if (!(sum <= 0x1p120f) || !(top <= 0x1p125f) || (sum < 0x1p-80f && p.eps < 0x1p-80f)) {
+        // below it) are scaled by a power of two first.  (A product below the
+        // normal range is off by several per cent, and codes made by such a
+        // maximum would pass 127.  Where all are 0, max |y| stays below 2^-100.)
+        if (!(sum <= 0x1p120f) || !(top <= 0x1p125f) || (sum < 0x1p-80f && p.eps < 0x1p-80f) || (top < 0x1p-100f && top > 0.0f)) {
           float most = 0.0f, none = 0.0f;
 #pragma unroll
           for (int c = 0; c < VPT; ++c)

@@ -538,3 +538,25 @@ def test_norm_of_contiguous_rows_of_any_width(cuda_lib, rows, dim):
         if rd:
             assert (np.abs(_np(got.residual) - s) <= np.abs(s) * (HALF[rd] + 2.0 ** -23) + 1e-37).all()
         _held(got.codes, got.scales, y, "int8")
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,dim,pad", [(3, 4096, 0), (3, 4097, 0), (5, 4096, 3), (700, 4096, 0), (700, 1027, 1)])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 2.0 ** -79])
+def test_weights_whose_products_leave_the_normal_range(cuda_lib, kind, rows, dim, pad, eps):
+    """Rows and weights whose products are subnormal, or 0, although y is not."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    g = _gen(dim + rows)
+    rand = lambda *s: torch.rand(*s, device="cuda", generator=g)  # noqa: E731
+    sign = lambda *s: torch.where(rand(*s) < 0.5, -1.0, 1.0)  # noqa: E731
+    for size, small in ((2.0 ** -45, 2.0 ** -100), (2.0 ** -41, 2.0 ** -98), (2.0 ** -30, 2.0 ** -110), (1.0, 2.0 ** -104)):
+        x = _cut((1 + rand(rows, dim)) * sign(rows, dim) * size, pad)
+        w = (1 + rand(dim)) * small
+        got = dense.add_rms_norm(x, w, None, eps, codes=_types()[kind], keep=True)
+        y, _ = od.add_rms_norm(_np(x), _np(w), None, float(np.float32(eps)))
+        assert (np.abs(_np(got.y) - y) <= np.abs(y) * 2.0 ** -17 + 2.0 ** -140).all()
+        _held(got.codes, got.scales, y, kind)
