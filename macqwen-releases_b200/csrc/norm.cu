@@ -370,10 +370,12 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[c][e]));
           reduce_row(none, most, G, part[turn ^= 1]);
-          // by 2^-e with 2^e about the larger of max |s| and sqrt(eps); by 1 where that is 0 or not finite
+          // by 2^-e with 2^e the power of two above max |s|, so that no product passes
+          // the weight, or about sqrt(eps) where that is larger; by 1 where max |s| is 0
+          // or not finite (2^-128 is below the normal range, but exact)
           int e2 = 0;
           if (most != 0.0f && most < __uint_as_float(kInfBits)) {
-            e2 = max(-126, min(126, ilogbf(most)));
+            e2 = max(-126, ilogbf(most) + 1);
             if (p.eps > 0.0f) e2 = max(e2, ilogbf(p.eps) / 2);
           }
           const float down = ldexpf(1.0f, -e2);

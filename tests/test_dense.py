@@ -560,3 +560,22 @@ def test_weights_whose_products_leave_the_normal_range(cuda_lib, kind, rows, dim
         y, _ = od.add_rms_norm(_np(x), _np(w), None, float(np.float32(eps)))
         assert (np.abs(_np(got.y) - y) <= np.abs(y) * 2.0 ** -17 + 2.0 ** -140).all()
         _held(got.codes, got.scales, y, kind)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,dim", [(2, 64), (3, 65), (600, 2048)])
+@pytest.mark.parametrize("size", [1.5, 1e-20, 3e38])
+def test_weights_next_to_the_largest_float(cuda_lib, kind, rows, dim, size):
+    """y is finite although a row's own values times the weight are not."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    g = _gen(dim + rows)
+    x = (1.0 - 2.0 ** -10 * torch.rand(rows, dim, device="cuda", generator=g)) * size
+    w = torch.full((dim,), 3.3e38, device="cuda")
+    got = dense.add_rms_norm(x, w, None, 0.0, codes=_types()[kind], keep=True)
+    y, _ = od.add_rms_norm(_np(x), _np(w), None, 0.0)
+    assert (np.abs(_np(got.y) - y) <= np.abs(y) * 2.0 ** -17).all()
+    _held(got.codes, got.scales, y, kind)
