@@ -32,8 +32,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-
 #include "async.cuh"
 #include "common.cuh"
 #include "q8_ranges.cuh"
@@ -234,21 +232,6 @@ __device__ __forceinline__ int page_col(const Q8View &p, int pos) {
 __device__ __forceinline__ int tokens_of(const Q8View &p, int b) {
   return max(0, min(p.ctx[b], p.width * p.page));
 }
-
-// A kernel's shared-memory limit, set once on each device (the attribute
-// belongs to the device's copy of the kernel).
-struct SmemLimit {
-  std::atomic<uint64_t> done{0};
-  cudaError_t set(const void *kernel, int bytes) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (e != cudaSuccess || (done.load(std::memory_order_acquire) & bit)) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-    return e;
-  }
-};
 
 // The many-row kernels (attention_q8_many.cu).
 int many_ctas(int head_dim);

@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace fnmoe {
 
 constexpr uint32_t kSlotBit = 0x80000000u;
@@ -243,5 +245,21 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
+
+// A kernel's shared-memory limit, set once on each device (the attribute
+// belongs to the device's copy of the kernel): to the most that any launch asks
+// for, since one thread's smaller limit could come between another's and its launch.
+struct SmemLimit {
+  std::atomic<uint64_t> done{0};
+  cudaError_t set(const void *kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (e != cudaSuccess || (done.load(std::memory_order_acquire) & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 }  // namespace fnmoe

@@ -499,12 +499,15 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(const uint8_t *codes, c
 
 bool misaligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
+// Bytes of a row's weights in shared memory (kFlat's eight columns of them and a zero; kOdd takes fewer).
+constexpr int weight_smem(uint32_t dim) { return static_cast<int>(((dim / 8 + 1) * 8 + 1) * sizeof(float)); }
+
 template <Deal D, int VPT, typename TX, typename TR>
 cudaError_t launch_k(const NormView &p, int per, int G, cudaStream_t s) {
-  const size_t smem = p.norm && D != kEven ? ((static_cast<size_t>(p.dim) / 8 + 1) * 8 + 1) * sizeof(float) : 0;
+  const size_t smem = p.norm && D != kEven ? weight_smem(static_cast<uint32_t>(p.dim)) : 0;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k_norm<D, VPT, TX, TR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
+    static SmemLimit limit;
+    const cudaError_t e = limit.set(reinterpret_cast<const void *>(k_norm<D, VPT, TX, TR>), weight_smem(kMaxDim));
     if (e != cudaSuccess) return e;
   }
   // as many CTAs as stay on the SMs: 1024 threads (512 where a thread holds more of a row)

@@ -765,18 +765,22 @@ cudaError_t launch(SampleView p, int rows, int sms, cudaStream_t s) {
   // CTAs of a row: as many as finish soonest, by rounds over the SMs (two CTAs
   // each) times a CTA's tokens and about 8000 tokens' time for its barriers.
   constexpr int kMost = 72 * 1024 / sizeof(T);  // tokens that leave room for a second CTA
+  constexpr int kMostBytes = 160 * 1024;         // of a CTA's tokens
+  constexpr size_t kFirst = (sizeof(Shared) + 15) / 16 * 16 + 16;
+  static_assert(kFirst + kMostBytes <= 227 * 1024, "shared memory");
   constexpr int64_t kFixed = 8000;
   int64_t least = INT64_MAX;
   for (int c = 1; c <= kMaxCtas; c *= 2) {
     const int64_t slice = (p.vocab + c - 1) / c;
-    if (slice > kMaxBlocks * kBlock || slice * sizeof(T) > 160 * 1024) continue;
+    if (slice > kMaxBlocks * kBlock || slice * sizeof(T) > kMostBytes) continue;
     const int64_t slots = static_cast<int64_t>(sms) * (slice > kMost ? 1 : 2);
     const int64_t time = (static_cast<int64_t>(rows) * c + slots - 1) / slots * (slice + kFixed);
     if (time < least) least = time, p.ctas = c;
   }
   p.slice = (p.vocab + p.ctas - 1) / p.ctas;
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + 16 + static_cast<size_t>(p.slice) * sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const size_t smem = kFirst + static_cast<size_t>(p.slice) * sizeof(T);
+  static SmemLimit limit;
+  cudaError_t e = limit.set(reinterpret_cast<const void *>(k_sample<T>), static_cast<int>(kFirst + kMostBytes));
   if (e == cudaSuccess && p.ctas > 8) e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};

@@ -365,3 +365,45 @@ def test_small_temperatures(cuda_lib, dtype, ties, temperature):
     u = torch.tensor([0.999, 0.3, 0.65], device="cuda")
     for form in ({"top_p": 0.5}, {"top_p": 0.97}, {"top_k": 400, "top_p": 0.8}, {"top_k": 2000}):
         _check(x.to(getattr(torch, dtype)), u, temperature=temperature, **form)
+
+
+@gpu
+def test_two_threads_with_rows_of_different_widths(cuda_lib):
+    """A call's shared memory depends on its rows: what one thread sets for its own must not refuse another's."""
+    import threading
+
+    import torch
+
+    from flashnext_b200 import dense, sampling
+
+    def draw(rows, vocab):
+        x, u = _rows(rows, vocab, torch.float32, vocab)
+        return lambda: sampling.sample(x, u, 0.8, 50, 0.9)
+
+    def norm(dim):
+        x, w = torch.randn(3, dim, device="cuda"), torch.ones(dim, device="cuda")
+        return lambda: dense.add_rms_norm(x, w)[:1]
+
+    for jobs in ((draw(1, 1000), draw(64, 131072), draw(3, 40000)), (norm(13001), norm(16375), norm(14003))):
+        want = [job() for job in jobs]
+        torch.cuda.synchronize()
+        start, wrong = threading.Barrier(len(jobs)), []
+
+        def work(job, out):
+            try:
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    start.wait()
+                    for _ in range(3000):
+                        got = job()
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, out)):
+                        wrong.append("another result")
+            except Exception as e:  # noqa: BLE001
+                wrong.append(str(e))
+
+        threads = [threading.Thread(target=work, args=j) for j in zip(jobs, want)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong
