@@ -457,7 +457,7 @@ typedef struct FnRowCodesArgs {
   uint32_t reserved;
   const void *codes;           /* [rows, dim] */
   const float *scales;         /* [rows] */
-  void *out;                   /* [rows, dim] */
+  void *out;                   /* [rows, dim]; overlaps neither codes nor scales */
 } FnRowCodesArgs;
 
 #define FNMOE_LINEAR_BF16 0u   /* bfloat16 x and weight, float32 sums */

@@ -648,8 +648,13 @@ int dequantize_rows(const FnRowCodesArgs *a, cudaStream_t s, std::string &err) {
     err = "scales and out must be aligned to their elements";
     return FNMOE_ERR_VALUE;
   }
-  const bool vec = !misaligned(a->codes, 16) && !misaligned(a->out, 16);
   const uint64_t count = static_cast<uint64_t>(a->rows) * a->dim;
+  const Span out{a->out, count * (f32 ? 4 : 2)};
+  if (out.meets(Span{a->codes, count}) || out.meets(Span{a->scales, static_cast<uint64_t>(a->rows) * 4})) {
+    err = "out overlaps codes or scales";
+    return FNMOE_ERR_VALUE;
+  }
+  const bool vec = !misaligned(a->codes, 16) && !misaligned(a->out, 16);
   const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((count + 4095) / 4096, 1u << 20)));
   const uint8_t *c = static_cast<const uint8_t *>(a->codes);
   cudaError_t e;

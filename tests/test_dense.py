@@ -579,3 +579,14 @@ def test_weights_next_to_the_largest_float(cuda_lib, kind, rows, dim, size):
     y, _ = od.add_rms_norm(_np(x), _np(w), None, 0.0)
     assert (np.abs(_np(got.y) - y) <= np.abs(y) * 2.0 ** -17).all()
     _held(got.codes, got.scales, y, kind)
+
+
+def test_values_that_overlap_codes_or_scales_are_refused():
+    lib = _lib.load()
+    a = _lib.FnRowCodesArgs(_lib.ABI_VERSION, 4, 64, 0, 0, 0, 0x1000, 0x2000, 0x3000)
+    run = lambda **kw: lib.fnmoe_dequantize_rows(ctypes.byref(_set(a, **kw)), None)  # noqa: E731
+    # 256 codes, 16 bytes of scales, 512 or 1024 bytes of values
+    for kw in ({"out": 0x1000}, {"out": 0x10FE}, {"out": 0xE02}, {"out": 0xC04, "out_dtype": 1}, {"out": 0x2000},
+               {"out": 0x200E}, {"out": 0x1E02}, {"out": 0x1C04, "out_dtype": 1}):
+        assert run(**kw) == _lib.ERR_VALUE, kw
+        assert "overlap" in _lib.last_error(lib)
