@@ -521,7 +521,7 @@ typedef struct FnSampleArgs {
   int32_t top_k;
   float top_p;
   float min_p;
-  int64_t *tokens;             /* [rows] */
+  int64_t *tokens;             /* [rows]; outputs overlap neither inputs nor one another */
   float *logprobs;             /* [rows] or NULL: the token's log-probability among the kept */
 } FnSampleArgs;
 

@@ -825,6 +825,15 @@ int sample(const FnSampleArgs *a, cudaStream_t s, std::string &err) {
     err = "arrays must be aligned to their elements";
     return FNMOE_ERR_VALUE;
   }
+  const uint64_t rows64 = a->rows;
+  const Span tokens{a->tokens, rows64 * 8}, logprobs{a->logprobs, rows64 * 4};
+  const Span inputs[] = {
+      {a->logits, ((rows64 - 1) * a->logits_stride + a->vocab) * (a->logits_dtype == FNMOE_DTYPE_F32 ? 4 : 2)},
+      {a->uniform, rows64 * 4}, {a->temperatures, rows64 * 4}, {a->top_ks, rows64 * 4}, {a->top_ps, rows64 * 4},
+      {a->min_ps, rows64 * 4}};
+  bool overlap = tokens.meets(logprobs);
+  for (const Span &in : inputs) overlap = overlap || tokens.meets(in) || logprobs.meets(in);
+  if (overlap) { err = "tokens and logprobs overlap inputs or one another"; return FNMOE_ERR_VALUE; }
   SampleView p{};
   p.logits = a->logits;
   p.uniform = a->uniform;

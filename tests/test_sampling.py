@@ -407,3 +407,24 @@ def test_two_threads_with_rows_of_different_widths(cuda_lib):
         for t in threads:
             t.join()
         assert not wrong
+
+
+def test_outputs_that_overlap_are_refused():
+    """Rows of a call are drawn side by side: a token written over another row's inputs would change that row's draw."""
+    lib = _lib.load()
+    a = _lib.FnSampleArgs(_lib.ABI_VERSION, 4, 100, 1, 0x10000, 128, 0x2000, 0x3000, 0x4000, 0x5000, 0x6000, 1.0, 0, 1.0, 0.0,
+                          0x7000, 0x8000)
+
+    def run(**kw):
+        b = _lib.FnSampleArgs.from_buffer_copy(a)
+        for k, v in kw.items():
+            setattr(b, k, v)
+        return lib.fnmoe_sample(ctypes.byref(b), None)
+
+    # 4 rows: 32 bytes of tokens, 16 of log-probabilities and of each setting, 1936 of logits (float32)
+    for kw in ({"tokens": 0x10000}, {"tokens": 0x10788}, {"tokens": 0xFFE8}, {"logprobs": 0x1078C}, {"logprobs": 0xFFF4},
+               {"tokens": 0x2008}, {"logprobs": 0x200C}, {"tokens": 0x2FE8}, {"logprobs": 0x3000}, {"tokens": 0x4000},
+               {"logprobs": 0x4004}, {"tokens": 0x5008}, {"logprobs": 0x4FF4}, {"tokens": 0x5FE8}, {"logprobs": 0x6008},
+               {"logprobs": 0x701C}, {"tokens": 0x8008}):
+        assert run(**kw) == _lib.ERR_VALUE, kw
+        assert "overlap" in _lib.last_error(lib)
