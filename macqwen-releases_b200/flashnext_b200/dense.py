@@ -169,8 +169,8 @@ def quantize_rows(x, codes=torch.int8):
     return q, scales
 
 
-def dequantize_rows(codes, scales, out_dtype=torch.bfloat16, out=None):
-    """The values ``codes[r] * scales[r]``, rounded once to ``out_dtype`` (bfloat16 or float32)."""
+def dequantize_rows(codes, scales, out_dtype=None, out=None):
+    """The values ``codes[r] * scales[r]``, rounded once to ``out_dtype`` (bfloat16, the default, or float32)."""
     ct = _CODES.get(codes.dtype)
     if ct is None:
         raise TypeError("codes must be an int8 or float8_e4m3fn tensor")
@@ -180,8 +180,10 @@ def dequantize_rows(codes, scales, out_dtype=torch.bfloat16, out=None):
     cp, sp = _want(codes, codes.dtype, shape, "codes", index), _want(scales, torch.float32, (shape[0],), "scales", index)
     stream = _ready_stream(index)
     if out is None:
-        out = _new(shape[0], shape[1], out_dtype, codes)
+        out = _new(shape[0], shape[1], torch.bfloat16 if out_dtype is None else out_dtype, codes)
         op = out.data_ptr()
+    elif out_dtype is not None and out.dtype is not out_dtype:
+        raise TypeError(f"out is {out.dtype}, out_dtype {out_dtype}")
     else:
         op = _want(out, out.dtype, shape, "out", index)
     code = _lib.packed["fnmoe_dequantize_rows"](_lib.pack_row_codes(

@@ -590,3 +590,23 @@ def test_values_that_overlap_codes_or_scales_are_refused():
                {"out": 0x200E}, {"out": 0x1E02}, {"out": 0x1C04, "out_dtype": 1}):
         assert run(**kw) == _lib.ERR_VALUE, kw
         assert "overlap" in _lib.last_error(lib)
+
+
+@gpu
+def test_values_out_and_out_dtype_have_to_agree(cuda_lib):
+    import torch
+
+    from flashnext_b200 import dense
+
+    codes, scales = dense.quantize_rows(torch.randn(3, 48, device="cuda"))
+    out = torch.empty(3, 48, device="cuda")
+    for call in (dense.dequantize_rows, lambda *a, **kw: dense.dequantize_rows(a[0].float().to(torch.float8_e4m3fn), *a[1:], **kw)):
+        with pytest.raises(TypeError):
+            call(codes, scales, torch.bfloat16, out)
+        with pytest.raises(TypeError):
+            call(codes, scales, out_dtype=torch.float32, out=out.bfloat16())
+        assert call(codes, scales, torch.float32, out) is out
+        assert call(codes, scales).dtype is torch.bfloat16 and call(codes, scales, out=out).dtype is torch.float32
+    buf = torch.zeros(3 * 48 * 4, dtype=torch.int8, device="cuda")
+    with pytest.raises(ValueError):  # values over their own codes
+        dense.dequantize_rows(buf[:144].view(3, 48), scales, out=buf.view(torch.float32).view(3, 48))
