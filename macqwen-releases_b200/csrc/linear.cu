@@ -170,10 +170,12 @@ __device__ __forceinline__ uint32_t peer_word(uint32_t a, uint32_t rank) {
 
 // Activations of U values, the choice made once for all of them.  Where the
 // result stays float32, by CUDA's exp and erfc.  Where it is rounded to bfloat16
-// (2^-9) the approximate exponential and quotient (2^-21) cost nothing that
-// shows, and GELU's erfc takes the five-term form of Abramowitz and Stegun
-// 7.1.26 (absolute error 1.5e-7): a tile's epilogue has to stay shorter than its
-// MMAs.
+// (2^-9) by the approximate exponential and quotient (2^-21) and, for GELU, by
+// erfc(z) = exp(-z^2) (c1 t + .. + c6 t^6), t = 1 / (1 + 0.41 z): a tile's
+// epilogue has to stay shorter than its MMAs.  The coefficients are a minimax fit
+// (linear programme over 1,900 points of [0, 9.6]) to the lesser of an absolute
+// and a relative error: at most 1e-7, and 2^-12 of the value as far as bfloat16
+// reaches (-13).  Five terms of that absolute error alone were 0.4% off at -6.
 template <int U>
 __device__ __forceinline__ void activate(float (&v)[U], uint32_t act, bool f32) {
   switch (act) {
@@ -195,8 +197,9 @@ __device__ __forceinline__ void activate(float (&v)[U], uint32_t act, bool f32) 
         for (int i = 0; i < U; ++i) {
           // max(v, 0) - |v| erfc(|v| / sqrt 2) / 2; beyond 20 the second term is 0
           const float m = fminf(fabsf(v[i]), 20.0f);
-          const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, m, 1.0f));
-          float q = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+          const float t = __fdividef(1.0f, fmaf(0.41f * 0.70710678f, m, 1.0f));
+          float q = fmaf(-0.179154054f, t, 0.575672936f);
+          q = fmaf(fmaf(fmaf(fmaf(q, t, -0.194078793f), t, 0.363653735f), t, 0.20013245f), t, 0.233773632f);
           q = q * t * __expf(-0.5f * m * m);
           v[i] = (v[i] > 0.0f ? v[i] : 0.0f * v[i]) - 0.5f * m * q;  // 0 * v: NaN stays
         }

@@ -610,3 +610,23 @@ def test_values_out_and_out_dtype_have_to_agree(cuda_lib):
     buf = torch.zeros(3 * 48 * 4, dtype=torch.int8, device="cuda")
     with pytest.raises(ValueError):  # values over their own codes
         dense.dequantize_rows(buf[:144].view(3, 48), scales, out=buf.view(torch.float32).view(3, 48))
+
+
+@gpu
+def test_gelu_of_large_negative_values(cuda_lib):
+    """bfloat16 results: erfc to 2^-12 of itself, its exponential and quotient to 2^-13 (-v^2 / 2 down to -84.5, twice
+    rounded), then half a step of bfloat16."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    v = -torch.arange(0, 1664, device="cuda").float() / 128
+    v = v.bfloat16().unique()
+    w = torch.zeros(v.numel(), 16, dtype=torch.bfloat16, device="cuda")
+    w[:, 3] = v
+    for rows in (3, 300):
+        x = torch.zeros(rows, 16, dtype=torch.bfloat16, device="cuda")
+        x[:, 3] = 1.0
+        got = dense.linear(x, w, activation="gelu")
+        want, _ = od.linear(_np(x), _np(w), None, "gelu")
+        assert (np.abs(_np(got) - want) <= np.abs(want) * (2.0 ** -8 + 2.0 ** -11) + 1e-37).all()
