@@ -358,44 +358,41 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
       reduce_row(sum, top, G, part[turn ^= 1]);
       float gain = 1.0f;
       if (p.norm) {
-        float rms_eps = p.eps;
-        // Rows whose squares or products leave float32's range (or lose bits
-        // below it) are scaled by a power of two first.  (A product below the
-        // normal range is off by several per cent, and codes made by such a
-        // maximum would pass 127.  Where all are 0, max |y| stays below 2^-100.)
-        if (!(sum <= 0x1p120f) || !(top <= 0x1p125f) || (sum < 0x1p-80f && p.eps < 0x1p-80f) || (top < 0x1p-100f && top > 0.0f)) {
+        gain = rsqrtf(fmaf(sum, per_dim, p.eps));  // to 2^-22
+        // Rows whose squares or products leave float32's range (or lose bits below
+        // it) are scaled by powers of two first.
+        if (!(sum <= 0x1p120f) || !(top <= 0x1p125f) || sum < 0x1p-80f || top < 0x1p-60f) {
           float most = 0.0f, none = 0.0f;
 #pragma unroll
           for (int c = 0; c < VPT; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[c][e]));
           reduce_row(none, most, G, part[turn ^= 1]);
-          // by 2^-e with 2^e the power of two above max |s|, so that no product passes
-          // the weight, or about sqrt(eps) where that is larger; by 1 where max |s| is 0
-          // or not finite (2^-128 is below the normal range, but exact)
-          int e2 = 0;
           if (most != 0.0f && most < __uint_as_float(kInfBits)) {
-            e2 = max(-126, ilogbf(most) + 1);
-            if (p.eps > 0.0f) e2 = max(e2, ilogbf(p.eps) / 2);
-          }
-          const float down = ldexpf(1.0f, -e2);
-          rms_eps = ldexpf(ldexpf(p.eps, -e2), -e2);
-          sum = 0.0f;
-          top = 0.0f;
+            // s by 2^-e2, to between 1/4 and 1/2 at most, the root by 2^-e3, 2^e3 about
+            // the larger of max |s| and sqrt(eps); s and the gain take half of
+            // 2^(e2 - e3) each.  (s in two steps, since one may be no float.)
+            const int e2 = ilogbf(most) + 2, e3 = p.eps > 0.0f ? max(e2, ilogbf(p.eps) / 2) : e2;
+            const int of_s = (e2 - e3) / 2, by = of_s - e2;
+            const float first = ldexpf(1.0f, by / 2), second = ldexpf(1.0f, by - by / 2), of_gain = ldexpf(1.0f, e2 - e3 - of_s);
+            sum = 0.0f;
+            top = 0.0f;
 #pragma unroll
-          for (int c = 0; c < VPT; ++c) {
-            float w[8];
-            weights(ra, c, w);
+            for (int c = 0; c < VPT; ++c) {
+              float w[8];
+              weights(ra, c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              s[c][e] *= down;
-              sum = fmaf(s[c][e], s[c][e], sum);
-              top = larger(top, fabsf(s[c][e] * w[e]));
+              for (int e = 0; e < 8; ++e) {
+                s[c][e] *= first;
+                s[c][e] *= second;
+                sum = fmaf(s[c][e], s[c][e], sum);
+                top = larger(top, fabsf(s[c][e] * w[e]));
+              }
             }
+            reduce_row(sum, top, G, part[turn ^= 1]);
+            gain = rsqrtf(sum * per_dim * of_gain * of_gain + ldexpf(ldexpf(p.eps, -e3), -e3)) * of_gain;
           }
-          reduce_row(sum, top, G, part[turn ^= 1]);
         }
-        gain = rsqrtf(fmaf(sum, per_dim, rms_eps));  // to 2^-22
       }
       float inv = 0.0f;
       bool codes_are_0 = false;
@@ -412,7 +409,7 @@ __global__ void __launch_bounds__(512, VPT <= 2 ? 2 : 1) k_norm(NormView p, int 
         float w[8];
         weights(ra, c, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[c][e] = s[c][e] * gain * w[e];
+        for (int e = 0; e < 8; ++e) s[c][e] = s[c][e] * w[e] * gain;  // in this order none passes top gain, nor a code 127
         if (p.y) store8<D>(static_cast<TX *>(p.y), k, ra, c, s[c]);
         if (p.codes) {
 #pragma unroll

@@ -630,3 +630,30 @@ def test_gelu_of_large_negative_values(cuda_lib):
         got = dense.linear(x, w, activation="gelu")
         want, _ = od.linear(_np(x), _np(w), None, "gelu")
         assert (np.abs(_np(got) - want) <= np.abs(want) * (2.0 ** -8 + 2.0 ** -11) + 1e-37).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,dim,pad", [(3, 512, 0), (3, 513, 0), (4, 512, 3), (700, 512, 0), (3, 1, 0)])
+def test_norm_where_eps_is_far_above_the_squares(cuda_lib, kind, rows, dim, pad):
+    """s / sqrt(eps) is subnormal, or 0, and the weight large: y and its codes are not; rows of zeros among them."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    g = _gen(dim + rows)
+    rand = lambda *s: torch.rand(*s, device="cuda", generator=g)  # noqa: E731
+    for size, large, eps in ((2.0 ** -119, 2.0 ** 59, 7e14), (2.0 ** -90, 2.0 ** 97, 2e25), (2.0 ** -130, 2.0 ** 110, 1e-6),
+                             (2.0 ** -140, 2.0 ** 120, 1e38), (2.0 ** -130, 1.0, 1e-20), (2.0 ** -130, 2.0 ** 110, 0.0),
+                             (2.0 ** -60, 2.0 ** 126, 3e38), (2.0 ** -148, 2.0 ** -100, 0.0)):
+        x = (1 + rand(rows, dim)) * torch.where(rand(rows, dim) < 0.5, -size, size)
+        if eps:
+            x[1] = 0.0
+        x, w = _cut(x, pad), (1 + rand(dim)) * large
+        got = dense.add_rms_norm(x, w, None, eps, codes=_types()[kind], keep=True)
+        y, _ = od.add_rms_norm(_np(x), _np(w), None, float(np.float32(eps)))
+        bound = np.abs(y) * 2.0 ** -17 + 2.0 ** -140
+        bad = np.isfinite(_np(got.y)) != (np.abs(y) < 2.0 ** 128)
+        live = (np.abs(y) < 2.0 ** 127.99).all(1)
+        assert not bad[live].any() and (np.abs(_np(got.y) - y) <= bound)[live].all()
+        _held(got.codes[torch.from_numpy(live).cuda()], got.scales[torch.from_numpy(live).cuda()], y[live], kind)
