@@ -502,7 +502,7 @@ constexpr int weight_smem(uint32_t dim) { return static_cast<int>(((dim / 8 + 1)
 template <Deal D, int VPT, typename TX, typename TR>
 cudaError_t launch_k(const NormView &p, int per, int G, cudaStream_t s) {
   const size_t smem = p.norm && D != kEven ? weight_smem(static_cast<uint32_t>(p.dim)) : 0;
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {  // (48 KB with the kernel's own need no leave)
     static SmemLimit limit;
     const cudaError_t e = limit.set(reinterpret_cast<const void *>(k_norm<D, VPT, TX, TR>), weight_smem(kMaxDim));
     if (e != cudaSuccess) return e;

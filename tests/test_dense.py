@@ -657,3 +657,18 @@ def test_norm_where_eps_is_far_above_the_squares(cuda_lib, kind, rows, dim, pad)
         live = (np.abs(y) < 2.0 ** 127.99).all(1)
         assert not bad[live].any() and (np.abs(_np(got.y) - y) <= bound)[live].all()
         _held(got.codes[torch.from_numpy(live).cuda()], got.scales[torch.from_numpy(live).cuda()], y[live], kind)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [10209, 10247, 12209, 12215, 12217, 12250, 12279, 12281, 12287, 12289])
+def test_norm_of_widths_whose_weights_nearly_fill_48_kb(cuda_lib, dim):
+    """The weights that lie in shared memory and the kernel's own variables there pass 48 KB together."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    w = 1 + 0.1 * torch.randn(dim, device="cuda", generator=_gen(dim))
+    for rows, pad in ((3, 0), (3, 1), (400, 0), (400, 1)):
+        x = _cut(torch.randn(rows, dim, device="cuda", generator=_gen(rows)), pad)
+        y, _ = od.add_rms_norm(_np(x), _np(w))
+        assert (np.abs(_np(dense.add_rms_norm(x, w).y) - y) <= np.abs(y) * (HALF["f32"] + 2.0 ** -18) + 1e-37).all()
