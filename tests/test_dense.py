@@ -672,3 +672,44 @@ def test_norm_of_widths_whose_weights_nearly_fill_48_kb(cuda_lib, dim):
         x = _cut(torch.randn(rows, dim, device="cuda", generator=_gen(rows)), pad)
         y, _ = od.add_rms_norm(_np(x), _np(w))
         assert (np.abs(_np(dense.add_rms_norm(x, w).y) - y) <= np.abs(y) * (HALF["f32"] + 2.0 ** -18) + 1e-37).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("m,k,n,rpad", [(3000, 528, 2100, 0), (5000, 2064, 1003, 5), (4000, 144, 2050, 1)])
+def test_linear_float32_results_of_several_items_a_pair(cuda_lib, kind, m, k, n, rpad):
+    """Chunks summed in registers, with accumulators and ring handed from item to item across a pair of CTAs."""
+    import torch
+
+    g = _gen(m + n)
+    res = _cut(torch.randn(m, n, device="cuda", generator=g), rpad)
+    x, w, xs, ws = _product(m, k, n, kind, m)
+    got = _check_linear(x, w, xs, ws, kind, "f32", None, "silu", res)
+    assert torch.equal(_check_linear(x, w, xs, ws, kind, "f32", None, "silu", res), got)
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim,pad,at", [(297, 513, 3, 1), (1200, 100, 1, 0), (700, 1027, 5, 3), (320, 2560, 1, 1),
+                                             (300, 4099, 2, 0), (297, 8200, 1, 1), (301, 15001, 3, 2)])
+@pytest.mark.parametrize("xd,rd,kind", [("bf16", None, "int8"), ("bf16", "bf16", "e4m3"), ("f32", None, "e4m3"),
+                                        ("f32", "f32", "int8"), ("bf16", "f32", None)])
+def test_norm_of_many_rows_off_boundaries(cuda_lib, rows, dim, pad, at, xd, rd, kind):
+    """Padded rows that start at any value, enough of them for a thread to hold several chunks of a row."""
+    import torch
+
+    from flashnext_b200 import dense
+
+    t, g = _types(), _gen(rows + dim)
+    randn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x = _cut(randn(rows, dim).to(t[xd]), pad, at)
+    res = None if rd is None else _cut(randn(rows, dim).to(t[rd]), pad, at)
+    w = (1 + 0.3 * randn(dim)).bfloat16()
+    got = dense.add_rms_norm(x, w, res, 1e-5, codes=None if kind is None else t[kind], keep=True)
+    y, s = od.add_rms_norm(_np(x), _np(w), None if res is None else _np(res), 1e-5)
+    assert (np.abs(_np(got.y) - y) <= np.abs(y) * (HALF[xd] + 2.0 ** -18) + 1e-37).all()
+    if rd:
+        assert (np.abs(_np(got.residual) - s) <= np.abs(s) * (HALF[rd] + 2.0 ** -23) + 1e-37).all()
+    if kind:
+        _held(got.codes, got.scales, y, kind)
+        codes, scales = dense.quantize_rows(x, t[kind])
+        _held(codes, scales, _np(x), kind)
