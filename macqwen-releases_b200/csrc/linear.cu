@@ -13,9 +13,10 @@
 // to 131071 keep 128^2 K below 2^31).  The epilogue works on float32 and rounds
 // once, to the output's type.
 //
-// Measured: 16 x 2048 > 131072 (a head) 87.5 us, 6.2 TB/s; 1 x 2048 > 5120 6.6 us;
-// 5000 x 2048 > 5120 with SiLU 83.5 us, 1,256 TFLOP/s of 1,653; 8192 x 4096 x 4096
-// int8 98 us, 2,800 TOPS.
+// Measured: 16 x 2048 > 131072 (a head) 88 us, 6.2 TB/s; 1 x 2048 > 5120 7.9 us;
+// 5000 x 2048 > 5120 with SiLU 84 us, 1,248 TFLOP/s of 1,653, with pauses between
+// the calls (98 us back to back, under the power limit); 8192 x 4096 x 4096 int8
+// 95 us, 2,890 TOPS.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -643,7 +644,8 @@ cudaError_t launch(const CUtensorMap &wm, const CUtensorMap &xm, LinearView p, i
   // about 2^-25 an addition that grows with their number (measured: 2.2e-6 of
   // the result after 128 of them).  Results that stay float32 are summed 16
   // additions at a time (32 in pairs, whose epilogue is busier) and those sums
-  // added with rounding; bfloat16 results do not show it, int8 sums are exact.
+  // added with rounding; bfloat16 results keep the bias (2^-12 at the largest width,
+  // where their rounding takes up to 2^-8), int8 sums are exact.
   p.chunk = KIND != kInt8 && p.out_f32 ? (PAIR ? 8 : 4) : p.k_steps;
   const int cluster = PAIR ? 2 : p.split;
   cudaLaunchConfig_t cfg = {};
@@ -673,7 +675,12 @@ int run(const FnLinearArgs *a, LinearView &p, cudaStream_t s, std::string &err) 
   constexpr uint64_t size = KIND == kBf16 ? 2 : 1;
   const int sms = device_info().sms;
   const bool sums = KIND != kInt8 && p.out_f32;
-  // pairs from 257 rows on, where there are two tiles of weight rows
+  // Pairs from 257 rows on, where there are two tiles of weight rows.  x 2048 > 5120,
+  // one CTA alone and in pairs, us: float32 results 26 and 18 at 512 rows, 60 and 44
+  // at 2,000, 129 and 114 at 5,000 (but 15.5 and 16.9 at 384); bfloat16 80 and 79 at
+  // 5,000, 37 and 38 at 2,000, 14.7 and 15.9 at 512; int8 (e4m3 much the same) 46.5
+  // and 46.5 at 5,000, 23 and 24.5 at 2,000, 10.5 and 11.5 at 512; 8192 x 4096 x 4096
+  // int8 117 and 94.
   const bool pair = p.rows > 256 && p.width > kLanes;
   const int nt = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : p.rows <= 128 ? 128 : !sums ? 256 : pair ? 192 : 128;
   const int64_t lanes = pair ? 2 * kLanes : kLanes, w_tiles = (p.width + lanes - 1) / lanes, step = pair ? 32 : 16;
@@ -682,6 +689,8 @@ int run(const FnLinearArgs *a, LinearView &p, cudaStream_t s, std::string &err) 
     // Tiles as wide as leaves the last round of items no emptier than the
     // others: fewest rounds x columns (and 48 columns' time for an item's start
     // and end).  1024 x 5120: 7 tiles of 160 in two rounds, not 4 of 256 in two.
+    // (5000 x 2048 > 5120 bfloat16: 118 us without the 48, 104 with 16, 79.5 with 48,
+    // 79.3 with 128; e4m3 70, 61, 49, 49; from 600 to 3,000 rows all alike.)
     const int64_t tiles0 = (p.rows + nt - 1) / nt, slots = pair ? sms / 2 : sms;
     int64_t least = INT64_MAX;
     for (int64_t n = tiles0; n <= 2 * tiles0 && n < tiles0 + 64; ++n) {

@@ -14,9 +14,11 @@
 // nothing).
 //
 // Bound by issue slots and HBM: CTAs stay on their SM and ask for rows ahead, and
-// nothing is chosen a value at a time.  5000 x 2048 bfloat16 with a residual: 17.5
-// us, 4.7 TB/s of 6.46 (41 instructions a value with codes, 55 in the first form);
-// one row of 2048: 2.0 us, of which a launch is most.
+// nothing is chosen a value at a time.  5000 x 2048 bfloat16 with a residual: 17 to 19
+// us, 4.3 to 4.8 TB/s of 6.46 (41 instructions a value with codes, 55 in the first
+// form); one row of 2048: 2.0 us, of which a launch is most.  Rows off boundaries that
+// are not contiguous (kOdd): 69 us padded to 2051, one value a load, and values of
+// two chunks that do not fit the registers.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>

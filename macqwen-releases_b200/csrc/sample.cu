@@ -19,9 +19,10 @@
 // flat distribution, whose borders lie 2^-17 apart.
 //
 // Bound by issue slots (57 to 163 instructions a token over all passes) and, for
-// few rows, by a chain of cluster barriers of about 1 us: 1 x 131072 with top-k 50,
-// top-p and min-p 10.4 us; 64 x 131072 33.4 us, with settings of their own 54.9 us,
-// top-p alone 77.5 us.
+// few rows, by short steps that follow one another (loads, the largest and its
+// barriers 3.6 us, then the bound's search, a list, its ranks and sums): 1 x 131072
+// with top-k 50, top-p and min-p 10.2 us; 64 x 131072 33.4 us, with settings of
+// their own 55 us, top-p alone 78 us.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -763,7 +764,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleView p) {
 template <typename T>
 cudaError_t launch(SampleView p, int rows, int sms, cudaStream_t s) {
   // CTAs of a row: as many as finish soonest, by rounds over the SMs (two CTAs
-  // each) times a CTA's tokens and about 8000 tokens' time for its barriers.
+  // each) times a CTA's tokens and about 8000 tokens' time for its barriers.  Top-p
+  // alone, us at 1, 2, 4, 8, 16 CTAs (131072 float32 tokens from 4 on): 296 x 32003
+  // bfloat16 54 73 113 203 490 (1 taken); 64 x 32000 36 27 29 45 102 (2); 64 x 131072
+  // 80 78 135 (8); 1 x 131072 38 27 22 (16).  It takes one step too many at 16 x 131072
+  // (39 35 47: 16 taken), 8 x 32000 (36 25 19 17 23: 16) and 300 x 32003 (84 88: 2).
   constexpr int kMost = 72 * 1024 / sizeof(T);  // tokens that leave room for a second CTA
   constexpr int kMostBytes = 160 * 1024;         // of a CTA's tokens
   constexpr size_t kFirst = (sizeof(Shared) + 15) / 16 * 16 + 16;

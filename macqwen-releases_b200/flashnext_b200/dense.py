@@ -155,7 +155,8 @@ def _code_rows(rows, dim, codes, like):
 def quantize_rows(x, codes=torch.int8):
     """``(codes, scales)`` of the rows of ``x`` [rows, dim] (bfloat16 or float32):
     ``scales[r] = max(max|x[r]|, 2^-100) / top`` and ``codes`` the nearest codes
-    of ``x / scales``, ``top`` 127 (torch.int8) or 448 (torch.float8_e4m3fn).
+    of ``x / scales``, ``top`` 127 (torch.int8) or 448 (torch.float8_e4m3fn); a
+    quotient as near the middle of two codes as 2^-21 of itself may take either.
     A row that is not finite gets NaN as its scale.  ``dim`` is at most 16384."""
     index = x.get_device()
     xd = _float(x, "x")
