@@ -171,7 +171,7 @@ __device__ __forceinline__ uint32_t peer_word(uint32_t a, uint32_t rank) {
 
 // Activations of U values, the choice made once for all of them.  Where the
 // result stays float32, by CUDA's exp and erfc.  Where it is rounded to bfloat16
-// (2^-9) by the approximate exponential and quotient (2^-21) and, for GELU, by
+// (2^-8) by the approximate exponential and quotient (2^-21) and, for GELU, by
 // erfc(z) = exp(-z^2) (c1 t + .. + c6 t^6), t = 1 / (1 + 0.41 z): a tile's
 // epilogue has to stay shorter than its MMAs.  The coefficients are a minimax fit
 // (linear programme over 1,900 points of [0, 9.6]) to the lesser of an absolute

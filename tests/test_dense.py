@@ -713,3 +713,42 @@ def test_norm_of_many_rows_off_boundaries(cuda_lib, rows, dim, pad, at, xd, rd, 
         _held(got.codes, got.scales, y, kind)
         codes, scales = dense.quantize_rows(x, t[kind])
         _held(codes, scales, _np(x), kind)
+
+
+@gpu
+def test_products_of_four_threads_at_once(cuda_lib):
+    """A split by clusters, tiles of one CTA and pairs side by side on streams of their own."""
+    import threading
+
+    import torch
+
+    from flashnext_b200 import dense
+
+    def job(m, k, n, kind):
+        x, w, xs, ws = _product(m, k, n, kind, m)
+        return lambda: dense.linear(x, w, x_scale=xs, weight_scale=ws, out_dtype=torch.float32)
+
+    jobs = [job(3, 2048, 1024, "bf16"), job(64, 512, 20000, "int8"), job(700, 1024, 2100, "e4m3"), job(300, 528, 1000, "bf16")]
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(len(jobs)), []
+
+    def work(j, out):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(40):
+                    got = [j() for _ in range(25)]
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(g, out) for g in got):
+                        wrong.append("another result")
+        except Exception as e:  # noqa: BLE001
+            wrong.append(str(e))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(jobs, want)]
+    for a in threads:
+        a.start()
+    for a in threads:
+        a.join()
+    assert not wrong
+    assert _lib.read_device_errors() == 0
